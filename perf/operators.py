@@ -5,11 +5,12 @@
   act8_save    activations into 8 bits with a power-of-two exponent for each 32 channels of a token, and restored
   act8_wgrad   the weight gradient of a linear layer, dW = base + X^T dY, from activations held that way
 
-Formats (also in include/subcuber_b200.h):
-  4-bit weights: codes[n][pitch] bytes, low nibble = even input, pitch = inputs / 2 rounded up to 16 bytes; scales[groups][n] in the
-  16-bit type of the activations, zeros[groups][n] bytes or none (then 8);  W[n][k] = scale * (code - zero).
+Formats:
+  4-bit weights: scales[groups][n] in the 16-bit type of the activations, zeros[groups][n] bytes or none (then 8);
+  W[n][k] = scale * (code - zero).  The plain form keeps two codes to a byte, low nibble = even input; the framework packs
+  codes in an order of its own.
   8-bit activations: codes[m][pitch] bytes, bit 7 = sign, bits 0-6 = magnitude, pitch = channels rounded up to 16 bytes;
-  exponents[m][blocks] bytes;  X[m][k] = +-magnitude * 2^(exponent - 127), exponent 255 = NaN.
+  exponents[m][blocks rounded up to 4] bytes;  X[m][k] = +-magnitude * 2^(exponent - 127), exponent 255 = NaN.
 """
 import math
 
@@ -141,7 +142,7 @@ def _act8_codes(x):
 
 def _act8_values(codes, exponents, k):
     """Activations [m, k] in 32 bits that bytes and exponents stand for."""
-    E = exponents.to(torch.int32)
+    E = exponents[:, : -(-k // BLOCK)].to(torch.int32)
     scale = torch.where(E == 255, torch.full_like(E, math.nan, dtype=torch.float32), _power(E.clamp(1, 254) - 127))
     c = codes[:, :k].to(torch.int32)
     v = _groups(torch.where(c > 127, 128 - c, c), BLOCK) * scale[:, :, None]
@@ -168,27 +169,31 @@ def prepare(case, seed):
             st["w"] = w
         else:
             q, s, z = _w4_codes(w, case["group"], case["symmetric"])
-            st["codes"], st["scales"] = _w4_pack(q), s.t().contiguous()
+            st["scales"] = s.t().contiguous()
             st["zeros"] = None if case["symmetric"] else z.to(torch.uint8).t().contiguous()
+            if own:
+                from subcuber_b200 import lowbit
+
+                st["weights"] = lowbit.pack_w4(q.to(torch.uint8), st["scales"], st["zeros"], group=case["group"])
+                st["workspace"] = lowbit.WorkspaceW4(case["m"], st["weights"])
+            else:
+                st["codes"] = _w4_pack(q)
             st["x"] = _activations(case["m"], case["k"], dtype, gen)
     else:
         x = _activations(case["m"], case["k"], dtype, gen)
         if op == "act8_save":
             st["x"] = x
         else:
-            q, st["exponents"] = _act8_codes(x)
+            q, E = _act8_codes(x)
+            st["exponents"] = torch.nn.functional.pad(E, (0, _up(E.shape[1], 4) - E.shape[1]), value=1).contiguous()
             st["codes"] = torch.nn.functional.pad(q, (0, _up(case["k"], 16) - case["k"])).contiguous()
             st["dy"] = (torch.randn(case["m"], case["n"], generator=gen, device="cuda") * 0.125).to(dtype)
             st["base"] = torch.randn(case["k"], case["n"], generator=gen, device="cuda").to(TYPES[case["out"]]) if case["base"] else None
-    if own:
-        from subcuber_b200 import lowbit
+            if own:
+                from subcuber_b200 import lowbit
 
-        if op == "w4_gemm":
-            st["weights"] = lowbit.WeightsW4(st["codes"], st["scales"], st["zeros"], k=case["k"], group=case["group"])
-            st["workspace"] = lowbit.WorkspaceW4(case["m"], st["weights"])
-        elif op == "act8_wgrad":
-            st["saved"] = lowbit.Checkpoint8(st["codes"], st["exponents"], k=case["k"], dtype=dtype)
-            st["workspace"] = lowbit.WorkspaceGrad8(st["saved"], case["n"])
+                st["saved"] = lowbit.Checkpoint8(st["codes"], st["exponents"], k=case["k"], dtype=dtype)
+                st["workspace"] = lowbit.WorkspaceGrad8(st["saved"], case["n"], TYPES[case["out"]])
     return st
 
 
@@ -253,7 +258,12 @@ def _step(e):
 
 
 def exact(case, seed):
-    st = prepare(case, seed)
+    global own
+    kept, own = own, False  # the plain codes, whichever side asks
+    try:
+        st = prepare(case, seed)
+    finally:
+        own = kept
     op, k = case["op"], case["k"]
     at = torch.arange(k, device="cuda")
     if op == "w4_gemm":
