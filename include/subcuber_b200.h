@@ -282,6 +282,56 @@ int sb200_peer_signal(int* const* peer_flags, int count, int value, sb200_stream
 int sb200_peer_wait(int* const* local_flags, int count, int value, unsigned wait_limit_us, int* status,
                     sb200_stream_t stream);
 
+/* ---- products with one operand held in few bits ---------------------------------------------------------------------
+ * What the linear layers of a language model need beside the GEMM above: weights in 4 bits (serving), activations saved
+ * in 8 bits for the backward pass (training).  dtype and out_dtype: 0 f16, 1 f32, 3 bf16.  All calls are asynchronous on
+ * `stream`, allocate nothing, and may be captured into graphs; a workspace belongs to one call at a time (two calls that
+ * may overlap need two).  Matrices are row-major with a leading dimension in elements; rows need no alignment beyond
+ * their elements'.  m = 0 is an empty batch.  No counterpart in the reference project.
+ *
+ * Weights in 4 bits, n outputs x k inputs, groups of G = 32, 64 or 128 inputs of an output:
+ *     W[n][k] = scale[k / G][n] * (code[n][k] - zero[k / G][n]),   code and zero in 0..15, zero = 8 where zeros == NULL
+ * scales (in the 16-bit type `dtype`) and zeros (bytes) are tables of ceil(k / G) rows of sb200_w4_table_rows(n) entries.
+ * codes (16-byte aligned, sb200_w4_codes_bytes(n, k) bytes) are tiles of 16 outputs x 128 inputs, 1 KiB each, along the inputs
+ * first: bytes 512 h + 16 (4 g + t) + 4 j of a tile hold the 32-bit word of output 8 h + g and inputs 32 j + 8 t + i, i = 0..7,
+ * input i in nibble (i >> 1) + 4 (i & 1).  sb200_w4_pack brings plain codes (one byte each) into this order. */
+size_t sb200_w4_codes_bytes(int n, int k);
+size_t sb200_w4_table_rows(int n);
+/* Quantise w (n x k, 16-bit), group by group.  zeros == NULL: scale = amax / 7, code = 8 + rint(w / scale).  Else, with
+ * lo = min(0, w) and hi = max(0, w): scale = (hi - lo) / 15, zero = rint(-lo / scale), code = zero + rint(w / scale).  The
+ * scale is rounded to `dtype` before the codes are made; codes are held within 0..15.  A group with an infinity or a NaN
+ * (or whose hi - lo overflows) gets a scale that is not finite: its weights stand for NaN. */
+int sb200_w4_quantize(int dtype, const void* w, long long ldw, int n, int k, int group, void* codes, void* scales, void* zeros,
+                      sb200_stream_t stream);
+/* Codes of another quantiser, one byte each in the low nibble, q[n][k], into the order above. */
+int sb200_w4_pack(const void* q, long long ldq, int n, int k, void* codes, sb200_stream_t stream);
+/* out[n][k] = W rounded once to `dtype`. */
+int sb200_w4_dequantize(int dtype, const void* codes, const void* scales, const void* zeros, int n, int k, int group, void* out,
+                        long long ldo, sb200_stream_t stream);
+/* y[m][n] = sum over k of x[m][k] W[n][k], sums in fp32, rounded once to `dtype`. */
+size_t sb200_w4_gemm_workspace_bytes(int dtype, int m, int n, int k, int group);
+int sb200_w4_gemm(int dtype, const void* x, long long ldx, const void* codes, const void* scales, const void* zeros, void* y,
+                  long long ldy, int m, int n, int k, int group, void* workspace, size_t workspace_bytes, sb200_stream_t stream);
+
+/* Activations in 8 bits, m tokens x k channels, a power-of-two step for each 32 channels of a token:
+ *     X[m][k] = +-magnitude * 2^(exponent[m][k / 32] - 127),   bit 7 of the byte = sign, bits 0-6 = magnitude
+ * Rows of codes start every `pitch` bytes (a multiple of 16, at least k), rows of exponents every `exp_pitch` (a multiple
+ * of 4, at least ceil(k / 32)); codes are 16-byte, exponents 4-byte aligned.  The step is 2^(floor(log2 amax) - 6), at least
+ * 2^-24 (f16) or 2^-126 (bf16); magnitude = min(127, rint(|x| / step)).  A block with an infinity or a NaN (bf16: or a
+ * magnitude of 2^127 and more) gets exponent 255 and reads as NaN.  Every other X is exact in `dtype`. */
+int sb200_act8_save(int dtype, const void* x, long long ldx, int m, int k, void* codes, long long pitch, void* exponents,
+                    long long exp_pitch, sb200_stream_t stream);
+int sb200_act8_restore(int dtype, const void* codes, long long pitch, const void* exponents, long long exp_pitch, int m, int k,
+                       void* x, long long ldx, sb200_stream_t stream);
+/* Weight gradient of y = x W (W is k x n, as B of sb200_gemm) from saved activations:
+ *     dw[k][n] = base[k][n] + sum over m of X[m][k] dy[m][n]
+ * dy in `dtype`; base (NULL: none; it may be dw itself) and dw in out_dtype, which is f32 or `dtype`.  Sums in fp32, rounded
+ * once.  m = 0 gives base, or zeros. */
+size_t sb200_act8_wgrad_workspace_bytes(int dtype, int out_dtype, int m, int n, int k);
+int sb200_act8_wgrad(int dtype, const void* codes, long long pitch, const void* exponents, long long exp_pitch, const void* dy,
+                     long long lddy, int out_dtype, const void* base, long long ldbase, void* dw, long long lddw, int m, int n,
+                     int k, void* workspace, size_t workspace_bytes, sb200_stream_t stream);
+
 /* Seeded synthetic inputs, bit-identical on host and device for dist 0 and 2 (dist 1 uses libm / device
  * math and agrees to rounding).  dtype: 0 f16, 1 f32, 2 f64, 3 bf16.  dist: 0 uniform[-1,1), 1 normal(0,1),
  * 2 the reference harness' value set (multiples of 0.25 in [-4,4] for f16, [-16,16] otherwise;

@@ -103,5 +103,20 @@ def load(build_if_missing: bool = True) -> C.CDLL:
     lib.sb200_peer_wait.argtypes = [C.POINTER(C.c_void_p), C.c_int, C.c_int, C.c_uint, C.c_void_p, C.c_void_p]
     lib.sb200_gemm_f16_sw_static_scratch.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int,
                                                      C.c_void_p, C.c_int]
+    p, i, ll, z = C.c_void_p, C.c_int, C.c_longlong, C.c_size_t
+    for name, res, args in (
+            ("sb200_w4_codes_bytes", z, [i, i]),
+            ("sb200_w4_table_rows", z, [i]),
+            ("sb200_w4_quantize", i, [i, p, ll, i, i, i, p, p, p, p]),
+            ("sb200_w4_pack", i, [p, ll, i, i, p, p]),
+            ("sb200_w4_dequantize", i, [i, p, p, p, i, i, i, p, ll, p]),
+            ("sb200_w4_gemm_workspace_bytes", z, [i, i, i, i, i]),
+            ("sb200_w4_gemm", i, [i, p, ll, p, p, p, p, ll, i, i, i, i, p, z, p]),
+            ("sb200_act8_save", i, [i, p, ll, i, i, p, ll, p, ll, p]),
+            ("sb200_act8_restore", i, [i, p, ll, p, ll, i, i, p, ll, p]),
+            ("sb200_act8_wgrad_workspace_bytes", z, [i, i, i, i, i]),
+            ("sb200_act8_wgrad", i, [i, p, ll, p, ll, p, ll, i, p, ll, p, ll, i, i, i, p, z, p])):
+        fn = getattr(lib, name)
+        fn.restype, fn.argtypes = res, args
     _lib = lib
     return lib

@@ -1,0 +1,232 @@
+// Activations saved in 8 bits (format ACT8 of lowbit_format.cuh): saving, restoring, and the weight gradient
+// dW = base + X^T dY of a linear layer from them.
+#include <stdint.h>
+
+#include "../../include/subcuber_b200.h"
+#include "lowbit_format.cuh"
+#include "lowbit_host.h"
+#include "simple_product.cuh"
+
+namespace sb200 {
+namespace lowbit {
+namespace {
+
+constexpr int kThreads = 256;
+
+// A thread handles 16 channels of a token, half a block.  `cols` threads (a power of two) stand along a row, the
+// others of the 256 on further rows.
+struct Cut {
+  int pieces;         // 16-channel pieces of a row
+  int cols_log2;      // threads along a row, as a power of two
+  long long parts;    // thread blocks along a row
+  long long blocks;   // thread blocks in all
+};
+
+Cut cut_of(int m, int k) {
+  Cut c;
+  c.pieces = 2 * ceil_div(k, kActBlock);  // whole blocks of 32: both halves take part in the block's maximum
+  c.cols_log2 = 1;
+  while (c.cols_log2 < 8 && (1 << c.cols_log2) < c.pieces) ++c.cols_log2;
+  c.parts = ceil_div(c.pieces, 1 << c.cols_log2);
+  c.blocks = c.parts * ceil_div(m, kThreads >> c.cols_log2);
+  return c;
+}
+
+template <typename T>
+__device__ __forceinline__ void load16(const T* row, int k0, int k, bool wide, T (&v)[16]) {
+  if (wide && k0 + 16 <= k) {
+    reinterpret_cast<uint4*>(v)[0] = __ldg(reinterpret_cast<const uint4*>(row + k0));
+    reinterpret_cast<uint4*>(v)[1] = __ldg(reinterpret_cast<const uint4*>(row + k0) + 1);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = k0 + i < k ? row[k0 + i] : from_f32<T>(0.f);
+  }
+}
+
+// The step of a block is 2^(floor(log2 amax) - 6): magnitudes reach 64..127 and the largest error is half a step, but
+// for magnitudes above 127.5 steps, which are held at 127 (off by less than one step, 0.8 %).  The exponent is read
+// from the bits of the largest magnitude; scaling by a power of two is exact, so rint() is the only rounding.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) act8_save_kernel(const T* __restrict__ x, long long ldx, int m, int k,
+                                                             uint8_t* __restrict__ codes, long long pitch,
+                                                             uint8_t* __restrict__ exps, long long exp_pitch, Cut cut, bool wide) {
+  const long long rb = blockIdx.x / cut.parts;
+  const int part = static_cast<int>(blockIdx.x % cut.parts);
+  const long long row = (rb << (8 - cut.cols_log2)) + (threadIdx.x >> cut.cols_log2);
+  const int piece = (part << cut.cols_log2) + (threadIdx.x & ((1 << cut.cols_log2) - 1));
+  const bool live = row < m && piece < cut.pieces;
+  const int k0 = piece * 16;
+  T v[16];
+  load16<T>(x + (live ? row : 0) * ldx, k0, live ? k : 0, wide, v);
+  uint32_t top = 0;  // magnitudes compare as their bits, NaN above infinity
+  float f[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    f[i] = to_f32(v[i]);
+    const uint32_t bits = __float_as_uint(f[i]) & 0x7fffffffu;
+    top = bits > top ? bits : top;
+  }
+  const uint32_t other = __shfl_xor_sync(0xffffffffu, top, 1);
+  top = other > top ? other : top;
+  int e = static_cast<int>(top >> 23) - 127 - 6;
+  const bool bad = top >= 0x7f800000u || e > ActRange<T>::hi;
+  if (e < ActRange<T>::lo) e = ActRange<T>::lo;
+  const float inv = __uint_as_float(static_cast<uint32_t>(127 - (bad ? 0 : e)) << 23);
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    w[j] = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float a = f[4 * j + i];
+      const uint32_t mag = bad ? 0u : static_cast<uint32_t>(fminf(rintf(fabsf(a) * inv), 127.f));
+      w[j] |= (mag | ((__float_as_uint(a) >> 24) & 128u)) << (8 * i);
+    }
+  }
+  if (!live) return;
+  // the second half of a row's last block may lie behind the row, which ends at k rounded up to 16
+  if (k0 < k) *reinterpret_cast<uint4*>(codes + row * pitch + k0) = make_uint4(w[0], w[1], w[2], w[3]);
+  if (!(piece & 1)) exps[row * exp_pitch + (piece >> 1)] = static_cast<uint8_t>(bad ? kActNaN : e + 127);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) act8_restore_kernel(const uint8_t* __restrict__ codes, long long pitch,
+                                                                const uint8_t* __restrict__ exps, long long exp_pitch, int m,
+                                                                int k, T* __restrict__ x, long long ldx, Cut cut, bool wide) {
+  const long long rb = blockIdx.x / cut.parts;
+  const int part = static_cast<int>(blockIdx.x % cut.parts);
+  const long long row = (rb << (8 - cut.cols_log2)) + (threadIdx.x >> cut.cols_log2);
+  const int piece = (part << cut.cols_log2) + (threadIdx.x & ((1 << cut.cols_log2) - 1));
+  const int k0 = piece * 16;
+  if (row >= m || k0 >= k) return;
+  const uint4 raw = __ldg(reinterpret_cast<const uint4*>(codes + row * pitch + k0));
+  const float step = act8_step(exps[row * exp_pitch + (piece >> 1)]);
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  T v[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = from_f32<T>(act8_value((w[i >> 2] >> (8 * (i & 3))) & 255u, step));
+  T* to = x + row * ldx + k0;
+  if (wide && k0 + 16 <= k) {
+    reinterpret_cast<uint4*>(to)[0] = reinterpret_cast<const uint4*>(v)[0];
+    reinterpret_cast<uint4*>(to)[1] = reinterpret_cast<const uint4*>(v)[1];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (k0 + i < k) to[i] = v[i];
+  }
+}
+
+struct ActLeft {  // X^T as the left operand of a product: (channel, token)
+  const uint8_t* codes;
+  long long pitch;
+  const uint8_t* exps;
+  long long exp_pitch;
+  int k, m;
+  __device__ float operator()(int ch, int t) const {
+    if (ch >= k || t >= m) return 0.f;
+    return act8_value(codes[t * pitch + ch], act8_step(exps[t * exp_pitch + ch / kActBlock]));
+  }
+};
+template <typename T>
+struct DenseRight {
+  const T* p;
+  long long ld;
+  int rows, cols;
+  __device__ float operator()(int k, int j) const { return k < rows && j < cols ? to_f32(p[k * ld + j]) : 0.f; }
+};
+
+inline bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+int check(const Act8& a) {
+  if (a.dtype != kF16 && a.dtype != kBF16) return kErrNotSupported;
+  if (a.m < 0 || a.k <= 0 || a.pitch < a.k || a.exp_pitch < ceil_div(a.k, kActBlock)) return kErrInvalidProblem;
+  if (a.m > 0 && (!a.codes || !a.exps)) return kErrInvalidProblem;
+  if (!aligned(a.codes, 16) || a.pitch % 16 || !aligned(a.exps, 4) || a.exp_pitch % 4) return kErrMisalignedOperand;
+  return kOk;
+}
+
+template <typename T>
+int save(const void* x, long long ldx, const Act8& a, cudaStream_t stream) {
+  const Cut cut = cut_of(a.m, a.k);
+  if (cut.blocks > 0x7fffffffll) return kErrNotSupported;
+  act8_save_kernel<T><<<static_cast<unsigned>(cut.blocks), kThreads, 0, stream>>>(
+      static_cast<const T*>(x), ldx, a.m, a.k, static_cast<uint8_t*>(const_cast<void*>(a.codes)), a.pitch,
+      static_cast<uint8_t*>(const_cast<void*>(a.exps)), a.exp_pitch, cut, aligned(x, 16) && ldx % 8 == 0);
+  return static_cast<int>(cudaGetLastError());
+}
+
+template <typename T>
+int restore(const Act8& a, void* x, long long ldx, cudaStream_t stream) {
+  const Cut cut = cut_of(a.m, a.k);
+  if (cut.blocks > 0x7fffffffll) return kErrNotSupported;
+  act8_restore_kernel<T><<<static_cast<unsigned>(cut.blocks), kThreads, 0, stream>>>(
+      static_cast<const uint8_t*>(a.codes), a.pitch, static_cast<const uint8_t*>(a.exps), a.exp_pitch, a.m, a.k,
+      static_cast<T*>(x), ldx, cut, aligned(x, 16) && ldx % 8 == 0);
+  return static_cast<int>(cudaGetLastError());
+}
+
+template <typename T, typename Out>
+int weight_grad(const Act8& a, const void* dy, long long lddy, const void* base, long long ldbase, void* dw, long long lddw,
+                int n, cudaStream_t stream) {
+  const ActLeft left{static_cast<const uint8_t*>(a.codes), a.pitch, static_cast<const uint8_t*>(a.exps), a.exp_pitch, a.k, a.m};
+  const DenseRight<T> right{static_cast<const T*>(dy), lddy, a.m, n};
+  return simple_product<Out>(left, right, static_cast<Out*>(dw), lddw, static_cast<const Out*>(base), ldbase, a.k, n, a.m, stream);
+}
+
+}  // namespace
+}  // namespace lowbit
+}  // namespace sb200
+
+using sb200::lowbit::Act8;
+
+extern "C" int sb200_act8_save(int dtype, const void* x, long long ldx, int m, int k, void* codes, long long pitch,
+                               void* exponents, long long exp_pitch, sb200_stream_t stream) {
+  const Act8 a{static_cast<sb200::DType>(dtype), m, k, codes, pitch, exponents, exp_pitch};
+  if (int rc = sb200::lowbit::check(a)) return rc;
+  if (ldx < k) return SB200_ERR_INVALID_PROBLEM;
+  if (m == 0) return SB200_OK;
+  if (!x) return SB200_ERR_INVALID_PROBLEM;
+  if (!sb200::lowbit::aligned(x, 2)) return SB200_ERR_MISALIGNED_OPERAND;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return dtype == sb200::kF16 ? sb200::lowbit::save<__half>(x, ldx, a, s) : sb200::lowbit::save<__nv_bfloat16>(x, ldx, a, s);
+}
+
+extern "C" int sb200_act8_restore(int dtype, const void* codes, long long pitch, const void* exponents, long long exp_pitch,
+                                  int m, int k, void* x, long long ldx, sb200_stream_t stream) {
+  const Act8 a{static_cast<sb200::DType>(dtype), m, k, codes, pitch, exponents, exp_pitch};
+  if (int rc = sb200::lowbit::check(a)) return rc;
+  if (ldx < k) return SB200_ERR_INVALID_PROBLEM;
+  if (m == 0) return SB200_OK;
+  if (!x) return SB200_ERR_INVALID_PROBLEM;
+  if (!sb200::lowbit::aligned(x, 2)) return SB200_ERR_MISALIGNED_OPERAND;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return dtype == sb200::kF16 ? sb200::lowbit::restore<__half>(a, x, ldx, s) : sb200::lowbit::restore<__nv_bfloat16>(a, x, ldx, s);
+}
+
+extern "C" size_t sb200_act8_wgrad_workspace_bytes(int dtype, int out_dtype, int m, int n, int k) {
+  (void)dtype; (void)out_dtype; (void)m; (void)n; (void)k;
+  return 256;
+}
+
+extern "C" int sb200_act8_wgrad(int dtype, const void* codes, long long pitch, const void* exponents, long long exp_pitch,
+                                const void* dy, long long lddy, int out_dtype, const void* base, long long ldbase, void* dw,
+                                long long lddw, int m, int n, int k, void* workspace, size_t workspace_bytes,
+                                sb200_stream_t stream) {
+  const Act8 a{static_cast<sb200::DType>(dtype), m, k, codes, pitch, exponents, exp_pitch};
+  if (int rc = sb200::lowbit::check(a)) return rc;
+  if (out_dtype != sb200::kF32 && out_dtype != dtype) return SB200_ERR_NOT_SUPPORTED;
+  if (n <= 0 || !dw || lddw < n || lddy < n || (m > 0 && !dy) || (base && ldbase < n)) return SB200_ERR_INVALID_PROBLEM;
+  const uintptr_t width = out_dtype == sb200::kF32 ? 4 : 2;
+  if (!sb200::lowbit::aligned(dy, 2) || !sb200::lowbit::aligned(dw, width) || !sb200::lowbit::aligned(base, width))
+    return SB200_ERR_MISALIGNED_OPERAND;
+  if (!workspace || workspace_bytes < sb200_act8_wgrad_workspace_bytes(dtype, out_dtype, m, n, k) ||
+      !sb200::lowbit::aligned(workspace, 256))
+    return SB200_ERR_WORKSPACE_NULL;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  using namespace sb200::lowbit;
+  if (dtype == sb200::kF16)
+    return out_dtype == sb200::kF32 ? weight_grad<__half, float>(a, dy, lddy, base, ldbase, dw, lddw, n, s)
+                                    : weight_grad<__half, __half>(a, dy, lddy, base, ldbase, dw, lddw, n, s);
+  return out_dtype == sb200::kF32 ? weight_grad<__nv_bfloat16, float>(a, dy, lddy, base, ldbase, dw, lddw, n, s)
+                                  : weight_grad<__nv_bfloat16, __nv_bfloat16>(a, dy, lddy, base, ldbase, dw, lddw, n, s);
+}

@@ -1,0 +1,63 @@
+// The two formats in which an operand of a product is held in few bits, and the element arithmetic on them.
+//
+//   W4     weights n x k in 4 bits:  W[n][k] = scale[k / G][n] * (code[n][k] - zero[k / G][n]),  code in 0..15, zero in 0..15
+//          (8 where there is no table of zeros), G = 32, 64 or 128.  Rows are padded to 16, inputs to 128.  A tile of 16 rows
+//          x 128 inputs is 1 KiB of consecutive bytes, tiles run along the inputs first.  Inside a tile the 16 bytes at
+//          512 h + 16 (4 g + t) belong to row 8 h + g; their word j holds the inputs 32 j + 8 t + (0..7), input i at nibble
+//          (i >> 1) + 4 (i & 1).  That is the fragment order of a 16 x 8 x 16 matrix instruction: lane 4 g + t loads its 16 bytes
+//          at once, one word lies within one group whatever G is, and the four pairs of nibbles that `w >> 4 p` leaves 16 bits
+//          apart are neighbouring inputs, so that an expanded word is 16 bytes in the order of the activations.
+//          Scales have the 16-bit type of the activations; scales and zeros are [groups][rows padded to 16].
+//   ACT8   activations m x k in 8 bits:  X[m][k] = +-magnitude * 2^(E[m][k / 32] - 127), bit 7 of the byte is the sign, bits 0-6
+//          the magnitude.  A magnitude has 7 bits and the step is a power of two, so every X is exact in bf16 and (with the
+//          steps kept to 2^-24 .. 2^9) in f16: a product of X is a product of 16-bit operands without another rounding.
+//          E = 255 marks a block that held an infinity or a NaN (bf16: or a magnitude of 2^127 and more); it reads as NaN.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace sb200 {
+namespace lowbit {
+
+constexpr int kW4Rows = 16;     // rows of a tile
+constexpr int kW4Block = 128;   // inputs of a tile
+constexpr int kW4TileBytes = kW4Rows * kW4Block / 2;
+constexpr int kActBlock = 32;   // channels that share an exponent
+constexpr int kActNaN = 255;    // the exponent of a block that reads as NaN
+
+__host__ __device__ inline int ceil_div(int a, int b) { return a / b + (a % b != 0); }
+__host__ __device__ inline int w4_blocks(int k) { return ceil_div(k, kW4Block); }
+__host__ __device__ inline int w4_row_tiles(int n) { return ceil_div(n, kW4Rows); }
+__host__ __device__ inline long long w4_padded_rows(int n) { return static_cast<long long>(w4_row_tiles(n)) * kW4Rows; }
+
+// Nibble of input i (0..7) in its word.
+__host__ __device__ constexpr int w4_nibble(int i) { return (i >> 1) + 4 * (i & 1); }
+
+// Exponent range of the steps of ACT8: bf16 steps start at the smallest normal number (matrix units may flush smaller
+// ones) and end where 2^(e + 7) is still finite; f16 steps cover the whole type, subnormals included.
+template <typename T> struct ActRange;
+template <> struct ActRange<__half> { static constexpr int lo = -24, hi = 9; };
+template <> struct ActRange<__nv_bfloat16> { static constexpr int lo = -126, hi = 120; };
+
+template <typename T> __device__ __forceinline__ float to_f32(T v);
+template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+
+// 2^(E - 127) of a stored exponent, NaN for kActNaN.  E is at least 1.
+__device__ __forceinline__ float act8_step(int e) {
+  return __uint_as_float(e == kActNaN ? 0x7fffffffu : static_cast<uint32_t>(e) << 23);
+}
+__device__ __forceinline__ float act8_value(uint32_t byte, float step) {
+  const float v = static_cast<float>(byte & 127u) * step;
+  return (byte & 128u) ? -v : v;
+}
+
+}  // namespace lowbit
+}  // namespace sb200

@@ -1,0 +1,315 @@
+// Weights in 4 bits (format W4 of lowbit_format.cuh): packing, quantisation, expansion, and the product y = x W^T.
+#include <stdint.h>
+
+#include "../../include/subcuber_b200.h"
+#include "lowbit_format.cuh"
+#include "lowbit_host.h"
+#include "simple_product.cuh"
+
+namespace sb200 {
+namespace lowbit {
+namespace {
+
+// A block of threads handles one row tile (16 rows) and kSpan inputs: warp w takes rows w and w + 8, a lane four
+// neighbouring inputs of each 128.  The codes are put together in shared memory and leave as whole tiles.
+constexpr int kSpanBlocks = 4;
+constexpr int kThreads = 256;
+
+// Four neighbouring 16-bit values, zeros behind `k`; `wide` says that 8-byte loads are aligned.
+template <typename T>
+__device__ __forceinline__ void load4(const T* row, int k0, int k, bool wide, T (&v)[4]) {
+  if (wide && k0 + 4 <= k) {
+    *reinterpret_cast<uint2*>(v) = __ldg(reinterpret_cast<const uint2*>(row + k0));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = k0 + i < k ? row[k0 + i] : from_f32<T>(0.f);
+  }
+}
+
+// Places the four codes of a lane (inputs 4 (lane & 1) .. + 3 of a word) in the word of its pair of lanes.
+__device__ __forceinline__ uint32_t join_codes(const uint32_t (&q)[4], int lane) {
+  const int first = (lane & 1) * 2;  // nibble of the lane's first input
+  uint32_t w = (q[0] | (q[1] << 16) | (q[2] << 4) | (q[3] << 20)) << (4 * first);
+  return w | __shfl_xor_sync(0xffffffffu, w, 1);
+}
+
+// Bytes of a tile where the word of (row, pair of lanes) goes: pair = 4 j + t.
+__device__ __forceinline__ int word_offset(int row, int pair) {
+  return (row >> 3) * 512 + ((row & 7) * 4 + (pair & 3)) * 16 + (pair >> 2) * 4;
+}
+
+// Quantisation, one group at a time.  Symmetric: scale = amax / 7 and codes 8 + rint(w / scale).  Else the range
+// [min(0, w), max(0, w)] is laid over 0..15, which keeps zero exact: scale = (hi - lo) / 15, zero = rint(-lo / scale).
+// The scale is rounded to the 16-bit type FIRST and the codes are made for the rounded one.  Divisions are the
+// correctly rounded ones, so that a code next to a border does not depend on how the quotient was formed.  A group with
+// an infinity or a NaN gets a scale that is not finite and stands for NaN.
+template <typename T, int G, bool SYM>
+__global__ void __launch_bounds__(kThreads) w4_quantize_kernel(const T* __restrict__ w, long long ldw, int n, int k,
+                                                               uint8_t* __restrict__ codes, T* __restrict__ scales,
+                                                               uint8_t* __restrict__ zeros, bool wide) {
+  __shared__ __align__(16) uint8_t tile[kSpanBlocks * kW4TileBytes];
+  const int blocks = w4_blocks(k), groups = ceil_div(k, G);
+  const int spans = ceil_div(blocks, kSpanBlocks);
+  const long long rows = w4_padded_rows(n);
+  const int rt = blockIdx.x / spans, span = blockIdx.x % spans;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = warp + 8 * h;
+    const int row = rt * kW4Rows + r;
+    T v[kSpanBlocks][4];
+#pragma unroll
+    for (int b = 0; b < kSpanBlocks; ++b)
+      load4<T>(w + (row < n ? row : 0) * ldw, (span * kSpanBlocks + b) * kW4Block + lane * 4, row < n ? k : 0, wide, v[b]);
+#pragma unroll
+    for (int b = 0; b < kSpanBlocks; ++b) {
+      const int k0 = (span * kSpanBlocks + b) * kW4Block + lane * 4;
+      float x[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = to_f32(v[b][i]);
+      // magnitudes compare as their bits, NaN above infinity
+      uint32_t top = 0;
+      float lo = 0.f, hi = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t bits = __float_as_uint(x[i]) & 0x7fffffffu;
+        top = bits > top ? bits : top;
+        lo = fminf(lo, x[i]);
+        hi = fmaxf(hi, x[i]);
+      }
+#pragma unroll
+      for (int s = G / 8; s >= 1; s >>= 1) {
+        const uint32_t o = __shfl_xor_sync(0xffffffffu, top, s);
+        top = o > top ? o : top;
+        if (!SYM) {
+          lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, s));
+          hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, s));
+        }
+      }
+      const float range = top > 0x7f800000u ? __uint_as_float(top) : (SYM ? __uint_as_float(top) : hi - lo);
+      const T s16 = from_f32<T>(__fdiv_rn(range, SYM ? 7.f : 15.f));
+      const float s = to_f32(s16);
+      const bool usable = s > 0.f && s < INFINITY;
+      float z = SYM ? 8.f : 0.f;
+      if (!SYM && usable) z = fminf(rintf(__fdiv_rn(-lo, s)), 15.f);
+      uint32_t q[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float c = usable ? rintf(__fdiv_rn(x[i], s)) + z : z;
+        q[i] = static_cast<uint32_t>(fminf(fmaxf(c, 0.f), 15.f));
+      }
+      const uint32_t word = join_codes(q, lane);
+      if (!(lane & 1)) *reinterpret_cast<uint32_t*>(tile + b * kW4TileBytes + word_offset(r, lane >> 1)) = word;
+      const int group = k0 / G;
+      if (lane % (G / 4) == 0 && group < groups) {
+        scales[group * rows + row] = s16;
+        if (!SYM) zeros[group * rows + row] = static_cast<uint8_t>(z);
+      }
+    }
+  }
+  __syncthreads();
+  const int block = span * kSpanBlocks + threadIdx.x / (kW4TileBytes / 16);
+  if (block < blocks)
+    reinterpret_cast<uint4*>(codes)[(static_cast<long long>(rt) * blocks + span * kSpanBlocks) * (kW4TileBytes / 16) +
+                                    threadIdx.x] = reinterpret_cast<const uint4*>(tile)[threadIdx.x];
+}
+
+// Codes that are there already, one byte each, into the format's order.  What the padding holds does not matter: padded
+// inputs meet activations that are zero, padded rows are not stored.
+__global__ void __launch_bounds__(kThreads) w4_pack_kernel(const uint8_t* __restrict__ q, long long ldq, int n, int k,
+                                                           uint8_t* __restrict__ codes) {
+  const int blocks = w4_blocks(k);
+  const int rt = blockIdx.x / blocks, block = blockIdx.x % blocks;
+  const int r = threadIdx.x >> 4, pair = threadIdx.x & 15;  // one word for each thread
+  const int row = rt * kW4Rows + r;
+  uint32_t word = 0;
+  for (int i = 0; i < 8; ++i) {
+    const int kk = block * kW4Block + pair * 8 + i;
+    uint32_t c = 8;
+    if (row < n && kk < k) c = q[row * ldq + kk] & 15u;
+    word |= c << (4 * w4_nibble(i));
+  }
+  *reinterpret_cast<uint32_t*>(codes + (static_cast<long long>(rt) * blocks + block) * kW4TileBytes + word_offset(r, pair)) = word;
+}
+
+// Expansion: a thread takes the 16 bytes of (row, t), four words of eight inputs.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) w4_dequantize_kernel(const uint8_t* __restrict__ codes, const T* __restrict__ scales,
+                                                                 const uint8_t* __restrict__ zeros, int n, int k, int G,
+                                                                 T* __restrict__ out, long long ldo, bool wide) {
+  const int blocks = w4_blocks(k);
+  const int spans = ceil_div(blocks, kSpanBlocks);
+  const long long rows = w4_padded_rows(n);
+  const int rt = blockIdx.x / spans, span = blockIdx.x % spans;
+  const int block = span * kSpanBlocks + (threadIdx.x >> 6);
+  const int piece = threadIdx.x & 63;
+  const int row = rt * kW4Rows + (piece >> 5) * 8 + ((piece & 31) >> 2), t = piece & 3;
+  if (block >= blocks || row >= n) return;
+  const uint4 raw = __ldg(reinterpret_cast<const uint4*>(codes) +
+                          (static_cast<long long>(rt) * blocks + block) * (kW4TileBytes / 16) + piece);
+  const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int k0 = block * kW4Block + 32 * j + 8 * t;
+    if (k0 >= k) break;
+    const long long at = (k0 / G) * rows + row;
+    const float s = to_f32(scales[at]);
+    const float z = zeros ? static_cast<float>(zeros[at]) : 8.f;
+    T v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      v[i] = from_f32<T>((static_cast<float>((words[j] >> (4 * w4_nibble(i))) & 15u) - z) * s);
+    T* to = out + row * ldo + k0;
+    if (wide && k0 + 8 <= k) {
+      *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (k0 + i < k) to[i] = v[i];
+    }
+  }
+}
+
+template <typename T>
+struct W4Right {  // W^T as the right operand of a product: (input, row)
+  const uint8_t* codes;
+  const T* scales;
+  const uint8_t* zeros;
+  int n, k, G, blocks;
+  long long rows;
+  __device__ float operator()(int kk, int row) const {
+    if (kk >= k || row >= n) return 0.f;
+    const int in = kk % kW4Block;
+    const uint32_t word = *reinterpret_cast<const uint32_t*>(
+        codes + (static_cast<long long>(row / kW4Rows) * blocks + kk / kW4Block) * kW4TileBytes + word_offset(row % kW4Rows, in / 8));
+    const float q = static_cast<float>((word >> (4 * w4_nibble(in % 8))) & 15u);
+    const long long at = (kk / G) * rows + row;
+    return (q - (zeros ? static_cast<float>(zeros[at]) : 8.f)) * to_f32(scales[at]);
+  }
+};
+
+template <typename T>
+int product(const void* x, long long ldx, const W4& w, void* y, long long ldy, int m, cudaStream_t stream) {
+  const DenseLeft<T> left{static_cast<const T*>(x), ldx, m, w.k};
+  const W4Right<T> right{static_cast<const uint8_t*>(w.codes), static_cast<const T*>(w.scales),
+                         static_cast<const uint8_t*>(w.zeros), w.n, w.k, w.group, w4_blocks(w.k), w4_padded_rows(w.n)};
+  return simple_product<T>(left, right, static_cast<T*>(y), ldy, static_cast<const T*>(nullptr), 0, m, w.n, w.k, stream);
+}
+
+inline bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+int check(const W4& w) {
+  if (w.dtype != kF16 && w.dtype != kBF16) return kErrNotSupported;
+  if (w.n <= 0 || w.k <= 0 || !w.codes || !w.scales) return kErrInvalidProblem;
+  if (w.group != 32 && w.group != 64 && w.group != 128) return kErrNotSupported;
+  if (!aligned(w.codes, 16) || !aligned(w.scales, 2)) return kErrMisalignedOperand;
+  return kOk;
+}
+
+// Thread blocks of a launch over (row tiles) x (parts of a row); the grid's x axis holds 2^31 - 1 of them.
+int grid_of(int n, int parts, unsigned* grid) {
+  const long long g = static_cast<long long>(w4_row_tiles(n)) * parts;
+  if (g > 0x7fffffffll) return kErrNotSupported;
+  *grid = static_cast<unsigned>(g);
+  return kOk;
+}
+
+template <typename T, int G>
+int quantize(const void* w, long long ldw, const W4& q, cudaStream_t stream) {
+  unsigned grid;
+  if (int rc = grid_of(q.n, ceil_div(w4_blocks(q.k), kSpanBlocks), &grid)) return rc;
+  const bool wide = aligned(w, 8) && ldw % 4 == 0;
+  const T* from = static_cast<const T*>(w);
+  uint8_t* codes = static_cast<uint8_t*>(const_cast<void*>(q.codes));
+  T* scales = static_cast<T*>(const_cast<void*>(q.scales));
+  uint8_t* zeros = static_cast<uint8_t*>(const_cast<void*>(q.zeros));
+  if (zeros) w4_quantize_kernel<T, G, false><<<grid, kThreads, 0, stream>>>(from, ldw, q.n, q.k, codes, scales, zeros, wide);
+  else w4_quantize_kernel<T, G, true><<<grid, kThreads, 0, stream>>>(from, ldw, q.n, q.k, codes, scales, zeros, wide);
+  return static_cast<int>(cudaGetLastError());
+}
+
+template <typename T>
+int quantize_any(const void* w, long long ldw, const W4& q, cudaStream_t stream) {
+  switch (q.group) {
+    case 32: return quantize<T, 32>(w, ldw, q, stream);
+    case 64: return quantize<T, 64>(w, ldw, q, stream);
+    default: return quantize<T, 128>(w, ldw, q, stream);
+  }
+}
+
+template <typename T>
+int dequantize(const W4& w, void* out, long long ldo, cudaStream_t stream) {
+  unsigned grid;
+  if (int rc = grid_of(w.n, ceil_div(w4_blocks(w.k), kSpanBlocks), &grid)) return rc;
+  w4_dequantize_kernel<T><<<grid, kThreads, 0, stream>>>(static_cast<const uint8_t*>(w.codes), static_cast<const T*>(w.scales),
+                                                         static_cast<const uint8_t*>(w.zeros), w.n, w.k, w.group,
+                                                         static_cast<T*>(out), ldo, aligned(out, 16) && ldo % 8 == 0);
+  return static_cast<int>(cudaGetLastError());
+}
+
+}  // namespace
+}  // namespace lowbit
+}  // namespace sb200
+
+using sb200::lowbit::W4;
+
+extern "C" size_t sb200_w4_codes_bytes(int n, int k) {
+  if (n <= 0 || k <= 0) return 0;
+  return static_cast<size_t>(sb200::lowbit::w4_row_tiles(n)) * sb200::lowbit::w4_blocks(k) * sb200::lowbit::kW4TileBytes;
+}
+
+extern "C" size_t sb200_w4_table_rows(int n) { return n <= 0 ? 0 : static_cast<size_t>(sb200::lowbit::w4_padded_rows(n)); }
+
+extern "C" int sb200_w4_quantize(int dtype, const void* w, long long ldw, int n, int k, int group, void* codes, void* scales,
+                                 void* zeros, sb200_stream_t stream) {
+  const W4 q{static_cast<sb200::DType>(dtype), n, k, group, codes, scales, zeros};
+  if (int rc = sb200::lowbit::check(q)) return rc;
+  if (!w || ldw < k) return SB200_ERR_INVALID_PROBLEM;
+  if (!sb200::lowbit::aligned(w, 2)) return SB200_ERR_MISALIGNED_OPERAND;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return dtype == sb200::kF16 ? sb200::lowbit::quantize_any<__half>(w, ldw, q, s)
+                              : sb200::lowbit::quantize_any<__nv_bfloat16>(w, ldw, q, s);
+}
+
+extern "C" int sb200_w4_pack(const void* q, long long ldq, int n, int k, void* codes, sb200_stream_t stream) {
+  if (n <= 0 || k <= 0 || !q || !codes || ldq < k) return SB200_ERR_INVALID_PROBLEM;
+  if (!sb200::lowbit::aligned(codes, 16)) return SB200_ERR_MISALIGNED_OPERAND;
+  unsigned grid;
+  if (int rc = sb200::lowbit::grid_of(n, sb200::lowbit::w4_blocks(k), &grid)) return rc;
+  sb200::lowbit::w4_pack_kernel<<<grid, sb200::lowbit::kThreads, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint8_t*>(q), ldq, n, k, static_cast<uint8_t*>(codes));
+  return static_cast<int>(cudaGetLastError());
+}
+
+extern "C" int sb200_w4_dequantize(int dtype, const void* codes, const void* scales, const void* zeros, int n, int k,
+                                   int group, void* out, long long ldo, sb200_stream_t stream) {
+  const W4 w{static_cast<sb200::DType>(dtype), n, k, group, codes, scales, zeros};
+  if (int rc = sb200::lowbit::check(w)) return rc;
+  if (!out || ldo < k) return SB200_ERR_INVALID_PROBLEM;
+  if (!sb200::lowbit::aligned(out, 2)) return SB200_ERR_MISALIGNED_OPERAND;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return dtype == sb200::kF16 ? sb200::lowbit::dequantize<__half>(w, out, ldo, s)
+                              : sb200::lowbit::dequantize<__nv_bfloat16>(w, out, ldo, s);
+}
+
+extern "C" size_t sb200_w4_gemm_workspace_bytes(int dtype, int m, int n, int k, int group) {
+  (void)dtype; (void)m; (void)n; (void)k; (void)group;
+  return 256;
+}
+
+extern "C" int sb200_w4_gemm(int dtype, const void* x, long long ldx, const void* codes, const void* scales,
+                             const void* zeros, void* y, long long ldy, int m, int n, int k, int group, void* workspace,
+                             size_t workspace_bytes, sb200_stream_t stream) {
+  const W4 w{static_cast<sb200::DType>(dtype), n, k, group, codes, scales, zeros};
+  if (int rc = sb200::lowbit::check(w)) return rc;
+  if (m < 0 || ldx < k || ldy < n) return SB200_ERR_INVALID_PROBLEM;
+  if (m == 0) return SB200_OK;
+  if (!x || !y) return SB200_ERR_INVALID_PROBLEM;
+  if (!sb200::lowbit::aligned(x, 2) || !sb200::lowbit::aligned(y, 2)) return SB200_ERR_MISALIGNED_OPERAND;
+  if (!workspace || workspace_bytes < sb200_w4_gemm_workspace_bytes(dtype, m, n, k, group) ||
+      !sb200::lowbit::aligned(workspace, 256))
+    return SB200_ERR_WORKSPACE_NULL;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return dtype == sb200::kF16 ? sb200::lowbit::product<__half>(x, ldx, w, y, ldy, m, s)
+                              : sb200::lowbit::product<__nv_bfloat16>(x, ldx, w, y, ldy, m, s);
+}

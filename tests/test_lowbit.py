@@ -1,0 +1,122 @@
+"""Products with one operand held in few bits, host side: argument checks of the C entry points and of the Python calls.
+Nothing here launches a kernel (the checks come before any CUDA call)."""
+import ctypes as C
+
+import pytest
+
+P = 1 << 20  # stands for a device address with every alignment; never dereferenced
+WS = 1 << 40  # more workspace than any call asks for
+
+
+def _w4_gemm(lib, dtype=0, x=P, ldx=256, codes=P, scales=P, zeros=P, y=P, ldy=64, m=1, n=64, k=256, group=128, ws=P, nbytes=WS):
+    return lib.sb200_w4_gemm(dtype, x, ldx, codes, scales, zeros, y, ldy, m, n, k, group, ws, nbytes, None)
+
+
+@pytest.mark.parametrize("change,rc", [
+    (dict(m=0), 0),                                   # an empty batch: nothing to do
+    (dict(m=0, x=None, y=None, ws=None), 0),
+    (dict(m=-1), 4), (dict(n=0), 4), (dict(k=0), 4), (dict(n=-5), 4),
+    (dict(x=None), 4), (dict(codes=None), 4), (dict(scales=None), 4), (dict(y=None), 4),
+    (dict(ldx=255), 4), (dict(ldy=63), 4),
+    (dict(dtype=1), 5), (dict(dtype=2), 5), (dict(dtype=7), 5),
+    (dict(group=0), 5), (dict(group=16), 5), (dict(group=96), 5), (dict(group=256), 5),
+    (dict(x=P + 1), 1), (dict(y=P + 1), 1), (dict(codes=P + 8), 1), (dict(scales=P + 1), 1),
+    (dict(ws=None), 6), (dict(nbytes=0), 6), (dict(ws=P + 16), 6),
+])
+def test_w4_gemm_refuses(lib, change, rc):
+    assert _w4_gemm(lib, **change) == rc
+
+
+def test_w4_sizes(lib):
+    assert lib.sb200_w4_codes_bytes(16, 128) == 1024 and lib.sb200_w4_codes_bytes(17, 129) == 4096
+    assert lib.sb200_w4_codes_bytes(1, 1) == 1024 and lib.sb200_w4_codes_bytes(0, 5) == 0
+    assert lib.sb200_w4_codes_bytes(1 << 20, 1 << 15) == 1 << 34   # offsets pass 32 bits
+    assert lib.sb200_w4_table_rows(1) == 16 and lib.sb200_w4_table_rows(16) == 16 and lib.sb200_w4_table_rows(17) == 32
+
+
+@pytest.mark.parametrize("args,rc", [
+    ((0, None, 64, 8, 64, 32, P, P, P), 4), ((0, P, 63, 8, 64, 32, P, P, P), 4), ((1, P, 64, 8, 64, 32, P, P, P), 5),
+    ((0, P, 64, 8, 64, 48, P, P, P), 5), ((0, P + 1, 64, 8, 64, 32, P, P, P), 1), ((0, P, 64, 0, 64, 32, P, P, P), 4),
+    ((3, P, 64, 8, 64, 32, P + 4, P, None), 1), ((3, P, 64, 8, 64, 32, P, None, None), 4),
+])
+def test_w4_quantize_refuses(lib, args, rc):
+    assert lib.sb200_w4_quantize(*args, None) == rc
+
+
+def test_w4_pack_and_dequantize_refuse(lib):
+    assert lib.sb200_w4_pack(None, 8, 4, 8, P, None) == 4
+    assert lib.sb200_w4_pack(P, 7, 4, 8, P, None) == 4
+    assert lib.sb200_w4_pack(P, 8, 4, 8, P + 1, None) == 1
+    assert lib.sb200_w4_dequantize(0, P, P, None, 4, 8, 32, None, 8, None) == 4
+    assert lib.sb200_w4_dequantize(0, P, P, None, 4, 8, 32, P, 7, None) == 4
+    assert lib.sb200_w4_dequantize(1, P, P, None, 4, 8, 32, P, 8, None) == 5
+    assert lib.sb200_w4_dequantize(0, P, P, None, 4, 8, 32, P + 1, 8, None) == 1
+
+
+def _save(lib, dtype=0, x=P, ldx=100, m=4, k=100, codes=P, pitch=112, exps=P, exp_pitch=4):
+    return lib.sb200_act8_save(dtype, x, ldx, m, k, codes, pitch, exps, exp_pitch, None)
+
+
+def _restore(lib, dtype=0, x=P, ldx=100, m=4, k=100, codes=P, pitch=112, exps=P, exp_pitch=4):
+    return lib.sb200_act8_restore(dtype, codes, pitch, exps, exp_pitch, m, k, x, ldx, None)
+
+
+@pytest.mark.parametrize("call", [_save, _restore])
+@pytest.mark.parametrize("change,rc", [
+    (dict(m=0), 0), (dict(m=0, x=None, codes=None, exps=None), 0),
+    (dict(m=-1), 4), (dict(k=0), 4), (dict(x=None), 4), (dict(codes=None), 4), (dict(exps=None), 4),
+    (dict(ldx=99), 4), (dict(pitch=96), 4), (dict(exp_pitch=0), 4), (dict(k=129, ldx=129, pitch=144), 4),
+    (dict(dtype=1), 5), (dict(dtype=2), 5),
+    (dict(x=P + 1), 1), (dict(codes=P + 8), 1), (dict(pitch=104), 1), (dict(exps=P + 2), 1), (dict(exp_pitch=6), 1),
+])
+def test_act8_save_and_restore_refuse(lib, call, change, rc):
+    assert call(lib, **change) == rc
+
+
+def _wgrad(lib, dtype=0, codes=P, pitch=112, exps=P, exp_pitch=4, dy=P, lddy=24, out_dtype=1, base=None, ldbase=24, dw=P,
+           lddw=24, m=4, n=24, k=100, ws=P, nbytes=WS):
+    return lib.sb200_act8_wgrad(dtype, codes, pitch, exps, exp_pitch, dy, lddy, out_dtype, base, ldbase, dw, lddw, m, n, k, ws,
+                                nbytes, None)
+
+
+@pytest.mark.parametrize("change,rc", [
+    (dict(m=-1), 4), (dict(n=0), 4), (dict(k=0), 4), (dict(codes=None), 4), (dict(exps=None), 4), (dict(dy=None), 4),
+    (dict(dw=None), 4), (dict(lddy=23), 4), (dict(lddw=23), 4), (dict(base=P, ldbase=23), 4), (dict(pitch=96), 4),
+    (dict(dtype=1), 5), (dict(out_dtype=3), 5), (dict(dtype=3, out_dtype=0), 5), (dict(out_dtype=2), 5),
+    (dict(codes=P + 8), 1), (dict(exps=P + 2), 1), (dict(dy=P + 1), 1), (dict(dw=P + 2), 1), (dict(base=P + 2), 1),
+    (dict(ws=None), 6), (dict(nbytes=0), 6), (dict(ws=P + 128), 6),
+])
+def test_act8_wgrad_refuses(lib, change, rc):
+    assert _wgrad(lib, **change) == rc
+
+
+def test_python_calls_refuse_host_tensors():
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    h = torch.zeros(16, 128, dtype=torch.float16)
+    for call in (lambda: lowbit.quantize_w4(h), lambda: lowbit.save8(h),
+                 lambda: lowbit.pack_w4(h.to(torch.uint8), torch.zeros(1, 16, dtype=torch.float16))):
+        with pytest.raises(ValueError, match="CUDA tensor"):
+            call()
+
+
+def test_python_handles_refuse_wrong_tables():
+    """The handles check shapes, types and devices before anything is launched (with meta tensors in place of device ones)."""
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    codes = torch.zeros(1024, dtype=torch.uint8)
+    scales = torch.zeros(1, 16, dtype=torch.float16)
+    with pytest.raises(ValueError):
+        lowbit.WeightsW4(codes, scales, None, 16, 128, 128)     # host tensors
+    with pytest.raises(ValueError):
+        lowbit.WeightsW4(codes, scales, None, 16, 128, 48)
+    with pytest.raises(ValueError):
+        lowbit.WeightsW4(codes, scales, None, 0, 128, 128)
+    with pytest.raises(ValueError):
+        lowbit.Checkpoint8(codes.view(8, 128), codes.view(8, 128), 100, torch.float32)
+    with pytest.raises(ValueError):
+        lowbit.Checkpoint8(codes.view(8, 128), codes.view(8, 128), 0, torch.float16)

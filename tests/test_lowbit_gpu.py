@@ -1,0 +1,656 @@
+"""Products with one operand held in few bits, on a B200, against plain implementations in 64 bits.
+
+Tolerances.  An output of 16 bits is off by at most half a step, eps / 2 relative, from the sum that was rounded; a sum in
+fp32 of terms t_i is off by at most (additions) * 2^-23 * sum |t_i| (every addition, chopped or rounded, is off by at most
+one unit of 2^-23 of a partial sum, which sum |t_i| bounds).  A matrix instruction adds 16 terms to its accumulator and
+counts for two additions (its own sum of products, and that to the accumulator); a group adds one more for its scale.  Products
+with many rows round the weights to 16 bits first: eps / 2 of every term more.  Codes, exponents and restored
+activations are compared bit for bit.
+"""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+HALF = ["f16", "bf16"]
+
+
+def T(name):
+    import torch
+
+    return {"f16": torch.float16, "bf16": torch.bfloat16, "f32": torch.float32}[name]
+
+
+def randn(shape, dtype, device, seed, scale=1.0):
+    import torch
+
+    g = torch.Generator(device=device)
+    g.manual_seed(seed)
+    return (torch.randn(shape, generator=g, device=device) * scale).to(dtype)
+
+
+# ------------------------------------------------------------------------------------------------ plain forms, 64 bits
+def plain_quantize(w, group, symmetric):
+    """codes [n, k], scales and zeros [n, groups], all 64 bits (scales hold values of w's type)."""
+    import torch
+
+    n, k = w.shape
+    q = torch.empty(n, k, dtype=torch.float64, device=w.device)
+    ss, zz = [], []
+    for g0 in range(0, k, group):
+        p = w[:, g0:g0 + group].double()
+        if symmetric:
+            r = p.abs().amax(1) / 7
+        else:
+            lo, hi = p.amin(1).clamp(max=0), p.amax(1).clamp(min=0)
+            r = (hi - lo) / 15
+        s = r.to(w.dtype).double()
+        ok = (s > 0) & torch.isfinite(s)
+        safe = torch.where(ok, s, torch.ones_like(s))
+        z = torch.full_like(s, 8) if symmetric else torch.where(ok, torch.round(-lo / safe), torch.zeros_like(s)).clamp(0, 15)
+        c = torch.where(ok[:, None], torch.round(p / safe[:, None]), torch.zeros_like(p))
+        q[:, g0:g0 + group] = (c + z[:, None]).clamp(0, 15)
+        ss.append(s)
+        zz.append(z)
+    return q, torch.stack(ss, 1), torch.stack(zz, 1)
+
+
+def unpack(w):
+    """Codes [n, k] of a WeightsW4, from the documented order."""
+    import torch
+
+    n_t, k_b = -(-w.n // 16), -(-w.k // 128)
+    words = w.codes.view(torch.int32).view(n_t, k_b, 2, 8, 4, 4)   # tile, block, h, g, t, j
+    out = torch.empty(n_t, k_b, 2, 8, 4, 4, 8, dtype=torch.int32, device=w.codes.device)
+    for i in range(8):
+        out[..., i] = (words >> (4 * ((i >> 1) + 4 * (i & 1)))) & 15
+    out = out.permute(0, 2, 3, 1, 5, 4, 6)                         # tile, h, g, block, j, t, i
+    return out.reshape(n_t * 16, k_b * 128)[:w.n, :w.k]
+
+
+def values(w):
+    """Weights [n, k] in 64 bits that a WeightsW4 stands for."""
+    import torch
+
+    at = torch.arange(w.k, device=w.codes.device) // w.group
+    s = w.scales.double()[at, :w.n].t()
+    z = 8.0 if w.zeros is None else w.zeros.double()[at, :w.n].t()
+    return (unpack(w).double() - z) * s
+
+
+def check_w4_gemm(y, x, w, exact_weights):
+    import torch
+
+    wv, xv = values(w), x.double()
+    want, size = xv @ wv.t(), xv.abs() @ wv.abs().t()
+    half = torch.finfo(w.dtype).eps / 2
+    sums = (2 * (w.k / 16 + 1) + w.k / 32 + 16) * 2.0 ** -23
+    tol = size * (sums + (0 if exact_weights else half)) * (1 + half) + want.abs() * half + torch.finfo(w.dtype).smallest_normal * half * 2
+    off = (y.double() - want).abs()
+    assert bool((off <= tol).all()), f"{int((off > tol).sum())} of {off.numel()} off, worst {float((off / tol).max()):.2f} x"
+
+
+def plain_save(x):
+    """(codes, exponents, values in 64 bits) of activations."""
+    import torch
+
+    m, k = x.shape
+    nb = -(-k // 32)
+    p = torch.nn.functional.pad(x.double(), (0, nb * 32 - k)).view(m, nb, 32)
+    amax = p.abs().amax(2)
+    lo, hi = (-24, 9) if x.dtype == torch.float16 else (-126, 120)
+    e = torch.frexp(amax).exponent - 7
+    bad = ~torch.isfinite(amax) | (e > hi)
+    e = torch.where(amax > 0, e.clamp(lo, 200), torch.full_like(e, lo))
+    e = torch.where(bad, torch.zeros_like(e), e)
+    step = ((e.long() + 1023) << 52).view(torch.float64)
+    mag = torch.round(p.abs() / step[..., None]).clamp(max=127)
+    mag = torch.where(bad[..., None], torch.zeros_like(mag), mag)
+    code = mag.to(torch.int32) | (torch.signbit(p).int() << 7)
+    val = torch.where(torch.signbit(p), -mag, mag) * step[..., None]
+    val = torch.where(bad[..., None], torch.full_like(val, float("nan")), val)
+    E = torch.where(bad, torch.full_like(e, 255), e + 127)
+    return code.view(m, -1)[:, :k], E, val.view(m, -1)[:, :k]
+
+
+def check_grad(dw, xv, dy, base, additions=None):
+    """xv: the saved activations' values in 64 bits."""
+    import torch
+
+    d = dy.double()
+    want, size = xv.t() @ d, xv.abs().t() @ d.abs()
+    if base is not None:
+        want, size = want + base.double(), size + base.double().abs()
+    half = torch.finfo(dw.dtype).eps / 2 if dw.dtype != torch.float32 else 0.0
+    n = (2 * (xv.shape[0] / 16 + 1) + 16) if additions is None else additions
+    tol = size * n * 2.0 ** -23 * (1 + half) + want.abs() * half + torch.finfo(dw.dtype).smallest_normal * torch.finfo(dw.dtype).eps
+    off = (dw.double() - want).abs()
+    assert bool((off <= tol).all()), f"{int((off > tol).sum())} of {off.numel()} off, worst {float((off / tol).max()):.2f} x"
+
+
+# ------------------------------------------------------------------------------------------------ 4-bit weights
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("n,k", [(1, 1), (16, 128), (17, 129), (33, 500), (5, 31), (64, 1024), (40, 515)])
+def test_quantize(cuda_device, dtype, symmetric, group, n, k):
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    w = randn((n, k), T(dtype), cuda_device, 1, 0.05)
+    w[0] = 0                                      # a row of zeros: scale 0
+    if n > 4:
+        w[3] = w[3].abs()                         # one sign only
+        w[4] = -w[4].abs()
+    got = lowbit.quantize_w4(w, group=group, symmetric=symmetric)
+    q, s, z = plain_quantize(w, group, symmetric)
+    assert torch.equal(unpack(got).double(), q)
+    assert torch.equal(got.scales.double()[:, :n].t(), s)
+    if not symmetric:
+        assert torch.equal(got.zeros.double()[:, :n].t(), z)
+    want = values(got).to(w.dtype)
+    assert torch.equal(lowbit.dequantize_w4(got), want)
+
+
+def test_quantize_rows_of_another_matrix(cuda_device):
+    """Rows with a pitch, off every vector alignment; an output with a pitch keeps what lies between its rows."""
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    big = randn((40, 300), torch.bfloat16, cuda_device, 2)
+    w = big[3:36, 7:270]
+    got = lowbit.quantize_w4(w, group=64)
+    assert torch.equal(unpack(got).double(), plain_quantize(w, 64, False)[0])
+    room = torch.full((33, 301), 7.0, dtype=torch.bfloat16, device=cuda_device)
+    lowbit.dequantize_w4(got, out=room[:, 5:268])
+    assert torch.equal(room[:, 5:268], values(got).to(torch.bfloat16))
+    assert bool((room[:, :5] == 7).all()) and bool((room[:, 268:] == 7).all())
+
+
+@pytest.mark.parametrize("dtype", HALF)
+def test_quantize_extremes(cuda_device, dtype):
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    fi = torch.finfo(T(dtype))
+    w = randn((8, 256), T(dtype), cuda_device, 3)
+    w[0] *= fi.smallest_normal * 4                # steps among the subnormal numbers
+    w[1] = fi.smallest_normal * fi.eps            # the smallest number: the scale rounds to 0 or to itself
+    w[2] = fi.max
+    w[3, ::2] = -fi.max / 2
+    for symmetric in (True, False):
+        got = lowbit.quantize_w4(w, group=128, symmetric=symmetric)
+        q, s, _ = plain_quantize(w, 128, symmetric)
+        assert torch.equal(got.scales.double()[:, :8].t(), s)
+        assert torch.equal(unpack(got).double(), q)
+
+
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_groups_that_are_not_finite_stand_for_nan(cuda_device, symmetric, bad):
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    w = randn((20, 256), torch.bfloat16, cuda_device, 4)
+    w[7, 130] = bad
+    got = lowbit.quantize_w4(w, group=128, symmetric=symmetric)
+    back = lowbit.dequantize_w4(got)
+    assert bool(torch.isnan(back[7, 128:]).all())
+    back[7, 128:] = 0
+    assert bool(torch.isfinite(back).all())
+    for m in (1, 5, 40, 200):
+        x = randn((m, 256), torch.bfloat16, cuda_device, 5)
+        y = lowbit.gemm_w4(x, got)
+        assert bool(torch.isnan(y[:, 7]).all())
+        y[:, 7] = 0
+        assert bool(torch.isfinite(y).all())
+
+
+def test_pack(cuda_device):
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    g = torch.Generator(device=cuda_device)
+    g.manual_seed(6)
+    for n, k, group in ((1, 1, 32), (19, 333, 64), (48, 256, 128)):
+        q = torch.randint(0, 16, (n, k), generator=g, device=cuda_device, dtype=torch.uint8)
+        scales = randn((-(-k // group), n), torch.float16, cuda_device, 7)
+        zeros = torch.randint(0, 16, scales.shape, generator=g, device=cuda_device, dtype=torch.uint8)
+        for zz in (zeros, None):
+            w = lowbit.pack_w4(q, scales, zz, group=group)
+            assert torch.equal(unpack(w), q.int())
+            at = torch.arange(k, device=cuda_device) // group
+            want = (q.double() - (8.0 if zz is None else zz.double()[at].t())) * scales.double()[at].t()
+            assert torch.equal(lowbit.dequantize_w4(w), want.half())
+    # rows of a wider matrix of codes
+    wide = torch.randint(0, 16, (10, 64), generator=g, device=cuda_device, dtype=torch.uint8)
+    w = lowbit.pack_w4(wide[:, 3:40], randn((2, 10), torch.float16, cuda_device, 7), group=32)
+    assert torch.equal(unpack(w), wide[:, 3:40].int())
+
+
+ROWS = [1, 2, 7, 8, 9, 16, 17, 32, 33, 64, 65, 129, 257]
+
+
+@pytest.mark.parametrize("m", ROWS)
+@pytest.mark.parametrize("n,k,group,symmetric,dtype", [
+    (16, 128, 128, True, "f16"), (128, 256, 32, False, "bf16"), (1, 1, 32, False, "f16"), (17, 33, 64, True, "bf16"),
+    (250, 1000, 64, False, "f16"), (515, 2047, 128, False, "bf16"), (384, 4096, 32, False, "f16"),
+])
+def test_gemm_w4(cuda_device, m, n, k, group, symmetric, dtype):
+    from subcuber_b200 import lowbit
+
+    w = lowbit.quantize_w4(randn((n, k), T(dtype), cuda_device, 8, k ** -0.5), group=group, symmetric=symmetric)
+    x = randn((m, k), T(dtype), cuda_device, 9)
+    check_w4_gemm(lowbit.gemm_w4(x, w), x, w, exact_weights=False)
+
+
+@pytest.mark.parametrize("m", [1, 5, 24, 40, 150])
+@pytest.mark.parametrize("n,k", [(300, 520), (260, 384)])
+def test_gemm_w4_rows_of_other_matrices(cuda_device, m, n, k):
+    """Activations and results with a pitch, aligned and not; what lies beside and behind the result stays."""
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    w = lowbit.quantize_w4(randn((n, k), torch.bfloat16, cuda_device, 10, 0.1), group=64)
+    for c0, ldx, d0, ldy in ((0, k + 8, 0, n + 4), (3, k + 5, 1, n + 3), (8, k + 16, 8, n + 20)):
+        x = randn((m + 2, ldx), torch.bfloat16, cuda_device, 11)[1:1 + m, c0:c0 + k]
+        room = torch.full((m + 3, ldy), 7.0, dtype=torch.bfloat16, device=cuda_device)
+        lowbit.gemm_w4(x, w, out=room[1:1 + m, d0:d0 + n])
+        check_w4_gemm(room[1:1 + m, d0:d0 + n], x, w, exact_weights=False)
+        room[1:1 + m, d0:d0 + n] = 7
+        assert bool((room == 7).all())
+
+
+@pytest.mark.parametrize("m", [1, 3, 20, 70, 140])
+def test_gemm_w4_keeps_rows_apart(cuda_device, m):
+    """An infinity or a NaN among the activations reaches its own row and no other."""
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    w = lowbit.quantize_w4(randn((70, 300), torch.float16, cuda_device, 12, 0.1), group=32)
+    x = randn((m, 300), torch.float16, cuda_device, 13)
+    want = lowbit.gemm_w4(x, w)
+    hit = m // 2
+    for bad in (float("inf"), float("nan"), float("-inf")):
+        y = x.clone()
+        y[hit, 299] = bad
+        got = lowbit.gemm_w4(y, w)
+        assert not bool(torch.isfinite(got[hit]).any()) or bool((values(w)[:, 299] == 0).any())
+        got[hit] = want[hit]
+        assert torch.equal(got, want)
+
+
+def test_gemm_w4_empty_batch(cuda_device):
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    w = lowbit.quantize_w4(randn((70, 300), torch.float16, cuda_device, 12))
+    assert lowbit.gemm_w4(torch.empty(0, 300, dtype=torch.float16, device=cuda_device), w).shape == (0, 70)
+
+
+@pytest.mark.parametrize("m", [1, 16, 64, 300])
+def test_gemm_w4_same_result_every_time(cuda_device, m):
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    w = lowbit.quantize_w4(randn((200, 4096), torch.bfloat16, cuda_device, 14, 0.02), group=128)
+    x = randn((m, 4096), torch.bfloat16, cuda_device, 15)
+    want = lowbit.gemm_w4(x, w)
+    for _ in range(20):
+        assert torch.equal(lowbit.gemm_w4(x, w), want)
+
+
+def test_gemm_w4_offsets_past_32_bits(cuda_device):
+    """More than 2^32 weights: 2^31 bytes of codes."""
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    n, k = 131072 + 37, 32768
+    part = lowbit.quantize_w4(randn((16384, k), torch.bfloat16, cuda_device, 16, 0.02), group=128, symmetric=True)
+    reps = -(-n // 16384)
+    rows = -(-n // 16) * 16
+    codes = part.codes.repeat(reps)[: rows * k // 2].clone()
+    scales = part.scales.repeat(1, reps)[:, :rows].contiguous()
+    w = lowbit.WeightsW4(codes, scales, None, n, k, 128)
+    tail = randn((37, k), torch.bfloat16, cuda_device, 17, 0.02)      # the last rows differ from the repeated ones
+    last = lowbit.quantize_w4(tail, group=128, symmetric=True)
+    codes[131072 * k // 2:] = last.codes
+    scales[:, 131072:] = last.scales
+    for m in (1, 17, 100):
+        x = randn((m, k), torch.bfloat16, cuda_device, 18)
+        y = lowbit.gemm_w4(x, w)
+        check_w4_gemm(y[:, 131072:], x, last, exact_weights=False)
+        assert torch.equal(y[:, 114688:131072], y[:, :16384])
+    del codes, scales, w
+    torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------------------------------------------ 8-bit activations
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("m,k", [(1, 1), (1, 32), (3, 33), (5, 15), (7, 16), (2, 31), (9, 100), (33, 512), (4, 2049), (300, 640)])
+def test_save_and_restore(cuda_device, dtype, m, k):
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    x = randn((m, k), T(dtype), cuda_device, 20, 3.0)
+    x[0] *= 0.001
+    saved = lowbit.save8(x)
+    code, E, val = plain_save(x)
+    assert torch.equal(saved.codes[:, :k].int(), code)
+    assert torch.equal(saved.exponents[:, :E.shape[1]].int(), E)
+    back = lowbit.restore8(saved)
+    assert torch.equal(back.double(), val)
+    step = ((E.long() - 127 + 1023) << 52).view(torch.float64).repeat_interleave(32, 1)[:, :k]
+    assert bool(((back.double() - x.double()).abs() <= step).all())
+
+
+@pytest.mark.parametrize("dtype", HALF)
+def test_save_extremes(cuda_device, dtype):
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    fi = torch.finfo(T(dtype))
+    x = randn((10, 96), T(dtype), cuda_device, 21)
+    x[0] = 0
+    x[1] = fi.smallest_normal * fi.eps            # the smallest number
+    x[2] *= fi.smallest_normal
+    x[3] = fi.max if dtype == "f16" else 2.0 ** 126
+    x[4] = -x[3]
+    x[5, ::3] = -0.0
+    x[6, 40] = float("inf")
+    x[7, 64] = float("nan")
+    x[8, 0] = float("-inf")
+    saved = lowbit.save8(x)
+    code, E, val = plain_save(x)
+    assert torch.equal(saved.exponents[:, :3].int(), E)
+    assert torch.equal(saved.codes.int() & 127, code & 127)
+    back = lowbit.restore8(saved)
+    assert torch.equal(torch.isnan(back), torch.isnan(val))
+    assert torch.equal(torch.nan_to_num(back.double()), torch.nan_to_num(val))
+    if dtype == "bf16":                           # 2^127 and more have no step whose largest value is finite
+        x[3] = fi.max
+        assert bool(torch.isnan(lowbit.restore8(lowbit.save8(x))[3]).all())
+
+
+def test_save_rows_of_another_matrix_into_a_buffer(cuda_device):
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    x = randn((50, 333), torch.float16, cuda_device, 22)[4:37, 9:300]
+    room = torch.full((40, 512), 9, dtype=torch.uint8, device=cuda_device)
+    ex = torch.full((40, 16), 9, dtype=torch.uint8, device=cuda_device)
+    out = lowbit.Checkpoint8(room[2:35, :304], ex[2:35, :12], 291, torch.float16)
+    lowbit.save8(x, out=out)
+    code, E, val = plain_save(x)
+    assert torch.equal(out.codes[:, :291].int(), code) and torch.equal(out.exponents[:, :10].int(), E)
+    assert bool((room[:2] == 9).all()) and bool((room[35:] == 9).all()) and bool((room[:, 304:] == 9).all())
+    assert bool((ex[:2] == 9).all()) and bool((ex[35:] == 9).all()) and bool((ex[:, 10:] == 9).all())
+    to = torch.full((33, 300), 7.0, dtype=torch.float16, device=cuda_device)
+    lowbit.restore8(out, out=to[:, 4:295])
+    assert torch.equal(to[:, 4:295].double(), val) and bool((to[:, :4] == 7).all()) and bool((to[:, 295:] == 7).all())
+
+
+def test_save_empty(cuda_device):
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    saved = lowbit.save8(torch.empty(0, 64, dtype=torch.float16, device=cuda_device))
+    assert lowbit.restore8(saved).shape == (0, 64)
+
+
+GRAD = [(1, 1, 1), (1, 128, 256), (63, 128, 256), (64, 128, 256), (65, 130, 260), (256, 256, 512), (1000, 100, 72), (333, 257, 129),
+        (2048, 384, 200), (5000, 64, 640)]
+
+
+@pytest.mark.parametrize("dtype,out", [("f16", "f32"), ("bf16", "f32"), ("f16", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("m,k,n", GRAD)
+def test_weight_grad(cuda_device, dtype, out, m, k, n):
+    from subcuber_b200 import lowbit
+
+    x = randn((m, k), T(dtype), cuda_device, 23, 2.0)
+    dy = randn((m, n), T(dtype), cuda_device, 24, 0.1)
+    saved = lowbit.save8(x)
+    xv = plain_save(x)[2]
+    check_grad(lowbit.weight_grad8(saved, dy, out_dtype=T(out)), xv, dy, None)
+    base = randn((k, n), T(out), cuda_device, 25)
+    got = base.clone()
+    lowbit.weight_grad8(saved, dy, base=got, out=got)      # in place
+    check_grad(got, xv, dy, base)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+def test_weight_grad_strides(cuda_device, dtype):
+    """dY, base and result as parts of wider matrices, aligned and not; what lies beside the result stays."""
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    m, k, n = 200, 150, 136
+    x = randn((m, k), T(dtype), cuda_device, 26)
+    saved = lowbit.save8(x)
+    xv = plain_save(x)[2]
+    for c0, ld in ((0, n + 8), (8, n + 24), (3, n + 7), (1, n + 1)):
+        dy = randn((m, ld), T(dtype), cuda_device, 27)[:, c0:c0 + n]
+        base = randn((k, ld), torch.float32, cuda_device, 28)[:, c0:c0 + n]
+        room = torch.full((k + 2, ld), 7.0, device=cuda_device)
+        lowbit.weight_grad8(saved, dy, base=base, out=room[1:1 + k, c0:c0 + n])
+        check_grad(room[1:1 + k, c0:c0 + n], xv, dy, base)
+        room[1:1 + k, c0:c0 + n] = 7
+        assert bool((room == 7).all())
+
+
+def test_weight_grad_no_tokens(cuda_device):
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    saved = lowbit.save8(torch.empty(0, 70, dtype=torch.float16, device=cuda_device))
+    dy = torch.empty(0, 40, dtype=torch.float16, device=cuda_device)
+    base = randn((70, 40), torch.float32, cuda_device, 29)
+    assert bool((lowbit.weight_grad8(saved, dy) == 0).all())
+    assert torch.equal(lowbit.weight_grad8(saved, dy, base=base), base)
+
+
+def test_weight_grad_not_finite(cuda_device):
+    """A token's block that was not finite reaches the rows of its 32 channels only; an infinity in dY its column only."""
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    x = randn((100, 128), torch.bfloat16, cuda_device, 30)
+    dy = randn((100, 64), torch.bfloat16, cuda_device, 31)
+    clean = lowbit.weight_grad8(lowbit.save8(x), dy)
+    x[50, 40] = float("inf")
+    got = lowbit.weight_grad8(lowbit.save8(x), dy)
+    assert bool(torch.isnan(got[32:64]).all())
+    got[32:64] = clean[32:64]
+    assert torch.equal(got, clean)
+    x[50, 40] = 1.0
+    saved = lowbit.save8(x)
+    clean = lowbit.weight_grad8(saved, dy)
+    dy[3, 9] = float("nan")
+    got = lowbit.weight_grad8(saved, dy)
+    assert bool(torch.isnan(got[:, 9]).all())
+    got[:, 9] = clean[:, 9]
+    assert torch.equal(got, clean)
+
+
+def test_weight_grad_extreme_steps(cuda_device):
+    """Blocks whose steps lie at both ends of the range, each type's own."""
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    for dtype, scales in (("f16", (2.0 ** -24, 2.0 ** -20, 2.0 ** -14, 1.0, 500.0, 15000.0)), ("bf16", (2.0 ** -120, 2.0 ** -60, 1.0, 2.0 ** 60, 2.0 ** 110))):
+        for s in scales:
+            x = (randn((96, 64), torch.float32, cuda_device, 32).clamp(-4, 4) * s).to(T(dtype))
+            dy = randn((96, 48), T(dtype), cuda_device, 33)
+            check_grad(lowbit.weight_grad8(lowbit.save8(x), dy), plain_save(x)[2], dy, None)
+
+
+def test_weight_grad_offsets_past_32_bits(cuda_device):
+    """More than 2^31 bytes of codes, and of dY."""
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    m, k, n = 262144 + 70, 8192 + 64, 16
+    saved = lowbit.Checkpoint8(torch.zeros(m, k, dtype=torch.uint8, device=cuda_device),
+                               torch.full((m, 260), 127, dtype=torch.uint8, device=cuda_device), k, torch.bfloat16)
+    x = randn((70, k), torch.bfloat16, cuda_device, 34)
+    part = lowbit.save8(x)
+    saved.codes[262144:] = part.codes
+    saved.exponents[262144:, :258] = part.exponents[:, :258]
+    dy = torch.zeros(m, n, dtype=torch.bfloat16, device=cuda_device)
+    dy[262144:] = randn((70, n), torch.bfloat16, cuda_device, 35)
+    check_grad(lowbit.weight_grad8(saved, dy), plain_save(x)[2], dy[262144:], None)
+    assert torch.equal(lowbit.restore8(saved)[262144:].double(), plain_save(x)[2])
+    del saved
+    torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------------------------------------------ as a user has them
+@pytest.mark.parametrize("dtype", HALF)
+def test_linear_layer_forward_and_backward(cuda_device, dtype):
+    """A linear layer trained with its input saved in 8 bits, then served with its weights in 4 bits.  The gradient is
+    checked against the formula and against differences of the loss L = sum(c * (X W))."""
+    import torch
+
+    from subcuber_b200 import lowbit, runner
+
+    m, k, n = 192, 256, 128
+    x = randn((m, k), T(dtype), cuda_device, 40)
+    w = randn((k, n), T(dtype), cuda_device, 41, k ** -0.5)
+    kernel = f"blackwell_{dtype}_cubic_2sm_256x256"
+    y = runner.gemm(kernel, x, w)
+    c = randn((m, n), T(dtype), cuda_device, 42)        # the loss's gradient with respect to y
+    saved = lowbit.save8(x)
+    del x
+    dx = runner.gemm(kernel, c, w.t().contiguous())
+    dw = lowbit.weight_grad8(saved, c)
+    xv = values_of(saved)
+    check_grad(dw, xv, c, None)
+    # differences: L is linear in W, so (L(W + h V) - L(W - h V)) / 2h = <dW, V> at any h
+    v = randn((k, n), torch.float64, cuda_device, 43)
+    loss = lambda weights: (c.double() * (xv @ weights)).sum()
+    diff = (loss(w.double() + 0.5 * v) - loss(w.double() - 0.5 * v))
+    assert abs(float(diff - (dw.double() * v).sum())) <= 1e-5 * float((dw.double() * v).abs().sum())
+    # a second micro batch on top of the first
+    saved2 = lowbit.save8(randn((64, k), T(dtype), cuda_device, 44))
+    c2 = randn((64, n), T(dtype), cuda_device, 45)
+    both = lowbit.weight_grad8(saved2, c2, base=dw)
+    check_grad(both, torch.cat([xv, values_of(saved2)]), torch.cat([c, c2]), None)
+    # serving: the same weights in 4 bits, a prompt and then one token
+    w4 = lowbit.quantize_w4(w.t().contiguous(), group=32)
+    for rows in (m, 1):
+        x = randn((rows, k), T(dtype), cuda_device, 46)
+        check_w4_gemm(lowbit.gemm_w4(x, w4), x, w4, exact_weights=False)
+    assert y.shape == (m, n) and dx.shape == (m, k)
+
+
+def values_of(saved):
+    import torch
+
+    k = saved.k
+    step = ((saved.exponents[:, :-(-k // 32)].long() - 127 + 1023) << 52).view(torch.float64).repeat_interleave(32, 1)[:, :k]
+    c = saved.codes[:, :k].int()
+    return torch.where(c > 127, -(c & 127), c).double() * step
+
+
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_other_stream_and_graphs(cuda_device, m):
+    """Calls on a side stream, and two captured graphs (each with its own workspace) replayed at once on two streams."""
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    w = lowbit.quantize_w4(randn((500, 1024), torch.float16, cuda_device, 50, 0.03))
+    xs = [randn((m, 1024), torch.float16, cuda_device, 51 + i) for i in range(2)]
+    want = [lowbit.gemm_w4(x, w) for x in xs]
+    saved = [lowbit.save8(x) for x in xs]
+    grads = [lowbit.weight_grad8(s, y) for s, y in zip(saved, want)]
+    streams = [torch.cuda.Stream(cuda_device) for _ in range(2)]
+    graphs, outs = [], []
+    for x, s in zip(xs, streams):
+        s.wait_stream(torch.cuda.current_stream(cuda_device))
+        ws, gs = lowbit.WorkspaceW4(m, w), lowbit.WorkspaceGrad8(saved[0], 500)
+        y = torch.empty(m, 500, dtype=torch.float16, device=cuda_device)
+        dw = torch.empty(1024, 500, device=cuda_device)
+        cp = lowbit.Checkpoint8(torch.empty_like(saved[0].codes), torch.empty_like(saved[0].exponents), 1024, torch.float16)
+        with torch.cuda.stream(s):
+            lowbit.gemm_w4(x, w, out=y, workspace=ws)
+        s.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            lowbit.gemm_w4(x, w, out=y, workspace=ws)
+            lowbit.save8(x, out=cp)
+            lowbit.weight_grad8(cp, y, out=dw, workspace=gs)
+        graphs.append(g)
+        outs.append((y, dw, ws, gs, cp))
+    for _ in range(10):
+        for o in outs:
+            o[0].fill_(float("nan"))
+            o[1].fill_(float("nan"))
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for o, y, dw in zip(outs, want, grads):
+            assert torch.equal(o[0], y) and torch.equal(o[1], dw)
+
+
+def test_python_refusals(cuda_device):
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    w = lowbit.quantize_w4(randn((64, 128), torch.float16, cuda_device, 60))
+    x = randn((4, 128), torch.float16, cuda_device, 61)
+    saved = lowbit.save8(x)
+    dy = randn((4, 64), torch.float16, cuda_device, 62)
+    bad = [
+        lambda: lowbit.gemm_w4(x.bfloat16(), w),
+        lambda: lowbit.gemm_w4(x[:, :100], w),
+        lambda: lowbit.gemm_w4(x.t(), w),
+        lambda: lowbit.gemm_w4(x[0], w),
+        lambda: lowbit.gemm_w4(x.cpu(), w),
+        lambda: lowbit.gemm_w4(x[:1].expand(4, 128).as_strided((4, 128), (64, 1)), w),
+        lambda: lowbit.gemm_w4(x, w, out=torch.empty(4, 63, dtype=torch.float16, device=cuda_device)),
+        lambda: lowbit.gemm_w4(x, w, out=torch.empty(4, 64, device=cuda_device)),
+        lambda: lowbit.quantize_w4(x.float()),
+        lambda: lowbit.quantize_w4(x, group=100),
+        lambda: lowbit.pack_w4(x.to(torch.uint8), torch.ones(2, 4, dtype=torch.float16, device=cuda_device)),
+        lambda: lowbit.save8(x.float()),
+        lambda: lowbit.save8(x, out=lowbit.save8(x[:3])),
+        lambda: lowbit.weight_grad8(saved, dy.bfloat16()),
+        lambda: lowbit.weight_grad8(saved, dy[:3]),
+        lambda: lowbit.weight_grad8(saved, dy[:, :0]),
+        lambda: lowbit.weight_grad8(saved, dy, out_dtype=torch.bfloat16),
+        lambda: lowbit.weight_grad8(saved, dy, base=torch.zeros(128, 64, dtype=torch.float16, device=cuda_device)),
+        lambda: lowbit.weight_grad8(saved, dy, base=torch.zeros(128, 60, device=cuda_device)),
+        lambda: lowbit.Checkpoint8(saved.codes[:, :120], saved.exponents, 120, torch.float16),
+        lambda: lowbit.WeightsW4(w.codes, w.scales[:, :8], None, 64, 128, 128),
+        lambda: lowbit.WeightsW4(w.codes[:512], w.scales, None, 64, 128, 128),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"call {i} was accepted")
+    small = lowbit.WorkspaceW4(1, w)
+    small.nbytes = 0
+    with pytest.raises(lowbit.KernelError):
+        lowbit.gemm_w4(x, w, workspace=small)
