@@ -290,21 +290,24 @@ int sb200_peer_wait(int* const* local_flags, int count, int value, unsigned wait
  * their elements'.  m = 0 is an empty batch.  No counterpart in the reference project.
  *
  * Weights in 4 bits, n outputs x k inputs, groups of G = 32, 64 or 128 inputs of an output:
- *     W[n][k] = scale[k / G][n] * (code[n][k] - zero[k / G][n]),   code and zero in 0..15, zero = 8 where zeros == NULL
- * scales (in the 16-bit type `dtype`) and zeros (bytes) are tables of ceil(k / G) rows of sb200_w4_table_rows(n) entries.
+ *     W[n][k] = scale(n, k / G) * (code[n][k] - zero(n, k / G)),   code and zero in 0..15, zero = 8 where zeros == NULL
  * codes (16-byte aligned, sb200_w4_codes_bytes(n, k) bytes) are tiles of 16 outputs x 128 inputs, 1 KiB each, along the inputs
  * first: bytes 512 h + 16 (4 g + t) + 4 j of a tile hold the 32-bit word of output 8 h + g and inputs 32 j + 8 t + i, i = 0..7,
- * input i in nibble (i >> 1) + 4 (i & 1).  sb200_w4_pack brings plain codes (one byte each) into this order. */
+ * input i in nibble (i >> 1) + 4 (i & 1).  scales (in the 16-bit type `dtype`, 8-byte aligned) and zeros (bytes, 4-byte aligned)
+ * hold sb200_w4_table_entries(n, k, group) entries: [tile of outputs][128 inputs][output of the tile][group of the 128 inputs].
+ * Outputs are padded to 16 and inputs to 128; the scales of padding are 0. */
 size_t sb200_w4_codes_bytes(int n, int k);
-size_t sb200_w4_table_rows(int n);
+size_t sb200_w4_table_entries(int n, int k, int group);
 /* Quantise w (n x k, 16-bit), group by group.  zeros == NULL: scale = amax / 7, code = 8 + rint(w / scale).  Else, with
  * lo = min(0, w) and hi = max(0, w): scale = (hi - lo) / 15, zero = rint(-lo / scale), code = zero + rint(w / scale).  The
  * scale is rounded to `dtype` before the codes are made; codes are held within 0..15.  A group with an infinity or a NaN
  * (or whose hi - lo overflows) gets a scale that is not finite: its weights stand for NaN. */
 int sb200_w4_quantize(int dtype, const void* w, long long ldw, int n, int k, int group, void* codes, void* scales, void* zeros,
                       sb200_stream_t stream);
-/* Codes of another quantiser, one byte each in the low nibble, q[n][k], into the order above. */
-int sb200_w4_pack(const void* q, long long ldq, int n, int k, void* codes, sb200_stream_t stream);
+/* Weights of another quantiser into the order above: codes q[n][k], one byte each, in the low nibble; scales
+ * q_scales[group][n] in `dtype`; zeros q_zeros[group][n], bytes, or NULL (then zeros is NULL too). */
+int sb200_w4_pack(int dtype, const void* q, long long ldq, const void* q_scales, long long lds, const void* q_zeros,
+                  long long ldz, int n, int k, int group, void* codes, void* scales, void* zeros, sb200_stream_t stream);
 /* out[n][k] = W rounded once to `dtype`. */
 int sb200_w4_dequantize(int dtype, const void* codes, const void* scales, const void* zeros, int n, int k, int group, void* out,
                         long long ldo, sb200_stream_t stream);

@@ -106,9 +106,9 @@ def load(build_if_missing: bool = True) -> C.CDLL:
     p, i, ll, z = C.c_void_p, C.c_int, C.c_longlong, C.c_size_t
     for name, res, args in (
             ("sb200_w4_codes_bytes", z, [i, i]),
-            ("sb200_w4_table_rows", z, [i]),
+            ("sb200_w4_table_entries", z, [i, i, i]),
             ("sb200_w4_quantize", i, [i, p, ll, i, i, i, p, p, p, p]),
-            ("sb200_w4_pack", i, [p, ll, i, i, p, p]),
+            ("sb200_w4_pack", i, [i, p, ll, p, ll, p, ll, i, i, i, p, p, p, p]),
             ("sb200_w4_dequantize", i, [i, p, p, p, i, i, i, p, ll, p]),
             ("sb200_w4_gemm_workspace_bytes", z, [i, i, i, i, i]),
             ("sb200_w4_gemm", i, [i, p, ll, p, p, p, p, ll, i, i, i, i, p, z, p]),

@@ -1,13 +1,15 @@
 // The two formats in which an operand of a product is held in few bits, and the element arithmetic on them.
 //
-//   W4     weights n x k in 4 bits:  W[n][k] = scale[k / G][n] * (code[n][k] - zero[k / G][n]),  code in 0..15, zero in 0..15
+//   W4     weights n x k in 4 bits:  W[n][k] = scale(n, k / G) * (code[n][k] - zero(n, k / G)),  code in 0..15, zero in 0..15
 //          (8 where there is no table of zeros), G = 32, 64 or 128.  Rows are padded to 16, inputs to 128.  A tile of 16 rows
 //          x 128 inputs is 1 KiB of consecutive bytes, tiles run along the inputs first.  Inside a tile the 16 bytes at
 //          512 h + 16 (4 g + t) belong to row 8 h + g; their word j holds the inputs 32 j + 8 t + (0..7), input i at nibble
 //          (i >> 1) + 4 (i & 1).  That is the fragment order of a 16 x 8 x 16 matrix instruction: lane 4 g + t loads its 16 bytes
 //          at once, one word lies within one group whatever G is, and the four pairs of nibbles that `w >> 4 p` leaves 16 bits
 //          apart are neighbouring inputs, so that an expanded word is 16 bytes in the order of the activations.
-//          Scales have the 16-bit type of the activations; scales and zeros are [groups][rows padded to 16].
+//          Scales have the 16-bit type of the activations, zeros are bytes; both tables run with the tiles:
+//          [row tile][128 inputs][row of the tile][group of the 128 inputs], so that the groups of a row in a tile are one load.
+//          What belongs to padding has scale 0.
 //   ACT8   activations m x k in 8 bits:  X[m][k] = +-magnitude * 2^(E[m][k / 32] - 127), bit 7 of the byte is the sign, bits 0-6
 //          the magnitude.  A magnitude has 7 bits and the step is a power of two, so every X is exact in bf16 and (with the
 //          steps kept to 2^-24 .. 2^9) in f16: a product of X is a product of 16-bit operands without another rounding.
@@ -31,6 +33,15 @@ __host__ __device__ inline int ceil_div(int a, int b) { return a / b + (a % b !=
 __host__ __device__ inline int w4_blocks(int k) { return ceil_div(k, kW4Block); }
 __host__ __device__ inline int w4_row_tiles(int n) { return ceil_div(n, kW4Rows); }
 __host__ __device__ inline long long w4_padded_rows(int n) { return static_cast<long long>(w4_row_tiles(n)) * kW4Rows; }
+
+// Entries of the tables, and where that of (row, group of the whole row) is.
+__host__ __device__ inline long long w4_table_entries(int n, int k, int G) {
+  return w4_padded_rows(n) * w4_blocks(k) * (kW4Block / G);
+}
+__host__ __device__ inline long long w4_table_at(int row, int group, int blocks, int G) {
+  const int per = kW4Block / G;
+  return ((static_cast<long long>(row / kW4Rows) * blocks + group / per) * kW4Rows + row % kW4Rows) * per + group % per;
+}
 
 // Nibble of input i (0..7) in its word.
 __host__ __device__ constexpr int w4_nibble(int i) { return (i >> 1) + 4 * (i & 1); }

@@ -84,24 +84,20 @@ class _Workspace:
 
 
 class WeightsW4:
-    """Weights in 4 bits: `codes` in the library's order, `scales` [groups, padded rows] in the activations' type,
-    `zeros` [groups, padded rows] uint8 or None (symmetric).  Made by `quantize_w4` or `pack_w4`."""
+    """Weights in 4 bits, in the library's order: `codes` uint8, `scales` in the activations' type, `zeros` uint8 or None
+    (symmetric), all flat.  Made by `quantize_w4` or `pack_w4`."""
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor], n: int, k: int, group: int):
         lib = _lib.load()
-        if n <= 0 or k <= 0:
-            raise ValueError("weights need at least one output and one input")
-        if group not in GROUPS:
-            raise ValueError(f"group must be one of {GROUPS}")
+        _check_w4(n, k, group)
         _same_device(codes, scales, zeros)
-        _matrix("scales", scales, HALF_TYPES)
-        table = (-(-k // group), int(lib.sb200_w4_table_rows(n)))
-        if codes.dtype != torch.uint8 or not codes.is_contiguous() or codes.numel() != int(lib.sb200_w4_codes_bytes(n, k)):
-            raise ValueError("codes must be a packed uint8 tensor of sb200_w4_codes_bytes(n, k) bytes")
-        if tuple(scales.shape) != table or not scales.is_contiguous():
-            raise ValueError(f"scales must be a packed {table[0]} x {table[1]} table")
-        if zeros is not None and (zeros.dtype != torch.uint8 or tuple(zeros.shape) != table or not zeros.is_contiguous()):
-            raise ValueError(f"zeros must be a packed {table[0]} x {table[1]} table of uint8")
+        nbytes, entries = int(lib.sb200_w4_codes_bytes(n, k)), int(lib.sb200_w4_table_entries(n, k, group))
+        if scales.dtype not in HALF_TYPES:
+            raise ValueError(f"scales must be one of {[str(d) for d in HALF_TYPES]}, not {scales.dtype}")
+        for name, t, dtype, count in (("codes", codes, torch.uint8, nbytes), ("scales", scales, scales.dtype, entries),
+                                      ("zeros", zeros, torch.uint8, entries)):
+            if t is not None and (not t.is_cuda or t.dtype != dtype or t.numel() != count or not t.is_contiguous()):
+                raise ValueError(f"{name} must be a packed CUDA tensor of {count} {dtype}")
         self.codes, self.scales, self.zeros = codes, scales, zeros
         self.n, self.k, self.group = n, k, group
         self.dtype, self.device = scales.dtype, scales.device
@@ -112,16 +108,20 @@ class WeightsW4:
         return sum(t.numel() * t.element_size() for t in (self.codes, self.scales, self.zeros) if t is not None)
 
 
-def _empty_w4(n: int, k: int, group: int, symmetric: bool, dtype, device) -> WeightsW4:
-    lib = _lib.load()
+def _check_w4(n: int, k: int, group: int) -> None:
     if group not in GROUPS:
         raise ValueError(f"group must be one of {GROUPS}")
     if n <= 0 or k <= 0:
         raise ValueError("weights need at least one output and one input")
-    table = (-(-k // group), int(lib.sb200_w4_table_rows(n)))
+
+
+def _empty_w4(n: int, k: int, group: int, symmetric: bool, dtype, device) -> WeightsW4:
+    lib = _lib.load()
+    _check_w4(n, k, group)
+    entries = int(lib.sb200_w4_table_entries(n, k, group))
     return WeightsW4(torch.empty(int(lib.sb200_w4_codes_bytes(n, k)), dtype=torch.uint8, device=device),
-                     torch.empty(table, dtype=dtype, device=device),
-                     None if symmetric else torch.empty(table, dtype=torch.uint8, device=device), n, k, group)
+                     torch.empty(entries, dtype=dtype, device=device),
+                     None if symmetric else torch.empty(entries, dtype=torch.uint8, device=device), n, k, group)
 
 
 def quantize_w4(weight: torch.Tensor, group: int = 128, symmetric: bool = False) -> WeightsW4:
@@ -141,14 +141,16 @@ def pack_w4(q: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor]
     _matrix("scales", scales, HALF_TYPES)
     n, k = q.shape
     _same_device(q, scales, zeros)
+    _check_w4(n, k, group)
+    if zeros is not None:
+        _matrix("zeros", zeros, (torch.uint8,))
+    for name, t in (("scales", scales), ("zeros", zeros)):
+        if t is not None and tuple(t.shape) != (-(-k // group), n):
+            raise ValueError(f"{name} must be a {-(-k // group)} x {n} table")
     w = _empty_w4(n, k, group, zeros is None, scales.dtype, q.device)
-    for name, table, to in (("scales", scales, w.scales), ("zeros", zeros, w.zeros)):
-        if table is not None:
-            if tuple(table.shape) != (to.shape[0], n) or table.dtype != to.dtype:
-                raise ValueError(f"{name} must be a {to.shape[0]} x {n} table of {to.dtype}")
-            to[:, n:] = 0
-            to[:, :n] = table
-    _call("pack_w4", _lib.load().sb200_w4_pack, q.device, q.data_ptr(), _ld(q), n, k, w.codes.data_ptr())
+    _call("pack_w4", _lib.load().sb200_w4_pack, q.device, DTYPE_CODE[w.dtype], q.data_ptr(), _ld(q), scales.data_ptr(),
+          _ld(scales), zeros.data_ptr() if zeros is not None else None, _ld(zeros) if zeros is not None else n, n, k, group,
+          w.codes.data_ptr(), w.scales.data_ptr(), w._zeros_ptr)
     return w
 
 

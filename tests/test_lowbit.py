@@ -31,7 +31,8 @@ def test_w4_sizes(lib):
     assert lib.sb200_w4_codes_bytes(16, 128) == 1024 and lib.sb200_w4_codes_bytes(17, 129) == 4096
     assert lib.sb200_w4_codes_bytes(1, 1) == 1024 and lib.sb200_w4_codes_bytes(0, 5) == 0
     assert lib.sb200_w4_codes_bytes(1 << 20, 1 << 15) == 1 << 34   # offsets pass 32 bits
-    assert lib.sb200_w4_table_rows(1) == 16 and lib.sb200_w4_table_rows(16) == 16 and lib.sb200_w4_table_rows(17) == 32
+    assert lib.sb200_w4_table_entries(1, 1, 128) == 16 and lib.sb200_w4_table_entries(17, 129, 32) == 32 * 8
+    assert lib.sb200_w4_table_entries(17, 129, 48) == 0 and lib.sb200_w4_table_entries(0, 1, 32) == 0
 
 
 @pytest.mark.parametrize("args,rc", [
@@ -44,9 +45,12 @@ def test_w4_quantize_refuses(lib, args, rc):
 
 
 def test_w4_pack_and_dequantize_refuse(lib):
-    assert lib.sb200_w4_pack(None, 8, 4, 8, P, None) == 4
-    assert lib.sb200_w4_pack(P, 7, 4, 8, P, None) == 4
-    assert lib.sb200_w4_pack(P, 8, 4, 8, P + 1, None) == 1
+    pack = lambda dtype=0, q=P, ldq=8, s=P, lds=4, z=P, ldz=4, n=4, k=8, group=32, codes=P, scales=P, zeros=P: lib.sb200_w4_pack(
+        dtype, q, ldq, s, lds, z, ldz, n, k, group, codes, scales, zeros, None)
+    assert pack(q=None) == 4 and pack(ldq=7) == 4 and pack(s=None) == 4 and pack(lds=3) == 4 and pack(ldz=3) == 4
+    assert pack(z=None) == 4 and pack(zeros=None) == 4 and pack(n=0) == 4 and pack(scales=None) == 4
+    assert pack(codes=P + 1) == 1 and pack(scales=P + 4) == 1 and pack(zeros=P + 2) == 1 and pack(s=P + 1) == 1
+    assert pack(dtype=1) == 5 and pack(group=16) == 5
     assert lib.sb200_w4_dequantize(0, P, P, None, 4, 8, 32, None, 8, None) == 4
     assert lib.sb200_w4_dequantize(0, P, P, None, 4, 8, 32, P, 7, None) == 4
     assert lib.sb200_w4_dequantize(1, P, P, None, 4, 8, 32, P, 8, None) == 5

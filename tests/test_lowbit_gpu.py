@@ -67,13 +67,19 @@ def unpack(w):
     return out.reshape(n_t * 16, k_b * 128)[:w.n, :w.k]
 
 
+def table(t, w):
+    """Entries [n, groups] of a table of a WeightsW4, from the documented order."""
+    n_t, k_b, per = -(-w.n // 16), -(-w.k // 128), 128 // w.group
+    return t.view(n_t, k_b, 16, per).permute(0, 2, 1, 3).reshape(n_t * 16, k_b * per)[:w.n, :-(-w.k // w.group)]
+
+
 def values(w):
     """Weights [n, k] in 64 bits that a WeightsW4 stands for."""
     import torch
 
     at = torch.arange(w.k, device=w.codes.device) // w.group
-    s = w.scales.double()[at, :w.n].t()
-    z = 8.0 if w.zeros is None else w.zeros.double()[at, :w.n].t()
+    s = table(w.scales, w).double()[:, at]
+    z = 8.0 if w.zeros is None else table(w.zeros, w).double()[:, at]
     return (unpack(w).double() - z) * s
 
 
@@ -145,9 +151,9 @@ def test_quantize(cuda_device, dtype, symmetric, group, n, k):
     got = lowbit.quantize_w4(w, group=group, symmetric=symmetric)
     q, s, z = plain_quantize(w, group, symmetric)
     assert torch.equal(unpack(got).double(), q)
-    assert torch.equal(got.scales.double()[:, :n].t(), s)
+    assert torch.equal(table(got.scales, got).double(), s)
     if not symmetric:
-        assert torch.equal(got.zeros.double()[:, :n].t(), z)
+        assert torch.equal(table(got.zeros, got).double(), z)
     want = values(got).to(w.dtype)
     assert torch.equal(lowbit.dequantize_w4(got), want)
 
@@ -183,7 +189,7 @@ def test_quantize_extremes(cuda_device, dtype):
     for symmetric in (True, False):
         got = lowbit.quantize_w4(w, group=128, symmetric=symmetric)
         q, s, _ = plain_quantize(w, 128, symmetric)
-        assert torch.equal(got.scales.double()[:, :8].t(), s)
+        assert torch.equal(table(got.scales, got).double(), s)
         assert torch.equal(unpack(got).double(), q)
 
 
@@ -319,12 +325,12 @@ def test_gemm_w4_offsets_past_32_bits(cuda_device):
     reps = -(-n // 16384)
     rows = -(-n // 16) * 16
     codes = part.codes.repeat(reps)[: rows * k // 2].clone()
-    scales = part.scales.repeat(1, reps)[:, :rows].contiguous()
+    scales = part.scales.repeat(reps)[: rows * k // 128].clone()
     w = lowbit.WeightsW4(codes, scales, None, n, k, 128)
     tail = randn((37, k), torch.bfloat16, cuda_device, 17, 0.02)      # the last rows differ from the repeated ones
     last = lowbit.quantize_w4(tail, group=128, symmetric=True)
     codes[131072 * k // 2:] = last.codes
-    scales[:, 131072:] = last.scales
+    scales[131072 * k // 128:] = last.scales
     for m in (1, 17, 100):
         x = randn((m, k), torch.bfloat16, cuda_device, 18)
         y = lowbit.gemm_w4(x, w)
@@ -643,7 +649,7 @@ def test_python_refusals(cuda_device):
         lambda: lowbit.weight_grad8(saved, dy, base=torch.zeros(128, 64, dtype=torch.float16, device=cuda_device)),
         lambda: lowbit.weight_grad8(saved, dy, base=torch.zeros(128, 60, device=cuda_device)),
         lambda: lowbit.Checkpoint8(saved.codes[:, :120], saved.exponents, 120, torch.float16),
-        lambda: lowbit.WeightsW4(w.codes, w.scales[:, :8], None, 64, 128, 128),
+        lambda: lowbit.WeightsW4(w.codes, w.scales[:8], None, 64, 128, 128),
         lambda: lowbit.WeightsW4(w.codes[:512], w.scales, None, 64, 128, 128),
     ]
     for i, call in enumerate(bad):
