@@ -285,8 +285,8 @@ int sb200_peer_wait(int* const* local_flags, int count, int value, unsigned wait
 /* ---- products with one operand held in few bits ---------------------------------------------------------------------
  * What the linear layers of a language model need beside the GEMM above: weights in 4 bits (serving), activations saved
  * in 8 bits for the backward pass (training).  dtype and out_dtype: 0 f16, 1 f32, 3 bf16.  All calls are asynchronous on
- * `stream`, allocate nothing, and may be captured into graphs; a workspace belongs to one call at a time (two calls that
- * may overlap need two).  Matrices are row-major with a leading dimension in elements; rows need no alignment beyond
+ * `stream`, allocate nothing, and may be captured into graphs; a workspace (256-byte aligned) belongs to one call at a time (two calls
+ * that may overlap need two); sb200_gemm_status reads the status word at its head after a product.  Matrices are row-major with a leading dimension in elements; rows need no alignment beyond
  * their elements'.  m = 0 is an empty batch.  No counterpart in the reference project.
  *
  * Weights in 4 bits, n outputs x k inputs, groups of G = 32, 64 or 128 inputs of an output:
@@ -311,8 +311,11 @@ int sb200_w4_pack(int dtype, const void* q, long long ldq, const void* q_scales,
 /* out[n][k] = W rounded once to `dtype`. */
 int sb200_w4_dequantize(int dtype, const void* codes, const void* scales, const void* zeros, int n, int k, int group, void* out,
                         long long ldo, sb200_stream_t stream);
-/* y[m][n] = sum over k of x[m][k] W[n][k], sums in fp32, rounded once to `dtype`. */
-size_t sb200_w4_gemm_workspace_bytes(int dtype, int m, int n, int k, int group);
+/* y[m][n] = sum over k of x[m][k] W[n][k], sums in fp32, rounded once to `dtype`.  Up to 32 rows the codes are multiplied
+ * exactly and the scales applied in fp32; with more the weights are rounded to `dtype` first (as sb200_w4_dequantize does).
+ * x_aligned: the rows of x start on 16 bytes (pointer and ldx); else the workspace holds a copy of x.  A workspace for m rows
+ * serves every smaller m. */
+size_t sb200_w4_gemm_workspace_bytes(int dtype, int m, int n, int k, int group, int x_aligned);
 int sb200_w4_gemm(int dtype, const void* x, long long ldx, const void* codes, const void* scales, const void* zeros, void* y,
                   long long ldy, int m, int n, int k, int group, void* workspace, size_t workspace_bytes, sb200_stream_t stream);
 
@@ -329,8 +332,9 @@ int sb200_act8_restore(int dtype, const void* codes, long long pitch, const void
 /* Weight gradient of y = x W (W is k x n, as B of sb200_gemm) from saved activations:
  *     dw[k][n] = base[k][n] + sum over m of X[m][k] dy[m][n]
  * dy in `dtype`; base (NULL: none; it may be dw itself) and dw in out_dtype, which is f32 or `dtype`.  Sums in fp32, rounded
- * once.  m = 0 gives base, or zeros. */
-size_t sb200_act8_wgrad_workspace_bytes(int dtype, int out_dtype, int m, int n, int k);
+ * once.  m = 0 gives base, or zeros.  dy_aligned: the rows of dy start on 16 bytes (pointer and lddy); else the workspace
+ * holds a copy of dy.  A workspace for m tokens serves every smaller m. */
+size_t sb200_act8_wgrad_workspace_bytes(int dtype, int out_dtype, int m, int n, int k, int dy_aligned);
 int sb200_act8_wgrad(int dtype, const void* codes, long long pitch, const void* exponents, long long exp_pitch, const void* dy,
                      long long lddy, int out_dtype, const void* base, long long ldbase, void* dw, long long lddw, int m, int n,
                      int k, void* workspace, size_t workspace_bytes, sb200_stream_t stream);

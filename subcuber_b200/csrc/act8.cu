@@ -5,7 +5,6 @@
 #include "../../include/subcuber_b200.h"
 #include "lowbit_format.cuh"
 #include "lowbit_host.h"
-#include "simple_product.cuh"
 
 namespace sb200 {
 namespace lowbit {
@@ -116,27 +115,6 @@ __global__ void __launch_bounds__(kThreads) act8_restore_kernel(const uint8_t* _
   }
 }
 
-struct ActLeft {  // X^T as the left operand of a product: (channel, token)
-  const uint8_t* codes;
-  long long pitch;
-  const uint8_t* exps;
-  long long exp_pitch;
-  int k, m;
-  __device__ float operator()(int ch, int t) const {
-    if (ch >= k || t >= m) return 0.f;
-    return act8_value(codes[t * pitch + ch], act8_step(exps[t * exp_pitch + ch / kActBlock]));
-  }
-};
-template <typename T>
-struct DenseRight {
-  const T* p;
-  long long ld;
-  int rows, cols;
-  __device__ float operator()(int k, int j) const { return k < rows && j < cols ? to_f32(p[k * ld + j]) : 0.f; }
-};
-
-inline bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
-
 int check(const Act8& a) {
   if (a.dtype != kF16 && a.dtype != kBF16) return kErrNotSupported;
   if (a.m < 0 || a.k <= 0 || a.pitch < a.k || a.exp_pitch < ceil_div(a.k, kActBlock)) return kErrInvalidProblem;
@@ -163,14 +141,6 @@ int restore(const Act8& a, void* x, long long ldx, cudaStream_t stream) {
       static_cast<const uint8_t*>(a.codes), a.pitch, static_cast<const uint8_t*>(a.exps), a.exp_pitch, a.m, a.k,
       static_cast<T*>(x), ldx, cut, aligned(x, 16) && ldx % 8 == 0);
   return static_cast<int>(cudaGetLastError());
-}
-
-template <typename T, typename Out>
-int weight_grad(const Act8& a, const void* dy, long long lddy, const void* base, long long ldbase, void* dw, long long lddw,
-                int n, cudaStream_t stream) {
-  const ActLeft left{static_cast<const uint8_t*>(a.codes), a.pitch, static_cast<const uint8_t*>(a.exps), a.exp_pitch, a.k, a.m};
-  const DenseRight<T> right{static_cast<const T*>(dy), lddy, a.m, n};
-  return simple_product<Out>(left, right, static_cast<Out*>(dw), lddw, static_cast<const Out*>(base), ldbase, a.k, n, a.m, stream);
 }
 
 }  // namespace
@@ -203,9 +173,11 @@ extern "C" int sb200_act8_restore(int dtype, const void* codes, long long pitch,
   return dtype == sb200::kF16 ? sb200::lowbit::restore<__half>(a, x, ldx, s) : sb200::lowbit::restore<__nv_bfloat16>(a, x, ldx, s);
 }
 
-extern "C" size_t sb200_act8_wgrad_workspace_bytes(int dtype, int out_dtype, int m, int n, int k) {
-  (void)dtype; (void)out_dtype; (void)m; (void)n; (void)k;
-  return 256;
+extern "C" size_t sb200_act8_wgrad_workspace_bytes(int dtype, int out_dtype, int m, int n, int k, int dy_aligned) {
+  (void)dtype;
+  (void)out_dtype;
+  if (m < 0 || n <= 0 || k <= 0) return 256;
+  return sb200::lowbit::expand_act8_workspace(m, n, k, dy_aligned != 0);
 }
 
 extern "C" int sb200_act8_wgrad(int dtype, const void* codes, long long pitch, const void* exponents, long long exp_pitch,
@@ -219,14 +191,9 @@ extern "C" int sb200_act8_wgrad(int dtype, const void* codes, long long pitch, c
   const uintptr_t width = out_dtype == sb200::kF32 ? 4 : 2;
   if (!sb200::lowbit::aligned(dy, 2) || !sb200::lowbit::aligned(dw, width) || !sb200::lowbit::aligned(base, width))
     return SB200_ERR_MISALIGNED_OPERAND;
-  if (!workspace || workspace_bytes < sb200_act8_wgrad_workspace_bytes(dtype, out_dtype, m, n, k) ||
+  if (!workspace || workspace_bytes < sb200_act8_wgrad_workspace_bytes(dtype, out_dtype, m, n, k, sb200::lowbit::tma_rows(dy, lddy)) ||
       !sb200::lowbit::aligned(workspace, 256))
     return SB200_ERR_WORKSPACE_NULL;
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  using namespace sb200::lowbit;
-  if (dtype == sb200::kF16)
-    return out_dtype == sb200::kF32 ? weight_grad<__half, float>(a, dy, lddy, base, ldbase, dw, lddw, n, s)
-                                    : weight_grad<__half, __half>(a, dy, lddy, base, ldbase, dw, lddw, n, s);
-  return out_dtype == sb200::kF32 ? weight_grad<__nv_bfloat16, float>(a, dy, lddy, base, ldbase, dw, lddw, n, s)
-                                  : weight_grad<__nv_bfloat16, __nv_bfloat16>(a, dy, lddy, base, ldbase, dw, lddw, n, s);
+  return sb200::lowbit::expand_act8(a, dy, lddy, out_dtype == sb200::kF32, base, ldbase, dw, lddw, n, workspace,
+                                    reinterpret_cast<cudaStream_t>(stream));
 }

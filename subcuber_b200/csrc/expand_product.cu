@@ -1,0 +1,203 @@
+// Host side of the products with an expanded operand: how a product is cut, workspace, launches.
+#include "expand_product.cuh"
+
+#include "lowbit_host.h"
+#include "per_device.h"
+
+namespace sb200 {
+namespace lowbit {
+namespace {
+
+inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
+
+constexpr int kMaxSlices = 16;
+constexpr size_t kPartBytes = size_t(64) << 20;  // most that the parts of a divided reduction may take
+
+struct Cut {
+  int bn, slices;
+};
+
+// Tile width and parts of the reduction.  A step of 64 costs a pair about 2 bn clocks on the tensor cores (256 rows x bn
+// columns x 64 at 8192 operations a clock and SM) and never less than the converters take; a unit more than that for filling its pipeline
+// and for its sums; dividing the reduction costs a pass over the parts, and a launch.  The cut with the least total of
+// the fullest pair wins; widths are what the instruction takes.
+Cut cut_of(long long rows, long long cols, int steps, int pairs) {
+  const double kConvert = 250, kUnit = 1500, kJoin = 6000, kBytesPerClock = 2500;
+  Cut best{kMaxCols, 1};
+  double least = 1e300;
+  for (int bn = kMaxCols; bn >= 32; bn -= 32) {
+    const double tiles = static_cast<double>(ceil_div(static_cast<int>(rows), kPairRows)) * ceil_div(static_cast<int>(cols), bn);
+    for (int s = 1; s <= kMaxSlices; ++s) {
+      if (s > 1 && (s > (steps + 1) / 2 || static_cast<double>(s) * rows * cols * 4 > kPartBytes)) break;
+      const double waves = ceil(tiles * s / pairs);
+      const double step = 2 * bn > kConvert ? 2 * bn : kConvert;
+      double t = waves * (2 * ceil((steps + 1) / 2 / static_cast<double>(s)) * step + kUnit);
+      if (s > 1) t += kJoin + (2.0 * s + 1) * rows * cols * 4 / kBytesPerClock;
+      if (t < least) { least = t; best = Cut{bn, s}; }
+    }
+  }
+  return best;
+}
+
+int pairs_of_device() {
+  const int sms = sm_count_of_current_device();
+  return (sms > 0 ? sms : 148) / 2;
+}
+
+size_t part_bytes(long long rows, long long cols) {
+  const size_t all = size_t(kMaxSlices) * rows * cols * 4;
+  return all < kPartBytes ? all : kPartBytes;
+}
+
+template <typename T, int KIND, int PER>
+int launch(const ExpandParams& p, int pairs, cudaStream_t stream) {
+  auto* kernel = expand_product_kernel<T, KIND, PER>;
+  static PerDeviceOnce once;
+  const int rc = once.run_once([&] {
+    // the warps trade registers: a block launched with fewer than the trade needs would wait for good
+    cudaFuncAttributes a;
+    cudaError_t e = cudaFuncGetAttributes(&a, kernel);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    if (a.numRegs != kRegsLaunch) return static_cast<int>(kErrInternal);
+    return static_cast<int>(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kExpandSmem));
+  });
+  if (rc) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
+  cfg.blockDim = dim3(kExpandThreads);
+  cfg.dynamicSmemBytes = kExpandSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {2, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, p));
+}
+
+template <typename Out>
+int join(const ExpandParams& p, int rows, int cols, cudaStream_t stream) {
+  const long long blocks = (static_cast<long long>(rows) * cols + 1023) / 1024;
+  const unsigned grid = static_cast<unsigned>(blocks < 148 * 16 ? blocks : 148 * 16);
+  join_slices_kernel<Out><<<grid, 256, 0, stream>>>(p.part, p.slices, rows, cols, static_cast<Out*>(p.out), p.ldo,
+                                                    static_cast<const Out*>(p.base), p.ldbase);
+  return static_cast<int>(cudaGetLastError());
+}
+
+// Fills in the cut; returns the pairs to launch, or 0 when there are too many units.
+int place(ExpandParams& p, int pairs) {
+  const Cut c = cut_of(p.rows, p.cols, p.steps, pairs);
+  p.bn = c.bn;
+  p.slices = c.slices;
+  p.tiles_r = ceil_div(p.rows, kPairRows);
+  p.tiles_c = ceil_div(p.cols, p.bn);
+  const long long units = static_cast<long long>(p.tiles_r) * p.tiles_c * p.slices;
+  if (units > 0x3fffffffll) return 0;
+  return units < pairs ? static_cast<int>(units) : pairs;
+}
+
+template <typename T>
+int run_w4(const ExpandParams& p, int group, int pairs, cudaStream_t stream) {
+  int rc;
+  if (group == 32) rc = launch<T, kExpandW4, 4>(p, pairs, stream);
+  else if (group == 64) rc = launch<T, kExpandW4, 2>(p, pairs, stream);
+  else rc = launch<T, kExpandW4, 1>(p, pairs, stream);
+  if (rc || p.slices == 1) return rc;
+  return join<T>(p, p.cols, p.rows, stream);
+}
+
+template <typename T>
+int run_act8(const ExpandParams& p, int pairs, cudaStream_t stream) {
+  if (p.steps > 0) {
+    const int rc = launch<T, kExpandAct8, 1>(p, pairs, stream);
+    if (rc || p.slices == 1) return rc;
+  }
+  return p.out_f32 ? join<float>(p, p.rows, p.cols, stream) : join<T>(p, p.rows, p.cols, stream);
+}
+
+constexpr unsigned long long kWaitNs = 2000000000ull;  // bound of every device-side wait
+constexpr size_t kStatusBytes = 256;
+
+size_t copy_bytes(long long rows, int cols, bool is_aligned) {
+  return is_aligned ? 0 : align_up(size_t(rows) * align_up(cols, 8) * 2, 256);
+}
+
+}  // namespace
+
+size_t expand_w4_workspace(int m, int n, int k, bool x_aligned) {
+  return kStatusBytes + copy_bytes(m, k, x_aligned) + part_bytes(m, n);
+}
+
+int expand_w4(const W4& w, const void* x, long long ldx, void* y, long long ldy, int m, void* workspace, cudaStream_t stream) {
+  ExpandParams p = {};
+  p.codes = static_cast<const uint8_t*>(w.codes);
+  p.scales = w.scales;
+  p.zeros = static_cast<const uint8_t*>(w.zeros);
+  p.rows = w.n;
+  p.cols = m;
+  p.depth = w.k;
+  p.steps = 2 * w4_blocks(w.k);
+  p.out = y;
+  p.ldo = ldy;
+  p.wait_ns = kWaitNs;
+  char* ws = static_cast<char*>(workspace);
+  p.status = reinterpret_cast<int*>(ws);
+  ws += kStatusBytes;
+  int rc;
+  if (!tma_rows(x, ldx)) {
+    const int cols = static_cast<int>(align_up(w.k, 8));
+    if ((rc = tc::copy_rows_16bit(ws, cols, x, m, w.k, ldx, stream))) return rc;
+    x = ws;
+    ldx = cols;
+    ws += copy_bytes(m, w.k, false);
+  }
+  p.part = reinterpret_cast<float*>(ws);
+  const int pairs = place(p, pairs_of_device());
+  if (!pairs) return kErrNotSupported;
+  if ((rc = tc::map_rows_16bit(&p.right, x, m, w.k, ldx, p.bn / 2))) return rc;
+  return w.dtype == kF16 ? run_w4<__half>(p, w.group, pairs, stream) : run_w4<__nv_bfloat16>(p, w.group, pairs, stream);
+}
+
+size_t expand_act8_workspace(int m, int n, int k, bool dy_aligned) {
+  return kStatusBytes + copy_bytes(m, n, dy_aligned) + part_bytes(k, n);
+}
+
+int expand_act8(const Act8& a, const void* dy, long long lddy, bool out_f32, const void* base, long long ldbase, void* dw,
+                long long lddw, int n, void* workspace, cudaStream_t stream) {
+  ExpandParams p = {};
+  p.codes = static_cast<const uint8_t*>(a.codes);
+  p.exps = static_cast<const uint8_t*>(a.exps);
+  p.pitch = a.pitch;
+  p.exp_pitch = a.exp_pitch;
+  p.rows = a.k;
+  p.cols = n;
+  p.depth = a.m;
+  p.steps = ceil_div(a.m, kStep);
+  p.out = dw;
+  p.ldo = lddw;
+  p.base = base;
+  p.ldbase = ldbase;
+  p.out_f32 = out_f32;
+  p.wait_ns = kWaitNs;
+  char* ws = static_cast<char*>(workspace);
+  p.status = reinterpret_cast<int*>(ws);
+  ws += kStatusBytes;
+  int pairs = 0;
+  if (p.steps > 0) {
+    int rc;
+    if (!tma_rows(dy, lddy)) {
+      const int cols = static_cast<int>(align_up(n, 8));
+      if ((rc = tc::copy_rows_16bit(ws, cols, dy, a.m, n, lddy, stream))) return rc;
+      dy = ws;
+      lddy = cols;
+      ws += copy_bytes(a.m, n, false);
+    }
+    p.part = reinterpret_cast<float*>(ws);
+    if (!(pairs = place(p, pairs_of_device()))) return kErrNotSupported;
+    if ((rc = tc::map_rows_16bit(&p.right, dy, a.m, n, lddy, kStep))) return rc;
+  }
+  return a.dtype == kF16 ? run_act8<__half>(p, pairs, stream) : run_act8<__nv_bfloat16>(p, pairs, stream);
+}
+
+}  // namespace lowbit
+}  // namespace sb200

@@ -1,0 +1,562 @@
+// Products whose left operand is held in few bits and is expanded to 16 bits on its way to the tensor cores:
+//     W4    y^T = W x^T      left rows = outputs of the layer,  right columns = rows of x,   reduction = inputs
+//     ACT8  dW  = X^T dY     left rows = channels,              right columns = columns of dY, reduction = tokens
+//
+// A pair of CTAs computes a tile of 256 left rows x `bn` columns with tcgen05.mma.cta_group::2.  Per step of 64 of the
+// reduction each CTA's eight converter warps expand the 128 x 64 values of its own left rows from registers (loaded a few
+// steps ahead) into the swizzled shared-memory tile that the tensor cores read; TMA brings the CTA's half of the right
+// operand.  The expansion therefore costs no pass over memory: the operand travels in 4 or 8 bits and is never written
+// out in 16.
+//   W4    the tile is K-major (a word of the format is the 16 bytes of eight neighbouring inputs); weights are rounded to 16
+//         bits once, code - zero is exact before.
+//   ACT8  the tile is MN-major (tokens are rows in memory, channels run along a row); every value is exact in 16 bits.
+//
+// Sums.  The tensor cores chop when they add to an accumulator (measured on B200, exact products of normal values:
+// relative error 3.4e-5 after 2048 additions, 1.5e-6 after 128, growing with their number), which is too coarse for a gradient kept in
+// fp32.  So an accumulator in tensor memory takes kSubSteps steps only; then eight epilogue warps add it to the tile's
+// running sum in their registers, rounding to nearest, while the MMAs go on in the other accumulator.  With 128 sums a thread
+// the epilogue warps need more registers than the others can spare at launch: the warps trade them (setmaxnreg).
+#pragma once
+#include <cuda.h>
+
+#include "lowbit_format.cuh"
+#include "ptx.cuh"
+
+namespace sb200 {
+namespace lowbit {
+
+enum ExpandKind { kExpandW4 = 0, kExpandAct8 = 1 };
+
+struct ExpandParams {
+  CUtensorMap right;        // x [tokens][inputs] (W4) or dY [tokens][columns] (ACT8)
+  const uint8_t* codes;
+  const void* scales;       // W4
+  const uint8_t* zeros;     // W4, or null
+  const uint8_t* exps;      // ACT8
+  long long pitch, exp_pitch;
+  int rows, cols;           // of the result: left rows, right columns
+  int depth;                // length of the reduction
+  int bn;                   // columns of a tile, a multiple of 32 up to 256
+  int tiles_r, tiles_c;
+  int steps;                // steps of 64 of the reduction
+  int slices;               // parts of the reduction; more than one: parts are written to `part` in fp32
+  void* out;                // ACT8: [rows][ldo]; W4: [cols][ldo] (transposed)
+  long long ldo;
+  const void* base;         // ACT8, or null
+  long long ldbase;
+  int out_f32;
+  float* part;              // [slices][the result's shape, packed]
+  int* status;
+  unsigned long long wait_ns;
+};
+
+constexpr int kPairRows = 256, kCtaRows = 128, kStep = 64, kMaxCols = 256;
+constexpr int kSubSteps = 8;       // steps that one accumulator takes: 32 additions
+constexpr int kStages = 6;
+constexpr int kLeftBytes = kCtaRows * 128;           // 128 x 64 values of 16 bits
+constexpr int kRightBytes = (kMaxCols / 2) * 128;    // at most 128 columns x 64
+constexpr int kStageBytes = kLeftBytes + kRightBytes;
+constexpr int kRightBlock = 64 * 128;                // 64 columns x 64 tokens (MN-major)
+constexpr int kExpandThreads = 640;  // warpgroups: 0 = producers and MMA, 1-2 = epilogue, 3-4 = converters
+constexpr int kEpilogueWarps = 8, kConvertWarps = 8;
+constexpr int kTransposeBytes = 32 * 32 * 4;         // per epilogue warp
+constexpr int kExpandSmem = 1024 + kStages * kStageBytes + kEpilogueWarps * kTransposeBytes + 1024;
+// registers a thread: at launch (all threads), and after the trade; the sum of what the warpgroups take must not
+// exceed what the block was launched with (the host checks the kernel's count before a launch)
+constexpr int kRegsLaunch = 96, kRegsControl = 24, kRegsEpilogue = 160, kRegsConvert = 64;
+static_assert(128 * kRegsControl + 256 * kRegsEpilogue + 256 * kRegsConvert <= kExpandThreads * kRegsLaunch, "register trade");
+static_assert(kExpandSmem <= 232448, "shared memory of a CTA");
+
+template <int N> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+template <typename T> struct Half;
+template <> struct Half<__half> {
+  static constexpr uint32_t fmt = 0;              // of the instruction descriptor
+  static constexpr uint32_t magic = 0x64006400u;  // 1024, last bit 1
+  typedef __half2 two;
+};
+template <> struct Half<__nv_bfloat16> {
+  static constexpr uint32_t fmt = 1;
+  static constexpr uint32_t magic = 0x43004300u;  // 128, last bit 1
+  typedef __nv_bfloat162 two;
+};
+template <typename T> __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
+  typedef typename Half<T>::two H;
+  const H r = __hsub2(*reinterpret_cast<const H*>(&a), *reinterpret_cast<const H*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+template <typename T> __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+  typedef typename Half<T>::two H;
+  const H r = __hmul2(*reinterpret_cast<const H*>(&a), *reinterpret_cast<const H*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// Eight codes of a word to eight weights, in the order of the inputs.  bias = magic + zero, scale twice.
+template <typename T>
+__device__ __forceinline__ uint4 expand_w4(uint32_t w, uint32_t bias, uint32_t scale) {
+  uint4 r;
+  r.x = mul2<T>(sub2<T>((w & 0x000f000fu) | Half<T>::magic, bias), scale);
+  r.y = mul2<T>(sub2<T>(((w >> 4) & 0x000f000fu) | Half<T>::magic, bias), scale);
+  r.z = mul2<T>(sub2<T>(((w >> 8) & 0x000f000fu) | Half<T>::magic, bias), scale);
+  r.w = mul2<T>(sub2<T>(((w >> 12) & 0x000f000fu) | Half<T>::magic, bias), scale);
+  return r;
+}
+
+// Two bytes (sign, 7 bits of magnitude) to two values.
+//   bf16  the magnitude is OR-ed under the exponent of 2^(e + 7), where its last bit is worth 2^e: the number is
+//         +-(2^(e+7) + magnitude 2^e), and subtracting its own leading term leaves the value.  `e` holds that exponent's
+//         bits twice; all ones (a block that reads as NaN) gives infinity - infinity or NaN.
+//   f16   the magnitude under the exponent of 1024 in the same way, then a product with 2^e (`s`), which is exact.
+template <typename T> struct Act8Step;
+template <> struct Act8Step<__nv_bfloat16> {
+  uint32_t e;
+  __device__ __forceinline__ explicit Act8Step(uint32_t exponent) {
+    const uint32_t field = exponent + 7u > 255u ? 255u : exponent + 7u;
+    e = (field << 7) | (field << 23);
+  }
+  __device__ __forceinline__ uint32_t two(uint32_t bytes_twice) const {
+    const uint32_t p = (bytes_twice & 0x807f807fu) | e;
+    return sub2<__nv_bfloat16>(p, p & 0xff80ff80u);
+  }
+};
+template <> struct Act8Step<__half> {
+  uint32_t s;
+  __device__ __forceinline__ explicit Act8Step(uint32_t exponent) {
+    const __half2 h = __float2half2_rn(act8_step(static_cast<int>(exponent)));
+    s = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  __device__ __forceinline__ uint32_t two(uint32_t bytes_twice) const {
+    const uint32_t p = (bytes_twice & 0x807f807fu) | 0x64006400u;
+    return mul2<__half>(sub2<__half>(p, p & 0xfc00fc00u), s);
+  }
+};
+template <typename T>
+__device__ __forceinline__ uint4 expand_act8(uint32_t w0, uint32_t w1, const Act8Step<T>& st) {  // eight channels
+  uint4 r;
+  r.x = st.two(__byte_perm(w0, 0, 0x1100));
+  r.y = st.two(__byte_perm(w0, 0, 0x3322));
+  r.z = st.two(__byte_perm(w1, 0, 0x1100));
+  r.w = st.two(__byte_perm(w1, 0, 0x3322));
+  return r;
+}
+
+struct ExpandUnit {
+  int row0, col0;  // of the pair's tile
+  int k0, k1;      // steps
+  int slice;
+};
+
+// Units in order: all tiles of a slice, tiles in bands of 16 tile rows, down the rows of a band first, so that the tiles that
+// run together share both operands' panels in L2.
+__device__ __forceinline__ ExpandUnit expand_unit(const ExpandParams& p, int u) {
+  constexpr int kBand = 16;
+  const int tiles = p.tiles_r * p.tiles_c;
+  ExpandUnit r;
+  r.slice = u / tiles;
+  int t = u - r.slice * tiles;
+  const int band = t / (kBand * p.tiles_c);
+  t -= band * kBand * p.tiles_c;
+  const int high = min(kBand, p.tiles_r - band * kBand);
+  r.row0 = (band * kBand + t % high) * kPairRows;
+  r.col0 = (t / high) * p.bn;
+  // slices are cut at whole pairs of steps (a tile of the 4-bit format is two)
+  const long long pairs = (p.steps + 1) / 2;
+  r.k0 = static_cast<int>(2 * (pairs * r.slice / p.slices));
+  r.k1 = min(p.steps, static_cast<int>(2 * (pairs * (r.slice + 1) / p.slices)));
+  return r;
+}
+
+__device__ __forceinline__ void give_up(const ExpandParams& p, volatile int* abort_flag, int code) {
+  *abort_flag = 1;
+  atomicCAS(p.status, 0, code);
+}
+
+template <typename T, int KIND, int PER>
+__global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const __grid_constant__ ExpandParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* after = smem + kStages * kStageBytes;
+  float* transpose = reinterpret_cast<float*>(after);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(after + kEpilogueWarps * kTransposeBytes);
+  uint64_t* empty_bar = full_bar + kStages;
+  uint64_t* slot_full = empty_bar + kStages;
+  uint64_t* slot_free = slot_full + 2;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(slot_free + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = ptx::cluster_ctarank();  // 0 = leader
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int units = p.tiles_r * p.tiles_c * p.slices;
+
+  if (threadIdx.x == 0) {
+    *abort_flag = 0;
+    // all blocks of the grid are resident, so this store comes long before any bounded wait can run out
+    if (blockIdx.x == 0) *p.status = 0;
+    for (int s = 0; s < kStages; ++s) {
+      ptx::mbar_init(&full_bar[s], 1 + 2 * kConvertWarps);  // the leader's producer, the converters of both CTAs
+      ptx::mbar_init(&empty_bar[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      ptx::mbar_init(&slot_full[s], 1);
+      ptx::mbar_init(&slot_free[s], 2 * kEpilogueWarps);
+    }
+    ptx::fence_mbar_init();
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc_pair(tmem_holder, 512);
+    ptx::tmem_relinquish_pair();
+  }
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  ptx::cluster_sync_all();
+  ptx::tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_holder;
+  const int half = p.bn / 2;  // columns of the right operand that a CTA brings
+
+  if (warp < 4) {
+    regs_dec<kRegsControl>();
+    if (warp == 0 || warp == 2) {
+      // ---- TMA producers: the loads of one warp complete one after the other, so two warps take the steps in turn
+      const int boxes = KIND == kExpandW4 ? 1 : (half + 63) / 64;
+      const uint32_t bytes = 2u * (KIND == kExpandW4 ? half * 128 : boxes * kRightBlock);  // both CTAs'
+      if (warp == 0 && lane == 0) ptx::prefetch_tmap(&p.right);
+      uint32_t stage = 0, phase = 0, turn = warp >> 1;
+      bool ok = true;
+      for (int u = pair; ok && u < units; u += pairs) {
+        const ExpandUnit w = expand_unit(p, u);
+        const int col0 = w.col0 + static_cast<int>(rank) * half;
+        for (int kk = w.k0; kk < w.k1; ++kk) {
+          if (turn == 0) {
+            if (!ptx::mbar_wait_warp<false>(&empty_bar[stage], phase ^ 1u, abort_flag, p.wait_ns)) {
+              if (lane == 0) give_up(p, abort_flag, 101);
+              ok = false;
+              break;
+            }
+            if (ptx::elect_one()) {
+              if (rank == 0) ptx::mbar_arrive_expect_tx(&full_bar[stage], bytes);
+              uint8_t* to = smem + stage * kStageBytes + kLeftBytes;
+              if (KIND == kExpandW4) {
+                ptx::tma_load_2d_pair(to, &p.right, &full_bar[stage], kk * kStep, col0);
+              } else {
+                for (int b = 0; b < boxes; ++b)
+                  ptx::tma_load_2d_pair(to + b * kRightBlock, &p.right, &full_bar[stage], col0 + b * 64, kk * kStep);
+              }
+            }
+            __syncwarp();
+          }
+          turn ^= 1u;
+          if (++stage == kStages) { stage = 0; phase ^= 1u; }
+        }
+      }
+    } else if (warp == 1 && rank == 0) {
+      // ---- MMA issuer (leader)
+      const uint32_t idesc = (1u << 4) | (Half<T>::fmt << 7) | (Half<T>::fmt << 10) |
+                             (KIND == kExpandAct8 ? (1u << 15) | (1u << 16) : 0u) |
+                             (static_cast<uint32_t>(p.bn >> 3) << 17) | (static_cast<uint32_t>(kPairRows >> 4) << 24);
+      const uint32_t lbo = KIND == kExpandW4 ? 16 : kRightBlock;
+      const uint32_t advance = (KIND == kExpandW4 ? 32 : 16 * 128) >> 4;  // 16 of the reduction
+      const uint64_t a0 = ptx::umma_desc_sw128(ptx::smem_u32(smem), lbo, 1024);
+      const uint64_t b0 = ptx::umma_desc_sw128(ptx::smem_u32(smem) + kLeftBytes, lbo, 1024);
+      uint32_t stage = 0, phase = 0, slot = 0, free_bits = 0;
+      bool ok = true;
+      for (int u = pair; ok && u < units; u += pairs) {
+        const ExpandUnit w = expand_unit(p, u);
+        int sub = 0;
+        for (int kk = w.k0; kk < w.k1; ++kk) {
+          if (sub == 0) {
+            if (!ptx::mbar_wait_warp<true>(&slot_free[slot], ((free_bits >> slot) & 1u) ^ 1u, abort_flag, p.wait_ns)) {
+              if (lane == 0) give_up(p, abort_flag, 102);
+              ok = false;
+              break;
+            }
+            free_bits ^= 1u << slot;
+            ptx::tc_fence_after_sync();
+          }
+          if (!ptx::mbar_wait_warp<true>(&full_bar[stage], phase, abort_flag, p.wait_ns)) {
+            if (lane == 0) give_up(p, abort_flag, 102);
+            ok = false;
+            break;
+          }
+          const uint64_t as = a0 + ((stage * kStageBytes) >> 4), bs = b0 + ((stage * kStageBytes) >> 4);
+          const bool last = sub == kSubSteps - 1 || kk == w.k1 - 1;
+          if (ptx::elect_one()) {
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+              ptx::umma_f16_pair(tmem_base + slot * kMaxCols, as + ks * advance, bs + ks * advance, idesc, (sub | ks) ? 1u : 0u);
+            ptx::umma_commit_pair(&empty_bar[stage], 3);
+            if (last) ptx::umma_commit_pair(&slot_full[slot], 3);
+          }
+          __syncwarp();
+          if (++stage == kStages) { stage = 0; phase ^= 1u; }
+          ++sub;
+          if (last) { sub = 0; slot ^= 1u; }
+        }
+      }
+    }
+  } else if (warp < 12) {
+    // ---- epilogue: warp = 32 rows (of its lane quarter) x half of the tile's columns
+    regs_inc<kRegsEpilogue>();
+    const int e = warp - 4, quarter = warp & 3, side = e >> 2;
+    float* swap = transpose + e * (kTransposeBytes / 4);
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    uint32_t slot = 0, full_bits = 0;
+    bool ok = true;
+    for (int u = pair; ok && u < units; u += pairs) {
+      const ExpandUnit w = expand_unit(p, u);
+      float sum[128];
+#pragma unroll
+      for (int i = 0; i < 128; ++i) sum[i] = 0.f;
+      for (int kk = w.k0; kk < w.k1; kk += kSubSteps) {
+        if (!ptx::mbar_wait_warp<true>(&slot_full[slot], (full_bits >> slot) & 1u, abort_flag, p.wait_ns)) {
+          if (lane == 0) give_up(p, abort_flag, 103);
+          ok = false;
+          break;
+        }
+        full_bits ^= 1u << slot;
+        ptx::tc_fence_after_sync();
+        const uint32_t from = tmem_base + lanes + slot * kMaxCols + side * half;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          if (c * 16 < half) {
+            uint32_t r[16];
+            tmem_ld_32x16(from + c * 16, r);
+            ptx::tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sum[c * 16 + i] += __uint_as_float(r[i]);
+          }
+        }
+        ptx::tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive_cluster(&slot_free[slot], 0);
+        slot ^= 1u;
+      }
+      if (!ok) break;
+      const int row0 = w.row0 + static_cast<int>(rank) * kCtaRows + quarter * 32;
+      const int col0 = w.col0 + side * half;
+      if (KIND == kExpandW4) {
+        // a column of the tile is a row of y: 32 lanes store 32 neighbours
+        const int row = row0 + lane;
+        float* part = p.part + static_cast<long long>(w.slice) * p.rows * p.cols;
+#pragma unroll
+        for (int c = 0; c < 128; ++c) {
+          if (c < half && col0 + c < p.cols && row < p.rows) {
+            if (p.slices > 1) part[static_cast<long long>(col0 + c) * p.rows + row] = sum[c];
+            else static_cast<T*>(p.out)[(col0 + c) * p.ldo + row] = from_f32<T>(sum[c]);
+          }
+        }
+      } else {
+        float* part = p.part + static_cast<long long>(w.slice) * p.rows * p.cols;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          if (c * 32 < half) {
+            // 32 x 32 values change places between lanes and registers, so that a row leaves as neighbours
+#pragma unroll
+            for (int i = 0; i < 32; ++i) swap[lane * 32 + (i ^ lane)] = sum[c * 32 + i];
+            __syncwarp();
+            const int col = col0 + c * 32 + lane;
+            const bool in = c * 32 + lane < half && col < p.cols;
+#pragma unroll 8
+            for (int i = 0; i < 32; ++i) {
+              const long long row = row0 + i;
+              if (in && row < p.rows) {
+                float v = swap[i * 32 + (lane ^ i)];
+                if (p.slices > 1) {
+                  part[row * p.cols + col] = v;
+                } else if (p.out_f32) {
+                  if (p.base) v += static_cast<const float*>(p.base)[row * p.ldbase + col];
+                  static_cast<float*>(p.out)[row * p.ldo + col] = v;
+                } else {
+                  if (p.base) v += to_f32(static_cast<const T*>(p.base)[row * p.ldbase + col]);
+                  static_cast<T*>(p.out)[row * p.ldo + col] = from_f32<T>(v);
+                }
+              }
+            }
+            __syncwarp();
+          }
+        }
+      }
+    }
+  } else {
+    // ---- converters
+    regs_dec<kRegsConvert>();
+    const int tid = threadIdx.x - 12 * 32;
+    const uint32_t left = ptx::smem_u32(smem);
+    uint32_t stage = 0, phase = 0;
+    bool ok = true;
+    auto acquire = [&]() -> bool {  // the stage's previous contents have been read
+      if (!ptx::mbar_wait_warp<true>(&empty_bar[stage], phase ^ 1u, abort_flag, p.wait_ns)) {
+        if (lane == 0) give_up(p, abort_flag, 104);
+        return false;
+      }
+      return true;
+    };
+    auto publish = [&]() {
+      ptx::fence_proxy_async_all();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive_cluster(&full_bar[stage], 0);
+      if (++stage == kStages) { stage = 0; phase ^= 1u; }
+    };
+    for (int u = pair; ok && u < units; u += pairs) {
+      const ExpandUnit w = expand_unit(p, u);
+      const int row0 = w.row0 + static_cast<int>(rank) * kCtaRows;
+      if (KIND == kExpandW4) {
+        // Two pieces a thread and tile of 128 inputs: 16 bytes (four words) of a row.  Words 0 and 1 belong to the first
+        // step, 2 and 3 to the second.  Lanes of odd rows store the second word of a step first, so that eight
+        // lanes always hit eight different 16-byte columns of the swizzled tile.
+        struct Raw { uint4 c; uint32_t s[(PER + 1) / 2]; uint32_t z; } raw[2][2];
+        const int blocks = w4_blocks(p.depth), tiles = w4_row_tiles(p.rows);
+        const int g = lane >> 2, t = lane & 3;
+        auto load = [&](int b, int buf) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int tile = row0 / kW4Rows + (tid >> 6) + 4 * i;
+            Raw& q = raw[buf][i];
+            q.c = make_uint4(0, 0, 0, 0);
+            q.z = 0;
+#pragma unroll
+            for (int j = 0; j < (PER + 1) / 2; ++j) q.s[j] = 0;
+            if (tile < tiles && 2 * b < w.k1) {
+              const long long at = static_cast<long long>(tile) * blocks + b;
+              q.c = ptx::ldg_nc_v4(p.codes + at * kW4TileBytes + (tid & 63) * 16);
+              const long long entry = (at * kW4Rows + 8 * ((tid >> 5) & 1) + g) * PER;
+              const uint16_t* s = static_cast<const uint16_t*>(p.scales) + entry;
+              if (PER == 1) q.s[0] = __ldg(s);
+              if (PER == 2) q.s[0] = __ldg(reinterpret_cast<const uint32_t*>(s));
+              if (PER == 4) {
+                const uint2 v = __ldg(reinterpret_cast<const uint2*>(s));
+                q.s[0] = v.x;
+                q.s[PER / 4] = v.y;
+              }
+              q.z = 0x08080808u;
+              if (p.zeros) {
+                if (PER == 1) q.z = __ldg(p.zeros + entry);
+                if (PER == 2) q.z = __ldg(reinterpret_cast<const uint16_t*>(p.zeros + entry));
+                if (PER == 4) q.z = __ldg(reinterpret_cast<const uint32_t*>(p.zeros + entry));
+              }
+            }
+          }
+        };
+        load(w.k0 / 2, 0);
+        load(w.k0 / 2 + 1, 1);
+        const int odd = g & 1;
+        for (int b = w.k0 / 2; ok && 2 * b < w.k1; b += 2) {
+#pragma unroll
+          for (int buf = 0; buf < 2; ++buf) {
+            if (2 * (b + buf) >= w.k1) break;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (2 * (b + buf) + h >= w.k1) break;
+              if (!acquire()) { ok = false; break; }
+              const uint32_t to = left + stage * kStageBytes;
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const Raw& q = raw[buf][i];
+                const int row = ((tid >> 6) + 4 * i) * kW4Rows + 8 * ((tid >> 5) & 1) + g;
+                uint4 v[2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                  const int word = 2 * h + j, group = word * PER / 4;
+                  const uint32_t z = (q.z >> (8 * group)) & 255u;
+                  const uint32_t s = (q.s[group / 2] >> (16 * (group & 1))) & 0xffffu;
+                  v[j] = expand_w4<T>((&q.c.x)[word], Half<T>::magic + (z | (z << 16)), s | (s << 16));
+                }
+                const uint4 a = odd ? v[1] : v[0], c = odd ? v[0] : v[1];
+                ptx::sts_v4(to + row * 128 + (((4 * odd + t) ^ (row & 7)) << 4), a);
+                ptx::sts_v4(to + row * 128 + (((4 * (1 - odd) + t) ^ (row & 7)) << 4), c);
+              }
+              publish();
+            }
+            if (!ok) break;
+            load(b + buf + 2, buf);
+          }
+        }
+      } else {
+        // Two pieces a thread and step: 16 channels of a token.  Eight neighbouring lanes hold a token's 128 channels; those
+        // of the second 64 store their second half first, which keeps eight lanes on eight different 16-byte columns.
+        struct Raw { uint4 c; uint32_t e; } raw[3][2];
+        const int piece = tid & 7, token = tid >> 3;
+        const int channel = row0 + piece * 16;
+        const bool in = channel < p.rows;
+        auto load = [&](int kk, int buf) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const long long tok = static_cast<long long>(kk) * kStep + token + 32 * i;
+            Raw& q = raw[buf][i];
+            q.c = make_uint4(0, 0, 0, 0);
+            q.e = 127;
+            if (in && kk < w.k1 && tok < p.depth) {
+              q.c = ptx::ldg_nc_v4(p.codes + tok * p.pitch + channel);
+              q.e = __ldg(p.exps + tok * p.exp_pitch + channel / kActBlock);
+            }
+          }
+        };
+#pragma unroll
+        for (int a = 0; a < 3; ++a) load(w.k0 + a, a);
+        const int second = piece >> 2;
+        for (int k0 = w.k0; ok && k0 < w.k1; k0 += 3) {
+#pragma unroll
+          for (int buf = 0; buf < 3; ++buf) {
+            const int kk = k0 + buf;
+            if (kk >= w.k1) break;
+            if (!acquire()) { ok = false; break; }
+            const uint32_t to = left + stage * kStageBytes + second * kRightBlock;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const Raw& q = raw[buf][i];
+              const int r = token + 32 * i;
+              const Act8Step<T> step(q.e);
+              const uint4 lo = expand_act8<T>(q.c.x, q.c.y, step), hi = expand_act8<T>(q.c.z, q.c.w, step);
+              const int c = 2 * (piece & 3);
+              ptx::sts_v4(to + r * 128 + (((c + second) ^ (r & 7)) << 4), second ? hi : lo);
+              ptx::sts_v4(to + r * 128 + (((c + 1 - second) ^ (r & 7)) << 4), second ? lo : hi);
+            }
+            publish();
+            load(kk + 3, buf);
+          }
+        }
+      }
+    }
+  }
+
+  // ---- teardown
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  if (*abort_flag) {  // copies in flight land before the shared memory goes
+    const uint64_t t0 = ptx::globaltimer_ns();
+    while (ptx::globaltimer_ns() - t0 < 2000000ull) __nanosleep(1000);
+  }
+  ptx::cluster_sync_all();
+  if (warp == 1) {
+    ptx::tc_fence_after_sync();
+    ptx::tmem_dealloc_pair(tmem_base, 512);
+  }
+}
+
+// out[r][c] = base[r][c] + the slices' parts in order.
+template <typename Out>
+__global__ void __launch_bounds__(256) join_slices_kernel(const float* __restrict__ part, int slices, int rows, int cols, Out* out,
+                                                          long long ldo, const Out* base, long long ldbase) {
+  const long long total = static_cast<long long>(rows) * cols;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+    const long long r = i / cols, c = i - r * cols;
+    float v = 0.f;
+    for (int s = 0; s < slices; ++s) v += part[s * total + i];
+    if (base) v += to_f32(base[r * ldbase + c]);
+    out[r * ldo + c] = from_f32<Out>(v);
+  }
+}
+
+}  // namespace lowbit
+}  // namespace sb200

@@ -1,5 +1,7 @@
 // Arguments of the products with an operand held in few bits (w4.cu, act8.cu).
 #pragma once
+#include <stdint.h>
+
 #include "sw_host.h"
 
 namespace sb200 {
@@ -23,6 +25,19 @@ struct Act8 {
   const void* exps;
   long long exp_pitch;
 };
+
+inline bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+// Rows of a 16-bit matrix that TMA can read as they are.
+inline bool tma_rows(const void* p, long long ld) { return aligned(p, 16) && ld % 8 == 0; }
+
+// The products on the tensor cores (expand_product.cu).  Workspace: a status word, a copy of the 16-bit operand where its
+// rows are not aligned, and the parts of a divided reduction.  The bytes asked for grow with m, so that a workspace serves
+// every smaller m.
+size_t expand_w4_workspace(int m, int n, int k, bool x_aligned);
+int expand_w4(const W4& w, const void* x, long long ldx, void* y, long long ldy, int m, void* workspace, cudaStream_t stream);
+size_t expand_act8_workspace(int m, int n, int k, bool dy_aligned);
+int expand_act8(const Act8& a, const void* dy, long long lddy, bool out_f32, const void* base, long long ldbase, void* dw,
+                long long lddw, int n, void* workspace, cudaStream_t stream);
 
 }  // namespace lowbit
 }  // namespace sb200

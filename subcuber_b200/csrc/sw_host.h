@@ -95,6 +95,11 @@ int launches_per_run(const GemmArgs& args);
 // the round-robin deal, tile, part, parts, k0, k1, hand-off slot, split slot) in list order, returns the number of
 // units and the worker count.  Host arithmetic only (tests read the plan through this).
 int deal_units(const GemmArgs& args, int sms, int* out, int max_units, int* workers);
+// Tensor map of a row-major matrix of 16-bit elements (`ld` elements from row to row, rows on 16 bytes) for boxes of 64
+// columns x `box_rows` rows with the 128-byte swizzle; elements outside read as zero.  `map` points to a CUtensorMap.
+int map_rows_16bit(void* map, const void* ptr, long long rows, long long cols, long long ld, int box_rows);
+// dst (rows x cols_d, packed, cols_d a multiple of 8) = src (rows x cols, leading dimension ld) of 16-bit elements, zeros behind.
+int copy_rows_16bit(void* dst, int cols_d, const void* src, int rows, int cols, long long ld, cudaStream_t stream);
 }  // namespace tc
 
 // fp64 path (dgemm_sw.cu): DMMA kernels, same four calls.

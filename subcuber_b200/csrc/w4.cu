@@ -5,7 +5,6 @@
 #include "lowbit_format.cuh"
 #include "lowbit_host.h"
 #include "per_device.h"
-#include "simple_product.cuh"
 #include "w4_rows.cuh"
 
 namespace sb200 {
@@ -179,29 +178,10 @@ __global__ void __launch_bounds__(kThreads) w4_dequantize_kernel(const uint8_t* 
   }
 }
 
-template <typename T>
-struct W4Right {  // W^T as the right operand of a product: (input, row)
-  const uint8_t* codes;
-  const T* scales;
-  const uint8_t* zeros;
-  int n, k, G, blocks;
-  __device__ float operator()(int kk, int row) const {
-    if (kk >= k || row >= n) return 0.f;
-    const int in = kk % kW4Block;
-    const uint32_t word = *reinterpret_cast<const uint32_t*>(
-        codes + (static_cast<long long>(row / kW4Rows) * blocks + kk / kW4Block) * kW4TileBytes + word_offset(row % kW4Rows, in / 8));
-    const float q = static_cast<float>((word >> (4 * w4_nibble(in % 8))) & 15u);
-    const long long at = w4_table_at(row, kk / G, blocks, G);
-    return (q - (zeros ? static_cast<float>(zeros[at]) : 8.f)) * to_f32(scales[at]);
-  }
-};
-
-inline bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
-
 template <typename T, int PER>
 int rows_product(const void* x, long long ldx, const W4& w, void* y, long long ldy, int m, cudaStream_t stream) {
   RowsParams p{x, ldx, static_cast<const uint8_t*>(w.codes), w.scales, static_cast<const uint8_t*>(w.zeros), y, ldy,
-               m, w.n, w.k, w4_blocks(w.k), aligned(x, 16) && ldx % 8 == 0};
+               m, w.n, w.k, w4_blocks(w.k), tma_rows(x, ldx)};
   // one row tile to a warp where that is at most two blocks an SM, else two (8192 x 8192, one row: 16.6 us, 19.9 with one)
   if (m <= 8)
     return w4_row_tiles(w.n) <= 2 * sm_count_of_current_device() ? launch_rows<T, PER, 1, 1, 2>(p, 1, stream)
@@ -211,17 +191,13 @@ int rows_product(const void* x, long long ldx, const W4& w, void* y, long long l
 }
 
 template <typename T>
-int product(const void* x, long long ldx, const W4& w, void* y, long long ldy, int m, cudaStream_t stream) {
-  if (m <= 64) {
-    if (w.group == 32) return rows_product<T, 4>(x, ldx, w, y, ldy, m, stream);
-    if (w.group == 64) return rows_product<T, 2>(x, ldx, w, y, ldy, m, stream);
-    return rows_product<T, 1>(x, ldx, w, y, ldy, m, stream);
-  }
-  const DenseLeft<T> left{static_cast<const T*>(x), ldx, m, w.k};
-  const W4Right<T> right{static_cast<const uint8_t*>(w.codes), static_cast<const T*>(w.scales),
-                         static_cast<const uint8_t*>(w.zeros), w.n, w.k, w.group, w4_blocks(w.k)};
-  return simple_product<T>(left, right, static_cast<T*>(y), ldy, static_cast<const T*>(nullptr), 0, m, w.n, w.k, stream);
+int rows_product_any(const void* x, long long ldx, const W4& w, void* y, long long ldy, int m, cudaStream_t stream) {
+  if (w.group == 32) return rows_product<T, 4>(x, ldx, w, y, ldy, m, stream);
+  if (w.group == 64) return rows_product<T, 2>(x, ldx, w, y, ldy, m, stream);
+  return rows_product<T, 1>(x, ldx, w, y, ldy, m, stream);
 }
+
+constexpr int kFewRows = 32;
 
 int check(const W4& w) {
   if (w.dtype != kF16 && w.dtype != kBF16) return kErrNotSupported;
@@ -325,24 +301,28 @@ extern "C" int sb200_w4_dequantize(int dtype, const void* codes, const void* sca
                               : sb200::lowbit::dequantize<__nv_bfloat16>(w, out, ldo, s);
 }
 
-extern "C" size_t sb200_w4_gemm_workspace_bytes(int dtype, int m, int n, int k, int group) {
-  (void)dtype; (void)m; (void)n; (void)k; (void)group;
-  return 256;
+extern "C" size_t sb200_w4_gemm_workspace_bytes(int dtype, int m, int n, int k, int group, int x_aligned) {
+  (void)dtype;
+  (void)group;
+  if (m <= sb200::lowbit::kFewRows || n <= 0 || k <= 0) return 256;
+  return sb200::lowbit::expand_w4_workspace(m, n, k, x_aligned != 0);
 }
 
 extern "C" int sb200_w4_gemm(int dtype, const void* x, long long ldx, const void* codes, const void* scales,
                              const void* zeros, void* y, long long ldy, int m, int n, int k, int group, void* workspace,
                              size_t workspace_bytes, sb200_stream_t stream) {
+  using namespace sb200::lowbit;
   const W4 w{static_cast<sb200::DType>(dtype), n, k, group, codes, scales, zeros};
-  if (int rc = sb200::lowbit::check(w)) return rc;
+  if (int rc = check(w)) return rc;
   if (m < 0 || ldx < k || ldy < n) return SB200_ERR_INVALID_PROBLEM;
   if (m == 0) return SB200_OK;
   if (!x || !y) return SB200_ERR_INVALID_PROBLEM;
-  if (!sb200::lowbit::aligned(x, 2) || !sb200::lowbit::aligned(y, 2)) return SB200_ERR_MISALIGNED_OPERAND;
-  if (!workspace || workspace_bytes < sb200_w4_gemm_workspace_bytes(dtype, m, n, k, group) ||
-      !sb200::lowbit::aligned(workspace, 256))
+  if (!aligned(x, 2) || !aligned(y, 2)) return SB200_ERR_MISALIGNED_OPERAND;
+  if (!workspace || !aligned(workspace, 256) ||
+      workspace_bytes < sb200_w4_gemm_workspace_bytes(dtype, m, n, k, group, tma_rows(x, ldx)))
     return SB200_ERR_WORKSPACE_NULL;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return dtype == sb200::kF16 ? sb200::lowbit::product<__half>(x, ldx, w, y, ldy, m, s)
-                              : sb200::lowbit::product<__nv_bfloat16>(x, ldx, w, y, ldy, m, s);
+  if (m > kFewRows) return expand_w4(w, x, ldx, y, ldy, m, workspace, s);
+  return dtype == sb200::kF16 ? rows_product_any<__half>(x, ldx, w, y, ldy, m, s)
+                              : rows_product_any<__nv_bfloat16>(x, ldx, w, y, ldy, m, s);
 }

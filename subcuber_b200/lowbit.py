@@ -77,10 +77,18 @@ def _call(what: str, fn, device: torch.device, *args) -> None:
 
 
 class _Workspace:
+    def check(self) -> None:
+        """Wait for the call that used the workspace last and raise if a device-side wait gave up."""
+        with torch.cuda.device(self.buf.device):
+            rc = _lib.load().sb200_gemm_status(self.ptr, torch.cuda.current_stream(self.buf.device).cuda_stream)
+        if rc != 0:
+            raise KernelError("workspace", rc)
+
     def _allocate(self, nbytes: int, device) -> None:
         self.nbytes = nbytes
         self.buf = torch.empty(nbytes + 256, dtype=torch.uint8, device=device)
         self.ptr = self.buf.data_ptr() + (-self.buf.data_ptr()) % 256
+        self.buf[:512].zero_()   # the status word
 
 
 class WeightsW4:
@@ -163,13 +171,19 @@ def dequantize_w4(w: WeightsW4, out: Optional[torch.Tensor] = None) -> torch.Ten
     return out
 
 
-class WorkspaceW4(_Workspace):
-    """Device workspace for `gemm_w4` with up to `m` rows; for one call at a time."""
+def _tma_rows(t: torch.Tensor) -> bool:
+    return t.data_ptr() % 16 == 0 and _ld(t) % 8 == 0
 
-    def __init__(self, m: int, w: WeightsW4):
+
+class WorkspaceW4(_Workspace):
+    """Device workspace for `gemm_w4` with up to `m` rows; for one call at a time.  `aligned`: the rows of x will start on 16
+    bytes (the default expects packed rows); else there is room for a copy of x."""
+
+    def __init__(self, m: int, w: WeightsW4, aligned: Optional[bool] = None):
         lib = _lib.load()
-        with torch.cuda.device(w.device):
-            self._allocate(int(lib.sb200_w4_gemm_workspace_bytes(DTYPE_CODE[w.dtype], m, w.n, w.k, w.group)), w.device)
+        with torch.cuda.device(w.device):  # a product is cut for the device that will run it
+            self._allocate(int(lib.sb200_w4_gemm_workspace_bytes(DTYPE_CODE[w.dtype], m, w.n, w.k, w.group,
+                                                                 int(w.k % 8 == 0 if aligned is None else aligned))), w.device)
 
 
 def gemm_w4(x: torch.Tensor, w: WeightsW4, out: Optional[torch.Tensor] = None,
@@ -182,7 +196,7 @@ def gemm_w4(x: torch.Tensor, w: WeightsW4, out: Optional[torch.Tensor] = None,
     out = _output("out", out, (m, w.n), w.dtype, x.device)
     _same_device(x, w.codes, out)
     if workspace is None:
-        workspace = WorkspaceW4(m, w)
+        workspace = WorkspaceW4(m, w, _tma_rows(x))
     _call("gemm_w4", _lib.load().sb200_w4_gemm, w.device, DTYPE_CODE[w.dtype], x.data_ptr(), _ld(x), w.codes.data_ptr(),
           w.scales.data_ptr(), w._zeros_ptr, out.data_ptr(), _ld(out), m, w.n, w.k, w.group, workspace.ptr, workspace.nbytes)
     return out
@@ -237,13 +251,15 @@ def restore8(saved: Checkpoint8, out: Optional[torch.Tensor] = None) -> torch.Te
 
 
 class WorkspaceGrad8(_Workspace):
-    """Device workspace for `weight_grad8` of `saved` against n output channels; for one call at a time."""
+    """Device workspace for `weight_grad8` of `saved` against n output channels; for one call at a time.  `aligned`: the
+    rows of dy will start on 16 bytes (the default expects packed rows); else there is room for a copy of dy."""
 
-    def __init__(self, saved: Checkpoint8, n: int, out_dtype: torch.dtype = torch.float32):
+    def __init__(self, saved: Checkpoint8, n: int, out_dtype: torch.dtype = torch.float32, aligned: Optional[bool] = None):
         lib = _lib.load()
         with torch.cuda.device(saved.device):
             self._allocate(int(lib.sb200_act8_wgrad_workspace_bytes(DTYPE_CODE[saved.dtype], DTYPE_CODE[out_dtype], saved.m,
-                                                                    n, saved.k)), saved.device)
+                                                                    n, saved.k, int(n % 8 == 0 if aligned is None else aligned))),
+                           saved.device)
 
 
 def weight_grad8(saved: Checkpoint8, dy: torch.Tensor, base: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
@@ -268,7 +284,7 @@ def weight_grad8(saved: Checkpoint8, dy: torch.Tensor, base: Optional[torch.Tens
     out = _output("out", out, (saved.k, n), out_dtype, dy.device)
     _same_device(dy, saved.codes, out, base)
     if workspace is None:
-        workspace = WorkspaceGrad8(saved, n, out_dtype)
+        workspace = WorkspaceGrad8(saved, n, out_dtype, _tma_rows(dy))
     _call("weight_grad8", _lib.load().sb200_act8_wgrad, saved.device, DTYPE_CODE[saved.dtype], saved.codes.data_ptr(),
           _ld(saved.codes), saved.exponents.data_ptr(), _ld(saved.exponents), dy.data_ptr(), _ld(dy), DTYPE_CODE[out_dtype],
           base.data_ptr() if base is not None else None, _ld(base) if base is not None else n, out.data_ptr(), _ld(out),
