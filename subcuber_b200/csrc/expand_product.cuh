@@ -192,7 +192,8 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
   uint64_t* empty_bar = full_bar + kStages;
   uint64_t* slot_full = empty_bar + kStages;
   uint64_t* slot_free = slot_full + 2;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(slot_free + 2);
+  uint64_t* left_bar = slot_free + 2;  // this CTA's left tile of a stage is written
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(left_bar + kStages);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -205,7 +206,8 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
     // all blocks of the grid are resident, so this store comes long before any bounded wait can run out
     if (blockIdx.x == 0) *p.status = 0;
     for (int s = 0; s < kStages; ++s) {
-      ptx::mbar_init(&full_bar[s], 1 + 2 * kConvertWarps);  // the leader's producer, the converters of both CTAs
+      ptx::mbar_init(&full_bar[s], 2);  // the leader's producer, the peer's left tile
+      ptx::mbar_init(&left_bar[s], kConvertWarps);
       ptx::mbar_init(&empty_bar[s], 1);
     }
     for (int s = 0; s < 2; ++s) {
@@ -289,6 +291,11 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
             ok = false;
             break;
           }
+          if (!ptx::mbar_wait_warp<false>(&left_bar[stage], phase, abort_flag, p.wait_ns)) {
+            if (lane == 0) give_up(p, abort_flag, 102);
+            ok = false;
+            break;
+          }
           const uint64_t as = a0 + ((stage * kStageBytes) >> 4), bs = b0 + ((stage * kStageBytes) >> 4);
           const bool last = sub == kSubSteps - 1 || kk == w.k1 - 1;
           if (ptx::elect_one()) {
@@ -302,6 +309,25 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
           if (++stage == kStages) { stage = 0; phase ^= 1u; }
           ++sub;
           if (last) { sub = 0; slot ^= 1u; }
+        }
+      }
+    }
+    else if (warp == 3 && rank == 1) {
+      // ---- passes on to the leader that the peer's left tile is written.  The converters themselves would have to release
+      // at cluster scope, which waits for the loads that they have in flight.
+      uint32_t stage = 0, phase = 0;
+      bool ok = true;
+      for (int u = pair; ok && u < units; u += pairs) {
+        const ExpandUnit w = expand_unit(p, u);
+        for (int kk = w.k0; kk < w.k1; ++kk) {
+          if (!ptx::mbar_wait_warp<false>(&left_bar[stage], phase, abort_flag, p.wait_ns)) {
+            if (lane == 0) give_up(p, abort_flag, 104);
+            ok = false;
+            break;
+          }
+          if (lane == 0) ptx::mbar_arrive_cluster(&full_bar[stage], 0);
+          __syncwarp();
+          if (++stage == kStages) { stage = 0; phase ^= 1u; }
         }
       }
     }
@@ -396,16 +422,16 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
     uint32_t stage = 0, phase = 0;
     bool ok = true;
     auto acquire = [&]() -> bool {  // the stage's previous contents have been read
-      if (!ptx::mbar_wait_warp<true>(&empty_bar[stage], phase ^ 1u, abort_flag, p.wait_ns)) {
+      if (!ptx::mbar_wait_warp<false>(&empty_bar[stage], phase ^ 1u, abort_flag, p.wait_ns)) {
         if (lane == 0) give_up(p, abort_flag, 104);
         return false;
       }
       return true;
     };
     auto publish = [&]() {
-      ptx::fence_proxy_async_all();
+      ptx::fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive_cluster(&full_bar[stage], 0);
+      if (lane == 0) ptx::mbar_arrive(&left_bar[stage]);
       if (++stage == kStages) { stage = 0; phase ^= 1u; }
     };
     for (int u = pair; ok && u < units; u += pairs) {
