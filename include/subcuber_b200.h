@@ -293,7 +293,7 @@ int sb200_peer_wait(int* const* local_flags, int count, int value, unsigned wait
  *     W[n][k] = scale(n, k / G) * (code[n][k] - zero(n, k / G)),   code and zero in 0..15, zero = 8 where zeros == NULL
  * codes (16-byte aligned, sb200_w4_codes_bytes(n, k) bytes) are tiles of 16 outputs x 128 inputs, 1 KiB each, along the inputs
  * first: bytes 512 h + 16 (4 g + t) + 4 j of a tile hold the 32-bit word of output 8 h + g and inputs 32 j + 8 t + i, i = 0..7,
- * input i in nibble (i >> 1) + 4 (i & 1).  scales (in the 16-bit type `dtype`, 8-byte aligned) and zeros (bytes, 4-byte aligned)
+ * input i in nibble (i >> 1) + 4 (i & 1).  scales (in the 16-bit type `dtype`) and zeros (bytes), both 16-byte aligned,
  * hold sb200_w4_table_entries(n, k, group) entries: [tile of outputs][128 inputs][output of the tile][group of the 128 inputs].
  * Outputs are padded to 16 and inputs to 128; the scales of padding are 0. */
 size_t sb200_w4_codes_bytes(int n, int k);

@@ -59,13 +59,14 @@ int launch(const ExpandParams& p, int pairs, cudaStream_t stream) {
     cudaError_t e = cudaFuncGetAttributes(&a, kernel);
     if (e != cudaSuccess) return static_cast<int>(e);
     if (a.numRegs != kRegsLaunch) return static_cast<int>(kErrInternal);
-    return static_cast<int>(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kExpandSmem));
+    return static_cast<int>(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 expand_smem(KIND, PER)));
   });
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
   cfg.blockDim = dim3(kExpandThreads);
-  cfg.dynamicSmemBytes = kExpandSmem;
+  cfg.dynamicSmemBytes = expand_smem(KIND, PER);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -130,7 +131,6 @@ size_t expand_w4_workspace(int m, int n, int k, bool x_aligned) {
 
 int expand_w4(const W4& w, const void* x, long long ldx, void* y, long long ldy, int m, void* workspace, cudaStream_t stream) {
   ExpandParams p = {};
-  p.codes = static_cast<const uint8_t*>(w.codes);
   p.scales = w.scales;
   p.zeros = static_cast<const uint8_t*>(w.zeros);
   p.rows = w.n;
@@ -155,6 +155,9 @@ int expand_w4(const W4& w, const void* x, long long ldx, void* y, long long ldy,
   const int pairs = place(p, pairs_of_device());
   if (!pairs) return kErrNotSupported;
   if ((rc = tc::map_rows_16bit(&p.right, x, m, w.k, ldx, p.bn / 2))) return rc;
+  // a row tile's codes are one row of 32-bit words; a box is 128 inputs of eight row tiles
+  if ((rc = tc::map_rows_plain(&p.codes_map, w.codes, 4, w4_row_tiles(w.n), 256ll * w4_blocks(w.k), 1024ll * w4_blocks(w.k), 8, 256)))
+    return rc;
   return w.dtype == kF16 ? run_w4<__half>(p, w.group, pairs, stream) : run_w4<__nv_bfloat16>(p, w.group, pairs, stream);
 }
 
@@ -165,9 +168,7 @@ size_t expand_act8_workspace(int m, int n, int k, bool dy_aligned) {
 int expand_act8(const Act8& a, const void* dy, long long lddy, bool out_f32, const void* base, long long ldbase, void* dw,
                 long long lddw, int n, void* workspace, cudaStream_t stream) {
   ExpandParams p = {};
-  p.codes = static_cast<const uint8_t*>(a.codes);
   p.exps = static_cast<const uint8_t*>(a.exps);
-  p.pitch = a.pitch;
   p.exp_pitch = a.exp_pitch;
   p.rows = a.k;
   p.cols = n;
@@ -195,6 +196,8 @@ int expand_act8(const Act8& a, const void* dy, long long lddy, bool out_f32, con
     p.part = reinterpret_cast<float*>(ws);
     if (!(pairs = place(p, pairs_of_device()))) return kErrNotSupported;
     if ((rc = tc::map_rows_16bit(&p.right, dy, a.m, n, lddy, kStep))) return rc;
+    if ((rc = tc::map_rows_plain(&p.codes_map, a.codes, 1, a.m, static_cast<long long>(align_up(a.k, 16)), a.pitch, kStep, kCtaRows)))
+      return rc;
   }
   return a.dtype == kF16 ? run_act8<__half>(p, pairs, stream) : run_act8<__nv_bfloat16>(p, pairs, stream);
 }

@@ -3,9 +3,10 @@
 //     ACT8  dW  = X^T dY     left rows = channels,              right columns = columns of dY, reduction = tokens
 //
 // A pair of CTAs computes a tile of 256 left rows x `bn` columns with tcgen05.mma.cta_group::2.  Per step of 64 of the
-// reduction each CTA's eight converter warps expand the 128 x 64 values of its own left rows from registers (loaded a few
-// steps ahead) into the swizzled shared-memory tile that the tensor cores read; TMA brings the CTA's half of the right
-// operand.  The expansion therefore costs no pass over memory: the operand travels in 4 or 8 bits and is never written
+// reduction each CTA's converter warps (two groups of four, in turn) expand the 128 x 64 values of its own left rows into the swizzled shared-memory
+// tile that the tensor cores read; TMA brings the codes and the CTA's half of the right operand.  (Codes loaded into the
+// converters' registers a few steps ahead were measured at less than half the speed: each fence that hands a tile to
+// the tensor cores then waits for the loads in flight.)  The expansion therefore costs no pass over memory: the operand travels in 4 or 8 bits and is never written
 // out in 16.
 //   W4    the tile is K-major (a word of the format is the 16 bytes of eight neighbouring inputs); weights are rounded to 16
 //         bits once, code - zero is exact before.
@@ -28,12 +29,12 @@ namespace lowbit {
 enum ExpandKind { kExpandW4 = 0, kExpandAct8 = 1 };
 
 struct ExpandParams {
+  CUtensorMap codes_map;    // W4: 32-bit words, a row for each row tile; ACT8: bytes, a row for each token
   CUtensorMap right;        // x [tokens][inputs] (W4) or dY [tokens][columns] (ACT8)
-  const uint8_t* codes;
   const void* scales;       // W4
   const uint8_t* zeros;     // W4, or null
   const uint8_t* exps;      // ACT8
-  long long pitch, exp_pitch;
+  long long exp_pitch;
   int rows, cols;           // of the result: left rows, right columns
   int depth;                // length of the reduction
   int bn;                   // columns of a tile, a multiple of 32 up to 256
@@ -52,20 +53,28 @@ struct ExpandParams {
 
 constexpr int kPairRows = 256, kCtaRows = 128, kStep = 64, kMaxCols = 256;
 constexpr int kSubSteps = 8;       // steps that one accumulator takes: 32 additions
-constexpr int kStages = 6;
+constexpr int kStages = 5;
+constexpr int kRawStages = 4;      // tiles of codes: a step (ACT8: 64 tokens x 128 channels) or two (W4: 128 rows x 128 inputs)
+constexpr int kRawBytes = 8192;
 constexpr int kLeftBytes = kCtaRows * 128;           // 128 x 64 values of 16 bits
 constexpr int kRightBytes = (kMaxCols / 2) * 128;    // at most 128 columns x 64
 constexpr int kStageBytes = kLeftBytes + kRightBytes;
 constexpr int kRightBlock = 64 * 128;                // 64 columns x 64 tokens (MN-major)
 constexpr int kExpandThreads = 640;  // warpgroups: 0 = producers and MMA, 1-2 = epilogue, 3-4 = converters
-constexpr int kEpilogueWarps = 8, kConvertWarps = 8;
+constexpr int kEpilogueWarps = 8;
+constexpr int kConvertWarps = 4;  // of a group; the two groups take the steps (W4: pairs of steps) in turn
 constexpr int kTransposeBytes = 32 * 32 * 4;         // per epilogue warp
-constexpr int kExpandSmem = 1024 + kStages * kStageBytes + kEpilogueWarps * kTransposeBytes + 1024;
+// scales and zeros of 128 rows (W4, PER groups each), or exponents of 64 tokens (ACT8, four blocks each)
+__host__ __device__ constexpr int table_bytes(int kind, int per) { return kind == kExpandW4 ? kCtaRows * 3 * per : kStep * 4; }
+__host__ __device__ constexpr int expand_smem(int kind, int per) {
+  return 1024 + kStages * kStageBytes + kRawStages * (kRawBytes + table_bytes(kind, per)) +
+         (kind == kExpandAct8 ? kEpilogueWarps * kTransposeBytes : 0) + 1024;
+}
 // registers a thread: at launch (all threads), and after the trade; the sum of what the warpgroups take must not
 // exceed what the block was launched with (the host checks the kernel's count before a launch)
-constexpr int kRegsLaunch = 96, kRegsControl = 24, kRegsEpilogue = 160, kRegsConvert = 64;
+constexpr int kRegsLaunch = 96, kRegsControl = 48, kRegsEpilogue = 152, kRegsConvert = 64;
 static_assert(128 * kRegsControl + 256 * kRegsEpilogue + 256 * kRegsConvert <= kExpandThreads * kRegsLaunch, "register trade");
-static_assert(kExpandSmem <= 232448, "shared memory of a CTA");
+static_assert(expand_smem(kExpandW4, 4) <= 232448 && expand_smem(kExpandAct8, 1) <= 232448, "shared memory of a CTA");
 
 template <int N> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -78,6 +87,23 @@ __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16])
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr)
       : "memory");
+}
+
+// Asynchronous copies of 4 and 16 bytes, zeros where `from` has none to give; a thread's arrival counts once they landed.
+__device__ __forceinline__ void copy_async_16(uint32_t to, const void* from, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_async_4(uint32_t to, const void* from, bool real) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(real ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(ptx::smem_u32(bar)) : "memory");
+}
+
+__device__ __forceinline__ uint2 lds_v2(uint32_t smem_addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(smem_addr));
+  return v;
 }
 
 template <typename T> struct Half;
@@ -186,14 +212,18 @@ template <typename T, int KIND, int PER>
 __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const __grid_constant__ ExpandParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* after = smem + kStages * kStageBytes;
-  float* transpose = reinterpret_cast<float*>(after);
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(after + kEpilogueWarps * kTransposeBytes);
+  constexpr int kTable = table_bytes(KIND, PER);
+  uint8_t* raw = smem + kStages * kStageBytes;
+  float* transpose = reinterpret_cast<float*>(raw + kRawStages * kRawBytes);
+  uint8_t* tables = raw + kRawStages * kRawBytes + (KIND == kExpandAct8 ? kEpilogueWarps * kTransposeBytes : 0);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(tables + kRawStages * kTable);
   uint64_t* empty_bar = full_bar + kStages;
   uint64_t* slot_full = empty_bar + kStages;
   uint64_t* slot_free = slot_full + 2;
   uint64_t* left_bar = slot_free + 2;  // this CTA's left tile of a stage is written
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(left_bar + kStages);
+  uint64_t* raw_full = left_bar + kStages;
+  uint64_t* raw_empty = raw_full + kRawStages;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(raw_empty + kRawStages);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -213,6 +243,10 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
     for (int s = 0; s < 2; ++s) {
       ptx::mbar_init(&slot_full[s], 1);
       ptx::mbar_init(&slot_free[s], 2 * kEpilogueWarps);
+    }
+    for (int s = 0; s < kRawStages; ++s) {
+      ptx::mbar_init(&raw_full[s], 1 + 32);  // the codes, and the loader's lanes' parts of the tables
+      ptx::mbar_init(&raw_empty[s], kConvertWarps);
     }
     ptx::fence_mbar_init();
   }
@@ -278,7 +312,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
         int sub = 0;
         for (int kk = w.k0; kk < w.k1; ++kk) {
           if (sub == 0) {
-            if (!ptx::mbar_wait_warp<true>(&slot_free[slot], ((free_bits >> slot) & 1u) ^ 1u, abort_flag, p.wait_ns)) {
+            if (!ptx::mbar_wait_warp<false>(&slot_free[slot], ((free_bits >> slot) & 1u) ^ 1u, abort_flag, p.wait_ns)) {
               if (lane == 0) give_up(p, abort_flag, 102);
               ok = false;
               break;
@@ -286,7 +320,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
             free_bits ^= 1u << slot;
             ptx::tc_fence_after_sync();
           }
-          if (!ptx::mbar_wait_warp<true>(&full_bar[stage], phase, abort_flag, p.wait_ns)) {
+          if (!ptx::mbar_wait_warp<false>(&full_bar[stage], phase, abort_flag, p.wait_ns)) {
             if (lane == 0) give_up(p, abort_flag, 102);
             ok = false;
             break;
@@ -312,7 +346,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
         }
       }
     }
-    else if (warp == 3 && rank == 1) {
+    else if (warp == 1) {
       // ---- passes on to the leader that the peer's left tile is written.  The converters themselves would have to release
       // at cluster scope, which waits for the loads that they have in flight.
       uint32_t stage = 0, phase = 0;
@@ -325,9 +359,54 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
             ok = false;
             break;
           }
-          if (lane == 0) ptx::mbar_arrive_cluster(&full_bar[stage], 0);
+          if (lane == 0) ptx::mbar_arrive_remote(&full_bar[stage], 0);
           __syncwarp();
           if (++stage == kStages) { stage = 0; phase ^= 1u; }
+        }
+      }
+    } else if (warp == 3) {
+      // ---- loader of codes (TMA) and tables (small asynchronous copies)
+      if (lane == 0) ptx::prefetch_tmap(&p.codes_map);
+      uint32_t stage = 0, phase = 0;
+      bool ok = true;
+      const int blocks = w4_blocks(p.depth), tiles = w4_row_tiles(p.rows);
+      for (int u = pair; ok && u < units; u += pairs) {
+        const ExpandUnit w = expand_unit(p, u);
+        const int row0 = w.row0 + static_cast<int>(rank) * kCtaRows;
+        for (int kk = w.k0; kk < w.k1; kk += KIND == kExpandW4 ? 2 : 1) {
+          if (!ptx::mbar_wait_warp<false>(&raw_empty[stage], phase ^ 1u, abort_flag, p.wait_ns)) {
+            if (lane == 0) give_up(p, abort_flag, 101);
+            ok = false;
+            break;
+          }
+          const uint32_t table = ptx::smem_u32(tables + stage * kTable);
+          if (ptx::elect_one()) {
+            ptx::mbar_arrive_expect_tx(&raw_full[stage], kRawBytes);
+            if (KIND == kExpandW4) ptx::tma_load_2d(raw + stage * kRawBytes, &p.codes_map, &raw_full[stage], kk / 2 * 256, row0 / kW4Rows);
+            else ptx::tma_load_2d(raw + stage * kRawBytes, &p.codes_map, &raw_full[stage], row0, kk * kStep);
+          }
+          __syncwarp();
+          if (KIND == kExpandW4) {
+            // 2 PER pieces of 16 bytes of scales for each of the eight row tiles, then PER of zeros
+            for (int i = lane; i < 24 * PER; i += 32) {
+              const bool zero = i >= 16 * PER;
+              const int j = zero ? i - 16 * PER : i, each = zero ? PER : 2 * PER;
+              const int tile = row0 / kW4Rows + j / each;
+              const bool real = tile < tiles && (!zero || p.zeros);
+              const long long at = (static_cast<long long>(tile) * blocks + kk / 2) * each + j % each;
+              const uint8_t* from = zero ? p.zeros : static_cast<const uint8_t*>(p.scales);
+              copy_async_16(table + i * 16, real ? from + at * 16 : static_cast<const uint8_t*>(p.scales), real);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const long long tok = static_cast<long long>(kk) * kStep + lane + 32 * i;
+              const bool real = tok < p.depth && row0 < p.rows;
+              copy_async_4(table + (lane + 32 * i) * 4, real ? p.exps + tok * p.exp_pitch + row0 / kActBlock : p.exps, real);
+            }
+          }
+          copy_async_arrive(&raw_full[stage]);
+          if (++stage == kRawStages) { stage = 0; phase ^= 1u; }
         }
       }
     }
@@ -341,11 +420,39 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
     bool ok = true;
     for (int u = pair; ok && u < units; u += pairs) {
       const ExpandUnit w = expand_unit(p, u);
+      const int row0 = w.row0 + static_cast<int>(rank) * kCtaRows + quarter * 32;
+      const int col0 = w.col0 + side * half;
       float sum[128];
 #pragma unroll
       for (int i = 0; i < 128; ++i) sum[i] = 0.f;
+      if (KIND == kExpandAct8 && p.base && p.slices == 1) {
+        // the sums start from the base, which is read while the tile's first MMAs run: 32 rows of 32 neighbours at a
+        // time, which then change places between lanes and registers
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          if (c * 32 < half) {
+            const int col = col0 + c * 32 + lane;
+            const bool in = c * 32 + lane < half && col < p.cols;
+            float v[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const long long row = row0 + i;
+              v[i] = 0.f;
+              if (in && row < p.rows)
+                v[i] = p.out_f32 ? static_cast<const float*>(p.base)[row * p.ldbase + col]
+                                 : to_f32(static_cast<const T*>(p.base)[row * p.ldbase + col]);
+            }
+#pragma unroll
+            for (int i = 0; i < 32; ++i) swap[i * 32 + (lane ^ i)] = v[i];
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) sum[c * 32 + i] = swap[lane * 32 + (i ^ lane)];
+            __syncwarp();
+          }
+        }
+      }
       for (int kk = w.k0; kk < w.k1; kk += kSubSteps) {
-        if (!ptx::mbar_wait_warp<true>(&slot_full[slot], (full_bits >> slot) & 1u, abort_flag, p.wait_ns)) {
+        if (!ptx::mbar_wait_warp<false>(&slot_full[slot], (full_bits >> slot) & 1u, abort_flag, p.wait_ns)) {
           if (lane == 0) give_up(p, abort_flag, 103);
           ok = false;
           break;
@@ -365,12 +472,10 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
         }
         ptx::tc_fence_before_sync();
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive_cluster(&slot_free[slot], 0);
+        if (lane == 0) ptx::mbar_arrive_remote(&slot_free[slot], 0);
         slot ^= 1u;
       }
       if (!ok) break;
-      const int row0 = w.row0 + static_cast<int>(rank) * kCtaRows + quarter * 32;
-      const int col0 = w.col0 + side * half;
       if (KIND == kExpandW4) {
         // a column of the tile is a row of y: 32 lanes store 32 neighbours
         const int row = row0 + lane;
@@ -397,14 +502,12 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
             for (int i = 0; i < 32; ++i) {
               const long long row = row0 + i;
               if (in && row < p.rows) {
-                float v = swap[i * 32 + (lane ^ i)];
+                const float v = swap[i * 32 + (lane ^ i)];
                 if (p.slices > 1) {
                   part[row * p.cols + col] = v;
                 } else if (p.out_f32) {
-                  if (p.base) v += static_cast<const float*>(p.base)[row * p.ldbase + col];
                   static_cast<float*>(p.out)[row * p.ldo + col] = v;
                 } else {
-                  if (p.base) v += to_f32(static_cast<const T*>(p.base)[row * p.ldbase + col]);
                   static_cast<T*>(p.out)[row * p.ldo + col] = from_f32<T>(v);
                 }
               }
@@ -417,140 +520,114 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
   } else {
     // ---- converters
     regs_dec<kRegsConvert>();
-    const int tid = threadIdx.x - 12 * 32;
-    const uint32_t left = ptx::smem_u32(smem);
-    uint32_t stage = 0, phase = 0;
+    const int group = (warp - 12) / kConvertWarps, tid = threadIdx.x % (kConvertWarps * 32);
+    const uint32_t left = ptx::smem_u32(smem), codes = ptx::smem_u32(raw);
+    uint32_t stage = 0, phase = 0, rstage = 0, rphase = 0, turn = group;
     bool ok = true;
+    auto next_stage = [&]() { if (++stage == kStages) { stage = 0; phase ^= 1u; } };
+    auto next_raw = [&]() { if (++rstage == kRawStages) { rstage = 0; rphase ^= 1u; } };
     auto acquire = [&]() -> bool {  // the stage's previous contents have been read
-      if (!ptx::mbar_wait_warp<false>(&empty_bar[stage], phase ^ 1u, abort_flag, p.wait_ns)) {
-        if (lane == 0) give_up(p, abort_flag, 104);
-        return false;
-      }
-      return true;
+      if (ptx::mbar_wait_warp<false>(&empty_bar[stage], phase ^ 1u, abort_flag, p.wait_ns)) return true;
+      if (lane == 0) give_up(p, abort_flag, 104);
+      return false;
     };
     auto publish = [&]() {
       ptx::fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(&left_bar[stage]);
-      if (++stage == kStages) { stage = 0; phase ^= 1u; }
+      next_stage();
+    };
+    auto raw_ready = [&]() -> bool {
+      if (ptx::mbar_wait_warp<false>(&raw_full[rstage], rphase, abort_flag, p.wait_ns)) return true;
+      if (lane == 0) give_up(p, abort_flag, 104);
+      return false;
+    };
+    auto raw_done = [&]() {  // every lane has read the codes and tables
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&raw_empty[rstage]);
+      next_raw();
     };
     for (int u = pair; ok && u < units; u += pairs) {
       const ExpandUnit w = expand_unit(p, u);
-      const int row0 = w.row0 + static_cast<int>(rank) * kCtaRows;
       if (KIND == kExpandW4) {
-        // Two pieces a thread and tile of 128 inputs: 16 bytes (four words) of a row.  Words 0 and 1 belong to the first
+        // Four pieces a thread and tile of 128 inputs: 16 bytes (four words) of a row.  Words 0 and 1 belong to the first
         // step, 2 and 3 to the second.  Lanes of odd rows store the second word of a step first, so that eight
         // lanes always hit eight different 16-byte columns of the swizzled tile.
-        struct Raw { uint4 c; uint32_t s[(PER + 1) / 2]; uint32_t z; } raw[2][2];
-        const int blocks = w4_blocks(p.depth), tiles = w4_row_tiles(p.rows);
-        const int g = lane >> 2, t = lane & 3;
-        auto load = [&](int b, int buf) {
+        const int g = lane >> 2, t = lane & 3, odd = g & 1;
+        const int row0 = (tid >> 6) * kW4Rows + 8 * ((tid >> 5) & 1) + g;  // of the first piece; the others 32 rows on
+        for (int kk = w.k0; kk < w.k1; kk += 2) {
+          turn ^= 1u;
+          if (turn == 0) {
+            next_raw();
+            next_stage();
+            next_stage();
+            continue;
+          }
+          if (!raw_ready()) { ok = false; break; }
+          const uint32_t from = codes + rstage * kRawBytes + tid * 16;
+          const uint8_t* table = tables + rstage * kTable;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int tile = row0 / kW4Rows + (tid >> 6) + 4 * i;
-            Raw& q = raw[buf][i];
-            q.c = make_uint4(0, 0, 0, 0);
-            q.z = 0;
+          for (int h = 0; h < 2; ++h) {
+            uint2 c[4];
+            uint32_t bias[4][2], scale[4][2];
 #pragma unroll
-            for (int j = 0; j < (PER + 1) / 2; ++j) q.s[j] = 0;
-            if (tile < tiles && 2 * b < w.k1) {
-              const long long at = static_cast<long long>(tile) * blocks + b;
-              q.c = ptx::ldg_nc_v4(p.codes + at * kW4TileBytes + (tid & 63) * 16);
-              const long long entry = (at * kW4Rows + 8 * ((tid >> 5) & 1) + g) * PER;
-              const uint16_t* s = static_cast<const uint16_t*>(p.scales) + entry;
-              if (PER == 1) q.s[0] = __ldg(s);
-              if (PER == 2) q.s[0] = __ldg(reinterpret_cast<const uint32_t*>(s));
-              if (PER == 4) {
-                const uint2 v = __ldg(reinterpret_cast<const uint2*>(s));
-                q.s[0] = v.x;
-                q.s[PER / 4] = v.y;
-              }
-              q.z = 0x08080808u;
-              if (p.zeros) {
-                if (PER == 1) q.z = __ldg(p.zeros + entry);
-                if (PER == 2) q.z = __ldg(reinterpret_cast<const uint16_t*>(p.zeros + entry));
-                if (PER == 4) q.z = __ldg(reinterpret_cast<const uint32_t*>(p.zeros + entry));
+            for (int i = 0; i < 4; ++i) {
+              c[i] = lds_v2(from + i * 2048 + h * 8);
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                if (PER < 4 && j == 1) { bias[i][1] = bias[i][0]; scale[i][1] = scale[i][0]; continue; }
+                const int at = (row0 + 32 * i) * PER + (2 * h + j) * PER / 4;
+                const uint32_t s = reinterpret_cast<const uint16_t*>(table)[at];
+                const uint32_t z = p.zeros ? table[kCtaRows * 2 * PER + at] : 8u;
+                scale[i][j] = s | (s << 16);
+                bias[i][j] = Half<T>::magic + (z | (z << 16));
               }
             }
-          }
-        };
-        load(w.k0 / 2, 0);
-        load(w.k0 / 2 + 1, 1);
-        const int odd = g & 1;
-        for (int b = w.k0 / 2; ok && 2 * b < w.k1; b += 2) {
-#pragma unroll
-          for (int buf = 0; buf < 2; ++buf) {
-            if (2 * (b + buf) >= w.k1) break;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              if (2 * (b + buf) + h >= w.k1) break;
-              if (!acquire()) { ok = false; break; }
-              const uint32_t to = left + stage * kStageBytes;
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const Raw& q = raw[buf][i];
-                const int row = ((tid >> 6) + 4 * i) * kW4Rows + 8 * ((tid >> 5) & 1) + g;
-                uint4 v[2];
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                  const int word = 2 * h + j, group = word * PER / 4;
-                  const uint32_t z = (q.z >> (8 * group)) & 255u;
-                  const uint32_t s = (q.s[group / 2] >> (16 * (group & 1))) & 0xffffu;
-                  v[j] = expand_w4<T>((&q.c.x)[word], Half<T>::magic + (z | (z << 16)), s | (s << 16));
-                }
-                const uint4 a = odd ? v[1] : v[0], c = odd ? v[0] : v[1];
-                ptx::sts_v4(to + row * 128 + (((4 * odd + t) ^ (row & 7)) << 4), a);
-                ptx::sts_v4(to + row * 128 + (((4 * (1 - odd) + t) ^ (row & 7)) << 4), c);
-              }
-              publish();
-            }
-            if (!ok) break;
-            load(b + buf + 2, buf);
-          }
-        }
-      } else {
-        // Two pieces a thread and step: 16 channels of a token.  Eight neighbouring lanes hold a token's 128 channels; those
-        // of the second 64 store their second half first, which keeps eight lanes on eight different 16-byte columns.
-        struct Raw { uint4 c; uint32_t e; } raw[3][2];
-        const int piece = tid & 7, token = tid >> 3;
-        const int channel = row0 + piece * 16;
-        const bool in = channel < p.rows;
-        auto load = [&](int kk, int buf) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const long long tok = static_cast<long long>(kk) * kStep + token + 32 * i;
-            Raw& q = raw[buf][i];
-            q.c = make_uint4(0, 0, 0, 0);
-            q.e = 127;
-            if (in && kk < w.k1 && tok < p.depth) {
-              q.c = ptx::ldg_nc_v4(p.codes + tok * p.pitch + channel);
-              q.e = __ldg(p.exps + tok * p.exp_pitch + channel / kActBlock);
-            }
-          }
-        };
-#pragma unroll
-        for (int a = 0; a < 3; ++a) load(w.k0 + a, a);
-        const int second = piece >> 2;
-        for (int k0 = w.k0; ok && k0 < w.k1; k0 += 3) {
-#pragma unroll
-          for (int buf = 0; buf < 3; ++buf) {
-            const int kk = k0 + buf;
-            if (kk >= w.k1) break;
             if (!acquire()) { ok = false; break; }
-            const uint32_t to = left + stage * kStageBytes + second * kRightBlock;
+            const uint32_t to = left + stage * kStageBytes;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const Raw& q = raw[buf][i];
-              const int r = token + 32 * i;
-              const Act8Step<T> step(q.e);
-              const uint4 lo = expand_act8<T>(q.c.x, q.c.y, step), hi = expand_act8<T>(q.c.z, q.c.w, step);
-              const int c = 2 * (piece & 3);
-              ptx::sts_v4(to + r * 128 + (((c + second) ^ (r & 7)) << 4), second ? hi : lo);
-              ptx::sts_v4(to + r * 128 + (((c + 1 - second) ^ (r & 7)) << 4), second ? lo : hi);
+            for (int i = 0; i < 4; ++i) {
+              const uint4 v0 = expand_w4<T>(c[i].x, bias[i][0], scale[i][0]), v1 = expand_w4<T>(c[i].y, bias[i][1], scale[i][1]);
+              const uint32_t line = to + (row0 + 32 * i) * 128;
+              ptx::sts_v4(line + (((4 * odd + t) ^ (g & 7)) << 4), odd ? v1 : v0);
+              ptx::sts_v4(line + (((4 * (1 - odd) + t) ^ (g & 7)) << 4), odd ? v0 : v1);
             }
             publish();
-            load(kk + 3, buf);
           }
+          if (!ok) break;
+          raw_done();
+        }
+      } else {
+        // Four pieces a thread and step: 16 channels of a token.  Eight neighbouring lanes hold a token's 128 channels; those
+        // of the second 64 store their second half first, which keeps eight lanes on eight different 16-byte columns.
+        const int piece = tid & 7, second = piece >> 2, token = tid >> 3;  // tokens 16 apart
+        const int at = 2 * (piece & 3);
+        for (int kk = w.k0; kk < w.k1; ++kk) {
+          turn ^= 1u;
+          if (turn == 0) {
+            next_raw();
+            next_stage();
+            continue;
+          }
+          if (!raw_ready()) { ok = false; break; }
+          uint4 c[4];
+          uint32_t e[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            c[i] = ptx::lds_v4(codes + rstage * kRawBytes + tid * 16 + i * 2048);
+            e[i] = tables[rstage * kTable + (token + 16 * i) * 4 + (piece >> 1)];
+          }
+          if (!acquire()) { ok = false; break; }
+          const uint32_t to = left + stage * kStageBytes + second * kRightBlock + token * 128;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const Act8Step<T> step(e[i]);
+            const uint4 lo = expand_act8<T>(c[i].x, c[i].y, step), hi = expand_act8<T>(c[i].z, c[i].w, step);
+            ptx::sts_v4(to + i * 2048 + (((at + second) ^ (token & 7)) << 4), second ? hi : lo);
+            ptx::sts_v4(to + i * 2048 + (((at + 1 - second) ^ (token & 7)) << 4), second ? lo : hi);
+          }
+          raw_done();
+          publish();
         }
       }
     }

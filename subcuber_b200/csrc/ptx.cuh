@@ -245,6 +245,20 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint64_t* bar, uint32_t cta)
       "r"(cta)
       : "memory");
 }
+// The same with release at CTA scope.  A release at cluster scope makes a thread wait until everything it wrote or read is
+// visible to the whole cluster, about 0.8 us on B200; this one is enough where the arrival announces nothing that the
+// other CTA's threads read themselves: accumulators read out of tensor memory, or tiles in this CTA's own shared memory that
+// only this SM's tensor core reads and that a proxy fence of their writers has already handed to it.
+__device__ __forceinline__ void mbar_arrive_remote(uint64_t* bar, uint32_t cta) {
+  asm volatile(
+      "{\n\t"
+      ".reg .b32 ra;\n\t"
+      "mapa.shared::cluster.u32 ra, %0, %1;\n\t"
+      "mbarrier.arrive.shared::cluster.b64 _, [ra];\n\t"
+      "}\n" ::"r"(smem_u32(bar)),
+      "r"(cta)
+      : "memory");
+}
 // 32-bit store into the shared memory of CTA `cta` of the cluster, at the offset of `local` in this CTA.
 __device__ __forceinline__ void st_shared_cluster_u32(const void* local, uint32_t cta, uint32_t value) {
   asm volatile(

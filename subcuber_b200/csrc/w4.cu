@@ -203,7 +203,7 @@ int check(const W4& w) {
   if (w.dtype != kF16 && w.dtype != kBF16) return kErrNotSupported;
   if (w.n <= 0 || w.k <= 0 || !w.codes || !w.scales) return kErrInvalidProblem;
   if (w.group != 32 && w.group != 64 && w.group != 128) return kErrNotSupported;
-  if (!aligned(w.codes, 16) || !aligned(w.scales, 8) || !aligned(w.zeros, 4)) return kErrMisalignedOperand;
+  if (!aligned(w.codes, 16) || !aligned(w.scales, 16) || !aligned(w.zeros, 16)) return kErrMisalignedOperand;
   return kOk;
 }
 
