@@ -63,6 +63,8 @@ constexpr int kRightBlock = 64 * 128;                // 64 columns x 64 tokens (
 constexpr int kExpandThreads = 640;  // warpgroups: 0 = producers and MMA, 1-2 = epilogue, 3-4 = converters
 constexpr int kEpilogueWarps = 8;
 constexpr int kConvertWarps = 4;  // of a group; the two groups take the steps (W4: pairs of steps) in turn
+constexpr int kPieces = kRawBytes / 16 / (32 * kConvertWarps);  // of 16 bytes of codes that a converter thread expands
+constexpr int kProducers = 3;
 constexpr int kTransposeBytes = 32 * 32 * 4;         // per epilogue warp
 // scales and zeros of 128 rows (W4, PER groups each), or exponents of 64 tokens (ACT8, four blocks each)
 __host__ __device__ constexpr int table_bytes(int kind, int per) { return kind == kExpandW4 ? kCtaRows * 3 * per : kStep * 4; }
@@ -73,20 +75,17 @@ __host__ __device__ constexpr int expand_smem(int kind, int per) {
 // registers a thread: at launch (all threads), and after the trade; the sum of what the warpgroups take must not
 // exceed what the block was launched with (the host checks the kernel's count before a launch)
 constexpr int kRegsLaunch = 96, kRegsControl = 48, kRegsEpilogue = 152, kRegsConvert = 64;
-static_assert(128 * kRegsControl + 256 * kRegsEpilogue + 256 * kRegsConvert <= kExpandThreads * kRegsLaunch, "register trade");
+static_assert(128 * kRegsControl + 256 * kRegsEpilogue + 64 * kConvertWarps * kRegsConvert <= kExpandThreads * kRegsLaunch, "register trade");
 static_assert(expand_smem(kExpandW4, 4) <= 232448 && expand_smem(kExpandAct8, 1) <= 232448, "shared memory of a CTA");
 
 template <int N> __device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
-__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr)
-      : "memory");
+__device__ __forceinline__ void tmem_ld_32x8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
 }
 
 // Asynchronous copies of 4 and 16 bytes, zeros where `from` has none to give; a thread's arrival counts once they landed.
@@ -103,6 +102,17 @@ __device__ __forceinline__ void copy_async_arrive(uint64_t* bar) {
 __device__ __forceinline__ uint2 lds_v2(uint32_t smem_addr) {
   uint2 v;
   asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(smem_addr));
+  return v;
+}
+
+__device__ __forceinline__ uint32_t lds_u16(uint32_t smem_addr) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(smem_addr));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds_u8(uint32_t smem_addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(smem_addr));
   return v;
 }
 
@@ -208,6 +218,69 @@ __device__ __forceinline__ void give_up(const ExpandParams& p, volatile int* abo
   atomicCAS(p.status, 0, code);
 }
 
+__device__ __forceinline__ float lds_f32(uint32_t a) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ void sts_f32(uint32_t a, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory"); }
+
+// A warp's 32 rows x 128 columns of sums, a row to a lane, from and to a row-major matrix: 32 x 32 values at a time change
+// places between lanes and registers in shared memory (`swap`, value (row, column) at word 32 row + (column ^ row)), so that
+// memory sees whole rows.
+template <typename E>
+__device__ __forceinline__ void load_tile_rows(float (&sum)[128], const E* base, long long ld, int row0, int col0, int nrows,
+                                               int ncols, uint32_t swap, int lane) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    if (c * 32 < ncols) {
+      const bool in = c * 32 + lane < ncols;
+      const E* from = base + row0 * ld + col0 + c * 32 + lane;
+#pragma unroll 1
+      for (int b = 0; b < 32; b += 8) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i, from += ld) v[i] = in && b + i < nrows ? to_f32(*from) : 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sts_f32(swap + (b + i) * 128 + ((lane ^ (b + i)) << 2), v[i]);
+      }
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 32; ++i) sum[c * 32 + i] = lds_f32(swap + lane * 128 + ((i ^ lane) << 2));
+      __syncwarp();
+    }
+  }
+}
+template <typename E>
+__device__ __forceinline__ void store_tile_rows(const float (&sum)[128], E* out, long long ld, int row0, int col0, int nrows,
+                                                int ncols, uint32_t swap, int lane) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    if (c * 32 < ncols) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) sts_f32(swap + lane * 128 + ((i ^ lane) << 2), sum[c * 32 + i]);
+      __syncwarp();
+      const bool in = c * 32 + lane < ncols;
+      E* to = out + row0 * ld + col0 + c * 32 + lane;
+#pragma unroll 8
+      for (int i = 0; i < 32; ++i, to += ld) {
+        const float v = lds_f32(swap + i * 128 + ((lane ^ i) << 2));
+        if (in && i < nrows) *to = from_f32<E>(v);
+      }
+      __syncwarp();
+    }
+  }
+}
+// The same to the transposed matrix: a column of the tile is a row there, 32 lanes store 32 neighbours.
+template <typename E>
+__device__ __forceinline__ void store_tile_cols(const float (&sum)[128], E* out, long long ld, int row0, int col0, int nrows,
+                                                int ncols, int lane) {
+  E* to = out + col0 * ld + row0 + lane;
+#pragma unroll
+  for (int c = 0; c < 128; ++c, to += ld)
+    if (c < ncols && lane < nrows) *to = from_f32<E>(sum[c]);
+}
+
 template <typename T, int KIND, int PER>
 __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const __grid_constant__ ExpandParams p) {
   extern __shared__ uint8_t smem_raw[];
@@ -245,7 +318,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
       ptx::mbar_init(&slot_free[s], 2 * kEpilogueWarps);
     }
     for (int s = 0; s < kRawStages; ++s) {
-      ptx::mbar_init(&raw_full[s], 1 + 32);  // the codes, and the loader's lanes' parts of the tables
+      ptx::mbar_init(&raw_full[s], 1 + 32);  // the codes, and a producer's lanes' parts of the tables
       ptx::mbar_init(&raw_empty[s], kConvertWarps);
     }
     ptx::fence_mbar_init();
@@ -263,37 +336,87 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
 
   if (warp < 4) {
     regs_dec<kRegsControl>();
-    if (warp == 0 || warp == 2) {
-      // ---- TMA producers: the loads of one warp complete one after the other, so two warps take the steps in turn
+    if (warp != 1) {
+      // ---- producers: codes, tables and the CTA's half of the right operand.  The loads of one warp complete one after the
+      // other (about 240 ns each, whatever they hold), so three warps take the steps (W4: pairs of steps) in turn.
+      const int blocks = w4_blocks(p.depth), tiles = w4_row_tiles(p.rows);
       const int boxes = KIND == kExpandW4 ? 1 : (half + 63) / 64;
       const uint32_t bytes = 2u * (KIND == kExpandW4 ? half * 128 : boxes * kRightBlock);  // both CTAs'
-      if (warp == 0 && lane == 0) ptx::prefetch_tmap(&p.right);
-      uint32_t stage = 0, phase = 0, turn = warp >> 1;
+      constexpr int kEach = KIND == kExpandW4 ? 2 : 1;  // steps of a tile of codes
+      if (warp == 0 && lane == 0) {
+        ptx::prefetch_tmap(&p.right);
+        ptx::prefetch_tmap(&p.codes_map);
+      }
+      uint32_t stage = 0, phase = 0, rstage = 0, rphase = 0;
+      int turn = warp == 0 ? 0 : warp - 1;
       bool ok = true;
       for (int u = pair; ok && u < units; u += pairs) {
         const ExpandUnit w = expand_unit(p, u);
+        const int row0 = w.row0 + static_cast<int>(rank) * kCtaRows;
         const int col0 = w.col0 + static_cast<int>(rank) * half;
-        for (int kk = w.k0; kk < w.k1; ++kk) {
-          if (turn == 0) {
-            if (!ptx::mbar_wait_warp<false>(&empty_bar[stage], phase ^ 1u, abort_flag, p.wait_ns)) {
+        for (int kk = w.k0; ok && kk < w.k1; kk += kEach) {
+          const bool mine = turn == 0;
+          turn = mine ? kProducers - 1 : turn - 1;
+          if (mine) {
+            if (!ptx::mbar_wait_warp<false>(&raw_empty[rstage], rphase ^ 1u, abort_flag, p.wait_ns)) {
               if (lane == 0) give_up(p, abort_flag, 101);
               ok = false;
               break;
             }
             if (ptx::elect_one()) {
-              if (rank == 0) ptx::mbar_arrive_expect_tx(&full_bar[stage], bytes);
-              uint8_t* to = smem + stage * kStageBytes + kLeftBytes;
-              if (KIND == kExpandW4) {
-                ptx::tma_load_2d_pair(to, &p.right, &full_bar[stage], kk * kStep, col0);
-              } else {
-                for (int b = 0; b < boxes; ++b)
-                  ptx::tma_load_2d_pair(to + b * kRightBlock, &p.right, &full_bar[stage], col0 + b * 64, kk * kStep);
-              }
+              ptx::mbar_arrive_expect_tx(&raw_full[rstage], kRawBytes);
+              if (KIND == kExpandW4) ptx::tma_load_2d(raw + rstage * kRawBytes, &p.codes_map, &raw_full[rstage], kk / 2 * 256, row0 / kW4Rows);
+              else ptx::tma_load_2d(raw + rstage * kRawBytes, &p.codes_map, &raw_full[rstage], row0, kk * kStep);
             }
             __syncwarp();
+            const uint32_t table = ptx::smem_u32(tables + rstage * kTable);
+            if (KIND == kExpandW4) {
+              // 2 PER pieces of 16 bytes of scales for each of the eight row tiles, then PER of zeros
+#pragma unroll
+              for (int i0 = 0; i0 < 24 * PER; i0 += 32) {
+                const int i = i0 + lane;
+                if (i >= 24 * PER) break;
+                const bool zero = i >= 16 * PER;
+                const int j = zero ? i - 16 * PER : i, each = zero ? PER : 2 * PER;
+                const int tile = row0 / kW4Rows + j / each;
+                const bool real = tile < tiles && (!zero || p.zeros);
+                const long long at = (static_cast<long long>(tile) * blocks + kk / 2) * each + j % each;
+                const uint8_t* from = zero ? p.zeros : static_cast<const uint8_t*>(p.scales);
+                copy_async_16(table + i * 16, real ? from + at * 16 : static_cast<const uint8_t*>(p.scales), real);
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const long long tok = static_cast<long long>(kk) * kStep + lane + 32 * i;
+                const bool real = tok < p.depth && row0 < p.rows;
+                copy_async_4(table + (lane + 32 * i) * 4, real ? p.exps + tok * p.exp_pitch + row0 / kActBlock : p.exps, real);
+              }
+            }
+            copy_async_arrive(&raw_full[rstage]);
           }
-          turn ^= 1u;
-          if (++stage == kStages) { stage = 0; phase ^= 1u; }
+          if (++rstage == kRawStages) { rstage = 0; rphase ^= 1u; }
+#pragma unroll
+          for (int h = 0; h < kEach; ++h) {
+            if (mine) {
+              if (!ptx::mbar_wait_warp<false>(&empty_bar[stage], phase ^ 1u, abort_flag, p.wait_ns)) {
+                if (lane == 0) give_up(p, abort_flag, 101);
+                ok = false;
+                break;
+              }
+              if (ptx::elect_one()) {
+                if (rank == 0) ptx::mbar_arrive_expect_tx(&full_bar[stage], bytes);
+                uint8_t* to = smem + stage * kStageBytes + kLeftBytes;
+                if (KIND == kExpandW4) {
+                  ptx::tma_load_2d_pair(to, &p.right, &full_bar[stage], (kk + h) * kStep, col0);
+                } else {
+                  for (int b = 0; b < boxes; ++b)
+                    ptx::tma_load_2d_pair(to + b * kRightBlock, &p.right, &full_bar[stage], col0 + b * 64, kk * kStep);
+                }
+              }
+              __syncwarp();
+            }
+            if (++stage == kStages) { stage = 0; phase ^= 1u; }
+          }
         }
       }
     } else if (warp == 1 && rank == 0) {
@@ -346,7 +469,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
         }
       }
     }
-    else if (warp == 1) {
+    else {
       // ---- passes on to the leader that the peer's left tile is written.  The converters themselves would have to release
       // at cluster scope, which waits for the loads that they have in flight.
       uint32_t stage = 0, phase = 0;
@@ -364,92 +487,27 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
           if (++stage == kStages) { stage = 0; phase ^= 1u; }
         }
       }
-    } else if (warp == 3) {
-      // ---- loader of codes (TMA) and tables (small asynchronous copies)
-      if (lane == 0) ptx::prefetch_tmap(&p.codes_map);
-      uint32_t stage = 0, phase = 0;
-      bool ok = true;
-      const int blocks = w4_blocks(p.depth), tiles = w4_row_tiles(p.rows);
-      for (int u = pair; ok && u < units; u += pairs) {
-        const ExpandUnit w = expand_unit(p, u);
-        const int row0 = w.row0 + static_cast<int>(rank) * kCtaRows;
-        for (int kk = w.k0; kk < w.k1; kk += KIND == kExpandW4 ? 2 : 1) {
-          if (!ptx::mbar_wait_warp<false>(&raw_empty[stage], phase ^ 1u, abort_flag, p.wait_ns)) {
-            if (lane == 0) give_up(p, abort_flag, 101);
-            ok = false;
-            break;
-          }
-          const uint32_t table = ptx::smem_u32(tables + stage * kTable);
-          if (ptx::elect_one()) {
-            ptx::mbar_arrive_expect_tx(&raw_full[stage], kRawBytes);
-            if (KIND == kExpandW4) ptx::tma_load_2d(raw + stage * kRawBytes, &p.codes_map, &raw_full[stage], kk / 2 * 256, row0 / kW4Rows);
-            else ptx::tma_load_2d(raw + stage * kRawBytes, &p.codes_map, &raw_full[stage], row0, kk * kStep);
-          }
-          __syncwarp();
-          if (KIND == kExpandW4) {
-            // 2 PER pieces of 16 bytes of scales for each of the eight row tiles, then PER of zeros
-            for (int i = lane; i < 24 * PER; i += 32) {
-              const bool zero = i >= 16 * PER;
-              const int j = zero ? i - 16 * PER : i, each = zero ? PER : 2 * PER;
-              const int tile = row0 / kW4Rows + j / each;
-              const bool real = tile < tiles && (!zero || p.zeros);
-              const long long at = (static_cast<long long>(tile) * blocks + kk / 2) * each + j % each;
-              const uint8_t* from = zero ? p.zeros : static_cast<const uint8_t*>(p.scales);
-              copy_async_16(table + i * 16, real ? from + at * 16 : static_cast<const uint8_t*>(p.scales), real);
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const long long tok = static_cast<long long>(kk) * kStep + lane + 32 * i;
-              const bool real = tok < p.depth && row0 < p.rows;
-              copy_async_4(table + (lane + 32 * i) * 4, real ? p.exps + tok * p.exp_pitch + row0 / kActBlock : p.exps, real);
-            }
-          }
-          copy_async_arrive(&raw_full[stage]);
-          if (++stage == kRawStages) { stage = 0; phase ^= 1u; }
-        }
-      }
     }
   } else if (warp < 12) {
     // ---- epilogue: warp = 32 rows (of its lane quarter) x half of the tile's columns
     regs_inc<kRegsEpilogue>();
-    const int e = warp - 4, quarter = warp & 3, side = e >> 2;
-    float* swap = transpose + e * (kTransposeBytes / 4);
-    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+    const int quarter = warp & 3, side = (warp - 4) >> 2;
+    const uint32_t swap = ptx::smem_u32(transpose) + (warp - 4) * kTransposeBytes;
+    const uint32_t tmem = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + side * half;
     uint32_t slot = 0, full_bits = 0;
     bool ok = true;
     for (int u = pair; ok && u < units; u += pairs) {
       const ExpandUnit w = expand_unit(p, u);
       const int row0 = w.row0 + static_cast<int>(rank) * kCtaRows + quarter * 32;
       const int col0 = w.col0 + side * half;
+      const int ncols = min(half, p.cols - col0), nrows = min(32, p.rows - row0);  // at most 0: outside
       float sum[128];
 #pragma unroll
       for (int i = 0; i < 128; ++i) sum[i] = 0.f;
       if (KIND == kExpandAct8 && p.base && p.slices == 1) {
-        // the sums start from the base, which is read while the tile's first MMAs run: 32 rows of 32 neighbours at a
-        // time, which then change places between lanes and registers
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          if (c * 32 < half) {
-            const int col = col0 + c * 32 + lane;
-            const bool in = c * 32 + lane < half && col < p.cols;
-            float v[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const long long row = row0 + i;
-              v[i] = 0.f;
-              if (in && row < p.rows)
-                v[i] = p.out_f32 ? static_cast<const float*>(p.base)[row * p.ldbase + col]
-                                 : to_f32(static_cast<const T*>(p.base)[row * p.ldbase + col]);
-            }
-#pragma unroll
-            for (int i = 0; i < 32; ++i) swap[i * 32 + (lane ^ i)] = v[i];
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) sum[c * 32 + i] = swap[lane * 32 + (i ^ lane)];
-            __syncwarp();
-          }
-        }
+        // the sums start from the base, which is read while the tile's first MMAs run
+        if (p.out_f32) load_tile_rows(sum, static_cast<const float*>(p.base), p.ldbase, row0, col0, nrows, ncols, swap, lane);
+        else load_tile_rows(sum, static_cast<const T*>(p.base), p.ldbase, row0, col0, nrows, ncols, swap, lane);
       }
       for (int kk = w.k0; kk < w.k1; kk += kSubSteps) {
         if (!ptx::mbar_wait_warp<false>(&slot_full[slot], (full_bits >> slot) & 1u, abort_flag, p.wait_ns)) {
@@ -459,15 +517,15 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
         }
         full_bits ^= 1u << slot;
         ptx::tc_fence_after_sync();
-        const uint32_t from = tmem_base + lanes + slot * kMaxCols + side * half;
+        const uint32_t from = tmem + slot * kMaxCols;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          if (c * 16 < half) {
-            uint32_t r[16];
-            tmem_ld_32x16(from + c * 16, r);
+        for (int c = 0; c < 16; ++c) {
+          if (c * 8 < half) {
+            uint32_t r[8];
+            tmem_ld_32x8(from + c * 8, r);
             ptx::tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sum[c * 16 + i] += __uint_as_float(r[i]);
+            for (int i = 0; i < 8; ++i) sum[c * 8 + i] += __uint_as_float(r[i]);
           }
         }
         ptx::tc_fence_before_sync();
@@ -477,44 +535,12 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
       }
       if (!ok) break;
       if (KIND == kExpandW4) {
-        // a column of the tile is a row of y: 32 lanes store 32 neighbours
-        const int row = row0 + lane;
-        float* part = p.part + static_cast<long long>(w.slice) * p.rows * p.cols;
-#pragma unroll
-        for (int c = 0; c < 128; ++c) {
-          if (c < half && col0 + c < p.cols && row < p.rows) {
-            if (p.slices > 1) part[static_cast<long long>(col0 + c) * p.rows + row] = sum[c];
-            else static_cast<T*>(p.out)[(col0 + c) * p.ldo + row] = from_f32<T>(sum[c]);
-          }
-        }
+        if (p.slices > 1) store_tile_cols(sum, p.part + static_cast<long long>(w.slice) * p.rows * p.cols, p.rows, row0, col0, nrows, ncols, lane);
+        else store_tile_cols(sum, static_cast<T*>(p.out), p.ldo, row0, col0, nrows, ncols, lane);
       } else {
-        float* part = p.part + static_cast<long long>(w.slice) * p.rows * p.cols;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          if (c * 32 < half) {
-            // 32 x 32 values change places between lanes and registers, so that a row leaves as neighbours
-#pragma unroll
-            for (int i = 0; i < 32; ++i) swap[lane * 32 + (i ^ lane)] = sum[c * 32 + i];
-            __syncwarp();
-            const int col = col0 + c * 32 + lane;
-            const bool in = c * 32 + lane < half && col < p.cols;
-#pragma unroll 8
-            for (int i = 0; i < 32; ++i) {
-              const long long row = row0 + i;
-              if (in && row < p.rows) {
-                const float v = swap[i * 32 + (lane ^ i)];
-                if (p.slices > 1) {
-                  part[row * p.cols + col] = v;
-                } else if (p.out_f32) {
-                  static_cast<float*>(p.out)[row * p.ldo + col] = v;
-                } else {
-                  static_cast<T*>(p.out)[row * p.ldo + col] = from_f32<T>(v);
-                }
-              }
-            }
-            __syncwarp();
-          }
-        }
+        if (p.slices > 1) store_tile_rows(sum, p.part + static_cast<long long>(w.slice) * p.rows * p.cols, p.cols, row0, col0, nrows, ncols, swap, lane);
+        else if (p.out_f32) store_tile_rows(sum, static_cast<float*>(p.out), p.ldo, row0, col0, nrows, ncols, swap, lane);
+        else store_tile_rows(sum, static_cast<T*>(p.out), p.ldo, row0, col0, nrows, ncols, swap, lane);
       }
     }
   } else {
@@ -550,11 +576,12 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
     for (int u = pair; ok && u < units; u += pairs) {
       const ExpandUnit w = expand_unit(p, u);
       if (KIND == kExpandW4) {
-        // Four pieces a thread and tile of 128 inputs: 16 bytes (four words) of a row.  Words 0 and 1 belong to the first
-        // step, 2 and 3 to the second.  Lanes of odd rows store the second word of a step first, so that eight
-        // lanes always hit eight different 16-byte columns of the swizzled tile.
+        // A thread takes four pieces of a tile of 128 inputs: 16 bytes (four words) of a row.  Words 0 and 1 belong to the first
+        // step, 2 and 3 to the second.  Lanes of odd rows take the second word of a step first, so that eight
+        // lanes always store to eight different 16-byte columns of the swizzled tile.
         const int g = lane >> 2, t = lane & 3, odd = g & 1;
         const int row0 = (tid >> 6) * kW4Rows + 8 * ((tid >> 5) & 1) + g;  // of the first piece; the others 32 rows on
+        const uint32_t line0 = row0 * 128 + (((4 * odd + t) ^ g) << 4), line1 = row0 * 128 + (((4 * (1 - odd) + t) ^ g) << 4);
         for (int kk = w.k0; kk < w.k1; kk += 2) {
           turn ^= 1u;
           if (turn == 0) {
@@ -565,43 +592,50 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
           }
           if (!raw_ready()) { ok = false; break; }
           const uint32_t from = codes + rstage * kRawBytes + tid * 16;
-          const uint8_t* table = tables + rstage * kTable;
+          const uint32_t table = ptx::smem_u32(tables) + rstage * kTable;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            uint2 c[4];
-            uint32_t bias[4][2], scale[4][2];
+            uint32_t word[kPieces][2], bias[kPieces][2], scale[kPieces][2];  // [piece][first, second to be stored]
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              c[i] = lds_v2(from + i * 2048 + h * 8);
+            for (int i = 0; i < kPieces; ++i) {
+              const uint2 c = lds_v2(from + i * (kRawBytes / kPieces) + h * 8);
+              word[i][0] = odd ? c.y : c.x;
+              word[i][1] = odd ? c.x : c.y;
 #pragma unroll
               for (int j = 0; j < 2; ++j) {
                 if (PER < 4 && j == 1) { bias[i][1] = bias[i][0]; scale[i][1] = scale[i][0]; continue; }
-                const int at = (row0 + 32 * i) * PER + (2 * h + j) * PER / 4;
-                const uint32_t s = reinterpret_cast<const uint16_t*>(table)[at];
-                const uint32_t z = p.zeros ? table[kCtaRows * 2 * PER + at] : 8u;
-                scale[i][j] = s | (s << 16);
-                bias[i][j] = Half<T>::magic + (z | (z << 16));
+                const int at = (row0 + (kCtaRows / kPieces) * i) * PER + (PER == 4 ? 2 * h + (j ^ odd) : PER == 2 ? h : 0);
+                const uint32_t s = lds_u16(table + 2 * at), z = p.zeros ? lds_u8(table + kCtaRows * 2 * PER + at) : 8u;
+                scale[i][j] = __byte_perm(s, 0, 0x1010);
+                bias[i][j] = Half<T>::magic + __byte_perm(z, 0, 0x4040);
               }
             }
             if (!acquire()) { ok = false; break; }
             const uint32_t to = left + stage * kStageBytes;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint4 v0 = expand_w4<T>(c[i].x, bias[i][0], scale[i][0]), v1 = expand_w4<T>(c[i].y, bias[i][1], scale[i][1]);
-              const uint32_t line = to + (row0 + 32 * i) * 128;
-              ptx::sts_v4(line + (((4 * odd + t) ^ (g & 7)) << 4), odd ? v1 : v0);
-              ptx::sts_v4(line + (((4 * (1 - odd) + t) ^ (g & 7)) << 4), odd ? v0 : v1);
-            }
+            for (int i = 0; i < kPieces; ++i)
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+                ptx::sts_v4(to + i * (kLeftBytes / kPieces) + (j ? line1 : line0), expand_w4<T>(word[i][j], bias[i][j], scale[i][j]));
             publish();
           }
           if (!ok) break;
           raw_done();
         }
       } else {
-        // Four pieces a thread and step: 16 channels of a token.  Eight neighbouring lanes hold a token's 128 channels; those
-        // of the second 64 store their second half first, which keeps eight lanes on eight different 16-byte columns.
-        const int piece = tid & 7, second = piece >> 2, token = tid >> 3;  // tokens 16 apart
-        const int at = 2 * (piece & 3);
+        // A thread takes four pieces of a step: 16 channels of a token, of the first 64 channels or the second.  Of eight
+        // neighbouring lanes four hold the first 64 channels of one token and four the second 64 of the token beside it:
+        // loads and stores then touch eight different 16-byte columns.
+        const int quarter = tid & 3, block = (tid >> 2) & 1, piece = quarter + 4 * block;
+        uint32_t from[2], exponent[2], line[2][2];  // of the first two pieces; the others 32 tokens on
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int token = 2 * (tid >> 3) + (block ^ i);
+          from[i] = token * 128 + piece * 16;
+          exponent[i] = token * 4 + (piece >> 1);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) line[i][j] = block * kRightBlock + token * 128 + (((2 * quarter + j) ^ (token & 7)) << 4);
+        }
         for (int kk = w.k0; kk < w.k1; ++kk) {
           turn ^= 1u;
           if (turn == 0) {
@@ -610,21 +644,20 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
             continue;
           }
           if (!raw_ready()) { ok = false; break; }
-          uint4 c[4];
-          uint32_t e[4];
+          uint4 c[kPieces];
+          uint32_t e[kPieces];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            c[i] = ptx::lds_v4(codes + rstage * kRawBytes + tid * 16 + i * 2048);
-            e[i] = tables[rstage * kTable + (token + 16 * i) * 4 + (piece >> 1)];
+          for (int i = 0; i < kPieces; ++i) {
+            c[i] = ptx::lds_v4(codes + rstage * kRawBytes + from[i & 1] + (i >> 1) * (32 * 128));
+            e[i] = lds_u8(ptx::smem_u32(tables) + rstage * kTable + exponent[i & 1] + (i >> 1) * (32 * 4));
           }
           if (!acquire()) { ok = false; break; }
-          const uint32_t to = left + stage * kStageBytes + second * kRightBlock + token * 128;
+          const uint32_t to = left + stage * kStageBytes;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int i = 0; i < kPieces; ++i) {
             const Act8Step<T> step(e[i]);
-            const uint4 lo = expand_act8<T>(c[i].x, c[i].y, step), hi = expand_act8<T>(c[i].z, c[i].w, step);
-            ptx::sts_v4(to + i * 2048 + (((at + second) ^ (token & 7)) << 4), second ? hi : lo);
-            ptx::sts_v4(to + i * 2048 + (((at + 1 - second) ^ (token & 7)) << 4), second ? lo : hi);
+            ptx::sts_v4(to + line[i & 1][0] + (i >> 1) * (32 * 128), expand_act8<T>(c[i].x, c[i].y, step));
+            ptx::sts_v4(to + line[i & 1][1] + (i >> 1) * (32 * 128), expand_act8<T>(c[i].z, c[i].w, step));
           }
           raw_done();
           publish();
