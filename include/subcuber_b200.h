@@ -311,7 +311,7 @@ int sb200_w4_pack(int dtype, const void* q, long long ldq, const void* q_scales,
 /* out[n][k] = W rounded once to `dtype`. */
 int sb200_w4_dequantize(int dtype, const void* codes, const void* scales, const void* zeros, int n, int k, int group, void* out,
                         long long ldo, sb200_stream_t stream);
-/* y[m][n] = sum over k of x[m][k] W[n][k], sums in fp32, rounded once to `dtype`.  Up to 32 rows the codes are multiplied
+/* y[m][n] = sum over k of x[m][k] W[n][k], sums in fp32, rounded once to `dtype`.  Up to 8 rows the codes are multiplied
  * exactly and the scales applied in fp32; with more the weights are rounded to `dtype` first (as sb200_w4_dequantize does).
  * x_aligned: the rows of x start on 16 bytes (pointer and ldx); else the workspace holds a copy of x.  A workspace for m rows
  * serves every smaller m. */

@@ -1,5 +1,6 @@
 // Host side of the products with an expanded operand: how a product is cut, workspace, launches.
 #include "expand_product.cuh"
+#include "w4_decode.cuh"
 
 #include "lowbit_host.h"
 #include "per_device.h"
@@ -45,7 +46,7 @@ int pairs_of_device() {
 }
 
 size_t part_bytes(long long rows, long long cols) {
-  const size_t all = size_t(kMaxSlices) * rows * cols * 4;
+  const size_t all = align_up(size_t(kMaxSlices) * rows * cols * 4, 256);
   return all < kPartBytes ? all : kPartBytes;
 }
 
@@ -117,19 +118,15 @@ int run_act8(const ExpandParams& p, int pairs, cudaStream_t stream) {
 }
 
 constexpr unsigned long long kWaitNs = 2000000000ull;  // bound of every device-side wait
-constexpr size_t kStatusBytes = 256;
-
-size_t copy_bytes(long long rows, int cols, bool is_aligned) {
-  return is_aligned ? 0 : align_up(size_t(rows) * align_up(cols, 8) * 2, 256);
-}
 
 }  // namespace
 
 size_t expand_w4_workspace(int m, int n, int k, bool x_aligned) {
-  return kStatusBytes + copy_bytes(m, k, x_aligned) + part_bytes(m, n);
+  return kStatusBytes + (x_aligned ? 0 : copy_bytes(m, k)) + (m > kDecodeMaxRows ? part_bytes(m, n) : 0);
 }
 
-int expand_w4(const W4& w, const void* x, long long ldx, void* y, long long ldy, int m, void* workspace, cudaStream_t stream) {
+int expand_w4(const W4& w, const void* x, long long ldx, void* y, long long ldy, int m, void* workspace, size_t workspace_bytes,
+              cudaStream_t stream) {
   ExpandParams p = {};
   p.scales = w.scales;
   p.zeros = static_cast<const uint8_t*>(w.zeros);
@@ -142,18 +139,10 @@ int expand_w4(const W4& w, const void* x, long long ldx, void* y, long long ldy,
   p.wait_ns = kWaitNs;
   char* ws = static_cast<char*>(workspace);
   p.status = reinterpret_cast<int*>(ws);
-  ws += kStatusBytes;
-  int rc;
-  if (!tma_rows(x, ldx)) {
-    const int cols = static_cast<int>(align_up(w.k, 8));
-    if ((rc = tc::copy_rows_16bit(ws, cols, x, m, w.k, ldx, stream))) return rc;
-    x = ws;
-    ldx = cols;
-    ws += copy_bytes(m, w.k, false);
-  }
-  p.part = reinterpret_cast<float*>(ws);
+  p.part = reinterpret_cast<float*>(ws + (workspace_bytes - part_bytes(m, w.n)) / 256 * 256);
   const int pairs = place(p, pairs_of_device());
   if (!pairs) return kErrNotSupported;
+  int rc;
   if ((rc = tc::map_rows_16bit(&p.right, x, m, w.k, ldx, p.bn / 2))) return rc;
   // a row tile's codes are one row of 32-bit words; a box is 128 inputs of eight row tiles
   if ((rc = tc::map_rows_plain(&p.codes_map, w.codes, 4, w4_row_tiles(w.n), 256ll * w4_blocks(w.k), 1024ll * w4_blocks(w.k), 8, 256)))
@@ -161,8 +150,67 @@ int expand_w4(const W4& w, const void* x, long long ldx, void* y, long long ldy,
   return w.dtype == kF16 ? run_w4<__half>(p, w.group, pairs, stream) : run_w4<__nv_bfloat16>(p, w.group, pairs, stream);
 }
 
+namespace {
+
+// CTAs that divide the inputs of 128 rows: as many as keep the grid within two CTAs for each SM.
+int decode_ranks(int n, int blocks) {
+  const int sms = sm_count_of_current_device();
+  const int room = 2 * (sms > 0 ? sms : 148), groups = ceil_div(n, kDecodeRows);
+  int ranks = 8;
+  while (ranks > 1 && (groups * static_cast<long long>(ranks) > room || ranks > blocks)) ranks /= 2;
+  return ranks;
+}
+
+template <typename T, int PER>
+int launch_decode(const DecodeParams& p, int ranks, cudaStream_t stream) {
+  auto* kernel = w4_decode_kernel<T, PER>;
+  static PerDeviceOnce attr;
+  const int rc = attr.run_once([&] {
+    return static_cast<int>(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, decode_smem(PER, kDecodeMaxRight)));
+  });
+  if (rc) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(ceil_div(p.n, kDecodeRows) * ranks));
+  cfg.blockDim = dim3(kDecodeThreads);
+  cfg.dynamicSmemBytes = decode_smem(PER, p.n16);
+  cfg.stream = stream;
+  cudaLaunchAttribute attrs[1];
+  attrs[0].id = cudaLaunchAttributeClusterDimension;
+  attrs[0].val.clusterDim = {static_cast<unsigned>(ranks), 1, 1};
+  cfg.attrs = attrs;
+  cfg.numAttrs = 1;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, p));
+}
+
+template <typename T>
+int run_decode(const DecodeParams& p, int group, int ranks, cudaStream_t stream) {
+  if (group == 32) return launch_decode<T, 4>(p, ranks, stream);
+  if (group == 64) return launch_decode<T, 2>(p, ranks, stream);
+  return launch_decode<T, 1>(p, ranks, stream);
+}
+
+}  // namespace
+
+int decode_w4(const W4& w, const void* x, long long ldx, void* y, long long ldy, int m, void* status, cudaStream_t stream) {
+  DecodeParams p = {};
+  p.codes = static_cast<const uint8_t*>(w.codes);
+  p.scales = static_cast<const uint8_t*>(w.scales);
+  p.zeros = static_cast<const uint8_t*>(w.zeros);
+  p.y = y;
+  p.ldy = ldy;
+  p.m = m;
+  p.n = w.n;
+  p.blocks = w4_blocks(w.k);
+  p.n16 = ceil_div(m, 16) * 16;
+  p.status = static_cast<int*>(status);
+  p.wait_ns = kWaitNs;
+  if (int rc = tc::map_rows_16bit(&p.right, x, m, w.k, ldx, p.n16)) return rc;
+  const int ranks = decode_ranks(w.n, p.blocks);
+  return w.dtype == kF16 ? run_decode<__half>(p, w.group, ranks, stream) : run_decode<__nv_bfloat16>(p, w.group, ranks, stream);
+}
+
 size_t expand_act8_workspace(int m, int n, int k, bool dy_aligned) {
-  return kStatusBytes + copy_bytes(m, n, dy_aligned) + part_bytes(k, n);
+  return kStatusBytes + (dy_aligned ? 0 : copy_bytes(m, n)) + part_bytes(k, n);
 }
 
 int expand_act8(const Act8& a, const void* dy, long long lddy, bool out_f32, const void* base, long long ldbase, void* dw,
@@ -191,7 +239,7 @@ int expand_act8(const Act8& a, const void* dy, long long lddy, bool out_f32, con
       if ((rc = tc::copy_rows_16bit(ws, cols, dy, a.m, n, lddy, stream))) return rc;
       dy = ws;
       lddy = cols;
-      ws += copy_bytes(a.m, n, false);
+      ws += copy_bytes(a.m, n);
     }
     p.part = reinterpret_cast<float*>(ws);
     if (!(pairs = place(p, pairs_of_device()))) return kErrNotSupported;

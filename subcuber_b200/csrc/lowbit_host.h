@@ -30,11 +30,21 @@ inline bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uint
 // Rows of a 16-bit matrix that TMA can read as they are.
 inline bool tma_rows(const void* p, long long ld) { return aligned(p, 16) && ld % 8 == 0; }
 
+// Bytes of a copy of a 16-bit matrix with rows that start on 16 bytes.
+inline size_t copy_bytes(long long rows, int cols) {
+  const size_t row = (static_cast<size_t>(cols) + 7) / 8 * 16;
+  return (static_cast<size_t>(rows) * row + 255) / 256 * 256;
+}
+
 // The products on the tensor cores (expand_product.cu).  Workspace: a status word, a copy of the 16-bit operand where its
-// rows are not aligned, and the parts of a divided reduction.  The bytes asked for grow with m, so that a workspace serves
-// every smaller m.
+// rows are not aligned, and the parts of a divided reduction at its end.  The bytes asked for grow with m, so that a
+// workspace serves every smaller m.
+constexpr size_t kStatusBytes = 256;
+constexpr int kDecodeMaxRows = 64;
 size_t expand_w4_workspace(int m, int n, int k, bool x_aligned);
-int expand_w4(const W4& w, const void* x, long long ldx, void* y, long long ldy, int m, void* workspace, cudaStream_t stream);
+int decode_w4(const W4& w, const void* x, long long ldx, void* y, long long ldy, int m, void* status, cudaStream_t stream);
+int expand_w4(const W4& w, const void* x, long long ldx, void* y, long long ldy, int m, void* workspace, size_t workspace_bytes,
+              cudaStream_t stream);
 size_t expand_act8_workspace(int m, int n, int k, bool dy_aligned);
 int expand_act8(const Act8& a, const void* dy, long long lddy, bool out_f32, const void* base, long long ldbase, void* dw,
                 long long lddw, int n, void* workspace, cudaStream_t stream);

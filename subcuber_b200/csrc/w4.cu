@@ -180,14 +180,12 @@ __global__ void __launch_bounds__(kThreads) w4_dequantize_kernel(const uint8_t* 
 
 template <typename T, int PER>
 int rows_product(const void* x, long long ldx, const W4& w, void* y, long long ldy, int m, cudaStream_t stream) {
-  RowsParams p{x, ldx, static_cast<const uint8_t*>(w.codes), w.scales, static_cast<const uint8_t*>(w.zeros), y, ldy,
-               m, w.n, w.k, w4_blocks(w.k), tma_rows(x, ldx)};
-  // one row tile to a warp where that is at most two blocks an SM, else two (8192 x 8192, one row: 16.6 us, 19.9 with one)
-  if (m <= 8)
-    return w4_row_tiles(w.n) <= 2 * sm_count_of_current_device() ? launch_rows<T, PER, 1, 1, 2>(p, 1, stream)
-                                                                 : launch_rows<T, PER, 1, 2, 2>(p, 1, stream);
-  if (m <= 16) return launch_rows<T, PER, 2, 1, 2>(p, 1, stream);
-  return launch_rows<T, PER, 4, 2, 1>(p, 1, stream);
+  const RowsParams p{x, ldx, static_cast<const uint8_t*>(w.codes), static_cast<const uint8_t*>(w.scales),
+                     static_cast<const uint8_t*>(w.zeros), y, ldy, m, w.n, w.k, w4_blocks(w.k)};
+  // one row tile to a warp while that is at most two blocks for each SM, else two, which read x half as often (one row, 2048 x
+  // 2048: 2.3 us, 3.2 with two; 8192 x 8192: 13.3 us, 14.5 with one; four row tiles were slower everywhere)
+  if (w4_row_tiles(w.n) <= 2 * sm_count_of_current_device()) return launch_rows<T, PER, 1, 1, 4>(p, stream);
+  return launch_rows<T, PER, 2, 1, 3>(p, stream);
 }
 
 template <typename T>
@@ -197,7 +195,9 @@ int rows_product_any(const void* x, long long ldx, const W4& w, void* y, long lo
   return rows_product<T, 1>(x, ldx, w, y, ldy, m, stream);
 }
 
-constexpr int kFewRows = 32;
+// Up to here the codes are multiplied as they are (w4_rows.cuh); a few rows more go to the tensor cores' own instruction
+// (w4_decode.cuh: 16 rows, 8192 x 8192: 18.2 us, and about as much for 64).
+constexpr int kFewRows = 8;
 
 int check(const W4& w) {
   if (w.dtype != kF16 && w.dtype != kBF16) return kErrNotSupported;
@@ -304,7 +304,7 @@ extern "C" int sb200_w4_dequantize(int dtype, const void* codes, const void* sca
 extern "C" size_t sb200_w4_gemm_workspace_bytes(int dtype, int m, int n, int k, int group, int x_aligned) {
   (void)dtype;
   (void)group;
-  if (m <= sb200::lowbit::kFewRows || n <= 0 || k <= 0) return 256;
+  if (n <= 0 || k <= 0 || m <= 0) return 0;
   return sb200::lowbit::expand_w4_workspace(m, n, k, x_aligned != 0);
 }
 
@@ -318,11 +318,19 @@ extern "C" int sb200_w4_gemm(int dtype, const void* x, long long ldx, const void
   if (m == 0) return SB200_OK;
   if (!x || !y) return SB200_ERR_INVALID_PROBLEM;
   if (!aligned(x, 2) || !aligned(y, 2)) return SB200_ERR_MISALIGNED_OPERAND;
-  if (!workspace || !aligned(workspace, 256) ||
-      workspace_bytes < sb200_w4_gemm_workspace_bytes(dtype, m, n, k, group, tma_rows(x, ldx)))
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < expand_w4_workspace(m, n, k, tma_rows(x, ldx)))
     return SB200_ERR_WORKSPACE_NULL;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (m > kFewRows) return expand_w4(w, x, ldx, y, ldy, m, workspace, s);
-  return dtype == sb200::kF16 ? rows_product_any<__half>(x, ldx, w, y, ldy, m, s)
-                              : rows_product_any<__nv_bfloat16>(x, ldx, w, y, ldy, m, s);
+  char* ws = static_cast<char*>(workspace);
+  if (!tma_rows(x, ldx)) {  // every kernel wants rows of x that start on 16 bytes
+    const int cols = (k + 7) / 8 * 8;
+    if (int rc = sb200::tc::copy_rows_16bit(ws + kStatusBytes, cols, x, m, k, ldx, s)) return rc;
+    x = ws + kStatusBytes;
+    ldx = cols;
+  }
+  if (m <= kFewRows)
+    return dtype == sb200::kF16 ? rows_product_any<__half>(x, ldx, w, y, ldy, m, s)
+                                : rows_product_any<__nv_bfloat16>(x, ldx, w, y, ldy, m, s);
+  if (m <= kDecodeMaxRows) return decode_w4(w, x, ldx, y, ldy, m, workspace, s);
+  return expand_w4(w, x, ldx, y, ldy, m, workspace, workspace_bytes, s);
 }

@@ -1,4 +1,4 @@
-// y = x W^T for a few rows of x (a decoding batch), weights in format W4: bound by the bytes of the weights.
+// y = x W^T for up to 8 rows of x, weights in format W4: bound by the bytes of the weights.
 //
 // Mathematics.  Codes are small whole numbers and exact in 16 bits, so that the matrix instruction multiplies (code -
 // zero) with x without any rounding; the sums of one group are scaled in fp32 afterwards:
@@ -6,16 +6,20 @@
 // A 4-bit code becomes a 16-bit number by bits alone: OR-ed into the last bits of 1024 (f16) or 128 (bf16) it adds exactly
 // its value, and one packed subtraction of (1024 | 128) + zero leaves code - zero, for two codes at a time.
 //
-// Split.  A warp holds RT row tiles (16 weights' rows each) and walks over tiles of 128 inputs, one 16-byte load per lane and
-// eight rows; the weights are the left operand of mma.m16n8k16 (16 rows x 16 inputs) and 8 NT rows of x the right one.  The
-// order of inputs inside an instruction is free as long as both operands have the same: a lane takes its word's eight
-// inputs as they lie in memory.  The warps of a block take the tiles of 128 inputs in turn, and where there are few row
-// tiles the CTAs of a cluster divide them further: the sums meet in shared memory, in the order of warps and ranks, so
-// that results do not change from call to call.
+// Split.  A warp walks over tiles of 16 rows x 128 inputs: the weights are the left operand of mma.m16n8k16 (16 rows x 16
+// inputs) and 8 rows of x the right one.  The order of inputs inside an instruction is free as long as both operands
+// have the same, so a lane takes its word's eight inputs as they lie in memory.  The eight warps of a block are WR rows of RT
+// row tiles x 8 / WR parts of the inputs, which they take in turn; their sums meet in shared memory in the order of the
+// warps, so that results do not change from call to call.
+//
+// Memory.  The kernel lives from bytes in flight (6.5 TB/s at about 1 us of latency under load are 44 KB for each SM), and
+// registers do not hold them: every warp has a ring of AHEAD stages in shared memory that it fills with 16-byte asynchronous
+// copies of its own, so that no barrier but the warp's own is needed.  Copies of x go through the first-level cache,
+// where the WR warps that work on the same inputs find them.
 #pragma once
-#include <cooperative_groups.h>
-
 #include "lowbit_format.cuh"
+#include "per_device.h"
+#include "ptx.cuh"
 
 namespace sb200 {
 namespace lowbit {
@@ -30,6 +34,10 @@ template <> struct Pair16<__half> {
     const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&r);
   }
+  // Codes 2 q and 2 q + 1 (in the order of the inputs) of a word, minus the zero point.
+  static __device__ __forceinline__ uint32_t code(uint32_t w, int q, uint32_t bias) {
+    return sub(((w >> (4 * q)) & 0x000f000fu) | magic, bias);
+  }
   static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -42,6 +50,9 @@ template <> struct Pair16<__nv_bfloat16> {
     const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
     return *reinterpret_cast<const uint32_t*>(&r);
   }
+  static __device__ __forceinline__ uint32_t code(uint32_t w, int q, uint32_t bias) {
+    return sub(((w >> (4 * q)) & 0x000f000fu) | magic, bias);
+  }
   static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -50,202 +61,175 @@ template <> struct Pair16<__nv_bfloat16> {
 };
 
 struct RowsParams {
-  const void* x;
+  const void* x;   // rows on 16 bytes
   long long ldx;
   const uint8_t* codes;
-  const void* scales;
+  const uint8_t* scales;
   const uint8_t* zeros;  // or null
   void* y;
   long long ldy;
   int m, n, k, blocks;
-  bool wide;  // rows of x start on 16 bytes
 };
 
-// What a lane needs of one row tile and 128 inputs: rows g and g + 8.
-template <int PER>  // groups in 128 inputs
-struct TileRaw {
-  uint4 w[2];
-  uint32_t s[2][(PER + 1) / 2];  // scales, two to a register
-  uint32_t z[2];                 // zeros, one to a byte
-};
-
-template <typename T, int PER>
-__device__ __forceinline__ void load_tile(TileRaw<PER>& t, const RowsParams& p, long long tile, int lane) {
-  const uint4* w = reinterpret_cast<const uint4*>(p.codes) + tile * (kW4TileBytes / 16) + lane;
-  t.w[0] = __ldcs(w);
-  t.w[1] = __ldcs(w + 32);
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const long long at = (tile * kW4Rows + 8 * h + (lane >> 2)) * PER;
-    const uint16_t* s = static_cast<const uint16_t*>(p.scales) + at;
-    if (PER == 1) t.s[h][0] = __ldg(s);
-    if (PER == 2) t.s[h][0] = __ldg(reinterpret_cast<const uint32_t*>(s));
-    if (PER == 4) {
-      const uint2 v = __ldg(reinterpret_cast<const uint2*>(s));
-      t.s[h][0] = v.x;
-      t.s[h][PER / 4] = v.y;
-    }
-    t.z[h] = 0x08080808u;
-    if (p.zeros) {
-      if (PER == 1) t.z[h] = __ldg(p.zeros + at);
-      if (PER == 2) t.z[h] = __ldg(reinterpret_cast<const uint16_t*>(p.zeros + at));
-      if (PER == 4) t.z[h] = __ldg(reinterpret_cast<const uint32_t*>(p.zeros + at));
-    }
-  }
+__device__ __forceinline__ void rows_copy_cg(uint32_t to, const void* from, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void rows_copy_ca(uint32_t to, const void* from, int bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ uint32_t rows_lds(uint32_t a, int bytes) {
+  uint32_t v;
+  uint16_t h;
+  if (bytes == 4) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+  else if (bytes == 2) { asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(a)); v = h; }
+  else asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(a));
+  return v;
 }
 
-template <typename T>
-__device__ __forceinline__ float scale_of(uint32_t two, int which) {
-  const uint16_t bits = static_cast<uint16_t>(two >> (16 * which));
-  return to_f32(*reinterpret_cast<const T*>(&bits));
-}
+// Bytes of a stage: codes, scales and zeros of RT row tiles, then 128 inputs of eight rows of x.
+__host__ __device__ constexpr int rows_tile_bytes(int per) { return kW4TileBytes + kW4Rows * 3 * per; }
+__host__ __device__ constexpr int rows_stage_bytes(int per, int rt) { return rt * rows_tile_bytes(per) + 8 * 256; }
+__host__ __device__ constexpr int rows_smem(int per, int rt, int ahead) { return kRowWarps * ahead * rows_stage_bytes(per, rt); }
 
-// Eight inputs of a row of x, zeros behind its end.
-template <typename T>
-__device__ __forceinline__ uint4 load_x(const T* row, int k0, int k, bool wide) {
-  if (wide && k0 + 8 <= k) return __ldg(reinterpret_cast<const uint4*>(row + k0));
-  uint4 r;
-  uint16_t v[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = k0 + i < k ? __ldg(reinterpret_cast<const uint16_t*>(row) + k0 + i) : uint16_t(0);
-  r.x = v[0] | (v[1] << 16); r.y = v[2] | (v[3] << 16); r.z = v[4] | (v[5] << 16); r.w = v[6] | (v[7] << 16);
-  return r;
-}
-
-template <typename T, int PER, int NT, int RT, int AHEAD>
+template <typename T, int PER, int RT, int WR, int AHEAD, bool ZEROS>
 __global__ void __launch_bounds__(kRowThreads) w4_rows_kernel(const RowsParams p) {
-  namespace cg = cooperative_groups;
-  __shared__ float part[kRowWarps][NT * 8][RT * 16 + 1];
-  cg::cluster_group cluster = cg::this_cluster();
-  const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  constexpr int WK = kRowWarps / WR;
+  constexpr int kTile = rows_tile_bytes(PER), kStage = rows_stage_bytes(PER, RT);
+  static_assert(kRowWarps * 8 * (RT * 16 + 1) * 4 <= rows_smem(PER, RT, AHEAD), "the sums reuse the rings");
+  extern __shared__ __align__(128) uint8_t smem_rows[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int tile0 = static_cast<int>(blockIdx.x / ranks) * RT;  // first row tile
-  const int tiles = w4_row_tiles(p.n);
-  const int m0 = blockIdx.y * (NT * 8);
-  const int first = rank * kRowWarps + warp, stride = ranks * kRowWarps;
-  float total[RT][NT][4] = {};
-  // a block's last row tiles may lie behind the weights: they read the last one and are not stored
-  long long base[RT];
-#pragma unroll
-  for (int r = 0; r < RT; ++r) base[r] = static_cast<long long>(min(tile0 + r, tiles - 1)) * p.blocks;
+  const int wk = warp % WK, wr = warp / WK;
+  const int tile0 = (static_cast<int>(blockIdx.x) * WR + wr) * RT;  // first row tile of the warp
+  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem_rows)) + warp * (AHEAD * kStage);
 
-  TileRaw<PER> raw[AHEAD][RT];
+  // where this lane's copies come from; they move on by WK tiles of 128 inputs
+  const uint8_t *codes[RT], *table[RT];
+  const bool copies_table = lane < 2 * PER || (ZEROS && lane < 3 * PER);  // 2 PER pieces of scales, PER of zeros
+  const int table_step = WK * kW4Rows * PER * (lane < 2 * PER ? 2 : 1);
 #pragma unroll
-  for (int a = 0; a < AHEAD; ++a)
-#pragma unroll
-    for (int r = 0; r < RT; ++r)
-      if (first + a * stride < p.blocks) load_tile<T, PER>(raw[a][r], p, base[r] + first + a * stride, lane);
-
-  for (int b0 = first; b0 < p.blocks; b0 += AHEAD * stride) {
-#pragma unroll
-    for (int a = 0; a < AHEAD; ++a) {
-      const int b = b0 + a * stride;
-      if (b >= p.blocks) break;
-      uint4 xv[NT][4];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const int row = m0 + nt * 8 + g;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          xv[nt][j] = make_uint4(0, 0, 0, 0);
-          if (row < p.m) xv[nt][j] = load_x(static_cast<const T*>(p.x) + row * p.ldx, b * kW4Block + 32 * j + 8 * t, p.k, p.wide);
-        }
-      }
-      TileRaw<PER> cur[RT];
+  for (int r = 0; r < RT; ++r) {
+    // row tiles behind the weights read the last one and are not stored
+    const long long tile = static_cast<long long>(min(tile0 + r, w4_row_tiles(p.n) - 1)) * p.blocks + wk;
+    codes[r] = p.codes + tile * kW4TileBytes + lane * 16;
+    table[r] = lane < 2 * PER ? p.scales + tile * (kW4Rows * 2 * PER) + lane * 16
+                              : p.zeros + tile * (kW4Rows * PER) + (lane - 2 * PER) * 16;
+  }
+  // Piece (row, c) of 16 of a row of x: eight inputs.  Odd rows keep their upper and lower eight pieces the other way
+  // round, so that eight lanes read eight different 16-byte columns.  Rows from m on are not copied: what the ring holds
+  // there reaches columns of the result that are not stored.
+  const int xc = lane & 15, xrow = lane >> 4;
+  const T* x = static_cast<const T*>(p.x) + xrow * p.ldx;
+  int fetch_k = wk * kW4Block + xc * 8, fetch_b = wk, fill = 0;
+  auto fetch = [&]() {
+    if (fetch_b < p.blocks) {
+      const uint32_t to = ring + fill * kStage;
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
-        cur[r] = raw[a][r];
-        if (b + AHEAD * stride < p.blocks) load_tile<T, PER>(raw[a][r], p, base[r] + b + AHEAD * stride, lane);
+        rows_copy_cg(to + r * kTile + lane * 16, codes[r], 16);
+        rows_copy_cg(to + r * kTile + 512 + lane * 16, codes[r] + 512, 16);
+        if (copies_table) rows_copy_cg(to + r * kTile + kW4TileBytes + lane * 16, table[r], 16);
+        codes[r] += WK * kW4TileBytes;
+        table[r] += table_step;
       }
+      const int left = min(max(p.k - fetch_k, 0), 8) * 2;
+      const T* from = x + (left ? fetch_k : 0);
 #pragma unroll
-      for (int r = 0; r < RT; ++r) {
+      for (int i = 0; i < 4; ++i)
+        if (2 * i + xrow < p.m)
+          rows_copy_ca(to + RT * kTile + (2 * i + xrow) * 256 + ((xc ^ (xrow << 2)) << 4), from + 2 * i * p.ldx, left);
+    }
+    fetch_b += WK;
+    fetch_k += WK * kW4Block;
+    fill = fill + 1 == AHEAD ? 0 : fill + 1;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+
+  float total[RT][4] = {};
 #pragma unroll
-        for (int gr = 0; gr < PER; ++gr) {
-          float acc[NT][4] = {};
-          uint32_t bias[2];
+  for (int a = 0; a < AHEAD - 1; ++a) fetch();
+  int stage = 0;
+  const uint32_t xat = g * 256 + ((t ^ ((g & 1) << 2)) << 4);  // of word 0; word j is 64 j further, exclusive-or
+  for (int b = wk; b < p.blocks; b += WK) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 2) : "memory");
+    __syncwarp();  // every lane's copies of this stage are there, and all have read the stage that is filled next
+    fetch();
+    const uint32_t at = ring + stage * kStage;
+    stage = stage + 1 == AHEAD ? 0 : stage + 1;
+    uint4 xv[4];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t z = (cur[r].z[h] >> (8 * gr)) & 255u;
-            bias[h] = Pair16<T>::magic + (z | (z << 16));
-          }
+    for (int j = 0; j < 4; ++j) xv[j] = ptx::lds_v4(at + RT * kTile + (xat ^ (j << 6)));
 #pragma unroll
-          for (int jj = 0; jj < 4 / PER; ++jj) {
-            const int j = gr * (4 / PER) + jj;
-            const uint32_t lo = (&cur[r].w[0].x)[j], hi = (&cur[r].w[1].x)[j];
-            uint32_t e[4][2];
+    for (int r = 0; r < RT; ++r) {
+      const uint32_t tile = at + r * kTile;
+      const uint4 lo4 = ptx::lds_v4(tile + lane * 16), hi4 = ptx::lds_v4(tile + 512 + lane * 16);
+      const uint32_t lo[4] = {lo4.x, lo4.y, lo4.z, lo4.w}, hi[4] = {hi4.x, hi4.y, hi4.z, hi4.w};
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              e[q][0] = Pair16<T>::sub(((lo >> (4 * q)) & 0x000f000fu) | Pair16<T>::magic, bias[0]);
-              e[q][1] = Pair16<T>::sub(((hi >> (4 * q)) & 0x000f000fu) | Pair16<T>::magic, bias[1]);
-            }
+      for (int gr = 0; gr < PER; ++gr) {
+        uint32_t bias[2];
+        float scale[2];
 #pragma unroll
-            for (int q = 0; q < 4; q += 2) {
-              const uint32_t a4[4] = {e[q][0], e[q][1], e[q + 1][0], e[q + 1][1]};
+        for (int h = 0; h < 2; ++h) {
+          const int entry = (8 * h + g) * PER + gr;
+          const uint16_t s = static_cast<uint16_t>(rows_lds(tile + kW4TileBytes + 2 * entry, 2));
+          scale[h] = to_f32(*reinterpret_cast<const T*>(&s));
+          bias[h] = Pair16<T>::magic +
+                    (ZEROS ? __byte_perm(rows_lds(tile + kW4TileBytes + kW4Rows * 2 * PER + entry, 1), 0, 0x4040) : 0x00080008u);
+        }
+        float acc[4] = {};
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-                Pair16<T>::mma(acc[nt], a4, (&xv[nt][j].x)[q], (&xv[nt][j].x)[q + 1]);
-            }
-          }
-          const float s0 = scale_of<T>(cur[r].s[0][gr / 2], gr & 1), s1 = scale_of<T>(cur[r].s[1][gr / 2], gr & 1);
+        for (int jj = 0; jj < 4 / PER; ++jj) {
+          const int j = gr * (4 / PER) + jj;
+          const uint32_t xw[4] = {xv[j].x, xv[j].y, xv[j].z, xv[j].w};
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            total[r][nt][0] = fmaf(s0, acc[nt][0], total[r][nt][0]);
-            total[r][nt][1] = fmaf(s0, acc[nt][1], total[r][nt][1]);
-            total[r][nt][2] = fmaf(s1, acc[nt][2], total[r][nt][2]);
-            total[r][nt][3] = fmaf(s1, acc[nt][3], total[r][nt][3]);
+          for (int q = 0; q < 4; q += 2) {
+            const uint32_t a4[4] = {Pair16<T>::code(lo[j], q, bias[0]), Pair16<T>::code(hi[j], q, bias[1]),
+                                    Pair16<T>::code(lo[j], q + 1, bias[0]), Pair16<T>::code(hi[j], q + 1, bias[1])};
+            Pair16<T>::mma(acc, a4, xw[q], xw[q + 1]);
           }
         }
+        total[r][0] = fmaf(scale[0], acc[0], total[r][0]);
+        total[r][1] = fmaf(scale[0], acc[1], total[r][1]);
+        total[r][2] = fmaf(scale[1], acc[2], total[r][2]);
+        total[r][3] = fmaf(scale[1], acc[3], total[r][3]);
       }
     }
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+  float(*part)[8][RT * 16 + 1] = reinterpret_cast<float(*)[8][RT * 16 + 1]>(smem_rows);
 #pragma unroll
   for (int r = 0; r < RT; ++r)
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) part[warp][nt * 8 + 2 * t + (i & 1)][r * 16 + g + 8 * (i >> 1)] = total[r][nt][i];
+    for (int i = 0; i < 4; ++i) part[warp][2 * t + (i & 1)][r * 16 + g + 8 * (i >> 1)] = total[r][i];
   __syncthreads();
-  if (ranks > 1) {
-    // the warps' sums of this CTA first, then rank 0 adds the ranks' in order
-    for (int e = threadIdx.x; e < NT * 8 * RT * 16; e += kRowThreads) {
-      float s = 0.f;
+  constexpr int kCols = WR * RT * 16;
+  for (int e = threadIdx.x; e < p.m * kCols; e += kRowThreads) {
+    const int row = e / kCols, c = e % kCols, col = static_cast<int>(blockIdx.x) * kCols + c;
+    float s = 0.f;
 #pragma unroll
-      for (int w = 0; w < kRowWarps; ++w) s += part[w][e / (RT * 16)][e % (RT * 16)];
-      part[0][e / (RT * 16)][e % (RT * 16)] = s;
-    }
-    cluster.sync();
+    for (int w = 0; w < WK; ++w) s += part[c / (RT * 16) * WK + w][row][c % (RT * 16)];
+    if (col < p.n) static_cast<T*>(p.y)[row * p.ldy + col] = from_f32<T>(s);
   }
-  if (rank == 0) {
-    for (int e = threadIdx.x; e < NT * 8 * RT * 16; e += kRowThreads) {
-      const int row = m0 + e / (RT * 16), col = tile0 * 16 + e % (RT * 16);
-      float s = 0.f;
-      if (ranks > 1) {
-        for (int c = 0; c < ranks; ++c) s += *cluster.map_shared_rank(&part[0][e / (RT * 16)][e % (RT * 16)], c);
-      } else {
-#pragma unroll
-        for (int w = 0; w < kRowWarps; ++w) s += part[w][e / (RT * 16)][e % (RT * 16)];
-      }
-      if (row < p.m && col < p.n) static_cast<T*>(p.y)[row * p.ldy + col] = from_f32<T>(s);
-    }
-  }
-  if (ranks > 1) cluster.sync();  // no CTA leaves while rank 0 reads its memory
 }
 
-template <typename T, int PER, int NT, int RT, int AHEAD>
-int launch_rows(const RowsParams& p, int ranks, cudaStream_t stream) {
-  const long long gx = static_cast<long long>(ceil_div(w4_row_tiles(p.n), RT)) * ranks;
-  const int gy = ceil_div(p.m, NT * 8);
-  if (gx > 0x7fffffffll || gy > 65535) return kErrNotSupported;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(gx), static_cast<unsigned>(gy));
-  cfg.blockDim = dim3(kRowThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim = {static_cast<unsigned>(ranks), 1, 1};
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, w4_rows_kernel<T, PER, NT, RT, AHEAD>, p));
+template <typename T, int PER, int RT, int WR, int AHEAD, bool ZEROS>
+int launch_rows_kernel(const RowsParams& p, cudaStream_t stream) {
+  constexpr int kSmem = rows_smem(PER, RT, AHEAD);
+  if (kSmem > 48 * 1024) {
+    static PerDeviceOnce attr;
+    const int rc = attr.run_once([] {
+      return static_cast<int>(cudaFuncSetAttribute(w4_rows_kernel<T, PER, RT, WR, AHEAD, ZEROS>,
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    });
+    if (rc) return rc;
+  }
+  w4_rows_kernel<T, PER, RT, WR, AHEAD, ZEROS><<<ceil_div(w4_row_tiles(p.n), RT * WR), kRowThreads, kSmem, stream>>>(p);
+  return static_cast<int>(cudaGetLastError());
+}
+template <typename T, int PER, int RT, int WR, int AHEAD>
+int launch_rows(const RowsParams& p, cudaStream_t stream) {
+  return p.zeros ? launch_rows_kernel<T, PER, RT, WR, AHEAD, true>(p, stream)
+                 : launch_rows_kernel<T, PER, RT, WR, AHEAD, false>(p, stream);
 }
 
 }  // namespace lowbit

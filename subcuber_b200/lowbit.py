@@ -31,43 +31,51 @@ GROUPS = (32, 64, 128)
 ACT_BLOCK = 32   # channels of a token that share a step
 
 
+# handle of the current stream of a device (the public call builds a Stream object, which takes 2 us)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _matrix(name: str, t: torch.Tensor, dtypes) -> None:
+    # (the stride of an axis of one element is never used)
+    if t.is_cuda and t.dtype in dtypes and t.dim() == 2:
+        rows, cols = t.shape
+        ld, step = t.stride()
+        if (step == 1 or cols <= 1) and (ld >= cols or rows <= 1):
+            return
+        raise ValueError(f"{name} must have its rows in consecutive elements, rows that do not overlap")
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor: this backend has no CPU path")
     if t.dim() != 2:
         raise ValueError(f"{name} must be a matrix")
-    if t.dtype not in dtypes:
-        raise ValueError(f"{name} must be one of {[str(d) for d in dtypes]}, not {t.dtype}")
-    # (the stride of an axis of one element is never used)
-    if t.shape[1] > 1 and t.stride(1) != 1:
-        raise ValueError(f"{name} must have its rows in consecutive elements")
-    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
-        raise ValueError(f"the rows of {name} must not overlap")
+    raise ValueError(f"{name} must be one of {[str(d) for d in dtypes]}, not {t.dtype}")
 
 
 def _ld(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+    rows, cols = t.shape
+    return t.stride(0) if rows > 1 else max(cols, 1)
 
 
-def _same_device(*tensors) -> None:
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) > 1:
-        raise ValueError(f"operands are on different devices: {sorted(map(str, devices))}")
+def _same_device(first, *others) -> None:
+    device = first.device
+    for t in others:
+        if t is not None and t.device != device:
+            raise ValueError(f"operands are on different devices: {device} and {t.device}")
 
 
-def _output(name: str, t: Optional[torch.Tensor], shape, dtype, device) -> torch.Tensor:
-    if t is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+def _output(name: str, t: torch.Tensor, shape, dtype, device) -> None:
     _matrix(name, t, (dtype,))
-    if tuple(t.shape) != tuple(shape):
+    if tuple(t.shape) != shape:
         raise ValueError(f"{name} must be {shape[0]} x {shape[1]}")
-    return t
+    if t.device != device:
+        raise ValueError(f"operands are on different devices: {device} and {t.device}")
 
 
-def _call(what: str, fn, device: torch.device, *args) -> None:
-    # the library works on the current device: make the operands' device current where it is not
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if torch.cuda.current_device() == device.index:
+def _call(what: str, device: torch.device, *args) -> None:
+    """Call the library's `what` on the current stream of `device`, with `device` current."""
+    fn = getattr(_lib.load(), what)
+    index = device.index
+    stream = _raw_stream(index)
+    if torch.cuda.current_device() == index:
         rc = fn(*args, stream)
     else:
         with torch.cuda.device(device):
@@ -76,44 +84,23 @@ def _call(what: str, fn, device: torch.device, *args) -> None:
         raise KernelError(what, rc)
 
 
-class _Workspace:
-    def check(self) -> None:
-        """Wait for the call that used the workspace last and raise if a device-side wait gave up."""
-        with torch.cuda.device(self.buf.device):
-            rc = _lib.load().sb200_gemm_status(self.ptr, torch.cuda.current_stream(self.buf.device).cuda_stream)
-        if rc != 0:
-            raise KernelError("workspace", rc)
+def _status(ptr: int, device) -> None:
+    with torch.cuda.device(device):
+        rc = _lib.load().sb200_gemm_status(ptr, _raw_stream(device.index))
+    if rc != 0:
+        raise KernelError("product with an operand in few bits", rc)
 
-    def _allocate(self, nbytes: int, device) -> None:
+
+class _Workspace:
+    def __init__(self, nbytes: int, device: torch.device):
         self.nbytes = nbytes
+        self.device = device
         self.buf = torch.empty(nbytes + 256, dtype=torch.uint8, device=device)
         self.ptr = self.buf.data_ptr() + (-self.buf.data_ptr()) % 256
-        self.buf[:512].zero_()   # the status word
 
-
-class WeightsW4:
-    """Weights in 4 bits, in the library's order: `codes` uint8, `scales` in the activations' type, `zeros` uint8 or None
-    (symmetric), all flat.  Made by `quantize_w4` or `pack_w4`."""
-
-    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor], n: int, k: int, group: int):
-        lib = _lib.load()
-        _check_w4(n, k, group)
-        _same_device(codes, scales, zeros)
-        nbytes, entries = int(lib.sb200_w4_codes_bytes(n, k)), int(lib.sb200_w4_table_entries(n, k, group))
-        if scales.dtype not in HALF_TYPES:
-            raise ValueError(f"scales must be one of {[str(d) for d in HALF_TYPES]}, not {scales.dtype}")
-        for name, t, dtype, count in (("codes", codes, torch.uint8, nbytes), ("scales", scales, scales.dtype, entries),
-                                      ("zeros", zeros, torch.uint8, entries)):
-            if t is not None and (not t.is_cuda or t.dtype != dtype or t.numel() != count or not t.is_contiguous()):
-                raise ValueError(f"{name} must be a packed CUDA tensor of {count} {dtype}")
-        self.codes, self.scales, self.zeros = codes, scales, zeros
-        self.n, self.k, self.group = n, k, group
-        self.dtype, self.device = scales.dtype, scales.device
-        self._zeros_ptr = zeros.data_ptr() if zeros is not None else None
-
-    @property
-    def nbytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in (self.codes, self.scales, self.zeros) if t is not None)
+    def check(self) -> None:
+        """Wait for the call that used the workspace last and raise if a device-side wait gave up."""
+        _status(self.ptr, self.device)
 
 
 def _check_w4(n: int, k: int, group: int) -> None:
@@ -123,22 +110,71 @@ def _check_w4(n: int, k: int, group: int) -> None:
         raise ValueError("weights need at least one output and one input")
 
 
-def _empty_w4(n: int, k: int, group: int, symmetric: bool, dtype, device) -> WeightsW4:
-    lib = _lib.load()
-    _check_w4(n, k, group)
-    entries = int(lib.sb200_w4_table_entries(n, k, group))
-    return WeightsW4(torch.empty(int(lib.sb200_w4_codes_bytes(n, k)), dtype=torch.uint8, device=device),
-                     torch.empty(entries, dtype=dtype, device=device),
-                     None if symmetric else torch.empty(entries, dtype=torch.uint8, device=device), n, k, group)
+class WeightsW4:
+    """Weights in 4 bits (out_features n x in_features k), in the library's order: `codes` uint8, `scales` in the activations'
+    type, `zeros` uint8 or None (symmetric), all flat.  Made by `quantize_w4` or `pack_w4`."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor], n: int, k: int, group: int):
+        lib = _lib.load()
+        _check_w4(n, k, group)
+        nbytes, entries = int(lib.sb200_w4_codes_bytes(n, k)), int(lib.sb200_w4_table_entries(n, k, group))
+        if scales.dtype not in HALF_TYPES:
+            raise ValueError(f"scales must be one of {[str(d) for d in HALF_TYPES]}, not {scales.dtype}")
+        for name, t, dtype, count in (("codes", codes, torch.uint8, nbytes), ("scales", scales, scales.dtype, entries),
+                                      ("zeros", zeros, torch.uint8, entries)):
+            if t is not None and (not t.is_cuda or t.dtype != dtype or t.numel() != count or not t.is_contiguous()):
+                raise ValueError(f"{name} must be a packed CUDA tensor of {count} {dtype}")
+        _same_device(codes, scales, zeros)
+        self._tensors = (codes, scales, zeros)
+        self._set(n, k, group, scales.dtype, scales.device, codes.data_ptr(), scales.data_ptr(),
+                  zeros.data_ptr() if zeros is not None else None)
+        # the status word of products that need no other workspace
+        self._own = torch.empty(512, dtype=torch.uint8, device=self.device)
+        self._status_ptr = self._own.data_ptr() + (-self._own.data_ptr()) % 256
+
+    def _set(self, n, k, group, dtype, device, codes_ptr, scales_ptr, zeros_ptr) -> None:
+        self.n, self.k, self.group, self.dtype, self.device = n, k, group, dtype, device
+        self._ptrs = (codes_ptr, scales_ptr, zeros_ptr)
+        self._code = DTYPE_CODE[dtype]
+
+    @classmethod
+    def _empty(cls, n: int, k: int, group: int, symmetric: bool, dtype, device) -> "WeightsW4":
+        """One allocation for everything; the tensors are made when they are asked for."""
+        _check_w4(n, k, group)
+        rows, blocks = -(-n // 16) * 16, -(-k // 128)
+        nbytes, entries = rows * blocks * 64, rows * blocks * (128 // group)
+        w = cls.__new__(cls)
+        buf = torch.empty(512 + nbytes + entries * (2 if symmetric else 3), dtype=torch.uint8, device=device)
+        base = buf.data_ptr()
+        w._own, w._tensors, w._sizes = buf, None, (nbytes, entries, symmetric)
+        w._status_ptr = base + (-base) % 256
+        codes = base + 512
+        w._set(n, k, group, dtype, device, codes, codes + nbytes, None if symmetric else codes + nbytes + 2 * entries)
+        return w
+
+    def _tensor(self, i: int):
+        if self._tensors is None:
+            nbytes, entries, symmetric = self._sizes
+            b = self._own[512:]
+            self._tensors = (b[:nbytes], b[nbytes:nbytes + 2 * entries].view(self.dtype),
+                             None if symmetric else b[nbytes + 2 * entries:])
+        return self._tensors[i]
+
+    codes = property(lambda self: self._tensor(0))
+    scales = property(lambda self: self._tensor(1))
+    zeros = property(lambda self: self._tensor(2))
+
+    @property
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.codes, self.scales, self.zeros) if t is not None)
 
 
 def quantize_w4(weight: torch.Tensor, group: int = 128, symmetric: bool = False) -> WeightsW4:
     """Quantise `weight` (out_features x in_features, f16 or bf16) to 4 bits, rounding to nearest within each group."""
     _matrix("weight", weight, HALF_TYPES)
     n, k = weight.shape
-    w = _empty_w4(n, k, group, symmetric, weight.dtype, weight.device)
-    _call("quantize_w4", _lib.load().sb200_w4_quantize, weight.device, DTYPE_CODE[weight.dtype], weight.data_ptr(), _ld(weight),
-          n, k, group, w.codes.data_ptr(), w.scales.data_ptr(), w._zeros_ptr)
+    w = WeightsW4._empty(n, k, group, symmetric, weight.dtype, weight.device)
+    _call("sb200_w4_quantize", w.device, w._code, weight.data_ptr(), _ld(weight), n, k, group, *w._ptrs)
     return w
 
 
@@ -148,31 +184,27 @@ def pack_w4(q: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor]
     _matrix("q", q, (torch.uint8,))
     _matrix("scales", scales, HALF_TYPES)
     n, k = q.shape
-    _same_device(q, scales, zeros)
     _check_w4(n, k, group)
     if zeros is not None:
         _matrix("zeros", zeros, (torch.uint8,))
     for name, t in (("scales", scales), ("zeros", zeros)):
         if t is not None and tuple(t.shape) != (-(-k // group), n):
             raise ValueError(f"{name} must be a {-(-k // group)} x {n} table")
-    w = _empty_w4(n, k, group, zeros is None, scales.dtype, q.device)
-    _call("pack_w4", _lib.load().sb200_w4_pack, q.device, DTYPE_CODE[w.dtype], q.data_ptr(), _ld(q), scales.data_ptr(),
-          _ld(scales), zeros.data_ptr() if zeros is not None else None, _ld(zeros) if zeros is not None else n, n, k, group,
-          w.codes.data_ptr(), w.scales.data_ptr(), w._zeros_ptr)
+    _same_device(q, scales, zeros)
+    w = WeightsW4._empty(n, k, group, zeros is None, scales.dtype, q.device)
+    _call("sb200_w4_pack", w.device, w._code, q.data_ptr(), _ld(q), scales.data_ptr(), _ld(scales),
+          zeros.data_ptr() if zeros is not None else None, _ld(zeros) if zeros is not None else n, n, k, group, *w._ptrs)
     return w
 
 
 def dequantize_w4(w: WeightsW4, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The weights (out_features x in_features) that `w` stands for, rounded once to its type."""
-    out = _output("out", out, (w.n, w.k), w.dtype, w.device)
-    _same_device(w.codes, out)
-    _call("dequantize_w4", _lib.load().sb200_w4_dequantize, w.device, DTYPE_CODE[w.dtype], w.codes.data_ptr(),
-          w.scales.data_ptr(), w._zeros_ptr, w.n, w.k, w.group, out.data_ptr(), _ld(out))
+    if out is None:
+        out = torch.empty((w.n, w.k), dtype=w.dtype, device=w.device)
+    else:
+        _output("out", out, (w.n, w.k), w.dtype, w.device)
+    _call("sb200_w4_dequantize", w.device, w._code, *w._ptrs, w.n, w.k, w.group, out.data_ptr(), _ld(out))
     return out
-
-
-def _tma_rows(t: torch.Tensor) -> bool:
-    return t.data_ptr() % 16 == 0 and _ld(t) % 8 == 0
 
 
 class WorkspaceW4(_Workspace):
@@ -180,25 +212,38 @@ class WorkspaceW4(_Workspace):
     bytes (the default expects packed rows); else there is room for a copy of x."""
 
     def __init__(self, m: int, w: WeightsW4, aligned: Optional[bool] = None):
-        lib = _lib.load()
+        aligned = w.k % 8 == 0 if aligned is None else aligned
         with torch.cuda.device(w.device):  # a product is cut for the device that will run it
-            self._allocate(int(lib.sb200_w4_gemm_workspace_bytes(DTYPE_CODE[w.dtype], m, w.n, w.k, w.group,
-                                                                 int(w.k % 8 == 0 if aligned is None else aligned))), w.device)
+            super().__init__(int(_lib.load().sb200_w4_gemm_workspace_bytes(w._code, m, w.n, w.k, w.group, int(aligned))), w.device)
 
 
-def gemm_w4(x: torch.Tensor, w: WeightsW4, out: Optional[torch.Tensor] = None,
-            workspace: Optional[WorkspaceW4] = None) -> torch.Tensor:
-    """x @ W^T (m x out_features) for x (m x in_features) of the weights' type; sums in fp32."""
+def gemm_w4(x: torch.Tensor, w: WeightsW4, out: Optional[torch.Tensor] = None, workspace: Optional[WorkspaceW4] = None,
+            check: bool = False) -> torch.Tensor:
+    """x @ W^T (m x out_features) for x (m x in_features) of the weights' type; sums in fp32.  `check` synchronises and raises
+    if a device-side wait gave up."""
     _matrix("x", x, (w.dtype,))
-    m = x.shape[0]
-    if x.shape[1] != w.k:
-        raise ValueError(f"x has {x.shape[1]} columns, the weights {w.k} inputs")
-    out = _output("out", out, (m, w.n), w.dtype, x.device)
-    _same_device(x, w.codes, out)
-    if workspace is None:
-        workspace = WorkspaceW4(m, w, _tma_rows(x))
-    _call("gemm_w4", _lib.load().sb200_w4_gemm, w.device, DTYPE_CODE[w.dtype], x.data_ptr(), _ld(x), w.codes.data_ptr(),
-          w.scales.data_ptr(), w._zeros_ptr, out.data_ptr(), _ld(out), m, w.n, w.k, w.group, workspace.ptr, workspace.nbytes)
+    m, k = x.shape
+    if k != w.k:
+        raise ValueError(f"x has {k} columns, the weights {w.k} inputs")
+    if out is None:
+        if x.device != w.device:
+            raise ValueError(f"operands are on different devices: {x.device} and {w.device}")
+        out = torch.empty((m, w.n), dtype=w.dtype, device=w.device)
+    else:
+        _output("out", out, (m, w.n), w.dtype, w.device)
+    ldx, x_ptr = _ld(x), x.data_ptr()
+    if workspace is not None:
+        ptr, nbytes = workspace.ptr, workspace.nbytes
+    elif m <= 64 and x_ptr % 16 == 0 and ldx % 8 == 0:
+        ptr, nbytes = w._status_ptr, 256     # the products of few rows need the status word only
+    else:
+        workspace = WorkspaceW4(m, w, x_ptr % 16 == 0 and ldx % 8 == 0)
+        ptr, nbytes = workspace.ptr, workspace.nbytes
+    _call("sb200_w4_gemm", w.device, w._code, x_ptr, ldx, *w._ptrs, out.data_ptr(), _ld(out), m, w.n, k, w.group, ptr, nbytes)
+    if check:
+        torch.cuda.current_stream(w.device).synchronize()
+        if m > 8:                            # (below, the kernel has no waits and leaves the word alone)
+            _status(ptr, w.device)
     return out
 
 
@@ -211,15 +256,41 @@ class Checkpoint8:
             raise ValueError("saved activations are f16 or bf16")
         if k <= 0:
             raise ValueError("activations need at least one channel")
-        _same_device(codes, exponents)
         for name, t, cols, unit in (("codes", codes, k, 16), ("exponents", exponents, -(-k // ACT_BLOCK), 4)):
             _matrix(name, t, (torch.uint8,))
             if t.shape[1] < cols or t.shape[1] % unit or _ld(t) % unit or t.data_ptr() % unit:
                 raise ValueError(f"rows of {name} must hold {cols} bytes, padded and aligned to {unit}")
         if codes.shape[0] != exponents.shape[0]:
             raise ValueError("codes and exponents must have the same tokens")
-        self.codes, self.exponents = codes, exponents
-        self.m, self.k, self.dtype, self.device = codes.shape[0], k, dtype, codes.device
+        _same_device(codes, exponents)
+        self._tensors = (codes, exponents)
+        self._set(codes.shape[0], k, dtype, codes.device, codes.data_ptr(), _ld(codes), exponents.data_ptr(), _ld(exponents))
+
+    def _set(self, m, k, dtype, device, codes_ptr, pitch, exp_ptr, exp_pitch) -> None:
+        self.m, self.k, self.dtype, self.device = m, k, dtype, device
+        self._layout = (codes_ptr, pitch, exp_ptr, exp_pitch)
+        self._code = DTYPE_CODE[dtype]
+
+    @classmethod
+    def _empty(cls, m: int, k: int, dtype, device) -> "Checkpoint8":
+        """One allocation for both; the tensors are made when they are asked for."""
+        if k <= 0:
+            raise ValueError("activations need at least one channel")
+        pitch, exp_pitch = -(-k // 16) * 16, -(-k // (4 * ACT_BLOCK)) * 4
+        c = cls.__new__(cls)
+        c._own, c._tensors = torch.empty(m * (pitch + exp_pitch), dtype=torch.uint8, device=device), None
+        base = c._own.data_ptr()
+        c._set(m, k, dtype, device, base, pitch, base + m * pitch, exp_pitch)
+        return c
+
+    def _tensor(self, i: int) -> torch.Tensor:
+        if self._tensors is None:
+            cut = self.m * self._layout[1]
+            self._tensors = (self._own[:cut].view(self.m, self._layout[1]), self._own[cut:].view(self.m, self._layout[3]))
+        return self._tensors[i]
+
+    codes = property(lambda self: self._tensor(0))
+    exponents = property(lambda self: self._tensor(1))
 
     @property
     def nbytes(self) -> int:
@@ -231,22 +302,22 @@ def save8(x: torch.Tensor, out: Optional[Checkpoint8] = None) -> Checkpoint8:
     _matrix("x", x, HALF_TYPES)
     m, k = x.shape
     if out is None:
-        out = Checkpoint8(torch.empty((m, -(-k // 16) * 16), dtype=torch.uint8, device=x.device),
-                          torch.empty((m, -(-k // (4 * ACT_BLOCK)) * 4), dtype=torch.uint8, device=x.device), k, x.dtype)
+        out = Checkpoint8._empty(m, k, x.dtype, x.device)
     elif (out.m, out.k, out.dtype) != (m, k, x.dtype):
         raise ValueError(f"out holds {out.m} x {out.k} {out.dtype}, x is {m} x {k} {x.dtype}")
-    _same_device(x, out.codes)
-    _call("save8", _lib.load().sb200_act8_save, x.device, DTYPE_CODE[x.dtype], x.data_ptr(), _ld(x), m, k, out.codes.data_ptr(),
-          _ld(out.codes), out.exponents.data_ptr(), _ld(out.exponents))
+    elif out.device != x.device:
+        raise ValueError(f"operands are on different devices: {x.device} and {out.device}")
+    _call("sb200_act8_save", out.device, out._code, x.data_ptr(), _ld(x), m, k, *out._layout)
     return out
 
 
 def restore8(saved: Checkpoint8, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The activations (tokens x channels) that `saved` stands for, exact in its type."""
-    out = _output("out", out, (saved.m, saved.k), saved.dtype, saved.device)
-    _same_device(saved.codes, out)
-    _call("restore8", _lib.load().sb200_act8_restore, saved.device, DTYPE_CODE[saved.dtype], saved.codes.data_ptr(),
-          _ld(saved.codes), saved.exponents.data_ptr(), _ld(saved.exponents), saved.m, saved.k, out.data_ptr(), _ld(out))
+    if out is None:
+        out = torch.empty((saved.m, saved.k), dtype=saved.dtype, device=saved.device)
+    else:
+        _output("out", out, (saved.m, saved.k), saved.dtype, saved.device)
+    _call("sb200_act8_restore", saved.device, saved._code, *saved._layout, saved.m, saved.k, out.data_ptr(), _ld(out))
     return out
 
 
@@ -255,38 +326,42 @@ class WorkspaceGrad8(_Workspace):
     rows of dy will start on 16 bytes (the default expects packed rows); else there is room for a copy of dy."""
 
     def __init__(self, saved: Checkpoint8, n: int, out_dtype: torch.dtype = torch.float32, aligned: Optional[bool] = None):
-        lib = _lib.load()
+        aligned = n % 8 == 0 if aligned is None else aligned
         with torch.cuda.device(saved.device):
-            self._allocate(int(lib.sb200_act8_wgrad_workspace_bytes(DTYPE_CODE[saved.dtype], DTYPE_CODE[out_dtype], saved.m,
-                                                                    n, saved.k, int(n % 8 == 0 if aligned is None else aligned))),
-                           saved.device)
+            super().__init__(int(_lib.load().sb200_act8_wgrad_workspace_bytes(saved._code, DTYPE_CODE[out_dtype], saved.m, n,
+                                                                              saved.k, int(aligned))), saved.device)
 
 
 def weight_grad8(saved: Checkpoint8, dy: torch.Tensor, base: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
-                 out_dtype: torch.dtype = torch.float32, workspace: Optional[WorkspaceGrad8] = None) -> torch.Tensor:
+                 out_dtype: torch.dtype = torch.float32, workspace: Optional[WorkspaceGrad8] = None,
+                 check: bool = False) -> torch.Tensor:
     """base + X^T @ dy (in_features x out_features, the layout of `gemm`'s B) for the saved activations X and the output
     gradient dy (tokens x out_features) of the same type.  The result is fp32 or has dy's type; `base` and `out` have
-    the result's type, and may be the same tensor."""
+    the result's type, and may be the same tensor.  `check` synchronises and raises if a device-side wait gave up."""
     _matrix("dy", dy, (saved.dtype,))
-    n = dy.shape[1]
-    if dy.shape[0] != saved.m:
-        raise ValueError(f"dy has {dy.shape[0]} rows, {saved.m} tokens were saved")
+    m, n = dy.shape
+    if m != saved.m:
+        raise ValueError(f"dy has {m} rows, {saved.m} tokens were saved")
     if n == 0:
         raise ValueError("dy needs at least one column")
     if out is not None:
         out_dtype = out.dtype
-    if out_dtype not in (torch.float32, saved.dtype):
+    if out_dtype != torch.float32 and out_dtype != saved.dtype:
         raise ValueError(f"the gradient is float32 or {saved.dtype}")
     if base is not None:
-        _matrix("base", base, (out_dtype,))
-        if tuple(base.shape) != (saved.k, n):
-            raise ValueError(f"base must be {saved.k} x {n}")
-    out = _output("out", out, (saved.k, n), out_dtype, dy.device)
-    _same_device(dy, saved.codes, out, base)
+        _output("base", base, (saved.k, n), out_dtype, saved.device)
+    if out is None:
+        if dy.device != saved.device:
+            raise ValueError(f"operands are on different devices: {dy.device} and {saved.device}")
+        out = torch.empty((saved.k, n), dtype=out_dtype, device=saved.device)
+    else:
+        _output("out", out, (saved.k, n), out_dtype, saved.device)
+    lddy, dy_ptr = _ld(dy), dy.data_ptr()
     if workspace is None:
-        workspace = WorkspaceGrad8(saved, n, out_dtype, _tma_rows(dy))
-    _call("weight_grad8", _lib.load().sb200_act8_wgrad, saved.device, DTYPE_CODE[saved.dtype], saved.codes.data_ptr(),
-          _ld(saved.codes), saved.exponents.data_ptr(), _ld(saved.exponents), dy.data_ptr(), _ld(dy), DTYPE_CODE[out_dtype],
-          base.data_ptr() if base is not None else None, _ld(base) if base is not None else n, out.data_ptr(), _ld(out),
-          saved.m, n, saved.k, workspace.ptr, workspace.nbytes)
+        workspace = WorkspaceGrad8(saved, n, out_dtype, dy_ptr % 16 == 0 and lddy % 8 == 0)
+    _call("sb200_act8_wgrad", saved.device, saved._code, *saved._layout, dy_ptr, lddy, DTYPE_CODE[out_dtype],
+          base.data_ptr() if base is not None else None, _ld(base) if base is not None else n, out.data_ptr(), _ld(out), m, n,
+          saved.k, workspace.ptr, workspace.nbytes)
+    if check:
+        workspace.check()
     return out

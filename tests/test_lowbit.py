@@ -1,7 +1,5 @@
 """Products with one operand held in few bits, host side: argument checks of the C entry points and of the Python calls.
 Nothing here launches a kernel (the checks come before any CUDA call)."""
-import ctypes as C
-
 import pytest
 
 P = 1 << 20  # stands for a device address with every alignment; never dereferenced
