@@ -31,14 +31,27 @@ Cut cut_of(int m, int k) {
   return c;
 }
 
+// 16 neighbouring values of a row, zeros behind `k`.  A row that does not start on 16 bytes is read in the aligned 8-byte
+// words that hold its values, which are shifted together.
 template <typename T>
 __device__ __forceinline__ void load16(const T* row, int k0, int k, bool wide, T (&v)[16]) {
   if (wide && k0 + 16 <= k) {
     reinterpret_cast<uint4*>(v)[0] = __ldg(reinterpret_cast<const uint4*>(row + k0));
     reinterpret_cast<uint4*>(v)[1] = __ldg(reinterpret_cast<const uint4*>(row + k0) + 1);
-  } else {
+    return;
+  }
+  const uintptr_t at = reinterpret_cast<uintptr_t>(row + k0), end = reinterpret_cast<uintptr_t>(row + k);
+  const uint32_t off = at & 7;
+  const unsigned long long* word = reinterpret_cast<const unsigned long long*>(at - off);
+  unsigned long long w[5];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = k0 + i < k ? row[k0 + i] : from_f32<T>(0.f);
+  for (int i = 0; i < 5; ++i) w[i] = k0 < k && at - off + 8 * i < end ? __ldg(word + i) : 0ull;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    unsigned long long x = off ? (w[i] >> (8 * off)) | (w[i + 1] << (64 - 8 * off)) : w[i];
+    const int left = k - k0 - 4 * i;
+    if (left < 4) x = left <= 0 ? 0ull : x & (~0ull >> (64 - 16 * left));
+    reinterpret_cast<unsigned long long*>(v)[i] = x;
   }
 }
 
@@ -97,13 +110,27 @@ __global__ void __launch_bounds__(kThreads) act8_restore_kernel(const uint8_t* _
   const long long row = (rb << (8 - cut.cols_log2)) + (threadIdx.x >> cut.cols_log2);
   const int piece = (part << cut.cols_log2) + (threadIdx.x & ((1 << cut.cols_log2) - 1));
   const int k0 = piece * 16;
-  if (row >= m || k0 >= k) return;
-  const uint4 raw = __ldg(reinterpret_cast<const uint4*>(codes + row * pitch + k0));
-  const float step = act8_step(exps[row * exp_pitch + (piece >> 1)]);
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-  T v[16];
+  // rows that do not start on 16 bytes leave through shared memory where a warp lies within one row
+  const bool staged = !wide && cut.cols_log2 >= 5;
+  __shared__ __align__(16) T stage[kThreads * 16];
+  if (row >= m || (k0 >= k && !staged)) return;
+  T v[16] = {};
+  if (k0 < k) {
+    const uint4 raw = __ldg(reinterpret_cast<const uint4*>(codes + row * pitch + k0));
+    const float step = act8_step(exps[row * exp_pitch + (piece >> 1)]);
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = from_f32<T>(act8_value((w[i >> 2] >> (8 * (i & 3))) & 255u, step));
+    for (int i = 0; i < 16; ++i) v[i] = from_f32<T>(act8_value((w[i >> 2] >> (8 * (i & 3))) & 255u, step));
+  }
+  if (staged) {
+    const int lane = threadIdx.x & 31, first = k0 - lane * 16;
+    T* mine = stage + (threadIdx.x - lane) * 16;
+    reinterpret_cast<uint4*>(mine + lane * 16)[0] = reinterpret_cast<const uint4*>(v)[0];
+    reinterpret_cast<uint4*>(mine + lane * 16)[1] = reinterpret_cast<const uint4*>(v)[1];
+    __syncwarp();
+    if (first < k) store_row<T>(x + row * ldx + first, mine, min(512, k - first), lane);
+    return;
+  }
   T* to = x + row * ldx + k0;
   if (wide && k0 + 16 <= k) {
     reinterpret_cast<uint4*>(to)[0] = reinterpret_cast<const uint4*>(v)[0];

@@ -70,5 +70,25 @@ __device__ __forceinline__ float act8_value(uint32_t byte, float step) {
   return (byte & 128u) ? -v : v;
 }
 
+// A warp stores `count` 16-bit values that lie in shared memory (on 16 bytes) to consecutive places of global memory.
+template <typename T>
+__device__ __forceinline__ void store_row(T* to, const T* from, int count, int lane) {
+  const uint32_t off = reinterpret_cast<uintptr_t>(to) & 15;
+  if (off == 0) {
+    for (int i = lane * 8; i + 8 <= count; i += 256) *reinterpret_cast<uint4*>(to + i) = *reinterpret_cast<const uint4*>(from + i);
+    const int done = count & ~7;
+    if (lane < count - done) to[done + lane] = from[done + lane];
+    return;
+  }
+  const int head = (off >> 1) & 1;  // a value before the first whole 4-byte word
+  if (head && lane == 0) to[0] = from[0];
+  const int pairs = (count - head) >> 1;
+  for (int i = lane; i < pairs; i += 32) {
+    const uint32_t a = *reinterpret_cast<const uint16_t*>(from + head + 2 * i), b = *reinterpret_cast<const uint16_t*>(from + head + 2 * i + 1);
+    *reinterpret_cast<uint32_t*>(to + head + 2 * i) = a | (b << 16);
+  }
+  if (((count - head) & 1) && lane == 0) to[count - 1] = from[count - 1];
+}
+
 }  // namespace lowbit
 }  // namespace sb200

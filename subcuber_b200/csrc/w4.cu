@@ -16,15 +16,26 @@ namespace {
 constexpr int kSpanBlocks = 4;
 constexpr int kThreads = 256;
 
-// Four neighbouring 16-bit values, zeros behind `k`; `wide` says that 8-byte loads are aligned.
+// Four neighbouring 16-bit values of a row for each lane, zeros behind `k`; the lanes of the warp take 128 neighbours.  A row
+// that does not start on 8 bytes is read in the aligned 8-byte words that hold it: a lane takes its word, the rest from
+// the lane behind (the last lane reads one more), and shifts the two together.  Words without a value of the row are
+// not read.
 template <typename T>
-__device__ __forceinline__ void load4(const T* row, int k0, int k, bool wide, T (&v)[4]) {
-  if (wide && k0 + 4 <= k) {
-    *reinterpret_cast<uint2*>(v) = __ldg(reinterpret_cast<const uint2*>(row + k0));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = k0 + i < k ? row[k0 + i] : from_f32<T>(0.f);
+__device__ __forceinline__ void load4(const T* row, int k0, int k, T (&v)[4], int lane) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(row + k0);
+  const uint32_t off = at & 7;  // the same for all lanes
+  const unsigned long long* word = reinterpret_cast<const unsigned long long*>(at - off);
+  const uintptr_t end = reinterpret_cast<uintptr_t>(row + k);
+  unsigned long long lo = 0;
+  if (k0 < k || at - off < end) lo = __ldg(word);
+  if (off) {
+    unsigned long long hi = __shfl_down_sync(0xffffffffu, lo, 1);
+    if (lane == 31) hi = at - off + 8 < end ? __ldg(word + 1) : 0ull;
+    lo = (lo >> (8 * off)) | (hi << (64 - 8 * off));
   }
+  const int left = k - k0;
+  if (left < 4) lo = left <= 0 ? 0ull : lo & (~0ull >> (64 - 16 * left));
+  *reinterpret_cast<unsigned long long*>(v) = lo;
 }
 
 // Places the four codes of a lane (inputs 4 (lane & 1) .. + 3 of a word) in the word of its pair of lanes.
@@ -47,7 +58,7 @@ __device__ __forceinline__ int word_offset(int row, int pair) {
 template <typename T, int G, bool SYM>
 __global__ void __launch_bounds__(kThreads) w4_quantize_kernel(const T* __restrict__ w, long long ldw, int n, int k,
                                                                uint8_t* __restrict__ codes, T* __restrict__ scales,
-                                                               uint8_t* __restrict__ zeros, bool wide) {
+                                                               uint8_t* __restrict__ zeros) {
   __shared__ __align__(16) uint8_t tile[kSpanBlocks * kW4TileBytes];
   const int blocks = w4_blocks(k);
   const int spans = ceil_div(blocks, kSpanBlocks);
@@ -60,7 +71,7 @@ __global__ void __launch_bounds__(kThreads) w4_quantize_kernel(const T* __restri
     T v[kSpanBlocks][4];
 #pragma unroll
     for (int b = 0; b < kSpanBlocks; ++b)
-      load4<T>(w + (row < n ? row : 0) * ldw, (span * kSpanBlocks + b) * kW4Block + lane * 4, row < n ? k : 0, wide, v[b]);
+      load4<T>(w + (row < n ? row : 0) * ldw, (span * kSpanBlocks + b) * kW4Block + lane * 4, row < n ? k : 0, v[b], lane);
 #pragma unroll
     for (int b = 0; b < kSpanBlocks; ++b) {
       const int k0 = (span * kSpanBlocks + b) * kW4Block + lane * 4;
@@ -141,40 +152,46 @@ __global__ void __launch_bounds__(kThreads) w4_pack_kernel(const uint8_t* __rest
   }
 }
 
-// Expansion: a thread takes the 16 bytes of (row, t), four words of eight inputs.
+// Expansion: a thread takes the 16 bytes of (row, t), four words of eight inputs, and leaves them in shared memory; a warp
+// then stores two rows of up to 512 neighbours in aligned words.  Rows that do not start on 16 bytes are stored in 4-byte words (or
+// 2-byte ones at their ends) of the values that fall into them.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) w4_dequantize_kernel(const uint8_t* __restrict__ codes, const T* __restrict__ scales,
                                                                  const uint8_t* __restrict__ zeros, int n, int k, int G,
-                                                                 T* __restrict__ out, long long ldo, bool wide) {
+                                                                 T* __restrict__ out, long long ldo) {
+  constexpr int kSpan = kSpanBlocks * kW4Block;
+  __shared__ __align__(16) T rows[kW4Rows][kSpan + 8];
   const int blocks = w4_blocks(k);
   const int spans = ceil_div(blocks, kSpanBlocks);
   const int rt = blockIdx.x / spans, span = blockIdx.x % spans;
   const int block = span * kSpanBlocks + (threadIdx.x >> 6);
   const int piece = threadIdx.x & 63;
-  const int row = rt * kW4Rows + (piece >> 5) * 8 + ((piece & 31) >> 2), t = piece & 3;
-  if (block >= blocks || row >= n) return;
-  const uint4 raw = __ldg(reinterpret_cast<const uint4*>(codes) +
-                          (static_cast<long long>(rt) * blocks + block) * (kW4TileBytes / 16) + piece);
-  const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+  const int r = (piece >> 5) * 8 + ((piece & 31) >> 2), t = piece & 3;
+  if (block < blocks) {
+    const uint4 raw = __ldg(reinterpret_cast<const uint4*>(codes) +
+                            (static_cast<long long>(rt) * blocks + block) * (kW4TileBytes / 16) + piece);
+    const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int k0 = block * kW4Block + 32 * j + 8 * t;
-    if (k0 >= k) break;
-    const long long at = w4_table_at(row, k0 / G, blocks, G);
-    const float s = to_f32(scales[at]);
-    const float z = zeros ? static_cast<float>(zeros[at]) : 8.f;
-    T v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      v[i] = from_f32<T>((static_cast<float>((words[j] >> (4 * w4_nibble(i))) & 15u) - z) * s);
-    T* to = out + row * ldo + k0;
-    if (wide && k0 + 8 <= k) {
-      *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(v);
-    } else {
+    for (int j = 0; j < 4; ++j) {
+      const int k0 = block * kW4Block + 32 * j + 8 * t;
+      const long long at = w4_table_at(rt * kW4Rows + r, k0 / G, blocks, G);
+      const float s = to_f32(scales[at]);
+      const float z = zeros ? static_cast<float>(zeros[at]) : 8.f;
+      T v[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (k0 + i < k) to[i] = v[i];
+        v[i] = from_f32<T>((static_cast<float>((words[j] >> (4 * w4_nibble(i))) & 15u) - z) * s);
+      *reinterpret_cast<uint4*>(&rows[r][k0 - span * kSpan]) = *reinterpret_cast<const uint4*>(v);
     }
+  }
+  __syncthreads();
+  const int first = span * kSpan, count = min(kSpan, k - first);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int row = rt * kW4Rows + warp + 8 * h;
+    if (row >= n) continue;
+    store_row<T>(out + row * ldo + first, rows[warp + 8 * h], count, lane);
   }
 }
 
@@ -219,13 +236,12 @@ template <typename T, int G>
 int quantize(const void* w, long long ldw, const W4& q, cudaStream_t stream) {
   unsigned grid;
   if (int rc = grid_of(q.n, ceil_div(w4_blocks(q.k), kSpanBlocks), &grid)) return rc;
-  const bool wide = aligned(w, 8) && ldw % 4 == 0;
   const T* from = static_cast<const T*>(w);
   uint8_t* codes = static_cast<uint8_t*>(const_cast<void*>(q.codes));
   T* scales = static_cast<T*>(const_cast<void*>(q.scales));
   uint8_t* zeros = static_cast<uint8_t*>(const_cast<void*>(q.zeros));
-  if (zeros) w4_quantize_kernel<T, G, false><<<grid, kThreads, 0, stream>>>(from, ldw, q.n, q.k, codes, scales, zeros, wide);
-  else w4_quantize_kernel<T, G, true><<<grid, kThreads, 0, stream>>>(from, ldw, q.n, q.k, codes, scales, zeros, wide);
+  if (zeros) w4_quantize_kernel<T, G, false><<<grid, kThreads, 0, stream>>>(from, ldw, q.n, q.k, codes, scales, zeros);
+  else w4_quantize_kernel<T, G, true><<<grid, kThreads, 0, stream>>>(from, ldw, q.n, q.k, codes, scales, zeros);
   return static_cast<int>(cudaGetLastError());
 }
 
@@ -244,7 +260,7 @@ int dequantize(const W4& w, void* out, long long ldo, cudaStream_t stream) {
   if (int rc = grid_of(w.n, ceil_div(w4_blocks(w.k), kSpanBlocks), &grid)) return rc;
   w4_dequantize_kernel<T><<<grid, kThreads, 0, stream>>>(static_cast<const uint8_t*>(w.codes), static_cast<const T*>(w.scales),
                                                          static_cast<const uint8_t*>(w.zeros), w.n, w.k, w.group,
-                                                         static_cast<T*>(out), ldo, aligned(out, 16) && ldo % 8 == 0);
+                                                         static_cast<T*>(out), ldo);
   return static_cast<int>(cudaGetLastError());
 }
 
