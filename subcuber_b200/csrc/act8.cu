@@ -84,16 +84,18 @@ __global__ void __launch_bounds__(kThreads) act8_save_kernel(const T* __restrict
   const bool bad = top >= 0x7f800000u || e > ActRange<T>::hi;
   if (e < ActRange<T>::lo) e = ActRange<T>::lo;
   const float inv = __uint_as_float(static_cast<uint32_t>(127 - (bad ? 0 : e)) << 23);
+  const uint32_t keep = bad ? 0x80808080u : 0xffffffffu;
   uint32_t w[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    w[j] = 0;
+    uint32_t q[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      // adding 2^23 rounds to a whole number (nearest, ties to even) in the last bits
       const float a = f[4 * j + i];
-      const uint32_t mag = bad ? 0u : static_cast<uint32_t>(fminf(rintf(fabsf(a) * inv), 127.f));
-      w[j] |= (mag | ((__float_as_uint(a) >> 24) & 128u)) << (8 * i);
+      q[i] = (__float_as_uint(fminf(fabsf(a) * inv, 127.f) + 8388608.f) & 0x7fu) | ((__float_as_uint(a) >> 24) & 128u);
     }
+    w[j] = (q[0] | (q[1] << 8) | (q[2] << 16) | (q[3] << 24)) & keep;
   }
   if (!live) return;
   // the second half of a row's last block may lie behind the row, which ends at k rounded up to 16
@@ -114,13 +116,12 @@ __global__ void __launch_bounds__(kThreads) act8_restore_kernel(const uint8_t* _
   const bool staged = !wide && cut.cols_log2 >= 5;
   __shared__ __align__(16) T stage[kThreads * 16];
   if (row >= m || (k0 >= k && !staged)) return;
-  T v[16] = {};
+  __align__(16) T v[16] = {};
   if (k0 < k) {
     const uint4 raw = __ldg(reinterpret_cast<const uint4*>(codes + row * pitch + k0));
-    const float step = act8_step(exps[row * exp_pitch + (piece >> 1)]);
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = from_f32<T>(act8_value((w[i >> 2] >> (8 * (i & 3))) & 255u, step));
+    const Act8Step<T> step(exps[row * exp_pitch + (piece >> 1)]);
+    reinterpret_cast<uint4*>(v)[0] = expand_act8<T>(raw.x, raw.y, step);
+    reinterpret_cast<uint4*>(v)[1] = expand_act8<T>(raw.z, raw.w, step);
   }
   if (staged) {
     const int lane = threadIdx.x & 31, first = k0 - lane * 16;

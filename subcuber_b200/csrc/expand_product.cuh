@@ -116,77 +116,6 @@ __device__ __forceinline__ uint32_t lds_u8(uint32_t smem_addr) {
   return v;
 }
 
-template <typename T> struct Half;
-template <> struct Half<__half> {
-  static constexpr uint32_t fmt = 0;              // of the instruction descriptor
-  static constexpr uint32_t magic = 0x64006400u;  // 1024, last bit 1
-  typedef __half2 two;
-};
-template <> struct Half<__nv_bfloat16> {
-  static constexpr uint32_t fmt = 1;
-  static constexpr uint32_t magic = 0x43004300u;  // 128, last bit 1
-  typedef __nv_bfloat162 two;
-};
-template <typename T> __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
-  typedef typename Half<T>::two H;
-  const H r = __hsub2(*reinterpret_cast<const H*>(&a), *reinterpret_cast<const H*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-template <typename T> __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
-  typedef typename Half<T>::two H;
-  const H r = __hmul2(*reinterpret_cast<const H*>(&a), *reinterpret_cast<const H*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-
-// Eight codes of a word to eight weights, in the order of the inputs.  bias = magic + zero, scale twice.
-template <typename T>
-__device__ __forceinline__ uint4 expand_w4(uint32_t w, uint32_t bias, uint32_t scale) {
-  uint4 r;
-  r.x = mul2<T>(sub2<T>((w & 0x000f000fu) | Half<T>::magic, bias), scale);
-  r.y = mul2<T>(sub2<T>(((w >> 4) & 0x000f000fu) | Half<T>::magic, bias), scale);
-  r.z = mul2<T>(sub2<T>(((w >> 8) & 0x000f000fu) | Half<T>::magic, bias), scale);
-  r.w = mul2<T>(sub2<T>(((w >> 12) & 0x000f000fu) | Half<T>::magic, bias), scale);
-  return r;
-}
-
-// Two bytes (sign, 7 bits of magnitude) to two values.
-//   bf16  the magnitude is OR-ed under the exponent of 2^(e + 7), where its last bit is worth 2^e: the number is
-//         +-(2^(e+7) + magnitude 2^e), and subtracting its own leading term leaves the value.  `e` holds that exponent's
-//         bits twice; all ones (a block that reads as NaN) gives infinity - infinity or NaN.
-//   f16   the magnitude under the exponent of 1024 in the same way, then a product with 2^e (`s`), which is exact.
-template <typename T> struct Act8Step;
-template <> struct Act8Step<__nv_bfloat16> {
-  uint32_t e;
-  __device__ __forceinline__ explicit Act8Step(uint32_t exponent) {
-    const uint32_t field = exponent + 7u > 255u ? 255u : exponent + 7u;
-    e = (field << 7) | (field << 23);
-  }
-  __device__ __forceinline__ uint32_t two(uint32_t bytes_twice) const {
-    const uint32_t p = (bytes_twice & 0x807f807fu) | e;
-    return sub2<__nv_bfloat16>(p, p & 0xff80ff80u);
-  }
-};
-template <> struct Act8Step<__half> {
-  uint32_t s;
-  __device__ __forceinline__ explicit Act8Step(uint32_t exponent) {
-    const __half2 h = __float2half2_rn(act8_step(static_cast<int>(exponent)));
-    s = *reinterpret_cast<const uint32_t*>(&h);
-  }
-  __device__ __forceinline__ uint32_t two(uint32_t bytes_twice) const {
-    const uint32_t p = (bytes_twice & 0x807f807fu) | 0x64006400u;
-    return mul2<__half>(sub2<__half>(p, p & 0xfc00fc00u), s);
-  }
-};
-template <typename T>
-__device__ __forceinline__ uint4 expand_act8(uint32_t w0, uint32_t w1, const Act8Step<T>& st) {  // eight channels
-  uint4 r;
-  r.x = st.two(__byte_perm(w0, 0, 0x1100));
-  r.y = st.two(__byte_perm(w0, 0, 0x3322));
-  r.z = st.two(__byte_perm(w1, 0, 0x1100));
-  r.w = st.two(__byte_perm(w1, 0, 0x3322));
-  return r;
-}
-
 struct ExpandUnit {
   int row0, col0;  // of the pair's tile
   int k0, k1;      // steps

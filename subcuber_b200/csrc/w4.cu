@@ -75,39 +75,49 @@ __global__ void __launch_bounds__(kThreads) w4_quantize_kernel(const T* __restri
 #pragma unroll
     for (int b = 0; b < kSpanBlocks; ++b) {
       const int k0 = (span * kSpanBlocks + b) * kW4Block + lane * 4;
+      // The largest value above zero and the largest magnitude below it, as bits: those of floats above zero are in the
+      // order of whole numbers, NaN above infinity.
       float x[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = to_f32(v[b][i]);
-      // magnitudes compare as their bits, NaN above infinity
-      uint32_t top = 0;
-      float lo = 0.f, hi = 0.f;
+      int hi = 0, lo = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t bits = __float_as_uint(x[i]) & 0x7fffffffu;
-        top = bits > top ? bits : top;
-        lo = fminf(lo, x[i]);
-        hi = fmaxf(hi, x[i]);
+        x[i] = to_f32(v[b][i]);
+        const int bits = __float_as_int(x[i]);
+        hi = max(hi, bits);
+        lo = max(lo, bits ^ static_cast<int>(0x80000000u));
       }
+      if (SYM) hi = max(hi, lo);
+      if (G == 128) {
+        hi = static_cast<int>(__reduce_max_sync(0xffffffffu, static_cast<uint32_t>(hi)));
+        if (!SYM) lo = static_cast<int>(__reduce_max_sync(0xffffffffu, static_cast<uint32_t>(lo)));
+      } else {
 #pragma unroll
-      for (int s = G / 8; s >= 1; s >>= 1) {
-        const uint32_t o = __shfl_xor_sync(0xffffffffu, top, s);
-        top = o > top ? o : top;
-        if (!SYM) {
-          lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, s));
-          hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, s));
+        for (int s = G / 8; s >= 1; s >>= 1) {
+          hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, s));
+          if (!SYM) lo = max(lo, __shfl_xor_sync(0xffffffffu, lo, s));
         }
       }
-      const float range = top > 0x7f800000u ? __uint_as_float(top) : (SYM ? __uint_as_float(top) : hi - lo);
+      const float range = SYM ? __int_as_float(hi) : __int_as_float(hi) + __int_as_float(lo);  // NaN and infinity stay
       const T s16 = from_f32<T>(__fdiv_rn(range, SYM ? 7.f : 15.f));
       const float s = to_f32(s16);
       const bool usable = s > 0.f && s < INFINITY;
-      float z = SYM ? 8.f : 0.f;
-      if (!SYM && usable) z = fminf(rintf(__fdiv_rn(-lo, s)), 15.f);
-      uint32_t q[4];
+      int z = SYM ? 8 : 0;
+      uint32_t q[4] = {static_cast<uint32_t>(z), static_cast<uint32_t>(z), static_cast<uint32_t>(z), static_cast<uint32_t>(z)};
+      if (usable) {
+        // rint(x / s) without a division.  x and s have 11 significant bits at most, so that a quotient up to 2^5 that is
+        // not halfway between two whole numbers is at least 2^-13 away from that; the product with the reciprocal is off by 2^-18 at
+        // most.  Adding and taking off 768 leaves multiples of 2^-14: a quotient that is halfway becomes exactly so, and no
+        // other one crosses.  Adding 1.5 * 2^23 then rounds to nearest, ties to even, as rint(x / s) does.
+        // Scales whose reciprocal is not a normal number take the division.
+        const bool plain = s < 0x1p-120f || s > 0x1p120f;
+        const float inv = plain ? 0.f : __frcp_rn(s);
+        auto code = [&](float a) {
+          const float r = plain ? __fdiv_rn(a, s) : __fadd_rn(__fadd_rn(__fmul_rn(a, inv), 768.f), -768.f);
+          return __float_as_int(__fadd_rn(r, 12582912.f)) - 0x4b400000;
+        };
+        if (!SYM) z = min(code(__int_as_float(lo)), 15);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float c = usable ? rintf(__fdiv_rn(x[i], s)) + z : z;
-        q[i] = static_cast<uint32_t>(fminf(fmaxf(c, 0.f), 15.f));
+        for (int i = 0; i < 4; ++i) q[i] = static_cast<uint32_t>(min(max(code(x[i]) + z, 0), 15));
       }
       const uint32_t word = join_codes(q, lane);
       if (!(lane & 1)) *reinterpret_cast<uint32_t*>(tile + b * kW4TileBytes + word_offset(r, lane >> 1)) = word;
@@ -171,17 +181,14 @@ __global__ void __launch_bounds__(kThreads) w4_dequantize_kernel(const uint8_t* 
     const uint4 raw = __ldg(reinterpret_cast<const uint4*>(codes) +
                             (static_cast<long long>(rt) * blocks + block) * (kW4TileBytes / 16) + piece);
     const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+    const int per = kW4Block / G;
+    const long long at = ((static_cast<long long>(rt) * blocks + block) * kW4Rows + r) * per;
+    T* to = &rows[r][(threadIdx.x >> 6) * kW4Block + 8 * t];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int k0 = block * kW4Block + 32 * j + 8 * t;
-      const long long at = w4_table_at(rt * kW4Rows + r, k0 / G, blocks, G);
-      const float s = to_f32(scales[at]);
-      const float z = zeros ? static_cast<float>(zeros[at]) : 8.f;
-      T v[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        v[i] = from_f32<T>((static_cast<float>((words[j] >> (4 * w4_nibble(i))) & 15u) - z) * s);
-      *reinterpret_cast<uint4*>(&rows[r][k0 - span * kSpan]) = *reinterpret_cast<const uint4*>(v);
+      const uint32_t s = reinterpret_cast<const uint16_t*>(scales)[at + j * per / 4], z = zeros ? zeros[at + j * per / 4] : 8u;
+      *reinterpret_cast<uint4*>(to + 32 * j) =
+          expand_w4<T>(words[j], Half<T>::magic + __byte_perm(z, 0, 0x4040), __byte_perm(s, 0, 0x1010));
     }
   }
   __syncthreads();
