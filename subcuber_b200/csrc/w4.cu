@@ -11,43 +11,46 @@ namespace sb200 {
 namespace lowbit {
 namespace {
 
-// A block of threads handles one row tile (16 rows) and kSpan inputs: warp w takes rows w and w + 8, a lane four
-// neighbouring inputs of each 128.  The codes are put together in shared memory and leave as whole tiles.
+// A block of threads handles one row tile (16 rows) and kSpanBlocks tiles of 128 inputs: half a warp takes a row, a lane eight
+// neighbouring inputs of each 128, which are one word of the format.  The codes are put together in shared memory and
+// leave as whole tiles.
 constexpr int kSpanBlocks = 4;
 constexpr int kThreads = 256;
 
-// Four neighbouring 16-bit values of a row for each lane, zeros behind `k`; the lanes of the warp take 128 neighbours.  A row
-// that does not start on 8 bytes is read in the aligned 8-byte words that hold it: a lane takes its word, the rest from
-// the lane behind (the last lane reads one more), and shifts the two together.  Words without a value of the row are
-// not read.
+// Eight neighbouring 16-bit values of a row for each lane, zeros behind `k`; the 16 lanes of half a warp take 128
+// neighbours.  A row that does not start on 8 bytes is read in the aligned 8-byte words that hold it: a lane takes two words, the
+// rest from the lane behind (the last lane reads one more), and shifts them together.  Words without a value of the
+// row are not read.
 template <typename T>
-__device__ __forceinline__ void load4(const T* row, int k0, int k, T (&v)[4], int lane) {
-  const uintptr_t at = reinterpret_cast<uintptr_t>(row + k0);
-  const uint32_t off = at & 7;  // the same for all lanes
-  const unsigned long long* word = reinterpret_cast<const unsigned long long*>(at - off);
-  const uintptr_t end = reinterpret_cast<uintptr_t>(row + k);
-  unsigned long long lo = 0;
-  if (k0 < k || at - off < end) lo = __ldg(word);
-  if (off) {
-    unsigned long long hi = __shfl_down_sync(0xffffffffu, lo, 1);
-    if (lane == 31) hi = at - off + 8 < end ? __ldg(word + 1) : 0ull;
-    lo = (lo >> (8 * off)) | (hi << (64 - 8 * off));
+__device__ __forceinline__ void load8(const T* row, int k0, int k, T (&v)[8], int lane) {
+  const uintptr_t at = reinterpret_cast<uintptr_t>(row + k0), end = reinterpret_cast<uintptr_t>(row + k);
+  unsigned long long* to = reinterpret_cast<unsigned long long*>(v);
+  const uint32_t off = at & 7;  // the same for the lanes of a row
+  if ((at & 15) == 0 && k0 + 8 <= k) {
+    *reinterpret_cast<uint4*>(v) = __ldg(reinterpret_cast<const uint4*>(at));
+  } else {
+    const unsigned long long* word = reinterpret_cast<const unsigned long long*>(at - off);
+    to[0] = k0 < k || at - off < end ? __ldg(word) : 0ull;
+    to[1] = at - off + 8 < end ? __ldg(word + 1) : 0ull;
   }
-  const int left = k - k0;
-  if (left < 4) lo = left <= 0 ? 0ull : lo & (~0ull >> (64 - 16 * left));
-  *reinterpret_cast<unsigned long long*>(v) = lo;
+  if (__any_sync(0xffffffffu, off)) {
+    unsigned long long next = __shfl_down_sync(0xffffffffu, to[0], 1, 16);
+    if (off) {
+      if ((lane & 15) == 15) next = at - off + 16 < end ? __ldg(reinterpret_cast<const unsigned long long*>(at - off) + 2) : 0ull;
+      to[0] = (to[0] >> (8 * off)) | (to[1] << (64 - 8 * off));
+      to[1] = (to[1] >> (8 * off)) | (next << (64 - 8 * off));
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int left = k - k0 - 4 * i;
+    if (left < 4) to[i] = left <= 0 ? 0ull : to[i] & (~0ull >> (64 - 16 * left));
+  }
 }
 
-// Places the four codes of a lane (inputs 4 (lane & 1) .. + 3 of a word) in the word of its pair of lanes.
-__device__ __forceinline__ uint32_t join_codes(const uint32_t (&q)[4], int lane) {
-  const int first = (lane & 1) * 2;  // nibble of the lane's first input
-  uint32_t w = (q[0] | (q[1] << 16) | (q[2] << 4) | (q[3] << 20)) << (4 * first);
-  return w | __shfl_xor_sync(0xffffffffu, w, 1);
-}
-
-// Bytes of a tile where the word of (row, pair of lanes) goes: pair = 4 j + t.
-__device__ __forceinline__ int word_offset(int row, int pair) {
-  return (row >> 3) * 512 + ((row & 7) * 4 + (pair & 3)) * 16 + (pair >> 2) * 4;
+// Bytes of a tile where the word of (row, eight inputs) goes: word = 4 j + t.
+__device__ __forceinline__ int word_offset(int row, int word) {
+  return (row >> 3) * 512 + ((row & 7) * 4 + (word & 3)) * 16 + (word >> 2) * 4;
 }
 
 // Quantisation, one group at a time.  Symmetric: scale = amax / 7 and codes 8 + rint(w / scale).  Else the range
@@ -63,74 +66,69 @@ __global__ void __launch_bounds__(kThreads) w4_quantize_kernel(const T* __restri
   const int blocks = w4_blocks(k);
   const int spans = ceil_div(blocks, kSpanBlocks);
   const int rt = blockIdx.x / spans, span = blockIdx.x % spans;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, word = lane & 15, r = threadIdx.x >> 4;
+  const int row = rt * kW4Rows + r;
+  const int first = span * (kSpanBlocks * kW4Block) + word * 8;
+  __align__(16) T v[kSpanBlocks][8];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int r = warp + 8 * h;
-    const int row = rt * kW4Rows + r;
-    T v[kSpanBlocks][4];
+  for (int b = 0; b < kSpanBlocks; ++b) load8<T>(w + (row < n ? row : 0) * ldw, first + b * kW4Block, row < n ? k : 0, v[b], lane);
 #pragma unroll
-    for (int b = 0; b < kSpanBlocks; ++b)
-      load4<T>(w + (row < n ? row : 0) * ldw, (span * kSpanBlocks + b) * kW4Block + lane * 4, row < n ? k : 0, v[b], lane);
+  for (int b = 0; b < kSpanBlocks; ++b) {
+    // The largest value above zero and the largest magnitude below it, as bits: those of floats above zero are in the
+    // order of whole numbers, NaN above infinity.
+    float x[8];
+    int hi = 0, lo = 0;
 #pragma unroll
-    for (int b = 0; b < kSpanBlocks; ++b) {
-      const int k0 = (span * kSpanBlocks + b) * kW4Block + lane * 4;
-      // The largest value above zero and the largest magnitude below it, as bits: those of floats above zero are in the
-      // order of whole numbers, NaN above infinity.
-      float x[4];
-      int hi = 0, lo = 0;
+    for (int i = 0; i < 8; ++i) {
+      x[i] = to_f32(v[b][i]);
+      const int bits = __float_as_int(x[i]);
+      hi = max(hi, SYM ? bits & 0x7fffffff : bits);
+      if (!SYM) lo = max(lo, bits ^ static_cast<int>(0x80000000u));
+    }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[i] = to_f32(v[b][i]);
-        const int bits = __float_as_int(x[i]);
-        hi = max(hi, bits);
-        lo = max(lo, bits ^ static_cast<int>(0x80000000u));
-      }
-      if (SYM) hi = max(hi, lo);
-      if (G == 128) {
-        hi = static_cast<int>(__reduce_max_sync(0xffffffffu, static_cast<uint32_t>(hi)));
-        if (!SYM) lo = static_cast<int>(__reduce_max_sync(0xffffffffu, static_cast<uint32_t>(lo)));
-      } else {
+    for (int s = G / 16; s >= 1; s >>= 1) {
+      hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, s));
+      if (!SYM) lo = max(lo, __shfl_xor_sync(0xffffffffu, lo, s));
+    }
+    // amax / 7 may be a product with 1 / 7: amax has 11 significant bits at most, so that the quotient is a fourteenth of a
+    // 16-bit step or more away from where the rounding to 16 bits changes.  hi - lo has more bits.
+    const float range = SYM ? __int_as_float(hi) : __int_as_float(hi) + __int_as_float(lo);  // NaN and infinity stay
+    const T s16 = from_f32<T>(SYM ? range * (1.f / 7.f) : __fdiv_rn(range, 15.f));
+    const float s = to_f32(s16);
+    const bool usable = s > 0.f && s < INFINITY;
+    int z = SYM ? 8 : 0;
+    int q[8];
 #pragma unroll
-        for (int s = G / 8; s >= 1; s >>= 1) {
-          hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, s));
-          if (!SYM) lo = max(lo, __shfl_xor_sync(0xffffffffu, lo, s));
-        }
-      }
-      const float range = SYM ? __int_as_float(hi) : __int_as_float(hi) + __int_as_float(lo);  // NaN and infinity stay
-      const T s16 = from_f32<T>(__fdiv_rn(range, SYM ? 7.f : 15.f));
-      const float s = to_f32(s16);
-      const bool usable = s > 0.f && s < INFINITY;
-      int z = SYM ? 8 : 0;
-      uint32_t q[4] = {static_cast<uint32_t>(z), static_cast<uint32_t>(z), static_cast<uint32_t>(z), static_cast<uint32_t>(z)};
-      if (usable) {
-        // rint(x / s) without a division.  x and s have 11 significant bits at most, so that a quotient up to 2^5 that is
-        // not halfway between two whole numbers is at least 2^-13 away from that; the product with the reciprocal is off by 2^-18 at
-        // most.  Adding and taking off 768 leaves multiples of 2^-14: a quotient that is halfway becomes exactly so, and no
-        // other one crosses.  Adding 1.5 * 2^23 then rounds to nearest, ties to even, as rint(x / s) does.
-        // Scales whose reciprocal is not a normal number take the division.
-        const bool plain = s < 0x1p-120f || s > 0x1p120f;
-        const float inv = plain ? 0.f : __frcp_rn(s);
-        auto code = [&](float a) {
-          const float r = plain ? __fdiv_rn(a, s) : __fadd_rn(__fadd_rn(__fmul_rn(a, inv), 768.f), -768.f);
-          return __float_as_int(__fadd_rn(r, 12582912.f)) - 0x4b400000;
-        };
-        if (!SYM) z = min(code(__int_as_float(lo)), 15);
+    for (int i = 0; i < 8; ++i) q[i] = z;
+    if (usable) {
+      // rint(x / s) without a division.  x and s have 11 significant bits at most, so that a quotient up to 2^5 that is
+      // not halfway between two whole numbers is at least 2^-13 away from that; the product with the reciprocal is off by
+      // 2^-17 at most.  Adding and taking off 768 leaves multiples of 2^-14: a quotient that is halfway becomes exactly so, and
+      // no other one crosses.  Adding 1.5 * 2^23 then rounds to nearest, ties to even, as rint(x / s) does.  Scales
+      // whose reciprocal is not a normal number take the division.
+      const bool plain = s < 0x1p-120f || s > 0x1p120f;
+      const float inv = plain ? 0.f : __fdividef(1.f, s);
+      auto code = [&](float a) {
+        const float r = plain ? __fdiv_rn(a, s) : __fadd_rn(__fadd_rn(__fmul_rn(a, inv), 768.f), -768.f);
+        return __float_as_int(__fadd_rn(r, 12582912.f)) - 0x4b400000;
+      };
+      if (!SYM) z = min(code(__int_as_float(lo)), 15);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) q[i] = static_cast<uint32_t>(min(max(code(x[i]) + z, 0), 15));
-      }
-      const uint32_t word = join_codes(q, lane);
-      if (!(lane & 1)) *reinterpret_cast<uint32_t*>(tile + b * kW4TileBytes + word_offset(r, lane >> 1)) = word;
-      if (lane % (G / 4) == 0 && k0 < blocks * kW4Block) {
-        const long long at = w4_table_at(row, k0 / G, blocks, G);
-        scales[at] = s16;
-        if (!SYM) zeros[at] = static_cast<uint8_t>(z);
-      }
+      for (int i = 0; i < 8; ++i) q[i] = min(max(code(x[i]) + z, 0), 15);
+    }
+    uint32_t packed = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) packed |= static_cast<uint32_t>(q[i]) << (4 * w4_nibble(i));
+    *reinterpret_cast<uint32_t*>(tile + b * kW4TileBytes + word_offset(r, word)) = packed;
+    const int block = span * kSpanBlocks + b;
+    if (word % (G / 8) == 0 && block < blocks) {
+      const long long at = ((static_cast<long long>(rt) * blocks + block) * kW4Rows + r) * (kW4Block / G) + word / (G / 8);
+      scales[at] = s16;
+      if (!SYM) zeros[at] = static_cast<uint8_t>(z);
     }
   }
   __syncthreads();
-  const int block = span * kSpanBlocks + threadIdx.x / (kW4TileBytes / 16);
-  if (block < blocks)
+  if (span * kSpanBlocks + static_cast<int>(threadIdx.x) / (kW4TileBytes / 16) < blocks)
     reinterpret_cast<uint4*>(codes)[(static_cast<long long>(rt) * blocks + span * kSpanBlocks) * (kW4TileBytes / 16) +
                                     threadIdx.x] = reinterpret_cast<const uint4*>(tile)[threadIdx.x];
 }
