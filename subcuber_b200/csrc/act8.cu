@@ -147,6 +147,7 @@ int check(const Act8& a) {
   if (a.dtype != kF16 && a.dtype != kBF16) return kErrNotSupported;
   if (a.m < 0 || a.k <= 0 || a.pitch < a.k || a.exp_pitch < ceil_div(a.k, kActBlock)) return kErrInvalidProblem;
   if (a.m > 0 && (!a.codes || !a.exps)) return kErrInvalidProblem;
+  if (a.exp_pitch > 0x7fffffffll) return kErrNotSupported;
   if (!aligned(a.codes, 16) || a.pitch % 16 || !aligned(a.exps, 4) || a.exp_pitch % 4) return kErrMisalignedOperand;
   return kOk;
 }

@@ -19,11 +19,12 @@ struct Cut {
 };
 
 // Tile width and parts of the reduction.  A step of 64 costs a pair about 2 bn clocks on the tensor cores (256 rows x bn
-// columns x 64 at 8192 operations a clock and SM) and never less than the converters take; a unit more than that for filling its pipeline
-// and for its sums; dividing the reduction costs a pass over the parts, and a launch.  The cut with the least total of
-// the fullest pair wins; widths are what the instruction takes.
+// columns x 64 at 8192 operations a clock and SM) and never less than what the hand-overs between the roles take (measured:
+// 0.37 us at every narrow tile); a unit more than that for filling its pipeline and for its sums; dividing the
+// reduction costs a pass over the parts, and a launch.  The cut with the least total of the fullest pair wins; widths
+// are what the instruction takes.  (128 rows through 4096 x 4096 4-bit weights: 16 tiles; in one part 38 us, in four 16 us.)
 Cut cut_of(long long rows, long long cols, int steps, int pairs) {
-  const double kConvert = 250, kUnit = 1500, kJoin = 6000, kBytesPerClock = 2500;
+  const double kStepLeast = 700, kUnit = 4000, kJoin = 4000, kBytesPerClock = 4000;
   Cut best{kMaxCols, 1};
   double least = 1e300;
   for (int bn = kMaxCols; bn >= 32; bn -= 32) {
@@ -31,7 +32,7 @@ Cut cut_of(long long rows, long long cols, int steps, int pairs) {
     for (int s = 1; s <= kMaxSlices; ++s) {
       if (s > 1 && (s > (steps + 1) / 2 || static_cast<double>(s) * rows * cols * 4 > kPartBytes)) break;
       const double waves = ceil(tiles * s / pairs);
-      const double step = 2 * bn > kConvert ? 2 * bn : kConvert;
+      const double step = 2 * bn > kStepLeast ? 2 * bn : kStepLeast;
       double t = waves * (2 * ceil((steps + 1) / 2 / static_cast<double>(s)) * step + kUnit);
       if (s > 1) t += kJoin + (2.0 * s + 1) * rows * cols * 4 / kBytesPerClock;
       if (t < least) { least = t; best = Cut{bn, s}; }
@@ -217,7 +218,7 @@ int expand_act8(const Act8& a, const void* dy, long long lddy, bool out_f32, con
                 long long lddw, int n, void* workspace, cudaStream_t stream) {
   ExpandParams p = {};
   p.exps = static_cast<const uint8_t*>(a.exps);
-  p.exp_pitch = a.exp_pitch;
+  p.exp_pitch = static_cast<int>(a.exp_pitch);
   p.rows = a.k;
   p.cols = n;
   p.depth = a.m;
@@ -243,7 +244,12 @@ int expand_act8(const Act8& a, const void* dy, long long lddy, bool out_f32, con
     }
     p.part = reinterpret_cast<float*>(ws);
     if (!(pairs = place(p, pairs_of_device()))) return kErrNotSupported;
-    if ((rc = tc::map_rows_16bit(&p.right, dy, a.m, n, lddy, kStep))) return rc;
+    // one load for a CTA's half of the columns where that is whole blocks of 64, and the matrix too (a partial last block
+    // would be read past the end of the row)
+    p.right_blocked = n % 64 == 0 && p.bn % 128 == 0;
+    if ((rc = p.right_blocked ? tc::map_blocks_16bit(&p.right, dy, a.m, n, lddy, kStep, p.bn / 128)
+                              : tc::map_rows_16bit(&p.right, dy, a.m, n, lddy, kStep)))
+      return rc;
     if ((rc = tc::map_rows_plain(&p.codes_map, a.codes, 1, a.m, static_cast<long long>(align_up(a.k, 16)), a.pitch, kStep, kCtaRows)))
       return rc;
   }

@@ -34,7 +34,8 @@ struct ExpandParams {
   const void* scales;       // W4
   const uint8_t* zeros;     // W4, or null
   const uint8_t* exps;      // ACT8
-  long long exp_pitch;
+  int exp_pitch;            // ACT8
+  int right_blocked;        // ACT8: `right` is [block of 64 columns][token][64], one box for a CTA's whole half
   int rows, cols;           // of the result: left rows, right columns
   int depth;                // length of the reduction
   int bn;                   // columns of a tile, a multiple of 32 up to 256
@@ -268,7 +269,6 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
     if (warp != 1) {
       // ---- producers: codes, tables and the CTA's half of the right operand.  The loads of one warp complete one after the
       // other (about 240 ns each, whatever they hold), so three warps take the steps (W4: pairs of steps) in turn.
-      const int blocks = w4_blocks(p.depth), tiles = w4_row_tiles(p.rows);
       const int boxes = KIND == kExpandW4 ? 1 : (half + 63) / 64;
       const uint32_t bytes = 2u * (KIND == kExpandW4 ? half * 128 : boxes * kRightBlock);  // both CTAs'
       constexpr int kEach = KIND == kExpandW4 ? 2 : 1;  // steps of a tile of codes
@@ -283,6 +283,26 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
         const ExpandUnit w = expand_unit(p, u);
         const int row0 = w.row0 + static_cast<int>(rank) * kCtaRows;
         const int col0 = w.col0 + static_cast<int>(rank) * half;
+        // where this lane's pieces of the tables come from; W4: of 24 PER pieces of 16 bytes (2 PER of scales for each of the
+        // eight row tiles, then PER of zeros), three at most; ACT8: the exponents of two tokens, 32 apart
+        constexpr int kCopies = KIND == kExpandW4 ? (24 * PER + 31) / 32 : 2;
+        const uint8_t* from[kCopies];
+        bool real[kCopies];
+#pragma unroll
+        for (int c = 0; c < kCopies; ++c) {
+          if (KIND == kExpandW4) {
+            const int i = c * 32 + lane;
+            const bool zero = i >= 16 * PER;
+            const int j = zero ? i - 16 * PER : i, each = zero ? PER : 2 * PER;
+            const int tile = row0 / kW4Rows + j / each;
+            real[c] = i < 24 * PER && tile < w4_row_tiles(p.rows) && (!zero || p.zeros);
+            from[c] = static_cast<const uint8_t*>(p.scales);
+            if (real[c]) from[c] = (zero ? p.zeros : from[c]) + (static_cast<long long>(tile) * w4_blocks(p.depth) * each + j % each) * 16;
+          } else {
+            real[c] = row0 < p.rows;
+            from[c] = p.exps + (real[c] ? row0 / kActBlock : 0);
+          }
+        }
         for (int kk = w.k0; ok && kk < w.k1; kk += kEach) {
           const bool mine = turn == 0;
           turn = mine ? kProducers - 1 : turn - 1;
@@ -299,26 +319,15 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
             }
             __syncwarp();
             const uint32_t table = ptx::smem_u32(tables + rstage * kTable);
-            if (KIND == kExpandW4) {
-              // 2 PER pieces of 16 bytes of scales for each of the eight row tiles, then PER of zeros
 #pragma unroll
-              for (int i0 = 0; i0 < 24 * PER; i0 += 32) {
-                const int i = i0 + lane;
-                if (i >= 24 * PER) break;
-                const bool zero = i >= 16 * PER;
-                const int j = zero ? i - 16 * PER : i, each = zero ? PER : 2 * PER;
-                const int tile = row0 / kW4Rows + j / each;
-                const bool real = tile < tiles && (!zero || p.zeros);
-                const long long at = (static_cast<long long>(tile) * blocks + kk / 2) * each + j % each;
-                const uint8_t* from = zero ? p.zeros : static_cast<const uint8_t*>(p.scales);
-                copy_async_16(table + i * 16, real ? from + at * 16 : static_cast<const uint8_t*>(p.scales), real);
-              }
-            } else {
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const long long tok = static_cast<long long>(kk) * kStep + lane + 32 * i;
-                const bool real = tok < p.depth && row0 < p.rows;
-                copy_async_4(table + (lane + 32 * i) * 4, real ? p.exps + tok * p.exp_pitch + row0 / kActBlock : p.exps, real);
+            for (int c = 0; c < kCopies; ++c) {
+              const int i = c * 32 + lane;
+              if (KIND == kExpandW4) {
+                if (i < 24 * PER) copy_async_16(table + i * 16, from[c] + (real[c] ? kk * (i >= 16 * PER ? 8 * PER : 16 * PER) : 0), real[c]);
+              } else {
+                const int token = kk * kStep + i;
+                const bool in = real[c] && token < p.depth;
+                copy_async_4(table + i * 4, from[c] + (in ? static_cast<long long>(token) * p.exp_pitch : 0), in);
               }
             }
             copy_async_arrive(&raw_full[rstage]);
@@ -337,6 +346,8 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
                 uint8_t* to = smem + stage * kStageBytes + kLeftBytes;
                 if (KIND == kExpandW4) {
                   ptx::tma_load_2d_pair(to, &p.right, &full_bar[stage], (kk + h) * kStep, col0);
+                } else if (p.right_blocked) {
+                  ptx::tma_load_3d_pair(to, &p.right, &full_bar[stage], 0, kk * kStep, col0 / 64);
                 } else {
                   for (int b = 0; b < boxes; ++b)
                     ptx::tma_load_2d_pair(to + b * kRightBlock, &p.right, &full_bar[stage], col0 + b * 64, kk * kStep);

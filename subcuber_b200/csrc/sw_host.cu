@@ -860,6 +860,15 @@ int map_rows_16bit(void* map, const void* ptr, long long rows, long long cols, l
   return r == CUDA_SUCCESS ? kOk : kErrInternal;
 }
 
+int map_blocks_16bit(void* map, const void* ptr, long long rows, long long cols, long long ld, int box_rows, int box_blocks) {
+  View v;
+  v.ptr = ptr;
+  v.rows = static_cast<int>(rows);
+  v.cols = static_cast<int>(cols);
+  v.ld = ld;
+  return make_tmap_b_blocked(static_cast<CUtensorMap*>(map), 2, v, box_rows, box_blocks, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
 int map_rows_plain(void* map, const void* ptr, int esize, long long rows, long long cols, long long pitch, int box_rows,
                    int box_cols) {
   EncodeTiledFn fn = encode_fn();

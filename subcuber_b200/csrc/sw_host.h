@@ -98,6 +98,9 @@ int deal_units(const GemmArgs& args, int sms, int* out, int max_units, int* work
 // Tensor map of a row-major matrix of 16-bit elements (`ld` elements from row to row, rows on 16 bytes) for boxes of 64
 // columns x `box_rows` rows with the 128-byte swizzle; elements outside read as zero.  `map` points to a CUtensorMap.
 int map_rows_16bit(void* map, const void* ptr, long long rows, long long cols, long long ld, int box_rows);
+// The same matrix (cols a multiple of 64) seen as [block of 64 columns][row][64]; boxes hold `box_rows` rows of `box_blocks`
+// blocks, block after block.
+int map_blocks_16bit(void* map, const void* ptr, long long rows, long long cols, long long ld, int box_rows, int box_blocks);
 // The same without a swizzle for elements of `esize` (1 or 4) bytes, rows `pitch` bytes apart, boxes of box_cols x box_rows.
 int map_rows_plain(void* map, const void* ptr, int esize, long long rows, long long cols, long long pitch, int box_rows,
                    int box_cols);
