@@ -12,8 +12,8 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// A thread handles 16 channels of a token, half a block.  `cols` threads (a power of two) stand along a row, the
-// others of the 256 on further rows.
+// A thread handles 16 channels of a token, half a block.  A power of two of threads stand along a row, the others of
+// the 256 on further rows.
 struct Cut {
   int pieces;         // 16-channel pieces of a row
   int cols_log2;      // threads along a row, as a power of two
@@ -21,9 +21,9 @@ struct Cut {
   long long blocks;   // thread blocks in all
 };
 
-Cut cut_of(int m, int k) {
+Cut cut_of(int m, int pieces) {
   Cut c;
-  c.pieces = 2 * ceil_div(k, kActBlock);  // whole blocks of 32: both halves take part in the block's maximum
+  c.pieces = pieces;
   c.cols_log2 = 1;
   while (c.cols_log2 < 8 && (1 << c.cols_log2) < c.pieces) ++c.cols_log2;
   c.parts = ceil_div(c.pieces, 1 << c.cols_log2);
@@ -103,6 +103,20 @@ __global__ void __launch_bounds__(kThreads) act8_save_kernel(const T* __restrict
   if (!(piece & 1)) exps[row * exp_pitch + (piece >> 1)] = static_cast<uint8_t>(bad ? kActNaN : e + 127);
 }
 
+// Rows of 16-bit values to rows on 16 bytes, zeros behind their ends.
+__global__ void __launch_bounds__(kThreads) copy_rows_kernel(uint16_t* __restrict__ dst, int cols_d, const uint16_t* __restrict__ src,
+                                                             int rows, int cols, long long ld, Cut cut) {
+  const long long row = ((blockIdx.x / cut.parts) << (8 - cut.cols_log2)) + (threadIdx.x >> cut.cols_log2);
+  const int piece = (static_cast<int>(blockIdx.x % cut.parts) << cut.cols_log2) + (threadIdx.x & ((1 << cut.cols_log2) - 1));
+  const int k0 = piece * 16;
+  if (row >= rows || k0 >= cols_d) return;
+  __align__(16) uint16_t v[16];
+  load16<uint16_t>(src + row * ld, k0, cols, false, v);
+  uint4* to = reinterpret_cast<uint4*>(dst + row * cols_d + k0);
+  to[0] = reinterpret_cast<const uint4*>(v)[0];
+  if (k0 + 8 < cols_d) to[1] = reinterpret_cast<const uint4*>(v)[1];
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads) act8_restore_kernel(const uint8_t* __restrict__ codes, long long pitch,
                                                                 const uint8_t* __restrict__ exps, long long exp_pitch, int m,
@@ -154,7 +168,7 @@ int check(const Act8& a) {
 
 template <typename T>
 int save(const void* x, long long ldx, const Act8& a, cudaStream_t stream) {
-  const Cut cut = cut_of(a.m, a.k);
+  const Cut cut = cut_of(a.m, 2 * ceil_div(a.k, kActBlock));  // whole blocks of 32: both halves take part in the maximum
   if (cut.blocks > 0x7fffffffll) return kErrNotSupported;
   act8_save_kernel<T><<<static_cast<unsigned>(cut.blocks), kThreads, 0, stream>>>(
       static_cast<const T*>(x), ldx, a.m, a.k, static_cast<uint8_t*>(const_cast<void*>(a.codes)), a.pitch,
@@ -164,7 +178,7 @@ int save(const void* x, long long ldx, const Act8& a, cudaStream_t stream) {
 
 template <typename T>
 int restore(const Act8& a, void* x, long long ldx, cudaStream_t stream) {
-  const Cut cut = cut_of(a.m, a.k);
+  const Cut cut = cut_of(a.m, 2 * ceil_div(a.k, kActBlock));  // whole blocks of 32: both halves take part in the maximum
   if (cut.blocks > 0x7fffffffll) return kErrNotSupported;
   act8_restore_kernel<T><<<static_cast<unsigned>(cut.blocks), kThreads, 0, stream>>>(
       static_cast<const uint8_t*>(a.codes), a.pitch, static_cast<const uint8_t*>(a.exps), a.exp_pitch, a.m, a.k,
@@ -173,6 +187,19 @@ int restore(const Act8& a, void* x, long long ldx, cudaStream_t stream) {
 }
 
 }  // namespace
+
+int copy_rows_16bit(void* dst, int cols_d, const void* src, int rows, int cols, long long ld, cudaStream_t stream) {
+  const Cut cut = cut_of(rows, ceil_div(cols_d, 16));
+  if (cut.blocks > 0x7fffffffll) return kErrNotSupported;
+  copy_rows_kernel<<<static_cast<unsigned>(cut.blocks), kThreads, 0, stream>>>(static_cast<uint16_t*>(dst), cols_d,
+                                                                               static_cast<const uint16_t*>(src), rows, cols, ld, cut);
+  return static_cast<int>(cudaGetLastError());
+}
+
+int restore_act8(const Act8& a, void* x, long long ldx, cudaStream_t stream) {
+  return a.dtype == kF16 ? restore<__half>(a, x, ldx, stream) : restore<__nv_bfloat16>(a, x, ldx, stream);
+}
+
 }  // namespace lowbit
 }  // namespace sb200
 
@@ -198,8 +225,7 @@ extern "C" int sb200_act8_restore(int dtype, const void* codes, long long pitch,
   if (m == 0) return SB200_OK;
   if (!x) return SB200_ERR_INVALID_PROBLEM;
   if (!sb200::lowbit::aligned(x, 2)) return SB200_ERR_MISALIGNED_OPERAND;
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return dtype == sb200::kF16 ? sb200::lowbit::restore<__half>(a, x, ldx, s) : sb200::lowbit::restore<__nv_bfloat16>(a, x, ldx, s);
+  return sb200::lowbit::restore_act8(a, x, ldx, reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" size_t sb200_act8_wgrad_workspace_bytes(int dtype, int out_dtype, int m, int n, int k, int dy_aligned) {

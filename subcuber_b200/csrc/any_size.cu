@@ -202,8 +202,4 @@ int run(const GemmArgs& a, void* workspace, size_t workspace_size, cudaStream_t 
   return mark();
 }
 
-int tc::copy_rows_16bit(void* dst, int cols_d, const void* src, int rows, int cols, long long ld, cudaStream_t stream) {
-  return pad_copy<unsigned short>(dst, rows, cols_d, src, rows, cols, ld, stream);
-}
-
 }  // namespace sb200

@@ -12,6 +12,7 @@ namespace {
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
 constexpr int kMaxSlices = 16;
+constexpr int kDenseColumns = 1280;  // measured: 1000 to 1024 rows through 8192 x 4096: 65 us on the way, 67 us in two passes
 constexpr size_t kPartBytes = size_t(64) << 20;  // most that the parts of a divided reduction may take
 
 struct Cut {
@@ -23,8 +24,8 @@ struct Cut {
 // 0.37 us at every narrow tile); a unit more than that for filling its pipeline and for its sums; dividing the
 // reduction costs a pass over the parts, and a launch.  The cut with the least total of the fullest pair wins; widths
 // are what the instruction takes.  (128 rows through 4096 x 4096 4-bit weights: 16 tiles; in one part 38 us, in four 16 us.)
-Cut cut_of(long long rows, long long cols, int steps, int pairs) {
-  const double kStepLeast = 700, kUnit = 4000, kJoin = 4000, kBytesPerClock = 4000;
+Cut cut_of(long long rows, long long cols, int steps, int pairs, bool dense) {
+  const double kStepLeast = dense ? 500 : 700, kUnit = 4000, kJoin = 4000, kBytesPerClock = 4000;
   Cut best{kMaxCols, 1};
   double least = 1e300;
   for (int bn = kMaxCols; bn >= 32; bn -= 32) {
@@ -51,24 +52,24 @@ size_t part_bytes(long long rows, long long cols) {
   return all < kPartBytes ? all : kPartBytes;
 }
 
-template <typename T, int KIND, int PER>
+template <typename T, int KIND, int PER, bool DENSE>
 int launch(const ExpandParams& p, int pairs, cudaStream_t stream) {
-  auto* kernel = expand_product_kernel<T, KIND, PER>;
+  auto* kernel = expand_product_kernel<T, KIND, PER, DENSE>;
+  constexpr int kSmem = DENSE ? kDenseSmem : expand_smem(KIND, PER);
   static PerDeviceOnce once;
   const int rc = once.run_once([&] {
     // the warps trade registers: a block launched with fewer than the trade needs would wait for good
     cudaFuncAttributes a;
     cudaError_t e = cudaFuncGetAttributes(&a, kernel);
     if (e != cudaSuccess) return static_cast<int>(e);
-    if (a.numRegs != kRegsLaunch) return static_cast<int>(kErrInternal);
-    return static_cast<int>(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 expand_smem(KIND, PER)));
+    if (!DENSE && a.numRegs != kRegsLaunch) return static_cast<int>(kErrInternal);
+    return static_cast<int>(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
   });
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
-  cfg.blockDim = dim3(kExpandThreads);
-  cfg.dynamicSmemBytes = expand_smem(KIND, PER);
+  cfg.blockDim = dim3(DENSE ? kDenseThreads : kExpandThreads);
+  cfg.dynamicSmemBytes = kSmem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -88,8 +89,8 @@ int join(const ExpandParams& p, int rows, int cols, cudaStream_t stream) {
 }
 
 // Fills in the cut; returns the pairs to launch, or 0 when there are too many units.
-int place(ExpandParams& p, int pairs) {
-  const Cut c = cut_of(p.rows, p.cols, p.steps, pairs);
+int place(ExpandParams& p, int pairs, bool dense) {
+  const Cut c = cut_of(p.rows, p.cols, p.steps, pairs, dense);
   p.bn = c.bn;
   p.slices = c.slices;
   p.tiles_r = ceil_div(p.rows, kPairRows);
@@ -100,30 +101,38 @@ int place(ExpandParams& p, int pairs) {
 }
 
 template <typename T>
-int run_w4(const ExpandParams& p, int group, int pairs, cudaStream_t stream) {
+int run_w4(const ExpandParams& p, int group, bool dense, int pairs, cudaStream_t stream) {
   int rc;
-  if (group == 32) rc = launch<T, kExpandW4, 4>(p, pairs, stream);
-  else if (group == 64) rc = launch<T, kExpandW4, 2>(p, pairs, stream);
-  else rc = launch<T, kExpandW4, 1>(p, pairs, stream);
+  if (dense) rc = launch<T, kExpandW4, 1, true>(p, pairs, stream);
+  else if (group == 32) rc = launch<T, kExpandW4, 4, false>(p, pairs, stream);
+  else if (group == 64) rc = launch<T, kExpandW4, 2, false>(p, pairs, stream);
+  else rc = launch<T, kExpandW4, 1, false>(p, pairs, stream);
   if (rc || p.slices == 1) return rc;
   return join<T>(p, p.cols, p.rows, stream);
 }
 
 template <typename T>
-int run_act8(const ExpandParams& p, int pairs, cudaStream_t stream) {
+int run_act8(const ExpandParams& p, bool dense, int pairs, cudaStream_t stream) {
   if (p.steps > 0) {
-    const int rc = launch<T, kExpandAct8, 1>(p, pairs, stream);
+    const int rc = dense ? launch<T, kExpandAct8, 1, true>(p, pairs, stream) : launch<T, kExpandAct8, 1, false>(p, pairs, stream);
     if (rc || p.slices == 1) return rc;
   }
   return p.out_f32 ? join<float>(p, p.rows, p.cols, stream) : join<T>(p, p.rows, p.cols, stream);
 }
+
+// Whether the left operand is expanded once, before the product: from so many columns on that the pass over memory (2.5 or 3
+// bytes a value) costs less than expanding every tile again for each tile of columns.
+bool dense_w4(int m) { return m >= kDenseColumns; }
+bool dense_act8(int n) { return n >= kDenseColumns; }
+size_t dense_bytes(long long rows, long long ld) { return align_up(size_t(rows) * ld * 2, 256); }
 
 constexpr unsigned long long kWaitNs = 2000000000ull;  // bound of every device-side wait
 
 }  // namespace
 
 size_t expand_w4_workspace(int m, int n, int k, bool x_aligned) {
-  return kStatusBytes + (x_aligned ? 0 : copy_bytes(m, k)) + (m > kDecodeMaxRows ? part_bytes(m, n) : 0);
+  return kStatusBytes + (x_aligned ? 0 : copy_bytes(m, k)) + (dense_w4(m) ? dense_bytes(n, align_up(k, 8)) : 0) +
+         (m > kDecodeMaxRows ? part_bytes(m, n) : 0);
 }
 
 int expand_w4(const W4& w, const void* x, long long ldx, void* y, long long ldy, int m, void* workspace, size_t workspace_bytes,
@@ -134,21 +143,29 @@ int expand_w4(const W4& w, const void* x, long long ldx, void* y, long long ldy,
   p.rows = w.n;
   p.cols = m;
   p.depth = w.k;
-  p.steps = 2 * w4_blocks(w.k);
+  p.steps = dense_w4(m) ? ceil_div(w.k, kStep) : 2 * w4_blocks(w.k);
   p.out = y;
   p.ldo = ldy;
   p.wait_ns = kWaitNs;
-  char* ws = static_cast<char*>(workspace);
-  p.status = reinterpret_cast<int*>(ws);
-  p.part = reinterpret_cast<float*>(ws + (workspace_bytes - part_bytes(m, w.n)) / 256 * 256);
-  const int pairs = place(p, pairs_of_device());
+  p.status = static_cast<int*>(workspace);
+  const bool dense = dense_w4(m);
+  char* part = static_cast<char*>(workspace) + (workspace_bytes - part_bytes(m, w.n)) / 256 * 256;
+  p.part = reinterpret_cast<float*>(part);
+  const int pairs = place(p, pairs_of_device(), dense);
   if (!pairs) return kErrNotSupported;
   int rc;
   if ((rc = tc::map_rows_16bit(&p.right, x, m, w.k, ldx, p.bn / 2))) return rc;
-  // a row tile's codes are one row of 32-bit words; a box is 128 inputs of eight row tiles
-  if ((rc = tc::map_rows_plain(&p.codes_map, w.codes, 4, w4_row_tiles(w.n), 256ll * w4_blocks(w.k), 1024ll * w4_blocks(w.k), 8, 256)))
+  if (dense) {
+    const long long ld = static_cast<long long>(align_up(w.k, 8));
+    char* left = part - dense_bytes(w.n, ld);
+    if ((rc = dequantize_w4(w, left, ld, stream))) return rc;
+    if ((rc = tc::map_rows_16bit(&p.left, left, w.n, w.k, ld, kCtaRows))) return rc;
+  } else if ((rc = tc::map_rows_plain(&p.left, w.codes, 4, w4_row_tiles(w.n), 256ll * w4_blocks(w.k), 1024ll * w4_blocks(w.k),
+                                      8, 256))) {  // a row tile's codes are one row of words; a box is 128 inputs of eight row tiles
     return rc;
-  return w.dtype == kF16 ? run_w4<__half>(p, w.group, pairs, stream) : run_w4<__nv_bfloat16>(p, w.group, pairs, stream);
+  }
+  return w.dtype == kF16 ? run_w4<__half>(p, w.group, dense, pairs, stream)
+                         : run_w4<__nv_bfloat16>(p, w.group, dense, pairs, stream);
 }
 
 namespace {
@@ -211,7 +228,7 @@ int decode_w4(const W4& w, const void* x, long long ldx, void* y, long long ldy,
 }
 
 size_t expand_act8_workspace(int m, int n, int k, bool dy_aligned) {
-  return kStatusBytes + (dy_aligned ? 0 : copy_bytes(m, n)) + part_bytes(k, n);
+  return kStatusBytes + (dy_aligned ? 0 : copy_bytes(m, n)) + (dense_act8(n) ? dense_bytes(m, align_up(k, 64)) : 0) + part_bytes(k, n);
 }
 
 int expand_act8(const Act8& a, const void* dy, long long lddy, bool out_f32, const void* base, long long ldbase, void* dw,
@@ -233,27 +250,36 @@ int expand_act8(const Act8& a, const void* dy, long long lddy, bool out_f32, con
   p.status = reinterpret_cast<int*>(ws);
   ws += kStatusBytes;
   int pairs = 0;
+  const bool dense = dense_act8(n);
   if (p.steps > 0) {
     int rc;
     if (!tma_rows(dy, lddy)) {
       const int cols = static_cast<int>(align_up(n, 8));
-      if ((rc = tc::copy_rows_16bit(ws, cols, dy, a.m, n, lddy, stream))) return rc;
+      if ((rc = copy_rows_16bit(ws, cols, dy, a.m, n, lddy, stream))) return rc;
       dy = ws;
       lddy = cols;
       ws += copy_bytes(a.m, n);
     }
-    p.part = reinterpret_cast<float*>(ws);
-    if (!(pairs = place(p, pairs_of_device()))) return kErrNotSupported;
+    if (!(pairs = place(p, pairs_of_device(), dense))) return kErrNotSupported;
     // one load for a CTA's half of the columns where that is whole blocks of 64, and the matrix too (a partial last block
     // would be read past the end of the row)
     p.right_blocked = n % 64 == 0 && p.bn % 128 == 0;
     if ((rc = p.right_blocked ? tc::map_blocks_16bit(&p.right, dy, a.m, n, lddy, kStep, p.bn / 128)
                               : tc::map_rows_16bit(&p.right, dy, a.m, n, lddy, kStep)))
       return rc;
-    if ((rc = tc::map_rows_plain(&p.codes_map, a.codes, 1, a.m, static_cast<long long>(align_up(a.k, 16)), a.pitch, kStep, kCtaRows)))
+    if (dense) {
+      // (channels behind k are not written: they reach rows of the result that are not stored)
+      const int ld = static_cast<int>(align_up(a.k, 64));
+      if ((rc = restore_act8(a, ws, ld, stream))) return rc;
+      if ((rc = tc::map_blocks_16bit(&p.left, ws, a.m, ld, ld, kStep, kCtaRows / 64))) return rc;
+      ws += dense_bytes(a.m, ld);
+    } else if ((rc = tc::map_rows_plain(&p.left, a.codes, 1, a.m, static_cast<long long>(align_up(a.k, 16)), a.pitch, kStep,
+                                        kCtaRows))) {
       return rc;
+    }
+    p.part = reinterpret_cast<float*>(ws);
   }
-  return a.dtype == kF16 ? run_act8<__half>(p, pairs, stream) : run_act8<__nv_bfloat16>(p, pairs, stream);
+  return a.dtype == kF16 ? run_act8<__half>(p, dense, pairs, stream) : run_act8<__nv_bfloat16>(p, dense, pairs, stream);
 }
 
 }  // namespace lowbit

@@ -12,6 +12,11 @@
 //         bits once, code - zero is exact before.
 //   ACT8  the tile is MN-major (tokens are rows in memory, channels run along a row); every value is exact in 16 bits.
 //
+// A left tile is expanded once for every tile of columns.  With many of those it is cheaper to expand the operand once into 16
+// bits in the workspace and to multiply that (DENSE: the left tiles come by TMA too, there are no converters): 4096 rows
+// through 8192 x 4096 4-bit weights take 196 us, expanded on the way 250 us;
+// a gradient of 4096 x 8192 from 16384 tokens 836 and 950 us.
+//
 // Sums.  The tensor cores chop when they add to an accumulator (measured on B200, exact products of normal values:
 // relative error 3.4e-5 after 2048 additions, 1.5e-6 after 128, growing with their number), which is too coarse for a gradient kept in
 // fp32.  So an accumulator in tensor memory takes kSubSteps steps only; then eight epilogue warps add it to the tile's
@@ -29,7 +34,8 @@ namespace lowbit {
 enum ExpandKind { kExpandW4 = 0, kExpandAct8 = 1 };
 
 struct ExpandParams {
-  CUtensorMap codes_map;    // W4: 32-bit words, a row for each row tile; ACT8: bytes, a row for each token
+  CUtensorMap left;         // codes: W4: 32-bit words, a row for each row tile; ACT8: bytes, a row for each token
+                            // dense: the left operand in 16 bits, [row][input] (W4), [block of 64 channels][token][64] (ACT8)
   CUtensorMap right;        // x [tokens][inputs] (W4) or dY [tokens][columns] (ACT8)
   const void* scales;       // W4
   const uint8_t* zeros;     // W4, or null
@@ -54,7 +60,7 @@ struct ExpandParams {
 
 constexpr int kPairRows = 256, kCtaRows = 128, kStep = 64, kMaxCols = 256;
 constexpr int kSubSteps = 8;       // steps that one accumulator takes: 32 additions
-constexpr int kStages = 5;
+constexpr int kExpandStages = 5;
 constexpr int kRawStages = 4;      // tiles of codes: a step (ACT8: 64 tokens x 128 channels) or two (W4: 128 rows x 128 inputs)
 constexpr int kRawBytes = 8192;
 constexpr int kLeftBytes = kCtaRows * 128;           // 128 x 64 values of 16 bits
@@ -70,9 +76,12 @@ constexpr int kTransposeBytes = 32 * 32 * 4;         // per epilogue warp
 // scales and zeros of 128 rows (W4, PER groups each), or exponents of 64 tokens (ACT8, four blocks each)
 __host__ __device__ constexpr int table_bytes(int kind, int per) { return kind == kExpandW4 ? kCtaRows * 3 * per : kStep * 4; }
 __host__ __device__ constexpr int expand_smem(int kind, int per) {
-  return 1024 + kStages * kStageBytes + kRawStages * (kRawBytes + table_bytes(kind, per)) +
+  return 1024 + kExpandStages * kStageBytes + kRawStages * (kRawBytes + table_bytes(kind, per)) +
          (kind == kExpandAct8 ? kEpilogueWarps * kTransposeBytes : 0) + 1024;
 }
+// The dense form has no converters; its ring takes what they leave.
+constexpr int kDenseStages = 6, kDenseThreads = 384;
+constexpr int kDenseSmem = 1024 + kDenseStages * kStageBytes + kEpilogueWarps * kTransposeBytes + 1024;
 // registers a thread: at launch (all threads), and after the trade; the sum of what the warpgroups take must not
 // exceed what the block was launched with (the host checks the kernel's count before a launch)
 constexpr int kRegsLaunch = 96, kRegsControl = 48, kRegsEpilogue = 152, kRegsConvert = 64;
@@ -211,15 +220,17 @@ __device__ __forceinline__ void store_tile_cols(const float (&sum)[128], E* out,
     if (c < ncols && lane < nrows) *to = from_f32<E>(sum[c]);
 }
 
-template <typename T, int KIND, int PER>
-__global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const __grid_constant__ ExpandParams p) {
+template <typename T, int KIND, int PER, bool DENSE>
+__global__ void __launch_bounds__(DENSE ? kDenseThreads : kExpandThreads, 1)
+expand_product_kernel(const __grid_constant__ ExpandParams p) {
+  constexpr int kStages = DENSE ? kDenseStages : kExpandStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   constexpr int kTable = table_bytes(KIND, PER);
   uint8_t* raw = smem + kStages * kStageBytes;
-  float* transpose = reinterpret_cast<float*>(raw + kRawStages * kRawBytes);
-  uint8_t* tables = raw + kRawStages * kRawBytes + (KIND == kExpandAct8 ? kEpilogueWarps * kTransposeBytes : 0);
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(tables + kRawStages * kTable);
+  float* transpose = reinterpret_cast<float*>(raw + (DENSE ? 0 : kRawStages * kRawBytes));
+  uint8_t* tables = reinterpret_cast<uint8_t*>(transpose) + (KIND == kExpandAct8 || DENSE ? kEpilogueWarps * kTransposeBytes : 0);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(tables + (DENSE ? 0 : kRawStages * kTable));
   uint64_t* empty_bar = full_bar + kStages;
   uint64_t* slot_full = empty_bar + kStages;
   uint64_t* slot_free = slot_full + 2;
@@ -239,7 +250,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
     // all blocks of the grid are resident, so this store comes long before any bounded wait can run out
     if (blockIdx.x == 0) *p.status = 0;
     for (int s = 0; s < kStages; ++s) {
-      ptx::mbar_init(&full_bar[s], 2);  // the leader's producer, the peer's left tile
+      ptx::mbar_init(&full_bar[s], DENSE ? 1 : 2);  // the leader's producer, the peer's left tile
       ptx::mbar_init(&left_bar[s], kConvertWarps);
       ptx::mbar_init(&empty_bar[s], 1);
     }
@@ -265,16 +276,16 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
   const int half = p.bn / 2;  // columns of the right operand that a CTA brings
 
   if (warp < 4) {
-    regs_dec<kRegsControl>();
+    if (!DENSE) regs_dec<kRegsControl>();
     if (warp != 1) {
       // ---- producers: codes, tables and the CTA's half of the right operand.  The loads of one warp complete one after the
       // other (about 240 ns each, whatever they hold), so three warps take the steps (W4: pairs of steps) in turn.
       const int boxes = KIND == kExpandW4 ? 1 : (half + 63) / 64;
-      const uint32_t bytes = 2u * (KIND == kExpandW4 ? half * 128 : boxes * kRightBlock);  // both CTAs'
-      constexpr int kEach = KIND == kExpandW4 ? 2 : 1;  // steps of a tile of codes
+      const uint32_t bytes = 2u * ((KIND == kExpandW4 ? half * 128 : boxes * kRightBlock) + (DENSE ? kLeftBytes : 0));  // both CTAs'
+      constexpr int kEach = KIND == kExpandW4 && !DENSE ? 2 : 1;  // steps of a tile of codes
       if (warp == 0 && lane == 0) {
         ptx::prefetch_tmap(&p.right);
-        ptx::prefetch_tmap(&p.codes_map);
+        ptx::prefetch_tmap(&p.left);
       }
       uint32_t stage = 0, phase = 0, rstage = 0, rphase = 0;
       int turn = warp == 0 ? 0 : warp - 1;
@@ -285,11 +296,12 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
         const int col0 = w.col0 + static_cast<int>(rank) * half;
         // where this lane's pieces of the tables come from; W4: of 24 PER pieces of 16 bytes (2 PER of scales for each of the
         // eight row tiles, then PER of zeros), three at most; ACT8: the exponents of two tokens, 32 apart
-        constexpr int kCopies = KIND == kExpandW4 ? (24 * PER + 31) / 32 : 2;
+        constexpr int kCopies = DENSE ? 1 : KIND == kExpandW4 ? (24 * PER + 31) / 32 : 2;
         const uint8_t* from[kCopies];
         bool real[kCopies];
 #pragma unroll
         for (int c = 0; c < kCopies; ++c) {
+          if (DENSE) break;
           if (KIND == kExpandW4) {
             const int i = c * 32 + lane;
             const bool zero = i >= 16 * PER;
@@ -306,7 +318,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
         for (int kk = w.k0; ok && kk < w.k1; kk += kEach) {
           const bool mine = turn == 0;
           turn = mine ? kProducers - 1 : turn - 1;
-          if (mine) {
+          if (mine && !DENSE) {
             if (!ptx::mbar_wait_warp<false>(&raw_empty[rstage], rphase ^ 1u, abort_flag, p.wait_ns)) {
               if (lane == 0) give_up(p, abort_flag, 101);
               ok = false;
@@ -314,8 +326,8 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
             }
             if (ptx::elect_one()) {
               ptx::mbar_arrive_expect_tx(&raw_full[rstage], kRawBytes);
-              if (KIND == kExpandW4) ptx::tma_load_2d(raw + rstage * kRawBytes, &p.codes_map, &raw_full[rstage], kk / 2 * 256, row0 / kW4Rows);
-              else ptx::tma_load_2d(raw + rstage * kRawBytes, &p.codes_map, &raw_full[rstage], row0, kk * kStep);
+              if (KIND == kExpandW4) ptx::tma_load_2d(raw + rstage * kRawBytes, &p.left, &raw_full[rstage], kk / 2 * 256, row0 / kW4Rows);
+              else ptx::tma_load_2d(raw + rstage * kRawBytes, &p.left, &raw_full[rstage], row0, kk * kStep);
             }
             __syncwarp();
             const uint32_t table = ptx::smem_u32(tables + rstage * kTable);
@@ -344,6 +356,10 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
               if (ptx::elect_one()) {
                 if (rank == 0) ptx::mbar_arrive_expect_tx(&full_bar[stage], bytes);
                 uint8_t* to = smem + stage * kStageBytes + kLeftBytes;
+                if (DENSE) {
+                  if (KIND == kExpandW4) ptx::tma_load_2d_pair(to - kLeftBytes, &p.left, &full_bar[stage], kk * kStep, row0);
+                  else ptx::tma_load_3d_pair(to - kLeftBytes, &p.left, &full_bar[stage], 0, kk * kStep, row0 / 64);
+                }
                 if (KIND == kExpandW4) {
                   ptx::tma_load_2d_pair(to, &p.right, &full_bar[stage], (kk + h) * kStep, col0);
                 } else if (p.right_blocked) {
@@ -388,7 +404,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
             ok = false;
             break;
           }
-          if (!ptx::mbar_wait_warp<false>(&left_bar[stage], phase, abort_flag, p.wait_ns)) {
+          if (!DENSE && !ptx::mbar_wait_warp<false>(&left_bar[stage], phase, abort_flag, p.wait_ns)) {
             if (lane == 0) give_up(p, abort_flag, 102);
             ok = false;
             break;
@@ -409,7 +425,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
         }
       }
     }
-    else {
+    else if (!DENSE) {
       // ---- passes on to the leader that the peer's left tile is written.  The converters themselves would have to release
       // at cluster scope, which waits for the loads that they have in flight.
       uint32_t stage = 0, phase = 0;
@@ -430,7 +446,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
     }
   } else if (warp < 12) {
     // ---- epilogue: warp = 32 rows (of its lane quarter) x half of the tile's columns
-    regs_inc<kRegsEpilogue>();
+    if (!DENSE) regs_inc<kRegsEpilogue>();
     const int quarter = warp & 3, side = (warp - 4) >> 2;
     const uint32_t swap = ptx::smem_u32(transpose) + (warp - 4) * kTransposeBytes;
     const uint32_t tmem = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + side * half;
@@ -483,9 +499,9 @@ __global__ void __launch_bounds__(kExpandThreads, 1) expand_product_kernel(const
         else store_tile_rows(sum, static_cast<T*>(p.out), p.ldo, row0, col0, nrows, ncols, swap, lane);
       }
     }
-  } else {
+  } else if (!DENSE) {
     // ---- converters
-    regs_dec<kRegsConvert>();
+    if (!DENSE) regs_dec<kRegsConvert>();
     const int group = (warp - 12) / kConvertWarps, tid = threadIdx.x % (kConvertWarps * 32);
     const uint32_t left = ptx::smem_u32(smem), codes = ptx::smem_u32(raw);
     uint32_t stage = 0, phase = 0, rstage = 0, rphase = 0, turn = group;

@@ -36,8 +36,15 @@ inline size_t copy_bytes(long long rows, int cols) {
   return (static_cast<size_t>(rows) * row + 255) / 256 * 256;
 }
 
+// dst (rows x cols_d, packed, cols_d the next multiple of 8) = src (rows x cols, leading dimension ld) of 16-bit elements,
+// zeros behind (act8.cu).
+int copy_rows_16bit(void* dst, int cols_d, const void* src, int rows, int cols, long long ld, cudaStream_t stream);
+// Expansion to 16 bits (w4.cu, act8.cu).
+int dequantize_w4(const W4& w, void* out, long long ldo, cudaStream_t stream);
+int restore_act8(const Act8& a, void* x, long long ldx, cudaStream_t stream);
+
 // The products on the tensor cores (expand_product.cu).  Workspace: a status word, a copy of the 16-bit operand where its
-// rows are not aligned, and the parts of a divided reduction at its end.  The bytes asked for grow with m, so that a
+// rows are not aligned, the operand in 16 bits where it is expanded first, and the parts of a divided reduction at its end.  The bytes asked for grow with m, so that a
 // workspace serves every smaller m.
 constexpr size_t kStatusBytes = 256;
 constexpr int kDecodeMaxRows = 64;

@@ -104,8 +104,6 @@ int map_blocks_16bit(void* map, const void* ptr, long long rows, long long cols,
 // The same without a swizzle for elements of `esize` (1 or 4) bytes, rows `pitch` bytes apart, boxes of box_cols x box_rows.
 int map_rows_plain(void* map, const void* ptr, int esize, long long rows, long long cols, long long pitch, int box_rows,
                    int box_cols);
-// dst (rows x cols_d, packed, cols_d a multiple of 8) = src (rows x cols, leading dimension ld) of 16-bit elements, zeros behind.
-int copy_rows_16bit(void* dst, int cols_d, const void* src, int rows, int cols, long long ld, cudaStream_t stream);
 }  // namespace tc
 
 // fp64 path (dgemm_sw.cu): DMMA kernels, same four calls.

@@ -270,6 +270,11 @@ int dequantize(const W4& w, void* out, long long ldo, cudaStream_t stream) {
 }
 
 }  // namespace
+
+int dequantize_w4(const W4& w, void* out, long long ldo, cudaStream_t stream) {
+  return w.dtype == kF16 ? dequantize<__half>(w, out, ldo, stream) : dequantize<__nv_bfloat16>(w, out, ldo, stream);
+}
+
 }  // namespace lowbit
 }  // namespace sb200
 
@@ -317,9 +322,7 @@ extern "C" int sb200_w4_dequantize(int dtype, const void* codes, const void* sca
   if (int rc = sb200::lowbit::check(w)) return rc;
   if (!out || ldo < k) return SB200_ERR_INVALID_PROBLEM;
   if (!sb200::lowbit::aligned(out, 2)) return SB200_ERR_MISALIGNED_OPERAND;
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return dtype == sb200::kF16 ? sb200::lowbit::dequantize<__half>(w, out, ldo, s)
-                              : sb200::lowbit::dequantize<__nv_bfloat16>(w, out, ldo, s);
+  return sb200::lowbit::dequantize_w4(w, out, ldo, reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" size_t sb200_w4_gemm_workspace_bytes(int dtype, int m, int n, int k, int group, int x_aligned) {
@@ -345,7 +348,7 @@ extern "C" int sb200_w4_gemm(int dtype, const void* x, long long ldx, const void
   char* ws = static_cast<char*>(workspace);
   if (!tma_rows(x, ldx)) {  // every kernel wants rows of x that start on 16 bytes
     const int cols = (k + 7) / 8 * 8;
-    if (int rc = sb200::tc::copy_rows_16bit(ws + kStatusBytes, cols, x, m, k, ldx, s)) return rc;
+    if (int rc = copy_rows_16bit(ws + kStatusBytes, cols, x, m, k, ldx, s)) return rc;
     x = ws + kStatusBytes;
     ldx = cols;
   }

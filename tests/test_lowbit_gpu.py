@@ -254,6 +254,32 @@ def test_gemm_w4(cuda_device, m, n, k, group, symmetric, dtype):
     check_w4_gemm(lowbit.gemm_w4(x, w), x, w, exact_weights=False)
 
 
+@pytest.mark.parametrize("m,n,k,group,symmetric,dtype", [
+    (1280, 256, 256, 32, True, "f16"), (1281, 515, 203, 64, False, "bf16"), (1500, 40, 1000, 128, False, "f16"), (4096, 130, 64, 128, True, "bf16"),
+    (1300, 1, 1, 32, False, "bf16"),
+])
+def test_gemm_w4_many_rows(cuda_device, m, n, k, group, symmetric, dtype):
+    """From 1280 rows on the weights are expanded once, before the product: the same values, and the same sums."""
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    w = lowbit.quantize_w4(randn((n, k), T(dtype), cuda_device, 8, k ** -0.5), group=group, symmetric=symmetric)
+    x = randn((m, k), T(dtype), cuda_device, 9)
+    ws = lowbit.WorkspaceW4(m, w)
+    y = lowbit.gemm_w4(x, w, workspace=ws, check=True)
+    check_w4_gemm(y, x, w, exact_weights=False)
+    # a workspace serves fewer rows too; rows do not depend on the others
+    for fewer in (1100, 100, 50, 3):
+        part = lowbit.gemm_w4(x[:fewer], w, workspace=ws)
+        check_w4_gemm(part, x[:fewer], w, exact_weights=False)
+    room = torch.full((m, n + 3), 7.0, dtype=T(dtype), device=cuda_device)
+    wide = randn((m, k + 3), T(dtype), cuda_device, 10)[:, 2:2 + k]     # off the 16-byte grid
+    lowbit.gemm_w4(wide, w, out=room[:, 1:1 + n])
+    check_w4_gemm(room[:, 1:1 + n], wide, w, exact_weights=False)
+    assert bool((room[:, :1] == 7).all()) and bool((room[:, 1 + n:] == 7).all())
+
+
 @pytest.mark.parametrize("m", [1, 5, 24, 40, 150])
 @pytest.mark.parametrize("n,k", [(300, 520), (260, 384)])
 def test_gemm_w4_rows_of_other_matrices(cuda_device, m, n, k):
@@ -418,7 +444,9 @@ def test_save_empty(cuda_device):
 
 
 GRAD = [(1, 1, 1), (1, 128, 256), (63, 128, 256), (64, 128, 256), (65, 130, 260), (256, 256, 512), (1000, 100, 72), (333, 257, 129),
-        (2048, 384, 200), (5000, 64, 640)]
+        (2048, 384, 200), (5000, 64, 640),
+        # from 1280 columns on the activations are expanded once, before the product
+        (1, 1, 1280), (100, 70, 1280), (333, 257, 1283), (2048, 300, 1500), (70, 33, 4096)]
 
 
 @pytest.mark.parametrize("dtype,out", [("f16", "f32"), ("bf16", "f32"), ("f16", "f16"), ("bf16", "bf16")])
