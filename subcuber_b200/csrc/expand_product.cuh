@@ -536,6 +536,7 @@ expand_product_kernel(const __grid_constant__ ExpandParams p) {
         // step, 2 and 3 to the second.  Lanes of odd rows take the second word of a step first, so that eight
         // lanes always store to eight different 16-byte columns of the swizzled tile.
         const int g = lane >> 2, t = lane & 3, odd = g & 1;
+        const uint32_t mask = in_register(0x000f000fu), magic = in_register(Half<T>::magic);
         const int row0 = (tid >> 6) * kW4Rows + 8 * ((tid >> 5) & 1) + g;  // of the first piece; the others 32 rows on
         const uint32_t line0 = row0 * 128 + (((4 * odd + t) ^ g) << 4), line1 = row0 * 128 + (((4 * (1 - odd) + t) ^ g) << 4);
         for (int kk = w.k0; kk < w.k1; kk += 2) {
@@ -572,7 +573,7 @@ expand_product_kernel(const __grid_constant__ ExpandParams p) {
             for (int i = 0; i < kPieces; ++i)
 #pragma unroll
               for (int j = 0; j < 2; ++j)
-                ptx::sts_v4(to + i * (kLeftBytes / kPieces) + (j ? line1 : line0), expand_w4<T>(word[i][j], bias[i][j], scale[i][j]));
+                ptx::sts_v4(to + i * (kLeftBytes / kPieces) + (j ? line1 : line0), expand_w4<T>(word[i][j], bias[i][j], scale[i][j], mask, magic));
             publish();
           }
           if (!ok) break;

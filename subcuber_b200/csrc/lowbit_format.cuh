@@ -89,14 +89,28 @@ template <typename T> __device__ __forceinline__ uint32_t mul2(uint32_t a, uint3
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+// (a & b) | c in one instruction.  The constants are kept in registers: with two of them written into the expression the
+// compiler takes two instructions, each of which has room for one.
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+__device__ __forceinline__ uint32_t in_register(uint32_t constant) {
+  uint32_t r;
+  asm volatile("mov.b32 %0, %1;" : "=r"(r) : "r"(constant));
+  return r;
+}
+
 // Eight codes of a word to eight weights, in the order of the inputs.  bias = magic + zero, scale twice.
+// mask = 0x000f000f and magic, both in registers.
 template <typename T>
-__device__ __forceinline__ uint4 expand_w4(uint32_t w, uint32_t bias, uint32_t scale) {
+__device__ __forceinline__ uint4 expand_w4(uint32_t w, uint32_t bias, uint32_t scale, uint32_t mask, uint32_t magic) {
   uint4 r;
-  r.x = mul2<T>(sub2<T>((w & 0x000f000fu) | Half<T>::magic, bias), scale);
-  r.y = mul2<T>(sub2<T>(((w >> 4) & 0x000f000fu) | Half<T>::magic, bias), scale);
-  r.z = mul2<T>(sub2<T>(((w >> 8) & 0x000f000fu) | Half<T>::magic, bias), scale);
-  r.w = mul2<T>(sub2<T>(((w >> 12) & 0x000f000fu) | Half<T>::magic, bias), scale);
+  r.x = mul2<T>(sub2<T>(and_or(w, mask, magic), bias), scale);
+  r.y = mul2<T>(sub2<T>(and_or(w >> 4, mask, magic), bias), scale);
+  r.z = mul2<T>(sub2<T>(and_or(w >> 8, mask, magic), bias), scale);
+  r.w = mul2<T>(sub2<T>(and_or(w >> 12, mask, magic), bias), scale);
   return r;
 }
 
@@ -113,18 +127,18 @@ template <> struct Act8Step<__nv_bfloat16> {
     e = (field << 7) | (field << 23);
   }
   __device__ __forceinline__ uint32_t two(uint32_t bytes_twice) const {
-    const uint32_t p = (bytes_twice & 0x807f807fu) | e;
+    const uint32_t p = and_or(bytes_twice, 0x807f807fu, e);
     return sub2<__nv_bfloat16>(p, p & 0xff80ff80u);
   }
 };
 template <> struct Act8Step<__half> {
-  uint32_t s;
-  __device__ __forceinline__ explicit Act8Step(uint32_t exponent) {
+  uint32_t s, magic;
+  __device__ __forceinline__ explicit Act8Step(uint32_t exponent) : magic(in_register(0x64006400u)) {
     const __half2 h = __float2half2_rn(act8_step(static_cast<int>(exponent)));
     s = *reinterpret_cast<const uint32_t*>(&h);
   }
   __device__ __forceinline__ uint32_t two(uint32_t bytes_twice) const {
-    const uint32_t p = (bytes_twice & 0x807f807fu) | 0x64006400u;
+    const uint32_t p = and_or(bytes_twice, 0x807f807fu, magic);
     return mul2<__half>(sub2<__half>(p, p & 0xfc00fc00u), s);
   }
 };

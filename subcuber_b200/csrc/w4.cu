@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kThreads) w4_dequantize_kernel(const uint8_t* 
     for (int j = 0; j < 4; ++j) {
       const uint32_t s = reinterpret_cast<const uint16_t*>(scales)[at + j * per / 4], z = zeros ? zeros[at + j * per / 4] : 8u;
       *reinterpret_cast<uint4*>(to + 32 * j) =
-          expand_w4<T>(words[j], Half<T>::magic + __byte_perm(z, 0, 0x4040), __byte_perm(s, 0, 0x1010));
+          expand_w4<T>(words[j], Half<T>::magic + __byte_perm(z, 0, 0x4040), __byte_perm(s, 0, 0x1010), 0x000f000fu, Half<T>::magic);
     }
   }
   __syncthreads();

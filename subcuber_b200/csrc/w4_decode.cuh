@@ -203,6 +203,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) w4_decode_kernel(const __gr
     uint32_t ls = group, lphase = 0;
     bool ok = true;
     const int r16 = lane & 15;
+    const uint32_t mask = in_register(0x000f000fu), magic = in_register(Half<T>::magic);
     for (int b = first; b < b1; b += 2) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 2) : "memory");
       __syncwarp();  // every lane's copies of this stage are there, and all have read the stage that is filled next
@@ -238,7 +239,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) w4_decode_kernel(const __gr
 #pragma unroll
           for (int t = 0; t < 4; ++t) {
             const int q = (2 * h + j) * PER / 4;
-            const uint4 v = expand_w4<T>(w[t][2 * h + j], bias[q], scale[q]);
+            const uint4 v = expand_w4<T>(w[t][2 * h + j], bias[q], scale[q], mask, magic);
             r[j * 16 + t * 4] = v.x; r[j * 16 + t * 4 + 1] = v.y; r[j * 16 + t * 4 + 2] = v.z; r[j * 16 + t * 4 + 3] = v.w;
           }
         tmem_st_32x32(to + h * 32, r);

@@ -35,8 +35,8 @@ template <> struct Pair16<__half> {
     return *reinterpret_cast<const uint32_t*>(&r);
   }
   // Codes 2 q and 2 q + 1 (in the order of the inputs) of a word, minus the zero point.
-  static __device__ __forceinline__ uint32_t code(uint32_t w, int q, uint32_t bias) {
-    return sub(((w >> (4 * q)) & 0x000f000fu) | magic, bias);
+  static __device__ __forceinline__ uint32_t code(uint32_t w, int q, uint32_t bias, uint32_t mask, uint32_t magic_in_register) {
+    return sub(and_or(w >> (4 * q), mask, magic_in_register), bias);
   }
   static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -50,8 +50,8 @@ template <> struct Pair16<__nv_bfloat16> {
     const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
     return *reinterpret_cast<const uint32_t*>(&r);
   }
-  static __device__ __forceinline__ uint32_t code(uint32_t w, int q, uint32_t bias) {
-    return sub(((w >> (4 * q)) & 0x000f000fu) | magic, bias);
+  static __device__ __forceinline__ uint32_t code(uint32_t w, int q, uint32_t bias, uint32_t mask, uint32_t magic_in_register) {
+    return sub(and_or(w >> (4 * q), mask, magic_in_register), bias);
   }
   static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -148,6 +148,7 @@ __global__ void __launch_bounds__(kRowThreads) w4_rows_kernel(const RowsParams p
 #pragma unroll
   for (int a = 0; a < AHEAD - 1; ++a) fetch();
   int stage = 0;
+  const uint32_t mask = in_register(0x000f000fu), magic = in_register(Pair16<T>::magic);
   const uint32_t xat = g * 256 + ((t ^ ((g & 1) << 2)) << 4);  // of word 0; word j is 64 j further, exclusive-or
   for (int b = wk; b < p.blocks; b += WK) {
     asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 2) : "memory");
@@ -182,8 +183,8 @@ __global__ void __launch_bounds__(kRowThreads) w4_rows_kernel(const RowsParams p
           const uint32_t xw[4] = {xv[j].x, xv[j].y, xv[j].z, xv[j].w};
 #pragma unroll
           for (int q = 0; q < 4; q += 2) {
-            const uint32_t a4[4] = {Pair16<T>::code(lo[j], q, bias[0]), Pair16<T>::code(hi[j], q, bias[1]),
-                                    Pair16<T>::code(lo[j], q + 1, bias[0]), Pair16<T>::code(hi[j], q + 1, bias[1])};
+            const uint32_t a4[4] = {Pair16<T>::code(lo[j], q, bias[0], mask, magic), Pair16<T>::code(hi[j], q, bias[1], mask, magic),
+                                    Pair16<T>::code(lo[j], q + 1, bias[0], mask, magic), Pair16<T>::code(hi[j], q + 1, bias[1], mask, magic)};
             Pair16<T>::mma(acc, a4, xw[q], xw[q + 1]);
           }
         }
