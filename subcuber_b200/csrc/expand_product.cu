@@ -81,10 +81,16 @@ int launch(const ExpandParams& p, int pairs, cudaStream_t stream) {
 
 template <typename Out>
 int join(const ExpandParams& p, int rows, int cols, cudaStream_t stream) {
-  const long long blocks = (static_cast<long long>(rows) * cols + 1023) / 1024;
-  const unsigned grid = static_cast<unsigned>(blocks < 148 * 16 ? blocks : 148 * 16);
-  join_slices_kernel<Out><<<grid, 256, 0, stream>>>(p.part, p.slices, rows, cols, static_cast<Out*>(p.out), p.ldo,
-                                                    static_cast<const Out*>(p.base), p.ldbase);
+  const bool wide = cols % 4 == 0;
+  const int pieces = wide ? cols / 4 : cols;
+  int cols_log2 = 0;
+  while (cols_log2 < 8 && (1 << cols_log2) < pieces) ++cols_log2;
+  const int row_parts = ceil_div(pieces, 1 << cols_log2);
+  const long long blocks = static_cast<long long>(row_parts) * ceil_div(rows, 256 >> cols_log2);
+  if (blocks > 0x7fffffffll) return kErrNotSupported;
+  auto* kernel = wide ? join_slices_kernel<Out, 4> : join_slices_kernel<Out, 1>;
+  kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(p.part, p.slices, rows, cols, static_cast<Out*>(p.out), p.ldo,
+                                                            static_cast<const Out*>(p.base), p.ldbase, cols_log2, row_parts);
   return static_cast<int>(cudaGetLastError());
 }
 

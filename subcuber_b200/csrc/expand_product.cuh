@@ -637,18 +637,31 @@ expand_product_kernel(const __grid_constant__ ExpandParams p) {
   }
 }
 
-// out[r][c] = base[r][c] + the slices' parts in order.
-template <typename Out>
+// out[r][c] = base[r][c] + the slices' parts in order.  A thread adds V neighbours (4 where rows of the parts start on 16 bytes:
+// cols a multiple of 4); 2^cols_log2 threads stand along a row.
+template <typename Out, int V>
 __global__ void __launch_bounds__(256) join_slices_kernel(const float* __restrict__ part, int slices, int rows, int cols, Out* out,
-                                                          long long ldo, const Out* base, long long ldbase) {
+                                                          long long ldo, const Out* base, long long ldbase, int cols_log2,
+                                                          int row_parts) {
+  const long long r = ((static_cast<long long>(blockIdx.x) / row_parts) << (8 - cols_log2)) + (threadIdx.x >> cols_log2);
+  const int c = (((blockIdx.x % row_parts) << cols_log2) + (threadIdx.x & ((1 << cols_log2) - 1))) * V;
+  if (r >= rows || c >= cols) return;
   const long long total = static_cast<long long>(rows) * cols;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-    const long long r = i / cols, c = i - r * cols;
-    float v = 0.f;
-    for (int s = 0; s < slices; ++s) v += part[s * total + i];
-    if (base) v += to_f32(base[r * ldbase + c]);
-    out[r * ldo + c] = from_f32<Out>(v);
+  const float* from = part + r * cols + c;
+  float v[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = base ? to_f32(base[r * ldbase + c + i]) : 0.f;
+#pragma unroll 4
+  for (int s = 0; s < slices; ++s, from += total) {
+    if (V == 4) {
+      const float4 x = __ldcs(reinterpret_cast<const float4*>(from));
+      v[0] += x.x; v[V > 1 ? 1 : 0] += x.y; v[V > 2 ? 2 : 0] += x.z; v[V > 3 ? 3 : 0] += x.w;
+    } else {
+      v[0] += __ldcs(from);
+    }
   }
+#pragma unroll
+  for (int i = 0; i < V; ++i) out[r * ldo + c + i] = from_f32<Out>(v[i]);
 }
 
 }  // namespace lowbit
