@@ -286,8 +286,10 @@ int sb200_peer_wait(int* const* local_flags, int count, int value, unsigned wait
  * What the linear layers of a language model need beside the GEMM above: weights in 4 bits (serving), activations saved
  * in 8 bits for the backward pass (training).  dtype and out_dtype: 0 f16, 1 f32, 3 bf16.  All calls are asynchronous on
  * `stream`, allocate nothing, and may be captured into graphs; a workspace (256-byte aligned) belongs to one call at a time (two calls
- * that may overlap need two); sb200_gemm_status reads the status word at its head after a product.  Matrices are row-major with a leading dimension in elements; rows need no alignment beyond
- * their elements'.  m = 0 is an empty batch.  No counterpart in the reference project.
+ * that may overlap need two); sb200_gemm_status reads the status word at its head after a
+ * product (sb200_w4_gemm: of more than 8 rows; a call of fewer has no waits and leaves the word alone).  Matrices are row-major with a leading dimension in elements; rows need no alignment beyond
+ * their elements'.  m = 0 is an empty batch.  The first call on a
+ * device should come before any stream capture (it loads the kernels).  No counterpart in the reference project.
  *
  * Weights in 4 bits, n outputs x k inputs, groups of G = 32, 64 or 128 inputs of an output:
  *     W[n][k] = scale(n, k / G) * (code[n][k] - zero(n, k / G)),   code and zero in 0..15, zero = 8 where zeros == NULL

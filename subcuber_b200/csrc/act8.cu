@@ -161,7 +161,7 @@ int check(const Act8& a) {
   if (a.dtype != kF16 && a.dtype != kBF16) return kErrNotSupported;
   if (a.m < 0 || a.k <= 0 || a.pitch < a.k || a.exp_pitch < ceil_div(a.k, kActBlock)) return kErrInvalidProblem;
   if (a.m > 0 && (!a.codes || !a.exps)) return kErrInvalidProblem;
-  if (a.exp_pitch > 0x7fffffffll) return kErrNotSupported;
+  if (a.m > kMaxExtent || a.k > kMaxExtent || a.exp_pitch > 0x7fffffffll) return kErrNotSupported;
   if (!aligned(a.codes, 16) || a.pitch % 16 || !aligned(a.exps, 4) || a.exp_pitch % 4) return kErrMisalignedOperand;
   return kOk;
 }
@@ -241,7 +241,7 @@ extern "C" int sb200_act8_wgrad(int dtype, const void* codes, long long pitch, c
                                 sb200_stream_t stream) {
   const Act8 a{static_cast<sb200::DType>(dtype), m, k, codes, pitch, exponents, exp_pitch};
   if (int rc = sb200::lowbit::check(a)) return rc;
-  if (out_dtype != sb200::kF32 && out_dtype != dtype) return SB200_ERR_NOT_SUPPORTED;
+  if ((out_dtype != sb200::kF32 && out_dtype != dtype) || n > sb200::lowbit::kMaxExtent) return SB200_ERR_NOT_SUPPORTED;
   if (n <= 0 || !dw || lddw < n || lddy < n || (m > 0 && !dy) || (base && ldbase < n)) return SB200_ERR_INVALID_PROBLEM;
   const uintptr_t width = out_dtype == sb200::kF32 ? 4 : 2;
   if (!sb200::lowbit::aligned(dy, 2) || !sb200::lowbit::aligned(dw, width) || !sb200::lowbit::aligned(base, width))

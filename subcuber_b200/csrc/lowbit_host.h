@@ -30,6 +30,9 @@ inline bool aligned(const void* p, uintptr_t to) { return (reinterpret_cast<uint
 // Rows of a 16-bit matrix that TMA can read as they are.
 inline bool tma_rows(const void* p, long long ld) { return aligned(p, 16) && ld % 8 == 0; }
 
+// Extents are held in 32 bits, rounded up to whole tiles too.
+constexpr int kMaxExtent = 0x7fffff00;
+
 // Bytes of a copy of a 16-bit matrix with rows that start on 16 bytes.
 inline size_t copy_bytes(long long rows, int cols) {
   const size_t row = (static_cast<size_t>(cols) + 7) / 8 * 16;

@@ -224,6 +224,7 @@ constexpr int kFewRows = 8;
 int check(const W4& w) {
   if (w.dtype != kF16 && w.dtype != kBF16) return kErrNotSupported;
   if (w.n <= 0 || w.k <= 0 || !w.codes || !w.scales) return kErrInvalidProblem;
+  if (w.n > kMaxExtent || w.k > kMaxExtent) return kErrNotSupported;
   if (w.group != 32 && w.group != 64 && w.group != 128) return kErrNotSupported;
   if (!aligned(w.codes, 16) || !aligned(w.scales, 16) || !aligned(w.zeros, 16)) return kErrMisalignedOperand;
   return kOk;
@@ -339,6 +340,7 @@ extern "C" int sb200_w4_gemm(int dtype, const void* x, long long ldx, const void
   const W4 w{static_cast<sb200::DType>(dtype), n, k, group, codes, scales, zeros};
   if (int rc = check(w)) return rc;
   if (m < 0 || ldx < k || ldy < n) return SB200_ERR_INVALID_PROBLEM;
+  if (m > kMaxExtent) return SB200_ERR_NOT_SUPPORTED;
   if (m == 0) return SB200_OK;
   if (!x || !y) return SB200_ERR_INVALID_PROBLEM;
   if (!aligned(x, 2) || !aligned(y, 2)) return SB200_ERR_MISALIGNED_OPERAND;

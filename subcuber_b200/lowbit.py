@@ -33,6 +33,7 @@ ACT_BLOCK = 32   # channels of a token that share a step
 
 # handle of the current stream of a device (the public call builds a Stream object, which takes 2 us)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _matrix(name: str, t: torch.Tensor, dtypes) -> None:
@@ -70,16 +71,20 @@ def _output(name: str, t: torch.Tensor, shape, dtype, device) -> None:
         raise ValueError(f"operands are on different devices: {device} and {t.device}")
 
 
+_functions: dict = {}
+
+
 def _call(what: str, device: torch.device, *args) -> None:
     """Call the library's `what` on the current stream of `device`, with `device` current."""
-    fn = getattr(_lib.load(), what)
+    fn = _functions.get(what)
+    if fn is None:
+        fn = _functions[what] = getattr(_lib.load(), what)
     index = device.index
-    stream = _raw_stream(index)
-    if torch.cuda.current_device() == index:
-        rc = fn(*args, stream)
+    if _current_device() == index:
+        rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, stream)
+            rc = fn(*args, _raw_stream(index))
     if rc != 0:
         raise KernelError(what, rc)
 
@@ -97,6 +102,12 @@ class _Workspace:
         self.device = device
         self.buf = torch.empty(nbytes + 256, dtype=torch.uint8, device=device)
         self.ptr = self.buf.data_ptr() + (-self.buf.data_ptr()) % 256
+        self.buf[:512].zero_()   # the status word: products of a few rows leave it alone
+
+    def _for(self, device: torch.device):
+        if self.device != device:
+            raise ValueError(f"the workspace is on {self.device}, the operands on {device}")
+        return self.ptr, self.nbytes
 
     def check(self) -> None:
         """Wait for the call that used the workspace last and raise if a device-side wait gave up."""
@@ -219,8 +230,8 @@ class WorkspaceW4(_Workspace):
 
 def gemm_w4(x: torch.Tensor, w: WeightsW4, out: Optional[torch.Tensor] = None, workspace: Optional[WorkspaceW4] = None,
             check: bool = False) -> torch.Tensor:
-    """x @ W^T (m x out_features) for x (m x in_features) of the weights' type; sums in fp32.  `check` synchronises and raises
-    if a device-side wait gave up."""
+    """x @ W^T (m x out_features) for x (m x in_features) of the weights' type; sums in fp32.  `out` must not overlap x.
+    `check` synchronises and raises if a device-side wait gave up."""
     _matrix("x", x, (w.dtype,))
     m, k = x.shape
     if k != w.k:
@@ -233,7 +244,7 @@ def gemm_w4(x: torch.Tensor, w: WeightsW4, out: Optional[torch.Tensor] = None, w
         _output("out", out, (m, w.n), w.dtype, w.device)
     ldx, x_ptr = _ld(x), x.data_ptr()
     if workspace is not None:
-        ptr, nbytes = workspace.ptr, workspace.nbytes
+        ptr, nbytes = workspace._for(w.device)
     elif m <= 64 and x_ptr % 16 == 0 and ldx % 8 == 0:
         ptr, nbytes = w._status_ptr, 256     # the products of few rows need the status word only
     else:
@@ -359,9 +370,10 @@ def weight_grad8(saved: Checkpoint8, dy: torch.Tensor, base: Optional[torch.Tens
     lddy, dy_ptr = _ld(dy), dy.data_ptr()
     if workspace is None:
         workspace = WorkspaceGrad8(saved, n, out_dtype, dy_ptr % 16 == 0 and lddy % 8 == 0)
+    ws_ptr, ws_bytes = workspace._for(saved.device)
     _call("sb200_act8_wgrad", saved.device, saved._code, *saved._layout, dy_ptr, lddy, DTYPE_CODE[out_dtype],
           base.data_ptr() if base is not None else None, _ld(base) if base is not None else n, out.data_ptr(), _ld(out), m, n,
-          saved.k, workspace.ptr, workspace.nbytes)
+          saved.k, ws_ptr, ws_bytes)
     if check:
         workspace.check()
     return out

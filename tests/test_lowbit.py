@@ -19,7 +19,9 @@ def _w4_gemm(lib, dtype=0, x=P, ldx=256, codes=P, scales=P, zeros=P, y=P, ldy=64
     (dict(dtype=1), 5), (dict(dtype=2), 5), (dict(dtype=7), 5),
     (dict(group=0), 5), (dict(group=16), 5), (dict(group=96), 5), (dict(group=256), 5),
     (dict(x=P + 1), 1), (dict(y=P + 1), 1), (dict(codes=P + 8), 1), (dict(scales=P + 1), 1),
+    (dict(n=(1 << 31) - 1, ldy=1 << 31), 5), (dict(k=(1 << 31) - 1, ldx=1 << 31), 5), (dict(m=(1 << 31) - 1), 5),
     (dict(ws=None), 6), (dict(nbytes=0), 6), (dict(ws=P + 16), 6),
+    (dict(m=65, nbytes=256), 6), (dict(m=9, k=255, ldx=255, nbytes=256), 6),    # parts of the sums, a copy of x
 ])
 def test_w4_gemm_refuses(lib, change, rc):
     assert _w4_gemm(lib, **change) == rc
@@ -86,10 +88,21 @@ def _wgrad(lib, dtype=0, codes=P, pitch=112, exps=P, exp_pitch=4, dy=P, lddy=24,
     (dict(dw=None), 4), (dict(lddy=23), 4), (dict(lddw=23), 4), (dict(base=P, ldbase=23), 4), (dict(pitch=96), 4),
     (dict(dtype=1), 5), (dict(out_dtype=3), 5), (dict(dtype=3, out_dtype=0), 5), (dict(out_dtype=2), 5),
     (dict(codes=P + 8), 1), (dict(exps=P + 2), 1), (dict(dy=P + 1), 1), (dict(dw=P + 2), 1), (dict(base=P + 2), 1),
+    (dict(exp_pitch=1 << 31), 5), (dict(n=(1 << 31) - 1, lddy=1 << 31, lddw=1 << 31), 5),
     (dict(ws=None), 6), (dict(nbytes=0), 6), (dict(ws=P + 128), 6),
 ])
 def test_act8_wgrad_refuses(lib, change, rc):
     assert _wgrad(lib, **change) == rc
+
+
+def test_workspaces_grow_with_the_rows(lib):
+    """A workspace for m rows serves every smaller m, whatever kernel that takes."""
+    for aligned in (0, 1):
+        w4 = [lib.sb200_w4_gemm_workspace_bytes(0, m, 1000, 500, 64, aligned) for m in (1, 8, 9, 64, 65, 500, 1279, 1280, 5000)]
+        assert w4 == sorted(w4) and w4[0] >= 256 and (aligned or w4[0] > 256)
+        g8 = [lib.sb200_act8_wgrad_workspace_bytes(3, 1, m, 1500, 300, aligned) for m in (0, 1, 64, 1000, 100000)]
+        assert g8 == sorted(g8) and g8[0] >= 256
+    assert lib.sb200_w4_gemm_workspace_bytes(0, 1, 1000, 512, 64, 1) == 256
 
 
 def test_python_calls_refuse_host_tensors():
