@@ -68,34 +68,33 @@ __global__ void __launch_bounds__(kThreads) act8_save_kernel(const T* __restrict
   const int piece = (part << cut.cols_log2) + (threadIdx.x & ((1 << cut.cols_log2) - 1));
   const bool live = row < m && piece < cut.pieces;
   const int k0 = piece * 16;
-  T v[16];
+  __align__(16) T v[16];
   load16<T>(x + (live ? row : 0) * ldx, k0, live ? k : 0, wide, v);
-  uint32_t top = 0;  // magnitudes compare as their bits, NaN above infinity
-  float f[16];
+  typedef typename Half<T>::two T2;
+  const T2* pair = reinterpret_cast<const T2*>(v);
+  T2 most = __habs2(pair[0]);  // NaN stays NaN
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    f[i] = to_f32(v[i]);
-    const uint32_t bits = __float_as_uint(f[i]) & 0x7fffffffu;
-    top = bits > top ? bits : top;
-  }
+  for (int i = 1; i < 8; ++i) most = __hmax2_nan(most, __habs2(pair[i]));
+  // magnitudes compare as their bits, NaN above infinity
+  uint32_t top = max(__float_as_uint(to_f32(low_of(most))), __float_as_uint(to_f32(high_of(most)))) & 0x7fffffffu;
   const uint32_t other = __shfl_xor_sync(0xffffffffu, top, 1);
   top = other > top ? other : top;
   int e = static_cast<int>(top >> 23) - 127 - 6;
   const bool bad = top >= 0x7f800000u || e > ActRange<T>::hi;
   if (e < ActRange<T>::lo) e = ActRange<T>::lo;
   const float inv = __uint_as_float(static_cast<uint32_t>(127 - (bad ? 0 : e)) << 23);
-  const uint32_t keep = bad ? 0x80808080u : 0xffffffffu;
+  const uint32_t keep = bad ? 0u : 0x7f7f7f7fu;
+  const uint32_t* words = reinterpret_cast<const uint32_t*>(v);
   uint32_t w[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     uint32_t q[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      // adding 2^23 rounds to a whole number (nearest, ties to even) in the last bits
-      const float a = f[4 * j + i];
-      q[i] = (__float_as_uint(fminf(fabsf(a) * inv, 127.f) + 8388608.f) & 0x7fu) | ((__float_as_uint(a) >> 24) & 128u);
-    }
-    w[j] = (q[0] | (q[1] << 8) | (q[2] << 16) | (q[3] << 24)) & keep;
+    for (int i = 0; i < 4; ++i)  // adding 2^23 rounds to a whole number (nearest, ties to even) in the last bits
+      q[i] = __float_as_uint(fminf(__fmaf_rn(fabsf(to_f32(v[4 * j + i])), inv, 8388608.f), 8388735.f));
+    const uint32_t mags = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+    const uint32_t signs = __byte_perm(words[2 * j], words[2 * j + 1], 0x7531);  // the upper bytes of four values
+    w[j] = (mags & keep) | (signs & 0x80808080u);
   }
   if (!live) return;
   // the second half of a row's last block may lie behind the row, which ends at k rounded up to 16

@@ -74,16 +74,22 @@ __global__ void __launch_bounds__(kThreads) w4_quantize_kernel(const T* __restri
   for (int b = 0; b < kSpanBlocks; ++b) load8<T>(w + (row < n ? row : 0) * ldw, first + b * kW4Block, row < n ? k : 0, v[b], lane);
 #pragma unroll
   for (int b = 0; b < kSpanBlocks; ++b) {
-    // The largest value above zero and the largest magnitude below it, as bits: those of floats above zero are in the
-    // order of whole numbers, NaN above infinity.
-    float x[8];
-    int hi = 0, lo = 0;
+    // The largest value above zero and the largest magnitude below it, two values at a time (NaN stays NaN), then as bits:
+    // those of floats above zero are in the order of whole numbers, NaN above infinity.
+    typedef typename Half<T>::two T2;
+    const T2* pair = reinterpret_cast<const T2*>(v[b]);
+    int hi, lo = 0;
+    {
+      T2 top = SYM ? __habs2(pair[0]) : pair[0], low = pair[0];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x[i] = to_f32(v[b][i]);
-      const int bits = __float_as_int(x[i]);
-      hi = max(hi, SYM ? bits & 0x7fffffff : bits);
-      if (!SYM) lo = max(lo, bits ^ static_cast<int>(0x80000000u));
+      for (int i = 1; i < 4; ++i) {
+        top = __hmax2_nan(top, SYM ? __habs2(pair[i]) : pair[i]);
+        if (!SYM) low = __hmin2_nan(low, pair[i]);
+      }
+      hi = max(max(__float_as_int(to_f32(low_of(top))), __float_as_int(to_f32(high_of(top)))), 0);
+      if (!SYM)
+        lo = max(max(__float_as_int(to_f32(low_of(low))) ^ static_cast<int>(0x80000000u),
+                     __float_as_int(to_f32(high_of(low))) ^ static_cast<int>(0x80000000u)), 0);
     }
 #pragma unroll
     for (int s = G / 16; s >= 1; s >>= 1) {
@@ -97,28 +103,26 @@ __global__ void __launch_bounds__(kThreads) w4_quantize_kernel(const T* __restri
     const float s = to_f32(s16);
     const bool usable = s > 0.f && s < INFINITY;
     int z = SYM ? 8 : 0;
-    int q[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) q[i] = z;
+    uint32_t packed = z * 0x11111111u;
     if (usable) {
       // rint(x / s) without a division.  x and s have 11 significant bits at most, so that a quotient up to 2^5 that is
       // not halfway between two whole numbers is at least 2^-13 away from that; the product with the reciprocal is off by
-      // 2^-17 at most.  Adding and taking off 768 leaves multiples of 2^-14: a quotient that is halfway becomes exactly so, and
-      // no other one crosses.  Adding 1.5 * 2^23 then rounds to nearest, ties to even, as rint(x / s) does.  Scales
-      // whose reciprocal is not a normal number take the division.
-      const bool plain = s < 0x1p-120f || s > 0x1p120f;
-      const float inv = plain ? 0.f : __fdividef(1.f, s);
-      auto code = [&](float a) {
-        const float r = plain ? __fdiv_rn(a, s) : __fadd_rn(__fadd_rn(__fmul_rn(a, inv), 768.f), -768.f);
-        return __float_as_int(__fadd_rn(r, 12582912.f)) - 0x4b400000;
+      // 2^-17 at most.  Adding it to 768 leaves multiples of 2^-14: a quotient that is halfway becomes exactly so, and no
+      // other one crosses.  Adding 1.5 * 2^23 - 768 then rounds to nearest, ties to even, as rint(x / s) does, and leaves the
+      // whole number in the last bits.  Scales whose reciprocal is not a normal number are brought into range first, the
+      // values with them (a power of two: exact).
+      const float shift = s < 0x1p-100f ? 0x1p64f : s > 0x1p100f ? 0x1p-64f : 1.f;
+      const float inv = __fdividef(1.f, s * shift);
+      auto whole = [&](float a) {  // 0x4b400000 + rint(a / s)
+        return __float_as_int(__fadd_rn(__fmaf_rn(__fmul_rn(a, shift), inv, 768.f), 12582144.f));
       };
-      if (!SYM) z = min(code(__int_as_float(lo)), 15);
+      if (!SYM) z = min(whole(__int_as_float(lo)) - 0x4b400000, 15);
+      const int least = 0x4b400000 - z;  // code 0
+      packed = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) q[i] = min(max(code(x[i]) + z, 0), 15);
+      for (int i = 0; i < 8; ++i)
+        packed += static_cast<uint32_t>(min(max(whole(to_f32(v[b][i])) - least, 0), 15)) << (4 * w4_nibble(i));
     }
-    uint32_t packed = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) packed |= static_cast<uint32_t>(q[i]) << (4 * w4_nibble(i));
     *reinterpret_cast<uint32_t*>(tile + b * kW4TileBytes + word_offset(r, word)) = packed;
     const int block = span * kSpanBlocks + b;
     if (word % (G / 8) == 0 && block < blocks) {
