@@ -52,8 +52,9 @@ def _matrix(name: str, t: torch.Tensor, dtypes) -> None:
 
 
 def _ld(t: torch.Tensor) -> int:
+    # (a single row has no second one that could start off the 16-byte grid)
     rows, cols = t.shape
-    return t.stride(0) if rows > 1 else max(cols, 1)
+    return t.stride(0) if rows > 1 else max(-(-cols // 8) * 8, 8)
 
 
 def _same_device(first, *others) -> None:
@@ -236,9 +237,9 @@ def gemm_w4(x: torch.Tensor, w: WeightsW4, out: Optional[torch.Tensor] = None, w
     m, k = x.shape
     if k != w.k:
         raise ValueError(f"x has {k} columns, the weights {w.k} inputs")
+    if x.device != w.device:
+        raise ValueError(f"operands are on different devices: {x.device} and {w.device}")
     if out is None:
-        if x.device != w.device:
-            raise ValueError(f"operands are on different devices: {x.device} and {w.device}")
         out = torch.empty((m, w.n), dtype=w.dtype, device=w.device)
     else:
         _output("out", out, (m, w.n), w.dtype, w.device)
@@ -337,6 +338,8 @@ class WorkspaceGrad8(_Workspace):
     rows of dy will start on 16 bytes (the default expects packed rows); else there is room for a copy of dy."""
 
     def __init__(self, saved: Checkpoint8, n: int, out_dtype: torch.dtype = torch.float32, aligned: Optional[bool] = None):
+        if out_dtype != torch.float32 and out_dtype != saved.dtype:
+            raise ValueError(f"the gradient is float32 or {saved.dtype}")
         aligned = n % 8 == 0 if aligned is None else aligned
         with torch.cuda.device(saved.device):
             super().__init__(int(_lib.load().sb200_act8_wgrad_workspace_bytes(saved._code, DTYPE_CODE[out_dtype], saved.m, n,
@@ -348,7 +351,7 @@ def weight_grad8(saved: Checkpoint8, dy: torch.Tensor, base: Optional[torch.Tens
                  check: bool = False) -> torch.Tensor:
     """base + X^T @ dy (in_features x out_features, the layout of `gemm`'s B) for the saved activations X and the output
     gradient dy (tokens x out_features) of the same type.  The result is fp32 or has dy's type; `base` and `out` have
-    the result's type, and may be the same tensor.  `check` synchronises and raises if a device-side wait gave up."""
+    the result's type, and may be the same tensor; `out` overlaps no other operand.  `check` synchronises and raises if a device-side wait gave up."""
     _matrix("dy", dy, (saved.dtype,))
     m, n = dy.shape
     if m != saved.m:
@@ -361,9 +364,9 @@ def weight_grad8(saved: Checkpoint8, dy: torch.Tensor, base: Optional[torch.Tens
         raise ValueError(f"the gradient is float32 or {saved.dtype}")
     if base is not None:
         _output("base", base, (saved.k, n), out_dtype, saved.device)
+    if dy.device != saved.device:
+        raise ValueError(f"operands are on different devices: {dy.device} and {saved.device}")
     if out is None:
-        if dy.device != saved.device:
-            raise ValueError(f"operands are on different devices: {dy.device} and {saved.device}")
         out = torch.empty((saved.k, n), dtype=out_dtype, device=saved.device)
     else:
         _output("out", out, (saved.k, n), out_dtype, saved.device)

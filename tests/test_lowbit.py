@@ -135,3 +135,69 @@ def test_python_handles_refuse_wrong_tables():
         lowbit.Checkpoint8(codes.view(8, 128), codes.view(8, 128), 100, torch.float32)
     with pytest.raises(ValueError):
         lowbit.Checkpoint8(codes.view(8, 128), codes.view(8, 128), 0, torch.float16)
+
+
+class _OnDevice:
+    """What the Python calls ask of a tensor, on a device that need not be there."""
+    is_cuda = True
+
+    def __init__(self, index, dtype, *shape):
+        import torch
+
+        self.device, self.dtype, self.shape = torch.device("cuda", index), dtype, shape
+
+    def dim(self):
+        return 2
+
+    def stride(self, axis=None):
+        return (self.shape[1], 1) if axis is None else (self.shape[1], 1)[axis]
+
+    def data_ptr(self):
+        return P
+
+
+def test_python_products_refuse_operands_on_different_devices(monkeypatch):
+    """Each operand on another device than the others, with and without an `out`."""
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    def launched(*args):
+        raise AssertionError("the call reached the library")
+
+    monkeypatch.setattr(lowbit, "_call", launched)
+    H, F = torch.float16, torch.float32
+    w = lowbit.WeightsW4.__new__(lowbit.WeightsW4)
+    w._set(64, 128, 128, H, torch.device("cuda", 0), P, P, None)
+    w._status_ptr = P
+    saved = lowbit.Checkpoint8.__new__(lowbit.Checkpoint8)
+    saved._set(4, 128, H, torch.device("cuda", 0), P, 128, P, 4)
+
+    class Room:
+        nbytes = WS
+        _for = lowbit._Workspace._for
+
+        def __init__(self, index):
+            self.device, self.ptr = torch.device("cuda", index), P
+
+    on = _OnDevice
+    for call in (
+        lambda: lowbit.gemm_w4(on(1, H, 4, 128), w),
+        lambda: lowbit.gemm_w4(on(1, H, 4, 128), w, out=on(0, H, 4, 64)),
+        lambda: lowbit.gemm_w4(on(0, H, 4, 128), w, out=on(1, H, 4, 64)),
+        lambda: lowbit.gemm_w4(on(0, H, 4, 128), w, out=on(0, H, 4, 64), workspace=Room(1)),
+        lambda: lowbit.dequantize_w4(w, out=on(1, H, 64, 128)),
+        lambda: lowbit.save8(on(1, H, 4, 128), out=saved),
+        lambda: lowbit.restore8(saved, out=on(1, H, 4, 128)),
+        lambda: lowbit.weight_grad8(saved, on(1, H, 4, 64), workspace=Room(0)),
+        lambda: lowbit.weight_grad8(saved, on(1, H, 4, 64), out=on(0, F, 128, 64), workspace=Room(0)),
+        lambda: lowbit.weight_grad8(saved, on(0, H, 4, 64), out=on(1, F, 128, 64), workspace=Room(0)),
+        lambda: lowbit.weight_grad8(saved, on(0, H, 4, 64), base=on(1, F, 128, 64), out=on(0, F, 128, 64), workspace=Room(0)),
+        lambda: lowbit.weight_grad8(saved, on(0, H, 4, 64), out=on(0, F, 128, 64), workspace=Room(1)),
+    ):
+        with pytest.raises(ValueError, match="device|workspace is on"):
+            call()
+    with pytest.raises(AssertionError):
+        lowbit.gemm_w4(on(0, H, 4, 128), w, out=on(0, H, 4, 64), workspace=Room(0))
+    with pytest.raises(ValueError):
+        lowbit.WorkspaceGrad8(saved, 64, torch.bfloat16)
