@@ -307,7 +307,7 @@ size_t sb200_w4_table_entries(int n, int k, int group);
 int sb200_w4_quantize(int dtype, const void* w, long long ldw, int n, int k, int group, void* codes, void* scales, void* zeros,
                       sb200_stream_t stream);
 /* Weights of another quantiser into the order above: codes q[n][k], one byte each, in the low nibble; scales
- * q_scales[group][n] in `dtype`; zeros q_zeros[group][n], bytes, or NULL (then zeros is NULL too). */
+ * q_scales[group][n] in `dtype`; zeros q_zeros[group][n], in the low nibble of bytes, or NULL (then zeros is NULL too). */
 int sb200_w4_pack(int dtype, const void* q, long long ldq, const void* q_scales, long long lds, const void* q_zeros,
                   long long ldz, int n, int k, int group, void* codes, void* scales, void* zeros, sb200_stream_t stream);
 /* out[n][k] = W rounded once to `dtype`. */

@@ -12,7 +12,9 @@ namespace {
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
 constexpr int kMaxSlices = 16;
-constexpr int kDenseColumns = 1280;  // measured: 1000 to 1024 rows through 8192 x 4096: 65 us on the way, 67 us in two passes
+constexpr int kDenseColumns = 1280;  // from here on two passes: rows through 8192 x 4096 4-bit weights, on the
+// way and in two passes: 512: 37 and 44 us, 1024: 64 and 63, 1280: 89 and 77, 4096: 202 and 181; columns of a gradient of 4096
+// channels from 4096 tokens: 512: 31 and 37 us, 1024: 41 and 42, 1280: 69 and 60, 2048: 72 and 64
 constexpr size_t kPartBytes = size_t(64) << 20;  // most that the parts of a divided reduction may take
 
 struct Cut {
@@ -23,7 +25,7 @@ struct Cut {
 // columns x 64 at 8192 operations a clock and SM) and never less than what the hand-overs between the roles take (measured:
 // 0.37 us at every narrow tile); a unit more than that for filling its pipeline and for its sums; dividing the
 // reduction costs a pass over the parts, and a launch.  The cut with the least total of the fullest pair wins; widths
-// are what the instruction takes.  (128 rows through 4096 x 4096 4-bit weights: 16 tiles; in one part 38 us, in four 16 us.)
+// are what the instruction takes.  (128 rows through 4096 x 4096 4-bit weights: 16 tiles; in one part 38 us, in four 17.5 us.)
 Cut cut_of(long long rows, long long cols, int steps, int pairs, bool dense) {
   const double kStepLeast = dense ? 500 : 700, kUnit = 4000, kJoin = 4000, kBytesPerClock = 4000;
   Cut best{kMaxCols, 1};

@@ -4,18 +4,23 @@
 //
 // A pair of CTAs computes a tile of 256 left rows x `bn` columns with tcgen05.mma.cta_group::2.  Per step of 64 of the
 // reduction each CTA's converter warps (two groups of four, in turn) expand the 128 x 64 values of its own left rows into the swizzled shared-memory
-// tile that the tensor cores read; TMA brings the codes and the CTA's half of the right operand.  (Codes loaded into the
-// converters' registers a few steps ahead were measured at less than half the speed: each fence that hands a tile to
-// the tensor cores then waits for the loads in flight.)  The expansion therefore costs no pass over memory: the operand travels in 4 or 8 bits and is never written
-// out in 16.
+// tile that the tensor cores read; TMA brings the codes and the CTA's half of the right operand, so that no
+// converter has a load of its own in flight when it hands a tile to the tensor cores.  The expansion costs no pass over
+// memory: the operand travels in 4 or 8 bits and is never written out in 16.
 //   W4    the tile is K-major (a word of the format is the 16 bytes of eight neighbouring inputs); weights are rounded to 16
 //         bits once, code - zero is exact before.
 //   ACT8  the tile is MN-major (tokens are rows in memory, channels run along a row); every value is exact in 16 bits.
 //
 // A left tile is expanded once for every tile of columns.  With many of those it is cheaper to expand the operand once into 16
 // bits in the workspace and to multiply that (DENSE: the left tiles come by TMA too, there are no converters): 4096 rows
-// through 8192 x 4096 4-bit weights take 196 us, expanded on the way 250 us;
-// a gradient of 4096 x 8192 from 16384 tokens 836 and 950 us.
+// through 8192 x 4096 4-bit weights take 181 us, expanded on the way 202 us; a gradient of 4096 x 2048 from 4096 tokens
+// 64 and 72 us.
+//
+// Bound.  Dense, a large product: the tensor pipe is busy for 79 % of the cycles, and under a long load the power limit lowers
+// the clock (4096 rows through 8192 x 4096: 1.5 PFLOP/s; a gradient of 4096 x 8192 from 16384 tokens 1.5 in a short run,
+// 1.1 in a long one).  Expanded on the way: tensor pipe 60 %, the converters issue in 41 % of the cycles, and
+// operands, codes and expanded tiles share the bandwidth of shared memory.  Small products: about 9 us for the launch, the
+// setup, the first loads, the last sums and the end, and 0.37 us for every step of 64 that a narrow tile takes.
 //
 // Sums.  The tensor cores chop when they add to an accumulator (measured on B200, exact products of normal values:
 // relative error 3.4e-5 after 2048 additions, 1.5e-6 after 128, growing with their number), which is too coarse for a gradient kept in
@@ -426,8 +431,8 @@ expand_product_kernel(const __grid_constant__ ExpandParams p) {
       }
     }
     else if (!DENSE) {
-      // ---- passes on to the leader that the peer's left tile is written.  The converters themselves would have to release
-      // at cluster scope, which waits for the loads that they have in flight.
+      // ---- passes on to the leader that the peer's left tile is written.  One thread's arrival crosses to the other CTA
+      // for each step instead of one from each converter warp.
       uint32_t stage = 0, phase = 0;
       bool ok = true;
       for (int u = pair; ok && u < units; u += pairs) {

@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(kThreads) w4_pack_kernel(const uint8_t* __rest
     const long long group = k0 / G, at = w4_table_at(row, k0 / G, blocks, G);
     const bool real = row < n && k0 < k;
     scales[at] = real ? s[group * lds + row] : 0;
-    if (z) zeros[at] = real ? z[group * ldz + row] : 0;
+    if (z) zeros[at] = real ? z[group * ldz + row] & 15u : 0;
   }
 }
 
@@ -238,7 +238,8 @@ int rows_product(const void* x, long long ldx, const W4& w, void* y, long long l
   const RowsParams p{x, ldx, static_cast<const uint8_t*>(w.codes), static_cast<const uint8_t*>(w.scales),
                      static_cast<const uint8_t*>(w.zeros), y, ldy, m, w.n, w.k, w4_blocks(w.k)};
   // one row tile to a warp while that is at most two blocks for each SM, else two, which read x half as often (one row, 2048 x
-  // 2048: 2.3 us, 3.2 with two; 8192 x 8192: 13.3 us, 14.5 with one; four row tiles were slower everywhere)
+  // 2048: 2.5 us, 3.0 with two; 4096 x 8192: 7.5 and 7.6; 8192 x 8192: 11.9 us, 13.4 with one; between, 6144 x 8192: 11.7 us,
+  // 10.7 with one, but 12.9 and 13.0 at eight rows of x, and 7104 x 2048 4.9 and 5.5; four row tiles were slower everywhere)
   if (w4_row_tiles(w.n) <= 2 * sm_count_of_current_device()) return launch_rows<T, PER, 1, 1, 4>(p, stream);
   return launch_rows<T, PER, 2, 1, 3>(p, stream);
 }
@@ -250,8 +251,8 @@ int rows_product_any(const void* x, long long ldx, const W4& w, void* y, long lo
   return rows_product<T, 1>(x, ldx, w, y, ldy, m, stream);
 }
 
-// Up to here the codes are multiplied as they are (w4_rows.cuh); a few rows more go to the tensor cores' own instruction
-// (w4_decode.cuh: 16 rows, 8192 x 8192: 18.2 us, and about as much for 64).
+// Up to here, the columns of one warp instruction, the codes are multiplied as they are (w4_rows.cuh); more rows go to
+// tcgen05.mma (w4_decode.cuh).  8192 x 8192: 1 row 11.9 us, the other kernel 16.4; 8 rows 13.1 and 16.6; 9 rows 17.0.
 constexpr int kFewRows = 8;
 
 int check(const W4& w) {

@@ -1,11 +1,15 @@
-// y = x W^T for up to 64 rows of x (a decoding batch), weights in format W4: bound by the bytes of the weights.
+// y = x W^T for up to 64 rows of x (a decoding batch), weights in format W4.
 //
-// Tensor-core instructions of a warp (mma.sync) are too slow here even for one row of x (measured on B200: about ten clocks of
-// an SM for each m16n8k16, which ends at 2.1 TB/s of weights; 8192 x 8192, 8 rows: 16 us).  So the weights go where
-// tcgen05.mma takes them from without another pass through shared memory: a thread expands a row of 128 inputs in its
-// registers and writes it to its lane of tensor memory, which is the left operand (128 rows x 16 inputs an instruction); x,
-// the right operand, comes to shared memory by TMA.  What is left is the expansion, about 15 instructions for eight
-// weights.
+// Up to 8 rows a warp's own matrix instruction takes the codes from registers (w4_rows.cuh), but that kernel is bound by the
+// instructions it issues, and every 8 rows more add a matrix instruction and the loads of x for each 16 x 16 codes.  Here the
+// weights go where tcgen05.mma takes them from without another pass through shared memory: a thread expands a row of
+// 128 inputs in its registers and writes it to its lane of tensor memory, which is the left operand (128 rows x 16 inputs
+// an instruction); x, the right operand, comes to shared memory by TMA.  What a batch costs is then almost independent of its
+// rows: 8192 x 8192, groups of 128: 9 rows 17.0 us, 16 rows 17.2, 32 rows 18.8, 64 rows 21.4 (the bytes: 5.3 us; 2.0 TB/s).
+//
+// Bound.  Neither memory nor the tensor cores (6 % busy) nor one pipe: the integer pipe is active for 37 % of the cycles, issue for
+// half, and the warps wait on one another (load, expand, store to tensor memory, hand over).  About 15 instructions for
+// eight weights are the expansion; the scales are multiplied in here, one rounding to 16 bits for each weight.
 //
 // Split.  A CTA holds 128 rows; where rows are few, the CTAs of a cluster divide the inputs and add their sums over
 // distributed shared memory, rank by rank, so that results do not change from call to call.  Two CTAs share an SM: one

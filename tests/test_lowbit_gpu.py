@@ -688,3 +688,89 @@ def test_python_refusals(cuda_device):
     small.nbytes = 0
     with pytest.raises(lowbit.KernelError):
         lowbit.gemm_w4(x, w, workspace=small)
+
+
+@pytest.mark.parametrize("m", [1, 3, 20, 64])
+@pytest.mark.parametrize("n,k,group,symmetric", [(4737, 300, 64, False), (9000, 200, 128, True), (19000, 130, 32, False)])
+def test_gemm_w4_many_outputs(cuda_device, m, n, k, group, symmetric):
+    """So many outputs that a warp takes two row tiles, and that fewer CTAs (at last one) divide the inputs of 128 rows."""
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    w = lowbit.quantize_w4(randn((n, k), torch.bfloat16, cuda_device, 70, k ** -0.5), group=group, symmetric=symmetric)
+    x = randn((m, k), torch.bfloat16, cuda_device, 71)
+    check_w4_gemm(lowbit.gemm_w4(x, w, check=True), x, w, exact_weights=False)
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("k", [1, 7, 131, 257])
+def test_single_rows_of_odd_length(cuda_device, dtype, k):
+    """A single row is taken where it lies, on 16 bytes or off; values behind its end are never used."""
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    w = lowbit.quantize_w4(randn((40, k), T(dtype), cuda_device, 72, k ** -0.5), group=32)
+    for first in (0, 3):
+        room = torch.full((1, k + 16), float("nan"), dtype=T(dtype), device=cuda_device)
+        x = room[:, first:first + k]
+        x.copy_(randn((1, k), T(dtype), cuda_device, 73))
+        check_w4_gemm(lowbit.gemm_w4(x, w), x, w, exact_weights=False)
+        saved = lowbit.save8(x)
+        codes, exps, _ = plain_save(x)
+        assert torch.equal(saved.codes[:, :k].int(), codes) and torch.equal(saved.exponents[:, :-(-k // 32)].long(), exps.long())
+        check_grad(lowbit.weight_grad8(saved, x), values_of(saved), x, None)
+        back = torch.full((1, k + 9), 7.0, dtype=T(dtype), device=cuda_device)
+        lowbit.restore8(saved, out=back[:, 1:1 + k])
+        assert torch.equal(back[:, 1:1 + k].double(), values_of(saved))
+        assert bool((back[:, :1] == 7).all()) and bool((back[:, 1 + k:] == 7).all())
+
+
+@pytest.mark.parametrize("m", [3, 24, 200])
+def test_two_streams_share_the_weights(cuda_device, m):
+    """Calls without workspaces on two streams at once, with the same weights and the same saved activations."""
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    w = lowbit.quantize_w4(randn((900, 512), torch.float16, cuda_device, 74, 0.05))
+    xs = [randn((m, 512), torch.float16, cuda_device, 75 + i) for i in range(2)]
+    want = [lowbit.gemm_w4(x, w) for x in xs]
+    saved = lowbit.save8(xs[0])
+    grads = [lowbit.weight_grad8(saved, y) for y in want]
+    streams = [torch.cuda.Stream(cuda_device) for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append((lowbit.gemm_w4(xs[i], w), lowbit.weight_grad8(saved, want[i])))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for y, dw in got[i]:
+            assert torch.equal(y, want[i]) and torch.equal(dw, grads[i])
+
+
+def test_status_and_workspace_sizes(cuda_device):
+    """`check` passes after good calls of every size; a workspace that is too small is refused, one that is larger serves."""
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    w = lowbit.quantize_w4(randn((300, 256), torch.bfloat16, cuda_device, 77, 0.06))
+    large = lowbit.WorkspaceW4(2000, w)
+    for m in (1, 9, 64, 65, 1300):
+        x = randn((m, 256), torch.bfloat16, cuda_device, 78)
+        y = lowbit.gemm_w4(x, w, check=True)
+        assert torch.equal(lowbit.gemm_w4(x, w, workspace=large, check=True), y)
+        large.check()
+    with pytest.raises(lowbit.KernelError):
+        lowbit.gemm_w4(randn((1300, 256), torch.bfloat16, cuda_device, 78), w, workspace=lowbit.WorkspaceW4(64, w))
+    for n in (5, 200, 1300):
+        dy = randn((70, n), torch.bfloat16, cuda_device, 79)
+        saved = lowbit.save8(randn((70, 100), torch.bfloat16, cuda_device, 80))
+        dw = lowbit.weight_grad8(saved, dy, check=True)
+        check_grad(dw, values_of(saved), dy, None)
+        with pytest.raises(lowbit.KernelError):
+            lowbit.weight_grad8(saved, dy, workspace=lowbit.WorkspaceW4(1, w))
