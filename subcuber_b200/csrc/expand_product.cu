@@ -182,7 +182,7 @@ namespace {
 int decode_ranks(int n, int blocks) {
   const int sms = sm_count_of_current_device();
   const int room = 2 * (sms > 0 ? sms : 148), groups = ceil_div(n, kDecodeRows);
-  int ranks = 8;
+  int ranks = kDecodeMaxRanks;
   while (ranks > 1 && (groups * static_cast<long long>(ranks) > room || ranks > blocks)) ranks /= 2;
   return ranks;
 }

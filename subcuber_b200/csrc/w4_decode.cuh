@@ -38,6 +38,7 @@ struct DecodeParams {
 
 constexpr int kDecodeThreads = 320;  // warps 0 and 1: TMA and MMA, 2-9: converters
 constexpr int kDecodeRows = 128, kDecodeMaxRight = 64;
+constexpr int kDecodeMaxRanks = 8;   // CTAs of a cluster
 constexpr int kAhead = 3;            // stages of a converter warp's ring
 constexpr int kLeftStages = 3;       // of 128 inputs in tensor memory, 64 columns each; the sums take the 64 behind
 constexpr int kRightStages = 3;      // of 128 inputs of x in shared memory
@@ -205,7 +206,6 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) w4_decode_kernel(const __gr
     int stage = 0, fill = kAhead - 1;
     // tiles of both groups take the left stages in order: this group starts at stage `group` and moves on by two
     uint32_t ls = group, lphase = 0;
-    bool ok = true;
     const int r16 = lane & 15;
     const uint32_t mask = in_register(0x000f000fu), magic = in_register(Half<T>::magic);
     for (int b = first; b < b1; b += 2) {
@@ -230,7 +230,6 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) w4_decode_kernel(const __gr
       }
       if (!ptx::mbar_wait_warp<false>(&left_empty[ls], lphase ^ 1u, abort_flag, p.wait_ns)) {
         give_up_here(104);
-        ok = false;
         break;
       }
       ptx::tc_fence_after_sync();
@@ -256,7 +255,6 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) w4_decode_kernel(const __gr
       if (ls >= kLeftStages) { ls -= kLeftStages; lphase ^= 1u; }
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
-    (void)ok;
   }
 
   // ---- the sums: row = lane of tensor memory, column = row of x
@@ -265,11 +263,11 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) w4_decode_kernel(const __gr
   float* part = reinterpret_cast<float*>(smem);  // [rows of x][128]
   const bool whole = !*abort_flag;
   __syncthreads();
-  if (whole && b1 > b0 && warp >= 2 && warp < 6) {
+  if (whole && b1 > b0 && warp >= 2) {  // two warps to a lane quarter, each takes eight of sixteen columns
     ptx::tc_fence_after_sync();
     const int quarter = warp & 3, row = row0 + quarter * 32 + lane;
     const uint32_t from = tmem_sums + (static_cast<uint32_t>(quarter * 32) << 16);
-    for (int c0 = 0; c0 < p.n16; c0 += 8) {
+    for (int c0 = (warp - 2) / 4 * 8; c0 < p.n16; c0 += 16) {
       uint32_t r[8];
       tmem_ld_32x8(from + c0, r);
       ptx::tmem_ld_wait();
@@ -283,11 +281,22 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) w4_decode_kernel(const __gr
   }
   if (ranks > 1) {
     cluster.sync();
-    for (int e = rank * kDecodeThreads + threadIdx.x; e < p.m * kDecodeRows; e += ranks * kDecodeThreads) {
-      float s = 0.f;
-      for (int c = 0; c < ranks; ++c) s += *cluster.map_shared_rank(part + e, c);
-      const int row = row0 + e % kDecodeRows;
-      if (row < p.n) static_cast<T*>(p.y)[(e / kDecodeRows) * p.ldy + row] = from_f32<T>(s);
+    // four neighbouring rows for each thread, all CTAs' parts asked for before the first is added
+    for (int e = rank * kDecodeThreads + threadIdx.x; e < p.m * (kDecodeRows / 4); e += ranks * kDecodeThreads) {
+      float4 v[kDecodeMaxRanks];
+#pragma unroll
+      for (int c = 0; c < kDecodeMaxRanks; ++c)
+        if (c < ranks) v[c] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(part + 4 * e, c));
+      float4 s = v[0];
+#pragma unroll
+      for (int c = 1; c < kDecodeMaxRanks; ++c)
+        if (c < ranks) { s.x += v[c].x; s.y += v[c].y; s.z += v[c].z; s.w += v[c].w; }
+      const int row = row0 + e % (kDecodeRows / 4) * 4;
+      T* to = static_cast<T*>(p.y) + (e / (kDecodeRows / 4)) * p.ldy + row;
+      const T four[4] = {from_f32<T>(s.x), from_f32<T>(s.y), from_f32<T>(s.z), from_f32<T>(s.w)};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (row + i < p.n) to[i] = four[i];
     }
     cluster.sync();  // no CTA leaves while others read its memory
   }
