@@ -2,6 +2,8 @@
 #include "expand_product.cuh"
 #include "w4_decode.cuh"
 
+#include <atomic>
+
 #include "lowbit_host.h"
 #include "per_device.h"
 
@@ -178,17 +180,8 @@ int expand_w4(const W4& w, const void* x, long long ldx, void* y, long long ldy,
 
 namespace {
 
-// CTAs that divide the inputs of 128 rows: as many as keep the grid within two CTAs for each SM.
-int decode_ranks(int n, int blocks) {
-  const int sms = sm_count_of_current_device();
-  const int room = 2 * (sms > 0 ? sms : 148), groups = ceil_div(n, kDecodeRows);
-  int ranks = kDecodeMaxRanks;
-  while (ranks > 1 && (groups * static_cast<long long>(ranks) > room || ranks > blocks)) ranks /= 2;
-  return ranks;
-}
-
 template <typename T, int PER>
-int launch_decode(const DecodeParams& p, int ranks, cudaStream_t stream) {
+int launch_decode(const DecodeParams& p, cudaStream_t stream) {
   auto* kernel = w4_decode_kernel<T, PER>;
   static PerDeviceOnce attr;
   const int rc = attr.run_once([&] {
@@ -196,23 +189,45 @@ int launch_decode(const DecodeParams& p, int ranks, cudaStream_t stream) {
   });
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(ceil_div(p.n, kDecodeRows) * ranks));
   cfg.blockDim = dim3(kDecodeThreads);
   cfg.dynamicSmemBytes = decode_smem(PER, p.n16);
   cfg.stream = stream;
   cudaLaunchAttribute attrs[1];
   attrs[0].id = cudaLaunchAttributeClusterDimension;
-  attrs[0].val.clusterDim = {static_cast<unsigned>(ranks), 1, 1};
   cfg.attrs = attrs;
   cfg.numAttrs = 1;
+  // CTAs that divide the inputs of 128 rows: as many as fit on the device at once, one for each SM, or two where they have eight
+  // tiles or more to go through (the runtime counts one).  A cluster lies within one group of SMs, which leaves some of
+  // them over.  16 rows, clusters of 1, 2, 4 and 8 CTAs in us: 128 x 4096: 15.9, 10.4, 7.5, 6.2; 4096 x 4096: 17.4, 11.7, 8.8,
+  // 9.8; 8192 x 1024: 7.2, 6.2, 7.2, 12.3; 8192 x 8192: 30.4, 18.6, 16.9, 21.8; 9472 x 4096: 17.8, 12.5, 16.9, 20.2;
+  // 16384 x 512: 5.6, 7.1, 10.9, 10.8; 16384 x 4096: 18.0, 17.0, 20.4, 29.7.
+  static std::atomic<int> room[kMaxDevices][kDecodeMaxRight / 16][4];  // clusters at once, plus one
+  const int groups = ceil_div(p.n, kDecodeRows);
+  int dev = -1, log2 = 3;
+  if (cudaError_t e = cudaGetDevice(&dev)) return static_cast<int>(e);
+  for (; log2 > 0; --log2) {
+    const int ranks = 1 << log2;
+    if (ranks > p.blocks || groups > 0x7fffffff / ranks) continue;
+    attrs[0].val.clusterDim = {static_cast<unsigned>(ranks), 1, 1};
+    cfg.gridDim = dim3(static_cast<unsigned>(groups) * ranks);
+    std::atomic<int>* cached = dev < kMaxDevices ? &room[dev][p.n16 / 16 - 1][log2] : nullptr;
+    int fit = cached ? cached->load(std::memory_order_relaxed) - 1 : -1;
+    if (fit < 0) {
+      if (cudaError_t e = cudaOccupancyMaxActiveClusters(&fit, kernel, &cfg)) return static_cast<int>(e);
+      if (cached) cached->store(fit + 1, std::memory_order_relaxed);
+    }
+    if (groups <= fit || (groups <= 2 * fit && p.blocks >= 8 * ranks)) break;
+  }
+  attrs[0].val.clusterDim = {1u << log2, 1, 1};
+  cfg.gridDim = dim3(static_cast<unsigned>(groups) << log2);
   return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, p));
 }
 
 template <typename T>
-int run_decode(const DecodeParams& p, int group, int ranks, cudaStream_t stream) {
-  if (group == 32) return launch_decode<T, 4>(p, ranks, stream);
-  if (group == 64) return launch_decode<T, 2>(p, ranks, stream);
-  return launch_decode<T, 1>(p, ranks, stream);
+int run_decode(const DecodeParams& p, int group, cudaStream_t stream) {
+  if (group == 32) return launch_decode<T, 4>(p, stream);
+  if (group == 64) return launch_decode<T, 2>(p, stream);
+  return launch_decode<T, 1>(p, stream);
 }
 
 }  // namespace
@@ -231,8 +246,7 @@ int decode_w4(const W4& w, const void* x, long long ldx, void* y, long long ldy,
   p.status = static_cast<int*>(status);
   p.wait_ns = kWaitNs;
   if (int rc = tc::map_rows_16bit(&p.right, x, m, w.k, ldx, p.n16)) return rc;
-  const int ranks = decode_ranks(w.n, p.blocks);
-  return w.dtype == kF16 ? run_decode<__half>(p, w.group, ranks, stream) : run_decode<__nv_bfloat16>(p, w.group, ranks, stream);
+  return w.dtype == kF16 ? run_decode<__half>(p, w.group, stream) : run_decode<__nv_bfloat16>(p, w.group, stream);
 }
 
 size_t expand_act8_workspace(int m, int n, int k, bool dy_aligned) {

@@ -5,7 +5,7 @@
 // weights go where tcgen05.mma takes them from without another pass through shared memory: a thread expands a row of
 // 128 inputs in its registers and writes it to its lane of tensor memory, which is the left operand (128 rows x 16 inputs
 // an instruction); x, the right operand, comes to shared memory by TMA.  What a batch costs is then almost independent of its
-// rows: 8192 x 8192, groups of 128: 9 rows 17.0 us, 16 rows 17.2, 32 rows 18.8, 64 rows 21.4 (the bytes: 5.3 us; 2.0 TB/s).
+// rows: 8192 x 8192, groups of 128: 16 rows 17.0 us, 64 rows 19.4 (the bytes: 5.3 us; 2.0 TB/s).
 //
 // Bound.  Neither memory nor the tensor cores (6 % busy) nor one pipe: the integer pipe is active for 37 % of the cycles, issue for
 // half, and the warps wait on one another (load, expand, store to tensor memory, hand over).  About 15 instructions for
@@ -298,7 +298,9 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) w4_decode_kernel(const __gr
       for (int i = 0; i < 4; ++i)
         if (row + i < p.n) to[i] = four[i];
     }
-    cluster.sync();  // no CTA leaves while others read its memory
+    // No CTA leaves while others read its memory.  Nothing but those reads has to be over, and their values have been used;
+    // an arrival that releases would wait for the stores to y.
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
   __syncthreads();
   if (*abort_flag) {
