@@ -11,45 +11,47 @@ namespace sb200 {
 namespace lowbit {
 namespace {
 
-// A block of threads handles one row tile (16 rows) and kSpanBlocks tiles of 128 inputs: half a warp takes a row, a lane eight
-// neighbouring inputs of each 128, which are one word of the format.  The codes are put together in shared memory and
-// leave as whole tiles.
-constexpr int kSpanBlocks = 4;
+// A block of threads handles one row tile (16 rows) and kSpanBlocks tiles of 128 inputs.  To quantise, half a warp takes a row and
+// a lane sixteen neighbouring inputs of each 256, two words of the format: what is done once for a group is then done by half
+// as many lanes as with one word (4096 x 4096, bf16, groups of 128 with zeros: 11.1 us, 13.0 with one).  The codes are put
+// together in shared memory and leave as whole tiles.
+constexpr int kSpanBlocks = 4, kSpan = kSpanBlocks * kW4Block;
 constexpr int kThreads = 256;
+constexpr int kLaneInputs = 16, kTurn = 16 * kLaneInputs, kTurns = kSpan / kTurn;
 
-// Eight neighbouring 16-bit values of a row for each lane and each of kSpanBlocks tiles, zeros behind `k`; the 16 lanes of half
-// a warp take 128 neighbours.  A row that does not start on 16 bytes is read in the aligned 8-byte words that hold it: a lane
-// takes two words, the rest from the lane behind (the last lane reads one more), and shifts them together.  Words without
-// a value of the row are not read.  All tiles' loads are issued before the first value
-// is used (4096 x 4096, bf16, groups of 128 with zeros: 13.0 us; tile after tile 17.1 us).
+// The lane's 16-bit values of a row for every turn, zeros behind `k`; the lanes of half a warp take neighbours.  A row that does
+// not start on 16 bytes is read in the aligned 8-byte words that hold it: a lane takes four words, the rest from the lane
+// behind (the last lane reads one more), and shifts them together.  Words without a value of the row are not read.  All loads
+// are issued before the first value is used (tile after tile, one word for a lane: 17.1 us in place of 13.0).
 template <typename T>
-__device__ __forceinline__ void load_words(const T* row, int first, int k, bool wide, T (&v)[kSpanBlocks][8], int lane) {
-  if (wide && first - (lane & 15) * 8 <= k - kSpanBlocks * kW4Block) {  // the same for the lanes of a row
+__device__ __forceinline__ void load_words(const T* row, int first, int k, bool wide, T (&v)[kTurns][kLaneInputs], int lane) {
+  if (wide && first - (lane & 15) * kLaneInputs <= k - kSpan) {  // the same for the lanes of a row
 #pragma unroll
-    for (int b = 0; b < kSpanBlocks; ++b) *reinterpret_cast<uint4*>(v[b]) = __ldg(reinterpret_cast<const uint4*>(row + first + b * kW4Block));
+    for (int b = 0; b < kTurns; ++b)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) reinterpret_cast<uint4*>(v[b])[i] = __ldg(reinterpret_cast<const uint4*>(row + first + b * kTurn) + i);
     return;
   }
   const uintptr_t end = reinterpret_cast<uintptr_t>(row + k);
-  const uint32_t off = reinterpret_cast<uintptr_t>(row + first) & 7;  // the same for the lanes of a row, and every tile
-  unsigned long long w[kSpanBlocks][3];
+  const uint32_t off = reinterpret_cast<uintptr_t>(row + first) & 7;  // the same for the lanes of a row, and every turn
+  unsigned long long w[kTurns][5];
 #pragma unroll
-  for (int b = 0; b < kSpanBlocks; ++b) {
-    const uintptr_t at = reinterpret_cast<uintptr_t>(row + first + b * kW4Block) - off;
+  for (int b = 0; b < kTurns; ++b) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(row + first + b * kTurn) - off;
     const unsigned long long* word = reinterpret_cast<const unsigned long long*>(at);
 #pragma unroll
-    for (int i = 0; i < 3; ++i)
-      w[b][i] = k > 0 && at + 8 * i < end && (i < 2 || (off && (lane & 15) == 15)) ? __ldg(word + i) : 0ull;
+    for (int i = 0; i < 5; ++i)
+      w[b][i] = k > 0 && at + 8 * i < end && (i < 4 || (off && (lane & 15) == 15)) ? __ldg(word + i) : 0ull;
   }
 #pragma unroll
-  for (int b = 0; b < kSpanBlocks; ++b) {
+  for (int b = 0; b < kTurns; ++b) {
     const unsigned long long behind = __shfl_down_sync(0xffffu << (lane & 16), w[b][0], 1, 16);
-    const unsigned long long next = (lane & 15) == 15 ? w[b][2] : behind;
+    if ((lane & 15) != 15) w[b][4] = behind;
     unsigned long long* to = reinterpret_cast<unsigned long long*>(v[b]);
-    to[0] = off ? (w[b][0] >> (8 * off)) | (w[b][1] << (64 - 8 * off)) : w[b][0];
-    to[1] = off ? (w[b][1] >> (8 * off)) | (next << (64 - 8 * off)) : w[b][1];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int left = k - (first + b * kW4Block) - 4 * i;
+    for (int i = 0; i < 4; ++i) {
+      to[i] = off ? (w[b][i] >> (8 * off)) | (w[b][i + 1] << (64 - 8 * off)) : w[b][i];
+      const int left = k - (first + b * kTurn) - 4 * i;
       if (left < 4) to[i] = left <= 0 ? 0ull : to[i] & (~0ull >> (64 - 16 * left));
     }
   }
@@ -84,20 +86,20 @@ __global__ void __launch_bounds__(kThreads) w4_quantize_kernel(const T* __restri
   const int blocks = w4_blocks(k);
   const int spans = ceil_div(blocks, kSpanBlocks);
   const int rt = blockIdx.x / spans, span = blockIdx.x % spans;
-  const int lane = threadIdx.x & 31, word = lane & 15, r = threadIdx.x >> 4;
+  const int lane = threadIdx.x & 31, word = (lane & 7) * 2, r = threadIdx.x >> 4;
   const int row = rt * kW4Rows + r;
-  const int first = span * (kSpanBlocks * kW4Block) + word * 8;
-  __align__(16) T v[kSpanBlocks][8];
+  const int first = span * kSpan + (lane & 15) * kLaneInputs;
+  __align__(16) T v[kTurns][kLaneInputs];
   load_words<T>(w + (row < n ? row : 0) * ldw, first, row < n ? k : 0, wide, v, lane);
 #pragma unroll
-  for (int b = 0; b < kSpanBlocks; ++b) {
+  for (int b = 0; b < kTurns; ++b) {
     // The largest value above zero and the largest magnitude below it (SYM: the largest magnitude), which travel as
     // one pair; NaN stays NaN.
     typedef typename Half<T>::two T2;
     const T2* pair = reinterpret_cast<const T2*>(v[b]);
     T2 top = SYM ? __habs2(pair[0]) : pair[0], low = pair[0];
 #pragma unroll
-    for (int i = 1; i < 4; ++i) {
+    for (int i = 1; i < kLaneInputs / 2; ++i) {
       top = __hmax2_nan(top, SYM ? __habs2(pair[i]) : pair[i]);
       if (!SYM) low = __hmin2_nan(low, pair[i]);
     }
@@ -109,7 +111,7 @@ __global__ void __launch_bounds__(kThreads) w4_quantize_kernel(const T* __restri
       most = max2<T>(max2<T>(__byte_perm(most, below, 0x5410), __byte_perm(most, below, 0x7632)), 0u);
     }
 #pragma unroll
-    for (int i = G / 16; i >= 1; i >>= 1) most = max2<T>(most, __shfl_xor_sync(0xffffffffu, most, i));
+    for (int i = G / kLaneInputs / 2; i >= 1; i >>= 1) most = max2<T>(most, __shfl_xor_sync(0xffffffffu, most, i));
     most &= 0x7fff7fffu;  // no zero keeps a sign
     const T2 ends = *reinterpret_cast<const T2*>(&most);
     const float hi = to_f32(low_of(ends)), lo = to_f32(high_of(ends));
@@ -119,7 +121,7 @@ __global__ void __launch_bounds__(kThreads) w4_quantize_kernel(const T* __restri
     const T s16 = from_f32<T>(SYM ? range * (1.f / 7.f) : __fdiv_rn(range, 15.f));
     const float s = to_f32(s16);
     int z = SYM ? 8 : 0;
-    uint32_t packed = z * 0x11111111u;
+    uint32_t packed[2] = {z * 0x11111111u, z * 0x11111111u};
     // rint(x / s) without a division.  x and s have 11 significant bits at most, so that a quotient up to 2^5 that is
     // not halfway between two whole numbers is at least 2^-13 away from that; the product with the reciprocal is off by
     // 2^-17 at most.  Adding it to 768 leaves multiples of 2^-14: a quotient that is halfway becomes exactly so, and no
@@ -134,12 +136,12 @@ __global__ void __launch_bounds__(kThreads) w4_quantize_kernel(const T* __restri
       const float inv = __fdividef(1.f, s);
       if (!SYM) z = whole(lo, inv) - kWhole;
       const int least = kWhole - z;  // code 0
-      packed = 0u - static_cast<uint32_t>(least) * 0x11111111u;
+      packed[0] = packed[1] = 0u - static_cast<uint32_t>(least) * 0x11111111u;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < kLaneInputs; ++i) {
         int c = whole(to_f32(v[b][i]), inv);
         if (!SYM) c = min(c, least + 15);
-        packed += static_cast<uint32_t>(c) << (4 * w4_nibble(i));
+        packed[i / 8] += static_cast<uint32_t>(c) << (4 * w4_nibble(i % 8));
       }
     } else if (s > 0.f && s < INFINITY) {
       // Scales that may have lost bits when they were rounded (subnormal ones), or whose reciprocal is not a normal number:
@@ -147,13 +149,15 @@ __global__ void __launch_bounds__(kThreads) w4_quantize_kernel(const T* __restri
       const float shift = s < 0x1p-100f ? 0x1p64f : s > 0x1p100f ? 0x1p-64f : 1.f;
       const float inv = __fdividef(1.f, s * shift);
       if (!SYM) z = min(whole(lo * shift, inv) - kWhole, 15);
-      packed = 0;
+      packed[0] = packed[1] = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        packed += static_cast<uint32_t>(min(max(whole(to_f32(v[b][i]) * shift, inv) - (kWhole - z), 0), 15)) << (4 * w4_nibble(i));
+      for (int i = 0; i < kLaneInputs; ++i)
+        packed[i / 8] += static_cast<uint32_t>(min(max(whole(to_f32(v[b][i]) * shift, inv) - (kWhole - z), 0), 15)) << (4 * w4_nibble(i % 8));
     }
-    *reinterpret_cast<uint32_t*>(tile + b * kW4TileBytes + word_offset(r, word)) = packed;
-    const int block = span * kSpanBlocks + b;
+    const int of_span = b * (kTurn / kW4Block) + ((lane >> 3) & 1), block = span * kSpanBlocks + of_span;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      *reinterpret_cast<uint32_t*>(tile + of_span * kW4TileBytes + word_offset(r, word + i)) = packed[i];
     if (word % (G / 8) == 0 && block < blocks) {
       const long long at = ((static_cast<long long>(rt) * blocks + block) * kW4Rows + r) * (kW4Block / G) + word / (G / 8);
       scales[at] = s16;
@@ -200,7 +204,6 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) w4_dequantize_kernel(const uint8_t* __restrict__ codes, const T* __restrict__ scales,
                                                                  const uint8_t* __restrict__ zeros, int n, int k, int G,
                                                                  T* __restrict__ out, long long ldo) {
-  constexpr int kSpan = kSpanBlocks * kW4Block;
   __shared__ __align__(16) T rows[kW4Rows][kSpan + 8];
   const int blocks = w4_blocks(k);
   const int spans = ceil_div(blocks, kSpanBlocks);

@@ -240,7 +240,7 @@ def gemm_w4(x: torch.Tensor, w: WeightsW4, out: Optional[torch.Tensor] = None, w
     if x.device != w.device:
         raise ValueError(f"operands are on different devices: {x.device} and {w.device}")
     if out is None:
-        out = torch.empty((m, w.n), dtype=w.dtype, device=w.device)
+        out = x.new_empty((m, w.n))   # (the type and device of the weights)
     else:
         _output("out", out, (m, w.n), w.dtype, w.device)
     ldx, x_ptr = _ld(x), x.data_ptr()
