@@ -255,7 +255,7 @@ int rows_product_any(const void* x, long long ldx, const W4& w, void* y, long lo
 }
 
 // Up to here, the columns of one warp instruction, the codes are multiplied as they are (w4_rows.cuh); more rows go to
-// tcgen05.mma (w4_decode.cuh).  8192 x 8192: 1 row 11.9 us, the other kernel 16.2; 8 rows 13.1 and 16.4; 9 rows 16.7.
+// tcgen05.mma (w4_decode.cuh).  8192 x 8192: 1 row 11.6 us, the other kernel 16.1; 8 rows 12.7 and 16.5; 9 rows 16.6.
 constexpr int kFewRows = 8;
 
 int check(const W4& w) {

@@ -5,7 +5,7 @@
 // weights go where tcgen05.mma takes them from without another pass through shared memory: a thread expands a row of
 // 128 inputs in its registers and writes it to its lane of tensor memory, which is the left operand (128 rows x 16 inputs
 // an instruction); x, the right operand, comes to shared memory by TMA.  What a batch costs is then almost independent of its
-// rows: 8192 x 8192, groups of 128: 16 rows 17.0 us, 64 rows 19.4 (the bytes: 5.3 us; 2.0 TB/s).
+// rows: 8192 x 8192, groups of 128: 9 rows 16.6 us, 16 rows 17.0, 32 rows 17.7, 64 rows 19.4 (the bytes: 5.3 us; 2.0 TB/s).
 //
 // Bound.  Neither memory nor the tensor cores (6 % busy) nor one pipe: the integer pipe is active for 37 % of the cycles, issue for
 // half, and the warps wait on one another (load, expand, store to tensor memory, hand over).  About 15 instructions for
