@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) w4_decode_kernel(const __gr
     }
     // No CTA leaves while others read its memory.  Nothing but those reads has to be over, and their values have been used;
     // an arrival that releases would wait for the stores to y.
-    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.arrive.relaxed;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
   }
   __syncthreads();
   if (*abort_flag) {
