@@ -281,26 +281,44 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) w4_decode_kernel(const __gr
   }
   if (ranks > 1) {
     cluster.sync();
-    // four neighbouring rows for each thread, all CTAs' parts asked for before the first is added
-    for (int e = rank * kDecodeThreads + threadIdx.x; e < p.m * (kDecodeRows / 4); e += ranks * kDecodeThreads) {
+    // Four neighbouring rows for each thread, all CTAs' parts asked for before the first is added.  Rows behind the weights are
+    // not fetched.
+    constexpr int kJoins = (kDecodeMaxRight * (kDecodeRows / 4) + 2 * kDecodeThreads - 1) / (2 * kDecodeThreads);
+    float4 sum[kJoins];
+    auto place = [&](int i, int& row, int& col) -> bool {  // of the thread's i-th four values
+      const int e = (i * ranks + rank) * kDecodeThreads + static_cast<int>(threadIdx.x);
+      row = row0 + e % (kDecodeRows / 4) * 4;
+      col = e / (kDecodeRows / 4);
+      return col < p.m && row < p.n;
+    };
+#pragma unroll
+    for (int i = 0; i < kJoins; ++i) {
+      int row, col;
+      if (!place(i, row, col)) continue;
+      const float* at = part + col * kDecodeRows + (row - row0);
       float4 v[kDecodeMaxRanks];
 #pragma unroll
       for (int c = 0; c < kDecodeMaxRanks; ++c)
-        if (c < ranks) v[c] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(part + 4 * e, c));
-      float4 s = v[0];
+        if (c < ranks) v[c] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(at, c));
+      sum[i] = v[0];
 #pragma unroll
       for (int c = 1; c < kDecodeMaxRanks; ++c)
-        if (c < ranks) { s.x += v[c].x; s.y += v[c].y; s.z += v[c].z; s.w += v[c].w; }
-      const int row = row0 + e % (kDecodeRows / 4) * 4;
-      T* to = static_cast<T*>(p.y) + (e / (kDecodeRows / 4)) * p.ldy + row;
-      const T four[4] = {from_f32<T>(s.x), from_f32<T>(s.y), from_f32<T>(s.z), from_f32<T>(s.w)};
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (row + i < p.n) to[i] = four[i];
+        if (c < ranks) { sum[i].x += v[c].x; sum[i].y += v[c].y; sum[i].z += v[c].z; sum[i].w += v[c].w; }
     }
-    // No CTA leaves while others read its memory.  Nothing but those reads has to be over, and their values have been used;
-    // an arrival that releases would wait for the stores to y.
-    asm volatile("barrier.cluster.arrive.relaxed;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+    // No CTA leaves while others read its memory: the arrival releases, so that this thread's reads are over before any CTA gets
+    // past the wait.  The stores to y come after it, so that it does not wait for them.
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < kJoins; ++i) {
+      int row, col;
+      if (!place(i, row, col)) continue;
+      T* to = static_cast<T*>(p.y) + col * p.ldy + row;
+      const T four[4] = {from_f32<T>(sum[i].x), from_f32<T>(sum[i].y), from_f32<T>(sum[i].z), from_f32<T>(sum[i].w)};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (row + j < p.n) to[j] = four[j];
+    }
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
   }
   __syncthreads();
   if (*abort_flag) {

@@ -774,3 +774,25 @@ def test_status_and_workspace_sizes(cuda_device):
         check_grad(dw, values_of(saved), dy, None)
         with pytest.raises(lowbit.KernelError):
             lowbit.weight_grad8(saved, dy, workspace=lowbit.WorkspaceW4(1, w))
+
+
+@pytest.mark.parametrize("m", [9, 16, 33, 64])
+@pytest.mark.parametrize("n,k,group", [(1, 1100, 64), (3, 2048, 128), (125, 1030, 32), (130, 2048, 64), (515, 4096, 128), (4097, 512, 32)])
+def test_gemm_w4_last_outputs_of_a_cluster(cuda_device, m, n, k, group):
+    """CTAs that divide the inputs of 128 outputs, the last of which are not there: results equal those of the same weights
+    with whole 128 outputs, which run in the same clusters, and what lies beside the result stays."""
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    full = randn((-(-n // 128) * 128, k), torch.bfloat16, cuda_device, 81, k ** -0.5)
+    x = randn((m, k), torch.bfloat16, cuda_device, 82)
+    want = lowbit.gemm_w4(x, lowbit.quantize_w4(full, group=group), check=True)
+    w = lowbit.quantize_w4(full[:n], group=group)
+    room = torch.full((m + 2, n + 3), 7.0, dtype=torch.bfloat16, device=cuda_device)
+    for _ in range(5):
+        room[1:1 + m, 1:1 + n] = 0
+        lowbit.gemm_w4(x, w, out=room[1:1 + m, 1:1 + n], check=True)
+        assert torch.equal(room[1:1 + m, 1:1 + n], want[:, :n])
+    room[1:1 + m, 1:1 + n] = 7
+    assert bool((room == 7).all())
