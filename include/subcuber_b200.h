@@ -174,7 +174,8 @@ typedef struct sb200_gemm_options {
   int wait_limit_us;    /* bound of every device-side wait in microseconds; 0 = 2 s */
   int drop_split_flags; /* test aid for the give-up path: the first K-halves of split tiles do not publish their flags,
                            the second halves' waits run out after wait_limit_us and the status word reads
-                           SB200_STATUS_SPLIT_TIMEOUT; the output of such a call is incomplete */
+                           SB200_STATUS_SPLIT_TIMEOUT; the output of such a call is incomplete.  Products with an operand in
+                           few bits: its tiles are not announced, and the first role to give up leaves its code */
 } sb200_gemm_options;
 size_t sb200_gemm_workspace_bytes_opt(const char* kernel, int m, int n, int k, const sb200_gemm_options* options);
 int sb200_gemm_opt(const char* kernel, const void* a, const void* b, void* d, int m, int n, int k, void* workspace,
@@ -320,6 +321,10 @@ int sb200_w4_dequantize(int dtype, const void* codes, const void* scales, const 
 size_t sb200_w4_gemm_workspace_bytes(int dtype, int m, int n, int k, int group, int x_aligned);
 int sb200_w4_gemm(int dtype, const void* x, long long ldx, const void* codes, const void* scales, const void* zeros, void* y,
                   long long ldy, int m, int n, int k, int group, void* workspace, size_t workspace_bytes, sb200_stream_t stream);
+/* The same with options (NULL: none); of those wait_limit_us and drop_split_flags are supported, the others must be 0. */
+int sb200_w4_gemm_opt(int dtype, const void* x, long long ldx, const void* codes, const void* scales, const void* zeros, void* y,
+                      long long ldy, int m, int n, int k, int group, void* workspace, size_t workspace_bytes,
+                      sb200_stream_t stream, const sb200_gemm_options* options);
 
 /* Activations in 8 bits, m tokens x k channels, a power-of-two step for each 32 channels of a token:
  *     X[m][k] = +-magnitude * 2^(exponent[m][k / 32] - 127),   bit 7 of the byte = sign, bits 0-6 = magnitude
@@ -340,6 +345,11 @@ size_t sb200_act8_wgrad_workspace_bytes(int dtype, int out_dtype, int m, int n, 
 int sb200_act8_wgrad(int dtype, const void* codes, long long pitch, const void* exponents, long long exp_pitch, const void* dy,
                      long long lddy, int out_dtype, const void* base, long long ldbase, void* dw, long long lddw, int m, int n,
                      int k, void* workspace, size_t workspace_bytes, sb200_stream_t stream);
+/* The same with options, as sb200_w4_gemm_opt. */
+int sb200_act8_wgrad_opt(int dtype, const void* codes, long long pitch, const void* exponents, long long exp_pitch,
+                         const void* dy, long long lddy, int out_dtype, const void* base, long long ldbase, void* dw,
+                         long long lddw, int m, int n, int k, void* workspace, size_t workspace_bytes, sb200_stream_t stream,
+                         const sb200_gemm_options* options);
 
 /* Seeded synthetic inputs, bit-identical on host and device for dist 0 and 2 (dist 1 uses libm / device
  * math and agrees to rounding).  dtype: 0 f16, 1 f32, 2 f64, 3 bf16.  dist: 0 uniform[-1,1), 1 normal(0,1),

@@ -112,10 +112,12 @@ def load(build_if_missing: bool = True) -> C.CDLL:
             ("sb200_w4_dequantize", i, [i, p, p, p, i, i, i, p, ll, p]),
             ("sb200_w4_gemm_workspace_bytes", z, [i, i, i, i, i, i]),
             ("sb200_w4_gemm", i, [i, p, ll, p, p, p, p, ll, i, i, i, i, p, z, p]),
+            ("sb200_w4_gemm_opt", i, [i, p, ll, p, p, p, p, ll, i, i, i, i, p, z, p, C.POINTER(GemmOptions)]),
             ("sb200_act8_save", i, [i, p, ll, i, i, p, ll, p, ll, p]),
             ("sb200_act8_restore", i, [i, p, ll, p, ll, i, i, p, ll, p]),
             ("sb200_act8_wgrad_workspace_bytes", z, [i, i, i, i, i, i]),
-            ("sb200_act8_wgrad", i, [i, p, ll, p, ll, p, ll, i, p, ll, p, ll, i, i, i, p, z, p])):
+            ("sb200_act8_wgrad", i, [i, p, ll, p, ll, p, ll, i, p, ll, p, ll, i, i, i, p, z, p]),
+            ("sb200_act8_wgrad_opt", i, [i, p, ll, p, ll, p, ll, i, p, ll, p, ll, i, i, i, p, z, p, C.POINTER(GemmOptions)])):
         fn = getattr(lib, name)
         fn.restype, fn.argtypes = res, args
     _lib = lib

@@ -234,12 +234,14 @@ extern "C" size_t sb200_act8_wgrad_workspace_bytes(int dtype, int out_dtype, int
   return sb200::lowbit::expand_act8_workspace(m, n, k, dy_aligned != 0);
 }
 
-extern "C" int sb200_act8_wgrad(int dtype, const void* codes, long long pitch, const void* exponents, long long exp_pitch,
-                                const void* dy, long long lddy, int out_dtype, const void* base, long long ldbase, void* dw,
-                                long long lddw, int m, int n, int k, void* workspace, size_t workspace_bytes,
-                                sb200_stream_t stream) {
+extern "C" int sb200_act8_wgrad_opt(int dtype, const void* codes, long long pitch, const void* exponents, long long exp_pitch,
+                                    const void* dy, long long lddy, int out_dtype, const void* base, long long ldbase, void* dw,
+                                    long long lddw, int m, int n, int k, void* workspace, size_t workspace_bytes,
+                                    sb200_stream_t stream, const sb200_gemm_options* options) {
   const Act8 a{static_cast<sb200::DType>(dtype), m, k, codes, pitch, exponents, exp_pitch};
+  sb200::lowbit::Waits waits;
   if (int rc = sb200::lowbit::check(a)) return rc;
+  if (int rc = sb200::lowbit::waits_of(options, &waits)) return rc;
   if ((out_dtype != sb200::kF32 && out_dtype != dtype) || n > sb200::lowbit::kMaxExtent) return SB200_ERR_NOT_SUPPORTED;
   if (n <= 0 || !dw || lddw < n || lddy < n || (m > 0 && !dy) || (base && ldbase < n)) return SB200_ERR_INVALID_PROBLEM;
   const uintptr_t width = out_dtype == sb200::kF32 ? 4 : 2;
@@ -248,6 +250,14 @@ extern "C" int sb200_act8_wgrad(int dtype, const void* codes, long long pitch, c
   if (!workspace || workspace_bytes < sb200_act8_wgrad_workspace_bytes(dtype, out_dtype, m, n, k, sb200::lowbit::tma_rows(dy, lddy)) ||
       !sb200::lowbit::aligned(workspace, 256))
     return SB200_ERR_WORKSPACE_NULL;
-  return sb200::lowbit::expand_act8(a, dy, lddy, out_dtype == sb200::kF32, base, ldbase, dw, lddw, n, workspace,
+  return sb200::lowbit::expand_act8(a, dy, lddy, out_dtype == sb200::kF32, base, ldbase, dw, lddw, n, workspace, waits,
                                     reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int sb200_act8_wgrad(int dtype, const void* codes, long long pitch, const void* exponents, long long exp_pitch,
+                                const void* dy, long long lddy, int out_dtype, const void* base, long long ldbase, void* dw,
+                                long long lddw, int m, int n, int k, void* workspace, size_t workspace_bytes,
+                                sb200_stream_t stream) {
+  return sb200_act8_wgrad_opt(dtype, codes, pitch, exponents, exp_pitch, dy, lddy, out_dtype, base, ldbase, dw, lddw, m, n, k,
+                              workspace, workspace_bytes, stream, nullptr);
 }

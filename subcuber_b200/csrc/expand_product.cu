@@ -136,8 +136,6 @@ bool dense_w4(int m) { return m >= kDenseColumns; }
 bool dense_act8(int n) { return n >= kDenseColumns; }
 size_t dense_bytes(long long rows, long long ld) { return align_up(size_t(rows) * ld * 2, 256); }
 
-constexpr unsigned long long kWaitNs = 2000000000ull;  // bound of every device-side wait
-
 }  // namespace
 
 size_t expand_w4_workspace(int m, int n, int k, bool x_aligned) {
@@ -146,7 +144,7 @@ size_t expand_w4_workspace(int m, int n, int k, bool x_aligned) {
 }
 
 int expand_w4(const W4& w, const void* x, long long ldx, void* y, long long ldy, int m, void* workspace, size_t workspace_bytes,
-              cudaStream_t stream) {
+              const Waits& waits, cudaStream_t stream) {
   ExpandParams p = {};
   p.scales = w.scales;
   p.zeros = static_cast<const uint8_t*>(w.zeros);
@@ -156,7 +154,7 @@ int expand_w4(const W4& w, const void* x, long long ldx, void* y, long long ldy,
   p.steps = dense_w4(m) ? ceil_div(w.k, kStep) : 2 * w4_blocks(w.k);
   p.out = y;
   p.ldo = ldy;
-  p.wait_ns = kWaitNs;
+  p.waits = waits;
   p.status = static_cast<int*>(workspace);
   const bool dense = dense_w4(m);
   char* part = static_cast<char*>(workspace) + (workspace_bytes - part_bytes(m, w.n)) / 256 * 256;
@@ -232,7 +230,8 @@ int run_decode(const DecodeParams& p, int group, cudaStream_t stream) {
 
 }  // namespace
 
-int decode_w4(const W4& w, const void* x, long long ldx, void* y, long long ldy, int m, void* status, cudaStream_t stream) {
+int decode_w4(const W4& w, const void* x, long long ldx, void* y, long long ldy, int m, void* status, const Waits& waits,
+              cudaStream_t stream) {
   DecodeParams p = {};
   p.codes = static_cast<const uint8_t*>(w.codes);
   p.scales = static_cast<const uint8_t*>(w.scales);
@@ -244,7 +243,7 @@ int decode_w4(const W4& w, const void* x, long long ldx, void* y, long long ldy,
   p.blocks = w4_blocks(w.k);
   p.n16 = ceil_div(m, 16) * 16;
   p.status = static_cast<int*>(status);
-  p.wait_ns = kWaitNs;
+  p.waits = waits;
   if (int rc = tc::map_rows_16bit(&p.right, x, m, w.k, ldx, p.n16)) return rc;
   return w.dtype == kF16 ? run_decode<__half>(p, w.group, stream) : run_decode<__nv_bfloat16>(p, w.group, stream);
 }
@@ -254,7 +253,7 @@ size_t expand_act8_workspace(int m, int n, int k, bool dy_aligned) {
 }
 
 int expand_act8(const Act8& a, const void* dy, long long lddy, bool out_f32, const void* base, long long ldbase, void* dw,
-                long long lddw, int n, void* workspace, cudaStream_t stream) {
+                long long lddw, int n, void* workspace, const Waits& waits, cudaStream_t stream) {
   ExpandParams p = {};
   p.exps = static_cast<const uint8_t*>(a.exps);
   p.exp_pitch = static_cast<int>(a.exp_pitch);
@@ -267,7 +266,7 @@ int expand_act8(const Act8& a, const void* dy, long long lddy, bool out_f32, con
   p.base = base;
   p.ldbase = ldbase;
   p.out_f32 = out_f32;
-  p.wait_ns = kWaitNs;
+  p.waits = waits;
   char* ws = static_cast<char*>(workspace);
   p.status = reinterpret_cast<int*>(ws);
   ws += kStatusBytes;

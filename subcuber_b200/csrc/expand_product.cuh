@@ -31,6 +31,7 @@
 #include <cuda.h>
 
 #include "lowbit_format.cuh"
+#include "lowbit_host.h"
 #include "ptx.cuh"
 
 namespace sb200 {
@@ -60,7 +61,7 @@ struct ExpandParams {
   int out_f32;
   float* part;              // [slices][the result's shape, packed]
   int* status;
-  unsigned long long wait_ns;
+  Waits waits;
 };
 
 constexpr int kPairRows = 256, kCtaRows = 128, kStep = 64, kMaxCols = 256;
@@ -324,7 +325,7 @@ expand_product_kernel(const __grid_constant__ ExpandParams p) {
           const bool mine = turn == 0;
           turn = mine ? kProducers - 1 : turn - 1;
           if (mine && !DENSE) {
-            if (!ptx::mbar_wait_warp<false>(&raw_empty[rstage], rphase ^ 1u, abort_flag, p.wait_ns)) {
+            if (!ptx::mbar_wait_warp<false>(&raw_empty[rstage], rphase ^ 1u, abort_flag, p.waits.ns)) {
               if (lane == 0) give_up(p, abort_flag, 101);
               ok = false;
               break;
@@ -353,12 +354,12 @@ expand_product_kernel(const __grid_constant__ ExpandParams p) {
 #pragma unroll
           for (int h = 0; h < kEach; ++h) {
             if (mine) {
-              if (!ptx::mbar_wait_warp<false>(&empty_bar[stage], phase ^ 1u, abort_flag, p.wait_ns)) {
+              if (!ptx::mbar_wait_warp<false>(&empty_bar[stage], phase ^ 1u, abort_flag, p.waits.ns)) {
                 if (lane == 0) give_up(p, abort_flag, 101);
                 ok = false;
                 break;
               }
-              if (ptx::elect_one()) {
+              if (!(DENSE && p.waits.drop) && ptx::elect_one()) {
                 if (rank == 0) ptx::mbar_arrive_expect_tx(&full_bar[stage], bytes);
                 uint8_t* to = smem + stage * kStageBytes + kLeftBytes;
                 if (DENSE) {
@@ -396,7 +397,7 @@ expand_product_kernel(const __grid_constant__ ExpandParams p) {
         int sub = 0;
         for (int kk = w.k0; kk < w.k1; ++kk) {
           if (sub == 0) {
-            if (!ptx::mbar_wait_warp<false>(&slot_free[slot], ((free_bits >> slot) & 1u) ^ 1u, abort_flag, p.wait_ns)) {
+            if (!ptx::mbar_wait_warp<false>(&slot_free[slot], ((free_bits >> slot) & 1u) ^ 1u, abort_flag, p.waits.ns)) {
               if (lane == 0) give_up(p, abort_flag, 102);
               ok = false;
               break;
@@ -404,12 +405,12 @@ expand_product_kernel(const __grid_constant__ ExpandParams p) {
             free_bits ^= 1u << slot;
             ptx::tc_fence_after_sync();
           }
-          if (!ptx::mbar_wait_warp<false>(&full_bar[stage], phase, abort_flag, p.wait_ns)) {
+          if (!ptx::mbar_wait_warp<false>(&full_bar[stage], phase, abort_flag, p.waits.ns)) {
             if (lane == 0) give_up(p, abort_flag, 102);
             ok = false;
             break;
           }
-          if (!DENSE && !ptx::mbar_wait_warp<false>(&left_bar[stage], phase, abort_flag, p.wait_ns)) {
+          if (!DENSE && !ptx::mbar_wait_warp<false>(&left_bar[stage], phase, abort_flag, p.waits.ns)) {
             if (lane == 0) give_up(p, abort_flag, 102);
             ok = false;
             break;
@@ -438,7 +439,7 @@ expand_product_kernel(const __grid_constant__ ExpandParams p) {
       for (int u = pair; ok && u < units; u += pairs) {
         const ExpandUnit w = expand_unit(p, u);
         for (int kk = w.k0; kk < w.k1; ++kk) {
-          if (!ptx::mbar_wait_warp<false>(&left_bar[stage], phase, abort_flag, p.wait_ns)) {
+          if (!ptx::mbar_wait_warp<false>(&left_bar[stage], phase, abort_flag, p.waits.ns)) {
             if (lane == 0) give_up(p, abort_flag, 104);
             ok = false;
             break;
@@ -471,7 +472,7 @@ expand_product_kernel(const __grid_constant__ ExpandParams p) {
         else load_tile_rows(sum, static_cast<const T*>(p.base), p.ldbase, row0, col0, nrows, ncols, swap, lane);
       }
       for (int kk = w.k0; kk < w.k1; kk += kSubSteps) {
-        if (!ptx::mbar_wait_warp<false>(&slot_full[slot], (full_bits >> slot) & 1u, abort_flag, p.wait_ns)) {
+        if (!ptx::mbar_wait_warp<false>(&slot_full[slot], (full_bits >> slot) & 1u, abort_flag, p.waits.ns)) {
           if (lane == 0) give_up(p, abort_flag, 103);
           ok = false;
           break;
@@ -514,18 +515,18 @@ expand_product_kernel(const __grid_constant__ ExpandParams p) {
     auto next_stage = [&]() { if (++stage == kStages) { stage = 0; phase ^= 1u; } };
     auto next_raw = [&]() { if (++rstage == kRawStages) { rstage = 0; rphase ^= 1u; } };
     auto acquire = [&]() -> bool {  // the stage's previous contents have been read
-      if (ptx::mbar_wait_warp<false>(&empty_bar[stage], phase ^ 1u, abort_flag, p.wait_ns)) return true;
+      if (ptx::mbar_wait_warp<false>(&empty_bar[stage], phase ^ 1u, abort_flag, p.waits.ns)) return true;
       if (lane == 0) give_up(p, abort_flag, 104);
       return false;
     };
     auto publish = [&]() {
       ptx::fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(&left_bar[stage]);
+      if (lane == 0 && !p.waits.drop) ptx::mbar_arrive(&left_bar[stage]);
       next_stage();
     };
     auto raw_ready = [&]() -> bool {
-      if (ptx::mbar_wait_warp<false>(&raw_full[rstage], rphase, abort_flag, p.wait_ns)) return true;
+      if (ptx::mbar_wait_warp<false>(&raw_full[rstage], rphase, abort_flag, p.waits.ns)) return true;
       if (lane == 0) give_up(p, abort_flag, 104);
       return false;
     };

@@ -2,6 +2,7 @@
 #pragma once
 #include <stdint.h>
 
+#include "../../include/subcuber_b200.h"
 #include "sw_host.h"
 
 namespace sb200 {
@@ -33,6 +34,22 @@ inline bool tma_rows(const void* p, long long ld) { return aligned(p, 16) && ld 
 // Extents are held in 32 bits, rounded up to whole tiles too.
 constexpr int kMaxExtent = 0x7fffff00;
 
+// The device-side waits of a product: how long one lasts at most, and the test aid that makes them run out (left tiles are not
+// announced to the matrix instructions).
+struct Waits {
+  unsigned long long ns;
+  int drop;
+};
+// From a call's options (null: 2 s); only those that concern waits are supported.
+inline int waits_of(const sb200_gemm_options* o, Waits* w) {
+  *w = Waits{2000000000ull, 0};
+  if (!o) return kOk;
+  if (o->sm_limit != 0 || o->no_split != 0) return kErrNotSupported;
+  if (o->wait_limit_us > 0) w->ns = 1000ull * static_cast<unsigned long long>(o->wait_limit_us);
+  w->drop = o->drop_split_flags != 0;
+  return kOk;
+}
+
 // Bytes of a copy of a 16-bit matrix with rows that start on 16 bytes.
 inline size_t copy_bytes(long long rows, int cols) {
   const size_t row = (static_cast<size_t>(cols) + 7) / 8 * 16;
@@ -52,12 +69,13 @@ int restore_act8(const Act8& a, void* x, long long ldx, cudaStream_t stream);
 constexpr size_t kStatusBytes = 256;
 constexpr int kDecodeMaxRows = 64;
 size_t expand_w4_workspace(int m, int n, int k, bool x_aligned);
-int decode_w4(const W4& w, const void* x, long long ldx, void* y, long long ldy, int m, void* status, cudaStream_t stream);
-int expand_w4(const W4& w, const void* x, long long ldx, void* y, long long ldy, int m, void* workspace, size_t workspace_bytes,
+int decode_w4(const W4& w, const void* x, long long ldx, void* y, long long ldy, int m, void* status, const Waits& waits,
               cudaStream_t stream);
+int expand_w4(const W4& w, const void* x, long long ldx, void* y, long long ldy, int m, void* workspace, size_t workspace_bytes,
+              const Waits& waits, cudaStream_t stream);
 size_t expand_act8_workspace(int m, int n, int k, bool dy_aligned);
 int expand_act8(const Act8& a, const void* dy, long long lddy, bool out_f32, const void* base, long long ldbase, void* dw,
-                long long lddw, int n, void* workspace, cudaStream_t stream);
+                long long lddw, int n, void* workspace, const Waits& waits, cudaStream_t stream);
 
 }  // namespace lowbit
 }  // namespace sb200

@@ -371,12 +371,14 @@ extern "C" size_t sb200_w4_gemm_workspace_bytes(int dtype, int m, int n, int k, 
   return sb200::lowbit::expand_w4_workspace(m, n, k, x_aligned != 0);
 }
 
-extern "C" int sb200_w4_gemm(int dtype, const void* x, long long ldx, const void* codes, const void* scales,
-                             const void* zeros, void* y, long long ldy, int m, int n, int k, int group, void* workspace,
-                             size_t workspace_bytes, sb200_stream_t stream) {
+extern "C" int sb200_w4_gemm_opt(int dtype, const void* x, long long ldx, const void* codes, const void* scales,
+                                 const void* zeros, void* y, long long ldy, int m, int n, int k, int group, void* workspace,
+                                 size_t workspace_bytes, sb200_stream_t stream, const sb200_gemm_options* options) {
   using namespace sb200::lowbit;
   const W4 w{static_cast<sb200::DType>(dtype), n, k, group, codes, scales, zeros};
+  Waits waits;
   if (int rc = check(w)) return rc;
+  if (int rc = waits_of(options, &waits)) return rc;
   if (m < 0 || ldx < k || ldy < n) return SB200_ERR_INVALID_PROBLEM;
   if (m > kMaxExtent) return SB200_ERR_NOT_SUPPORTED;
   if (m == 0) return SB200_OK;
@@ -395,6 +397,13 @@ extern "C" int sb200_w4_gemm(int dtype, const void* x, long long ldx, const void
   if (m <= kFewRows)
     return dtype == sb200::kF16 ? rows_product_any<__half>(x, ldx, w, y, ldy, m, s)
                                 : rows_product_any<__nv_bfloat16>(x, ldx, w, y, ldy, m, s);
-  if (m <= kDecodeMaxRows) return decode_w4(w, x, ldx, y, ldy, m, workspace, s);
-  return expand_w4(w, x, ldx, y, ldy, m, workspace, workspace_bytes, s);
+  if (m <= kDecodeMaxRows) return decode_w4(w, x, ldx, y, ldy, m, workspace, waits, s);
+  return expand_w4(w, x, ldx, y, ldy, m, workspace, workspace_bytes, waits, s);
+}
+
+extern "C" int sb200_w4_gemm(int dtype, const void* x, long long ldx, const void* codes, const void* scales,
+                             const void* zeros, void* y, long long ldy, int m, int n, int k, int group, void* workspace,
+                             size_t workspace_bytes, sb200_stream_t stream) {
+  return sb200_w4_gemm_opt(dtype, x, ldx, codes, scales, zeros, y, ldy, m, n, k, group, workspace, workspace_bytes, stream,
+                           nullptr);
 }

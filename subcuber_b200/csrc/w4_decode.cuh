@@ -33,7 +33,7 @@ struct DecodeParams {
   int m, n, blocks;
   int n16;            // rows of x rounded up to 16
   int* status;
-  unsigned long long wait_ns;
+  Waits waits;
 };
 
 constexpr int kDecodeThreads = 320;  // warps 0 and 1: TMA and MMA, 2-9: converters
@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) w4_decode_kernel(const __gr
     if (lane == 0) ptx::prefetch_tmap(&p.right);
     uint32_t stage = 0, phase = 0;
     for (int b = b0; b < b1; ++b) {
-      if (!ptx::mbar_wait_warp<false>(&right_empty[stage], phase ^ 1u, abort_flag, p.wait_ns)) {
+      if (!ptx::mbar_wait_warp<false>(&right_empty[stage], phase ^ 1u, abort_flag, p.waits.ns)) {
         give_up_here(101);
         break;
       }
@@ -149,8 +149,8 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) w4_decode_kernel(const __gr
     uint32_t rs = 0, rphase = 0, ls = 0, lphase = 0;
     bool ok = true;
     for (int b = b0; b < b1; ++b) {
-      if (!ptx::mbar_wait_warp<false>(&right_full[rs], rphase, abort_flag, p.wait_ns) ||
-          !ptx::mbar_wait_warp<false>(&left_full[ls], lphase, abort_flag, p.wait_ns)) {
+      if (!ptx::mbar_wait_warp<false>(&right_full[rs], rphase, abort_flag, p.waits.ns) ||
+          !ptx::mbar_wait_warp<false>(&left_full[ls], lphase, abort_flag, p.waits.ns)) {
         give_up_here(102);
         ok = false;
         break;
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) w4_decode_kernel(const __gr
         const uint32_t z = p.zeros ? lds_u8(at + kW4TileBytes + kW4Rows * 2 * PER + r16 * PER + q) : 8u;
         bias[q] = Half<T>::magic + __byte_perm(z, 0, 0x4040);
       }
-      if (!ptx::mbar_wait_warp<false>(&left_empty[ls], lphase ^ 1u, abort_flag, p.wait_ns)) {
+      if (!ptx::mbar_wait_warp<false>(&left_empty[ls], lphase ^ 1u, abort_flag, p.waits.ns)) {
         give_up_here(104);
         break;
       }
@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) w4_decode_kernel(const __gr
       tmem_st_wait();
       ptx::tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(&left_full[ls]);
+      if (lane == 0 && !p.waits.drop) ptx::mbar_arrive(&left_full[ls]);
       ls += 2;
       if (ls >= kLeftStages) { ls -= kLeftStages; lphase ^= 1u; }
     }
@@ -259,10 +259,10 @@ __global__ void __launch_bounds__(kDecodeThreads, 2) w4_decode_kernel(const __gr
 
   // ---- the sums: row = lane of tensor memory, column = row of x
   __syncthreads();  // the rings are free (and every role is done, or has given up)
-  if (!*abort_flag && !ptx::mbar_wait_warp<false>(sums_full, 0, abort_flag, p.wait_ns)) give_up_here(103);
+  if (!ptx::mbar_wait_warp<false>(sums_full, 0, abort_flag, p.waits.ns)) give_up_here(103);
   float* part = reinterpret_cast<float*>(smem);  // [rows of x][128]
-  const bool whole = !*abort_flag;
   __syncthreads();
+  const bool whole = !*abort_flag;  // read where no warp writes it any more: the same for all threads of the CTA
   if (whole && b1 > b0 && warp >= 2) {  // two warps to a lane quarter, each takes eight of sixteen columns
     ptx::tc_fence_after_sync();
     const int quarter = warp & 3, row = row0 + quarter * 32 + lane;

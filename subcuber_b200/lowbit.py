@@ -18,6 +18,7 @@ are replayed at once) need one each.  The reference project has no counterpart.
 """
 from __future__ import annotations
 
+import ctypes as C
 from typing import Optional
 
 import torch
@@ -75,17 +76,17 @@ def _output(name: str, t: torch.Tensor, shape, dtype, device) -> None:
 _functions: dict = {}
 
 
-def _call(what: str, device: torch.device, *args) -> None:
-    """Call the library's `what` on the current stream of `device`, with `device` current."""
+def _call(what: str, device: torch.device, *args, behind=()) -> None:
+    """Call the library's `what` on the current stream of `device`, with `device` current (`behind`: what follows the stream)."""
     fn = _functions.get(what)
     if fn is None:
         fn = _functions[what] = getattr(_lib.load(), what)
     index = device.index
     if _current_device() == index:
-        rc = fn(*args, _raw_stream(index))
+        rc = fn(*args, _raw_stream(index), *behind)
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, _raw_stream(index))
+            rc = fn(*args, _raw_stream(index), *behind)
     if rc != 0:
         raise KernelError(what, rc)
 
@@ -230,9 +231,9 @@ class WorkspaceW4(_Workspace):
 
 
 def gemm_w4(x: torch.Tensor, w: WeightsW4, out: Optional[torch.Tensor] = None, workspace: Optional[WorkspaceW4] = None,
-            check: bool = False) -> torch.Tensor:
+            check: bool = False, opts=None) -> torch.Tensor:
     """x @ W^T (m x out_features) for x (m x in_features) of the weights' type; sums in fp32.  `out` must not overlap x.
-    `check` synchronises and raises if a device-side wait gave up."""
+    `check` synchronises and raises if a device-side wait gave up; `opts` (`runner.options`): the bound of those waits."""
     _matrix("x", x, (w.dtype,))
     m, k = x.shape
     if k != w.k:
@@ -251,7 +252,11 @@ def gemm_w4(x: torch.Tensor, w: WeightsW4, out: Optional[torch.Tensor] = None, w
     else:
         workspace = WorkspaceW4(m, w, x_ptr % 16 == 0 and ldx % 8 == 0)
         ptr, nbytes = workspace.ptr, workspace.nbytes
-    _call("sb200_w4_gemm", w.device, w._code, x_ptr, ldx, *w._ptrs, out.data_ptr(), _ld(out), m, w.n, k, w.group, ptr, nbytes)
+    args = (w._code, x_ptr, ldx, *w._ptrs, out.data_ptr(), _ld(out), m, w.n, k, w.group, ptr, nbytes)
+    if opts is None:
+        _call("sb200_w4_gemm", w.device, *args)
+    else:
+        _call("sb200_w4_gemm_opt", w.device, *args, behind=(C.byref(opts),))
     if check:
         torch.cuda.current_stream(w.device).synchronize()
         if m > 8:                            # (below, the kernel has no waits and leaves the word alone)
@@ -348,10 +353,10 @@ class WorkspaceGrad8(_Workspace):
 
 def weight_grad8(saved: Checkpoint8, dy: torch.Tensor, base: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
                  out_dtype: torch.dtype = torch.float32, workspace: Optional[WorkspaceGrad8] = None,
-                 check: bool = False) -> torch.Tensor:
+                 check: bool = False, opts=None) -> torch.Tensor:
     """base + X^T @ dy (in_features x out_features, the layout of `gemm`'s B) for the saved activations X and the output
     gradient dy (tokens x out_features) of the same type.  The result is fp32 or has dy's type; `base` and `out` have
-    the result's type, and may be the same tensor; `out` overlaps no other operand.  `check` synchronises and raises if a device-side wait gave up."""
+    the result's type, and may be the same tensor; `out` overlaps no other operand.  `check` and `opts` as in `gemm_w4`."""
     _matrix("dy", dy, (saved.dtype,))
     m, n = dy.shape
     if m != saved.m:
@@ -374,9 +379,12 @@ def weight_grad8(saved: Checkpoint8, dy: torch.Tensor, base: Optional[torch.Tens
     if workspace is None:
         workspace = WorkspaceGrad8(saved, n, out_dtype, dy_ptr % 16 == 0 and lddy % 8 == 0)
     ws_ptr, ws_bytes = workspace._for(saved.device)
-    _call("sb200_act8_wgrad", saved.device, saved._code, *saved._layout, dy_ptr, lddy, DTYPE_CODE[out_dtype],
-          base.data_ptr() if base is not None else None, _ld(base) if base is not None else n, out.data_ptr(), _ld(out), m, n,
-          saved.k, ws_ptr, ws_bytes)
+    args = (saved._code, *saved._layout, dy_ptr, lddy, DTYPE_CODE[out_dtype], base.data_ptr() if base is not None else None,
+            _ld(base) if base is not None else n, out.data_ptr(), _ld(out), m, n, saved.k, ws_ptr, ws_bytes)
+    if opts is None:
+        _call("sb200_act8_wgrad", saved.device, *args)
+    else:
+        _call("sb200_act8_wgrad_opt", saved.device, *args, behind=(C.byref(opts),))
     if check:
         workspace.check()
     return out

@@ -201,3 +201,15 @@ def test_python_products_refuse_operands_on_different_devices(monkeypatch):
         lowbit.gemm_w4(on(0, H, 4, 128), w, out=on(0, H, 4, 64), workspace=Room(0))
     with pytest.raises(ValueError):
         lowbit.WorkspaceGrad8(saved, 64, torch.bfloat16)
+
+
+@pytest.mark.parametrize("options,rc", [(dict(sm_limit=4), 5), (dict(no_split=1), 5), (dict(wait_limit_us=1000, drop_split_flags=1), 0), (None, 0)])
+def test_products_take_the_options_of_waits_only(lib, options, rc):
+    import ctypes as C
+
+    from subcuber_b200 import _lib
+
+    o = None if options is None else C.byref(_lib.GemmOptions(**options))
+    assert lib.sb200_w4_gemm_opt(0, P, 256, P, P, P, P, 64, 0, 64, 256, 128, P, WS, None, o) == rc       # no rows: nothing runs
+    got = lib.sb200_act8_wgrad_opt(0, P, 112, P, 4, P, 24, 1, None, 24, P, 24, 4, 24, 100, None, WS, None, o)
+    assert got == (rc or 6)                                                                              # no workspace

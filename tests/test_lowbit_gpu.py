@@ -796,3 +796,56 @@ def test_gemm_w4_last_outputs_of_a_cluster(cuda_device, m, n, k, group):
         assert torch.equal(room[1:1 + m, 1:1 + n], want[:, :n])
     room[1:1 + m, 1:1 + n] = 7
     assert bool((room == 7).all())
+
+
+@pytest.mark.parametrize("m,n,k", [(20, 300, 2048), (64, 128, 4096), (16, 19000, 256), (100, 300, 2048), (1300, 300, 512)])
+def test_gemm_w4_waits_that_run_out_are_reported(cuda_device, m, n, k):
+    """Tiles that are never announced: every role gives up within the (shortened) limit, the call says so, and the next call on
+    the same device is right.  One CTA and clusters, the products on the way and in two passes."""
+    import torch
+
+    from subcuber_b200 import lowbit, runner
+
+    w = lowbit.quantize_w4(randn((n, k), torch.float16, cuda_device, 83, k ** -0.5))
+    x = randn((m, k), torch.float16, cuda_device, 84)
+    want = lowbit.gemm_w4(x, w, check=True)
+    ws = lowbit.WorkspaceW4(m, w)
+    opts = runner.options(wait_limit_us=1000, drop_split_flags=True)
+    for kw in (dict(check=True), dict(check=True, workspace=ws)):
+        with pytest.raises(lowbit.KernelError) as exc:
+            lowbit.gemm_w4(x, w, opts=opts, **kw)
+        assert exc.value.code in (101, 102, 103, 104)
+    lowbit.gemm_w4(x, w, opts=opts, workspace=ws)
+    with pytest.raises(lowbit.KernelError):
+        ws.check()
+    assert torch.equal(lowbit.gemm_w4(x, w, workspace=ws, check=True, opts=runner.options(wait_limit_us=1000000)), want)
+    ws.check()
+
+
+@pytest.mark.parametrize("m,k,n", [(500, 300, 200), (64, 128, 256), (500, 300, 1300)])
+def test_weight_grad_waits_that_run_out_are_reported(cuda_device, m, k, n):
+    import torch
+
+    from subcuber_b200 import lowbit, runner
+
+    saved = lowbit.save8(randn((m, k), torch.bfloat16, cuda_device, 85))
+    dy = randn((m, n), torch.bfloat16, cuda_device, 86)
+    want = lowbit.weight_grad8(saved, dy, check=True)
+    opts = runner.options(wait_limit_us=1000, drop_split_flags=True)
+    with pytest.raises(lowbit.KernelError) as exc:
+        lowbit.weight_grad8(saved, dy, check=True, opts=opts)
+    assert exc.value.code in (101, 102, 103, 104)
+    assert torch.equal(lowbit.weight_grad8(saved, dy, check=True), want)
+
+
+def test_rows_without_waits_take_options(cuda_device):
+    import torch
+
+    from subcuber_b200 import lowbit, runner
+
+    w = lowbit.quantize_w4(randn((300, 512), torch.float16, cuda_device, 87, 0.05))
+    x = randn((3, 512), torch.float16, cuda_device, 88)
+    opts = runner.options(wait_limit_us=1000, drop_split_flags=True)
+    assert torch.equal(lowbit.gemm_w4(x, w, check=True, opts=opts), lowbit.gemm_w4(x, w))
+    with pytest.raises(lowbit.KernelError):
+        lowbit.gemm_w4(x, w, opts=runner.options(sm_limit=8))
