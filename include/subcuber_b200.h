@@ -298,7 +298,8 @@ int sb200_peer_wait(int* const* local_flags, int count, int value, unsigned wait
  * first: bytes 512 h + 16 (4 g + t) + 4 j of a tile hold the 32-bit word of output 8 h + g and inputs 32 j + 8 t + i, i = 0..7,
  * input i in nibble (i >> 1) + 4 (i & 1).  scales (in the 16-bit type `dtype`) and zeros (bytes), both 16-byte aligned,
  * hold sb200_w4_table_entries(n, k, group) entries: [tile of outputs][128 inputs][output of the tile][group of the 128 inputs].
- * Outputs are padded to 16 and inputs to 128; the scales of padding are 0. */
+ * Outputs are padded to 16 and inputs to 128; the scales of padding are 0, and inputs behind k in a group that has some before it
+ * have its zero point as their code. */
 size_t sb200_w4_codes_bytes(int n, int k);
 size_t sb200_w4_table_entries(int n, int k, int group);
 /* Quantise w (n x k, 16-bit), group by group.  zeros == NULL: scale = amax / 7, code = 8 + rint(w / scale).  Else, with

@@ -180,20 +180,22 @@ __global__ void __launch_bounds__(kThreads) w4_pack_kernel(const uint8_t* __rest
   const int rt = blockIdx.x / blocks, block = blockIdx.x % blocks;
   const int r = threadIdx.x >> 4, pair = threadIdx.x & 15;  // one word for each thread
   const int row = rt * kW4Rows + r;
+  const int k0 = block * kW4Block + pair * 8;
+  const long long group = k0 / G;
+  const bool real = row < n && group * G < k;
+  const uint32_t zero = z && real ? z[group * ldz + row] & 15u : 8u;
   uint32_t word = 0;
   for (int i = 0; i < 8; ++i) {
-    const int kk = block * kW4Block + pair * 8 + i;
-    uint32_t c = 8;
+    const int kk = k0 + i;
+    uint32_t c = zero;  // inputs behind k stand for 0: another code times a large scale would be infinite
     if (row < n && kk < k) c = q[row * ldq + kk] & 15u;
     word |= c << (4 * w4_nibble(i));
   }
   *reinterpret_cast<uint32_t*>(codes + (static_cast<long long>(rt) * blocks + block) * kW4TileBytes + word_offset(r, pair)) = word;
-  const int k0 = block * kW4Block + pair * 8;
   if (k0 % G == 0) {
-    const long long group = k0 / G, at = w4_table_at(row, k0 / G, blocks, G);
-    const bool real = row < n && k0 < k;
+    const long long at = w4_table_at(row, k0 / G, blocks, G);
     scales[at] = real ? s[group * lds + row] : 0;
-    if (z) zeros[at] = real ? z[group * ldz + row] & 15u : 0;
+    if (z) zeros[at] = real ? zero : 0;
   }
 }
 

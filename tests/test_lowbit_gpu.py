@@ -849,3 +849,24 @@ def test_rows_without_waits_take_options(cuda_device):
     assert torch.equal(lowbit.gemm_w4(x, w, check=True, opts=opts), lowbit.gemm_w4(x, w))
     with pytest.raises(lowbit.KernelError):
         lowbit.gemm_w4(x, w, opts=runner.options(sm_limit=8))
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("k", [5, 40, 131, 200])
+def test_inputs_behind_the_last_stand_for_zero(cuda_device, k, group):
+    """Codes and scales of another quantiser whose values are finite, but would not be with a code of 8 behind the last input."""
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    groups = -(-k // group)
+    q = torch.ones(20, k, dtype=torch.uint8, device=cuda_device)
+    scales = torch.full((groups, 20), 20000.0, dtype=torch.float16, device=cuda_device)
+    for zero in (0, 3, 15):
+        q.fill_(min(zero + 1, 15) if zero < 15 else 14)
+        zeros = torch.full((groups, 20), zero, dtype=torch.uint8, device=cuda_device)
+        w = lowbit.pack_w4(q, scales, zeros, group=group)
+        assert bool(torch.isfinite(lowbit.dequantize_w4(w)).all())
+        for m in (1, 9, 40, 100, 1300):
+            x = randn((m, k), torch.float16, cuda_device, 89, 2.0 ** -10)
+            check_w4_gemm(lowbit.gemm_w4(x, w), x, w, exact_weights=False)
