@@ -30,6 +30,7 @@ DTYPE_CODE = {torch.float16: 0, torch.float32: 1, torch.bfloat16: 3}
 HALF_TYPES = (torch.float16, torch.bfloat16)
 GROUPS = (32, 64, 128)
 ACT_BLOCK = 32   # channels of a token that share a step
+MAX_EXTENT = 0x7fffff00  # of any axis: the library holds extents, rounded up to whole tiles, in 32 bits (ctypes would cut more bits off)
 
 
 # handle of the current stream of a device (the public call builds a Stream object, which takes 2 us)
@@ -42,14 +43,21 @@ def _matrix(name: str, t: torch.Tensor, dtypes) -> None:
     if t.is_cuda and t.dtype in dtypes and t.dim() == 2:
         rows, cols = t.shape
         ld, step = t.stride()
-        if (step == 1 or cols <= 1) and (ld >= cols or rows <= 1):
+        if (step == 1 or cols <= 1) and (ld >= cols or rows <= 1) and rows <= MAX_EXTENT and cols <= MAX_EXTENT:
             return
+        _extent(f"{name}'s rows", rows)
+        _extent(f"{name}'s columns", cols)
         raise ValueError(f"{name} must have its rows in consecutive elements, rows that do not overlap")
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor: this backend has no CPU path")
     if t.dim() != 2:
         raise ValueError(f"{name} must be a matrix")
     raise ValueError(f"{name} must be one of {[str(d) for d in dtypes]}, not {t.dtype}")
+
+
+def _extent(name: str, count: int) -> None:
+    if not 0 <= count <= MAX_EXTENT:
+        raise ValueError(f"{name}: {count}, must be 0 to {MAX_EXTENT}")
 
 
 def _ld(t: torch.Tensor) -> int:
@@ -121,6 +129,8 @@ def _check_w4(n: int, k: int, group: int) -> None:
         raise ValueError(f"group must be one of {GROUPS}")
     if n <= 0 or k <= 0:
         raise ValueError("weights need at least one output and one input")
+    _extent("outputs", n)
+    _extent("inputs", k)
 
 
 class WeightsW4:
@@ -225,6 +235,7 @@ class WorkspaceW4(_Workspace):
     bytes (the default expects packed rows); else there is room for a copy of x."""
 
     def __init__(self, m: int, w: WeightsW4, aligned: Optional[bool] = None):
+        _extent("rows", m)
         aligned = w.k % 8 == 0 if aligned is None else aligned
         with torch.cuda.device(w.device):  # a product is cut for the device that will run it
             super().__init__(int(_lib.load().sb200_w4_gemm_workspace_bytes(w._code, m, w.n, w.k, w.group, int(aligned))), w.device)
@@ -345,6 +356,7 @@ class WorkspaceGrad8(_Workspace):
     def __init__(self, saved: Checkpoint8, n: int, out_dtype: torch.dtype = torch.float32, aligned: Optional[bool] = None):
         if out_dtype != torch.float32 and out_dtype != saved.dtype:
             raise ValueError(f"the gradient is float32 or {saved.dtype}")
+        _extent("output channels", n)
         aligned = n % 8 == 0 if aligned is None else aligned
         with torch.cuda.device(saved.device):
             super().__init__(int(_lib.load().sb200_act8_wgrad_workspace_bytes(saved._code, DTYPE_CODE[out_dtype], saved.m, n,

@@ -213,3 +213,42 @@ def test_products_take_the_options_of_waits_only(lib, options, rc):
     assert lib.sb200_w4_gemm_opt(0, P, 256, P, P, P, P, 64, 0, 64, 256, 128, P, WS, None, o) == rc       # no rows: nothing runs
     got = lib.sb200_act8_wgrad_opt(0, P, 112, P, 4, P, 24, 1, None, 24, P, 24, 4, 24, 100, None, WS, None, o)
     assert got == (rc or 6)                                                                              # no workspace
+
+
+def test_python_calls_refuse_extents_past_32_bits(monkeypatch):
+    """Counts that ctypes would cut to 32 bits (2^32 tokens to none, 2^32 + 5 to five) are refused, wherever they come from."""
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    def launched(*args):
+        raise AssertionError("the call reached the library")
+
+    monkeypatch.setattr(lowbit, "_call", launched)
+    monkeypatch.setattr(lowbit.WeightsW4, "_empty", launched)
+    monkeypatch.setattr(lowbit.Checkpoint8, "_empty", launched)
+    H, U, on = torch.float16, torch.uint8, _OnDevice
+    w = lowbit.WeightsW4.__new__(lowbit.WeightsW4)
+    w._set(64, 128, 128, H, torch.device("cuda", 0), P, P, None)
+    w._status_ptr = P
+    for many in (1 << 32, (1 << 32) + 5, (1 << 31) - 1):
+        saved = lowbit.Checkpoint8.__new__(lowbit.Checkpoint8)
+        saved._set(many, 128, H, torch.device("cuda", 0), P, 128, P, 4)
+        for call in (
+            lambda: lowbit.gemm_w4(on(0, H, many, 128), w, out=on(0, H, many, 64)),
+            lambda: lowbit.quantize_w4(on(0, H, many, 128)),
+            lambda: lowbit.quantize_w4(on(0, H, 16, many)),
+            lambda: lowbit.pack_w4(on(0, U, many, 128), on(0, H, 1, many)),
+            lambda: lowbit.save8(on(0, H, many, 128)),
+            lambda: lowbit.save8(on(0, H, 4, many)),
+            lambda: lowbit.save8(on(0, H, many, 128), out=saved),
+            lambda: lowbit.restore8(saved, out=on(0, H, many, 128)),
+            lambda: lowbit.weight_grad8(saved, on(0, H, many, 64)),
+            lambda: lowbit.WorkspaceW4(many, w),
+            lambda: lowbit.WorkspaceW4(-1, w),
+            lambda: lowbit.WorkspaceGrad8(saved, many),
+            lambda: lowbit.WeightsW4(on(0, U, 1, 1), on(0, H, 1, 1), None, many, 128, 128),
+            lambda: lowbit.WeightsW4(on(0, U, 1, 1), on(0, H, 1, 1), None, 16, many, 128),
+        ):
+            with pytest.raises(ValueError, match=str(many) + "|-1"):
+                call()
