@@ -113,6 +113,12 @@ def kernels(dtype: Optional[str] = None, level: Optional[int] = None, regex: Opt
     return out
 
 
+def _check_extents(*extents: int):
+    # the library holds extents in 32 bits; ctypes would cut more bits off
+    if not all(0 <= x < 1 << 31 for x in extents):
+        raise ValueError(f"extents must fit 31 bits: {' x '.join(map(str, extents))}")
+
+
 def _check_inputs(a: torch.Tensor, b: torch.Tensor):
     if not (a.is_cuda and b.is_cuda):
         raise ValueError("operands must be CUDA tensors: this backend has no CPU path")
@@ -122,6 +128,7 @@ def _check_inputs(a: torch.Tensor, b: torch.Tensor):
         raise ValueError("operands must be packed row-major")
     if a.dtype != b.dtype:
         raise ValueError("A and B must have the same dtype")
+    _check_extents(*a.shape, b.shape[1])
 
 
 def run_kernel(name: str, a: torch.Tensor, b: torch.Tensor, d: Optional[torch.Tensor] = None, warmup: int = 1,
@@ -165,6 +172,7 @@ class Workspace:
 
     def __init__(self, kernel: str, m: int, n: int, k: int, device, opts=None):
         lib = _lib.load()
+        _check_extents(m, n, k)
         rc = lib.sb200_gemm_can_implement(kernel.encode(), m, n, k)
         if rc != 0:
             raise KernelError(kernel, rc)
@@ -311,6 +319,7 @@ def gemm_host(kernel: str, a, b):
     b = np.ascontiguousarray(b)
     m, k = a.shape
     n = b.shape[1]
+    _check_extents(m, n, k)
     d = np.empty((m, n), dtype=a.dtype)
     rc = lib.sb200_gemm_host(kernel.encode(), a.ctypes.data_as(C.c_void_p), b.ctypes.data_as(C.c_void_p),
                              d.ctypes.data_as(C.c_void_p), m, n, k)

@@ -150,3 +150,37 @@ def test_cpu_only_call_fails_loudly():
     a = torch.zeros((128, 64), dtype=torch.float16)
     with pytest.raises(ValueError):
         runner.gemm("blackwell_f16_cubic_128x256", a, a.t().contiguous())
+
+
+@pytest.mark.parametrize("many", [1 << 32, (1 << 32) + 256, 1 << 31])
+def test_extents_past_32_bits_are_refused(many):
+    """ctypes would cut them: 2^32 rows to none, 2^32 + 256 to 256."""
+    import numpy as np
+    import torch
+
+    from subcuber_b200 import runner
+
+    class OnDevice:
+        is_cuda, dtype, device = True, torch.float16, torch.device("cuda", 0)
+
+        def __init__(self, *shape):
+            self.shape = shape
+
+        def dim(self):
+            return 2
+
+        def is_contiguous(self):
+            return True
+
+    kernel = "blackwell_f16_sw_interleaved_presum"
+    for call in (
+        lambda: runner.gemm(kernel, OnDevice(many, 256), OnDevice(256, 256)),
+        lambda: runner.gemm(kernel, OnDevice(256, 256), OnDevice(256, many)),
+        lambda: runner.gemm(kernel, OnDevice(256, many), OnDevice(many, 256)),
+        lambda: runner.run_kernel(kernel, OnDevice(many, 256), OnDevice(256, 256)),
+        lambda: runner.gemm_colmajor(kernel, OnDevice(256, many), OnDevice(256, 256), many, 256, 256),
+        lambda: runner.Workspace(kernel, many, 256, 256, "cuda:0"),
+        lambda: runner.gemm_host(kernel, np.broadcast_to(np.float16(0), (many, 0)), np.zeros((0, 8), np.float16)),
+    ):
+        with pytest.raises(ValueError, match=str(many)):
+            call()
