@@ -168,8 +168,8 @@ int expand_w4(const W4& w, const void* x, long long ldx, void* y, long long ldy,
     char* left = part - dense_bytes(w.n, ld);
     if ((rc = dequantize_w4(w, left, ld, stream))) return rc;
     if ((rc = tc::map_rows_16bit(&p.left, left, w.n, w.k, ld, kCtaRows))) return rc;
-  } else if ((rc = tc::map_rows_plain(&p.left, w.codes, 4, w4_row_tiles(w.n), 256ll * w4_blocks(w.k), 1024ll * w4_blocks(w.k),
-                                      8, 256))) {  // a row tile's codes are one row of words; a box is 128 inputs of eight row tiles
+  } else if ((rc = tc::map_rows_plain(&p.left, w.codes, 8, w4_row_tiles(w.n), 128ll * w4_blocks(w.k), 1024ll * w4_blocks(w.k),
+                                      8, 128))) {  // a row tile's codes are one row of words; a box is 128 inputs of eight row tiles
     return rc;
   }
   return w.dtype == kF16 ? run_w4<__half>(p, w.group, dense, pairs, stream)

@@ -40,7 +40,8 @@ namespace lowbit {
 enum ExpandKind { kExpandW4 = 0, kExpandAct8 = 1 };
 
 struct ExpandParams {
-  CUtensorMap left;         // codes: W4: 32-bit words, a row for each row tile; ACT8: bytes, a row for each token
+  CUtensorMap left;         // codes: W4: 64-bit words (one for each input, so that coordinates fit), a row for each row tile;
+                            // ACT8: bytes, a row for each token
                             // dense: the left operand in 16 bits, [row][input] (W4), [block of 64 channels][token][64] (ACT8)
   CUtensorMap right;        // x [tokens][inputs] (W4) or dY [tokens][columns] (ACT8)
   const void* scales;       // W4
@@ -332,7 +333,7 @@ expand_product_kernel(const __grid_constant__ ExpandParams p) {
             }
             if (ptx::elect_one()) {
               ptx::mbar_arrive_expect_tx(&raw_full[rstage], kRawBytes);
-              if (KIND == kExpandW4) ptx::tma_load_2d(raw + rstage * kRawBytes, &p.left, &raw_full[rstage], kk / 2 * 256, row0 / kW4Rows);
+              if (KIND == kExpandW4) ptx::tma_load_2d(raw + rstage * kRawBytes, &p.left, &raw_full[rstage], kk * kStep, row0 / kW4Rows);
               else ptx::tma_load_2d(raw + rstage * kRawBytes, &p.left, &raw_full[rstage], row0, kk * kStep);
             }
             __syncwarp();

@@ -101,7 +101,7 @@ int map_rows_16bit(void* map, const void* ptr, long long rows, long long cols, l
 // The same matrix (cols a multiple of 64) seen as [block of 64 columns][row][64]; boxes hold `box_rows` rows of `box_blocks`
 // blocks, block after block.
 int map_blocks_16bit(void* map, const void* ptr, long long rows, long long cols, long long ld, int box_rows, int box_blocks);
-// The same without a swizzle for elements of `esize` (1 or 4) bytes, rows `pitch` bytes apart, boxes of box_cols x box_rows.
+// The same without a swizzle for elements of `esize` (1 or 8) bytes, rows `pitch` bytes apart, boxes of box_cols x box_rows.
 int map_rows_plain(void* map, const void* ptr, int esize, long long rows, long long cols, long long pitch, int box_rows,
                    int box_cols);
 }  // namespace tc

@@ -870,3 +870,28 @@ def test_inputs_behind_the_last_stand_for_zero(cuda_device, k, group):
         for m in (1, 9, 40, 100, 1300):
             x = randn((m, k), torch.float16, cuda_device, 89, 2.0 ** -10)
             check_w4_gemm(lowbit.gemm_w4(x, w), x, w, exact_weights=False)
+
+
+def test_gemm_w4_more_inputs_than_half_of_31_bits(cuda_device):
+    """More than 2^30 inputs: what copies count in, and where the last inputs of 9 and 65 rows are found."""
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    k, n, last = (1 << 30) + 384, 16, 1000
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info(cuda_device)[0] < 165 << 30:
+        pytest.skip("needs 165 GB of free device memory")
+    tail = lowbit.quantize_w4(randn((n, 1024), torch.float16, cuda_device, 90, 0.05), group=128, symmetric=True)
+    codes = torch.full((n * k // 2,), 0x88, dtype=torch.uint8, device=cuda_device)          # zeros
+    scales = torch.ones(n * k // 128, dtype=torch.float16, device=cuda_device)
+    codes[-tail.codes.numel():] = tail.codes
+    scales[-tail.scales.numel():] = tail.scales
+    w = lowbit.WeightsW4(codes, scales, None, n, k, 128)
+    x = torch.zeros(65, k, dtype=torch.float16, device=cuda_device)
+    x[:, -last:] = randn((65, last), torch.float16, cuda_device, 91)
+    for m in (65, 9, 1):
+        y = lowbit.gemm_w4(x[:m], w, check=True)
+        check_w4_gemm(y, x[:m, -1024:], tail, exact_weights=False)
+    del x, codes, scales, w
+    torch.cuda.empty_cache()
