@@ -151,7 +151,7 @@ class WeightsW4:
         self._tensors = (codes, scales, zeros)
         self._set(n, k, group, scales.dtype, scales.device, codes.data_ptr(), scales.data_ptr(),
                   zeros.data_ptr() if zeros is not None else None)
-        # the status word of products that need no other workspace
+        # the status word of products that need no other workspace and are not checked
         self._own = torch.empty(512, dtype=torch.uint8, device=self.device)
         self._status_ptr = self._own.data_ptr() + (-self._own.data_ptr()) % 256
 
@@ -258,8 +258,8 @@ def gemm_w4(x: torch.Tensor, w: WeightsW4, out: Optional[torch.Tensor] = None, w
     ldx, x_ptr = _ld(x), x.data_ptr()
     if workspace is not None:
         ptr, nbytes = workspace._for(w.device)
-    elif m <= 64 and x_ptr % 16 == 0 and ldx % 8 == 0:
-        ptr, nbytes = w._status_ptr, 256     # the products of few rows need the status word only
+    elif m <= 64 and x_ptr % 16 == 0 and ldx % 8 == 0 and not check:
+        ptr, nbytes = w._status_ptr, 256     # few rows need a status word only; calls at once may share one that is not read
     else:
         workspace = WorkspaceW4(m, w, x_ptr % 16 == 0 and ldx % 8 == 0)
         ptr, nbytes = workspace.ptr, workspace.nbytes

@@ -252,3 +252,37 @@ def test_python_calls_refuse_extents_past_32_bits(monkeypatch):
         ):
             with pytest.raises(ValueError, match=str(many) + "|-1"):
                 call()
+
+
+def test_checked_products_have_a_status_word_of_their_own(monkeypatch):
+    """Two checked calls at once with the same weights: the second must not clear what the first will read."""
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    class Reached(Exception):
+        pass
+
+    words = []
+
+    def call(what, device, *args):
+        words.append(args[-2])
+        raise Reached
+
+    class Room:
+        nbytes = 256
+
+        def __init__(self, m, w, aligned):
+            self.ptr = P + 4096 * (1 + len(words))
+
+    monkeypatch.setattr(lowbit, "_call", call)
+    monkeypatch.setattr(lowbit, "WorkspaceW4", Room)
+    w = lowbit.WeightsW4.__new__(lowbit.WeightsW4)
+    w._set(64, 128, 128, torch.float16, torch.device("cuda", 0), P, P, None)
+    w._status_ptr = P
+    x, y = _OnDevice(0, torch.float16, 40, 128), _OnDevice(0, torch.float16, 40, 64)
+    for check in (True, True, False, False):
+        with pytest.raises(Reached):
+            lowbit.gemm_w4(x, w, out=y, check=check)
+    assert len(set(words[:2])) == 2 and P not in words[:2]
+    assert words[2:] == [P, P]       # not read by anyone
