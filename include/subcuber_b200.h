@@ -317,6 +317,8 @@ int sb200_w4_dequantize(int dtype, const void* codes, const void* scales, const 
                         long long ldo, sb200_stream_t stream);
 /* y[m][n] = sum over k of x[m][k] W[n][k], sums in fp32, rounded once to `dtype`.  Up to 8 rows the codes are multiplied
  * exactly and the scales applied in fp32; with more the weights are rounded to `dtype` first (as sb200_w4_dequantize does).
+ * Of 9 to 64 rows a tensor-core accumulator, which chops, takes up to 16384 inputs (k / 8 from 131072 inputs on), and every 16 of
+ * them may cost a few units of 2^-23 of the partial sum; of more rows it takes 512 inputs.
  * x_aligned: the rows of x start on 16 bytes (pointer and ldx); else the workspace holds a copy of x.  A workspace for m rows
  * serves every smaller m. */
 size_t sb200_w4_gemm_workspace_bytes(int dtype, int m, int n, int k, int group, int x_aligned);

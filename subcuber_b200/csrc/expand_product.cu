@@ -201,9 +201,10 @@ int launch_decode(const DecodeParams& p, cudaStream_t stream) {
   // 16384 x 512: 5.6, 7.1, 10.9, 10.8; 16384 x 4096: 18.0, 17.0, 20.4, 29.7.
   static std::atomic<int> room[kMaxDevices][kDecodeMaxRight / 16][4];  // clusters at once, plus one
   const int groups = ceil_div(p.n, kDecodeRows);
-  int dev = -1, log2 = 3;
+  int dev = -1, log2 = 3, least = 0;
+  while (least < 3 && p.blocks > (kDecodeBlocks << least)) ++least;
   if (cudaError_t e = cudaGetDevice(&dev)) return static_cast<int>(e);
-  for (; log2 > 0; --log2) {
+  for (; log2 > least; --log2) {
     const int ranks = 1 << log2;
     if (ranks > p.blocks || groups > 0x7fffffff / ranks) continue;
     attrs[0].val.clusterDim = {static_cast<unsigned>(ranks), 1, 1};

@@ -895,3 +895,28 @@ def test_gemm_w4_more_inputs_than_half_of_31_bits(cuda_device):
         check_w4_gemm(y, x[:m, -1024:], tail, exact_weights=False)
     del x, codes, scales, w
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("m", [9, 16, 64])
+def test_gemm_w4_long_sums_of_many_outputs(cuda_device, m):
+    """A large term first, its negative last, small ones between: an accumulator that chops loses about two units in the last place of
+    the large term with each addition (eight for 128 inputs).  It takes 16384 inputs, so that 1024 of the 8192 additions meet the
+    large term; with all of them the sum was off by 2.25."""
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    n, k = 149 * 128, 131072
+    q = torch.full((n, k), 9, dtype=torch.uint8, device=cuda_device)
+    w = lowbit.pack_w4(q, torch.ones(k // 128, n, dtype=torch.float16, device=cuda_device), group=128)    # ones
+    del q
+    g = torch.Generator(device=cuda_device)
+    g.manual_seed(92)
+    x = ((torch.rand(m, k, generator=g, device=cuda_device) + 1) * 2.0 ** -10).half()
+    want = x[:, 1:-1].double().sum(1, keepdim=True)
+    x[:, 0], x[:, -1] = 1024, -1024
+    y = lowbit.gemm_w4(x, w, check=True).double()
+    unit = 2.0 ** (10 - 23)                                    # of sums from 1024 to 2048
+    assert float(want.max()) < 1024
+    tol = 2 * 1024 * unit + 8192 * 2 * 2.0 ** -23 * 256 / 8 + 16 * unit + want * 2.0 ** -11   # large, small terms, join, rounding
+    assert bool(((y - want).abs() <= tol).all()), f"worst {float(((y - want).abs() / tol).max()):.2f} x"
