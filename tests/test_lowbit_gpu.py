@@ -920,3 +920,70 @@ def test_gemm_w4_long_sums_of_many_outputs(cuda_device, m):
     assert float(want.max()) < 1024
     tol = 2 * 1024 * unit + 8192 * 2 * 2.0 ** -23 * 256 / 8 + 16 * unit + want * 2.0 ** -11   # large, small terms, join, rounding
     assert bool(((y - want).abs() <= tol).all()), f"worst {float(((y - want).abs() / tol).max()):.2f} x"
+
+
+def _strict_bound(x, wv, k, dtype):
+    """The product with weights wv (64 bits), and how far a sum of exact products may be from it: the additions, and half a step of
+    the result.  Nothing for a rounding of the weights."""
+    import torch
+
+    xv = x.double()
+    want, size = xv @ wv.t(), xv.abs() @ wv.abs().t()
+    half = torch.finfo(dtype).eps / 2
+    sums = (2 * (k / 16 + 1) + k / 32 + 16) * 2.0 ** -23
+    return want, size * sums * (1 + half) + want.abs() * half + torch.finfo(dtype).smallest_normal * half * 2
+
+
+@pytest.mark.parametrize("m", [1, 2, 5, 8])
+@pytest.mark.parametrize("n,k,group,symmetric,dtype", [
+    (16, 128, 128, True, "f16"), (128, 256, 32, False, "bf16"), (17, 33, 64, True, "bf16"), (250, 1000, 64, False, "f16"),
+    (515, 260, 128, False, "bf16"), (384, 512, 32, True, "f16"), (5000, 200, 64, False, "bf16"),
+])
+def test_gemm_w4_few_rows_have_exact_weights(cuda_device, m, n, k, group, symmetric, dtype):
+    """Up to 8 rows codes are multiplied exactly and scales applied in 32 bits.  A product with weights rounded to 16 bits, in 64
+    bits otherwise, would not pass."""
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    w = lowbit.quantize_w4(randn((n, k), T(dtype), cuda_device, 93, k ** -0.5), group=group, symmetric=symmetric)
+    x = randn((m, k), T(dtype), cuda_device, 94)
+    want, tol = _strict_bound(x, values(w), k, w.dtype)
+    off = (lowbit.gemm_w4(x, w).double() - want).abs()
+    assert bool((off <= tol).all()), f"{int((off > tol).sum())} of {off.numel()} off, worst {float((off / tol).max()):.2f} x"
+    if m * n >= 500:
+        rounded = (x.double() @ lowbit.dequantize_w4(w).double().t()).to(w.dtype).double()
+        assert bool(((rounded - want).abs() > tol).any())
+
+
+@pytest.mark.parametrize("m", [9, 16, 17, 33, 64, 65, 129, 257, 1280])
+@pytest.mark.parametrize("n,k,group,symmetric,dtype", [
+    (16, 128, 128, True, "f16"), (128, 256, 32, False, "bf16"), (1, 1, 32, False, "f16"), (17, 33, 64, True, "bf16"),
+    (250, 1000, 64, False, "f16"), (515, 2047, 128, False, "bf16"), (384, 4096, 32, False, "f16"), (19100, 520, 64, False, "f16"),
+])
+def test_gemm_w4_more_rows_multiply_what_dequantize_gives(cuda_device, m, n, k, group, symmetric, dtype):
+    """From 9 rows on the weights are those that dequantize_w4 gives (checked bit for bit above), and their products are exact."""
+    from subcuber_b200 import lowbit
+
+    w = lowbit.quantize_w4(randn((n, k), T(dtype), cuda_device, 95, k ** -0.5), group=group, symmetric=symmetric)
+    x = randn((m, k), T(dtype), cuda_device, 96)
+    want, tol = _strict_bound(x, lowbit.dequantize_w4(w).double(), k, w.dtype)
+    off = (lowbit.gemm_w4(x, w).double() - want).abs()
+    assert bool((off <= tol).all()), f"{int((off > tol).sum())} of {off.numel()} off, worst {float((off / tol).max()):.2f} x"
+
+
+@pytest.mark.parametrize("m", [1, 17, 100])
+def test_gemm_w4_every_input_counts(cuda_device, m):
+    """One row at a time, a single input of x that is not zero: each result is one weight times 1, exactly."""
+    import torch
+
+    from subcuber_b200 import lowbit
+
+    n, k = 300, 32768 - 77
+    w = lowbit.quantize_w4(randn((n, k), torch.bfloat16, cuda_device, 97, 0.05), group=128)
+    wv = lowbit.dequantize_w4(w) if m > 8 else values(w).bfloat16()
+    for first in (0, 127, 16384, k - m):
+        x = torch.zeros(m, k, dtype=torch.bfloat16, device=cuda_device)
+        at = torch.arange(m, device=cuda_device)
+        x[at, first + at] = 1
+        assert torch.equal(lowbit.gemm_w4(x, w), wv[:, first:first + m].t())
