@@ -177,7 +177,7 @@ int save(const void* x, long long ldx, const Act8& a, cudaStream_t stream) {
 
 template <typename T>
 int restore(const Act8& a, void* x, long long ldx, cudaStream_t stream) {
-  const Cut cut = cut_of(a.m, 2 * ceil_div(a.k, kActBlock));  // whole blocks of 32: both halves take part in the maximum
+  const Cut cut = cut_of(a.m, ceil_div(a.k, 16));
   if (cut.blocks > 0x7fffffffll) return kErrNotSupported;
   act8_restore_kernel<T><<<static_cast<unsigned>(cut.blocks), kThreads, 0, stream>>>(
       static_cast<const uint8_t*>(a.codes), a.pitch, static_cast<const uint8_t*>(a.exps), a.exp_pitch, a.m, a.k,

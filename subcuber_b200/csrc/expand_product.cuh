@@ -105,13 +105,7 @@ __device__ __forceinline__ void tmem_ld_32x8(uint32_t taddr, uint32_t (&r)[8]) {
                : "memory");
 }
 
-// Asynchronous copies of 4 and 16 bytes, zeros where `from` has none to give; a thread's arrival counts once they landed.
-__device__ __forceinline__ void copy_async_16(uint32_t to, const void* from, bool real) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(real ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copy_async_4(uint32_t to, const void* from, bool real) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(real ? 4 : 0) : "memory");
-}
+// The calling thread arrives at `bar` once its asynchronous copies have landed.
 __device__ __forceinline__ void copy_async_arrive(uint64_t* bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(ptx::smem_u32(bar)) : "memory");
 }
@@ -119,17 +113,6 @@ __device__ __forceinline__ void copy_async_arrive(uint64_t* bar) {
 __device__ __forceinline__ uint2 lds_v2(uint32_t smem_addr) {
   uint2 v;
   asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(smem_addr));
-  return v;
-}
-
-__device__ __forceinline__ uint32_t lds_u16(uint32_t smem_addr) {
-  uint16_t v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(smem_addr));
-  return v;
-}
-__device__ __forceinline__ uint32_t lds_u8(uint32_t smem_addr) {
-  uint32_t v;
-  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(smem_addr));
   return v;
 }
 

@@ -156,6 +156,24 @@ __device__ __forceinline__ uint4 expand_act8(uint32_t w0, uint32_t w1, const Act
   return r;
 }
 
+// Asynchronous copies of 4 and 16 bytes, zeros where `from` has none to give.
+__device__ __forceinline__ void copy_async_16(uint32_t to, const void* from, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_async_4(uint32_t to, const void* from, bool real) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(real ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ uint32_t lds_u16(uint32_t smem_addr) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(smem_addr));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds_u8(uint32_t smem_addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(smem_addr));
+  return v;
+}
+
 // A warp stores `count` 16-bit values that lie in shared memory (on 16 bytes) to consecutive places of global memory.
 template <typename T>
 __device__ __forceinline__ void store_row(T* to, const T* from, int count, int lane) {

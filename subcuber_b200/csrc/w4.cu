@@ -245,8 +245,8 @@ int rows_product(const void* x, long long ldx, const W4& w, void* y, long long l
   // one row tile to a warp while that is at most two blocks for each SM, else two, which read x half as often (one row, 2048 x
   // 2048: 2.5 us, 3.0 with two; 4096 x 8192: 7.5 and 7.6; 8192 x 8192: 11.9 us, 13.4 with one; between, 6144 x 8192: 11.7 us,
   // 10.7 with one, but 12.9 and 13.0 at eight rows of x, and 7104 x 2048 4.9 and 5.5; four row tiles were slower everywhere)
-  if (w4_row_tiles(w.n) <= 2 * sm_count_of_current_device()) return launch_rows<T, PER, 1, 1, 4>(p, stream);
-  return launch_rows<T, PER, 2, 1, 3>(p, stream);
+  if (w4_row_tiles(w.n) <= 2 * sm_count_of_current_device()) return launch_rows<T, PER, 1, 4>(p, stream);
+  return launch_rows<T, PER, 2, 3>(p, stream);
 }
 
 template <typename T>

@@ -14,14 +14,16 @@
 //
 // Split.  A warp walks over tiles of 16 rows x 128 inputs: the weights are the left operand of mma.m16n8k16 (16 rows x 16
 // inputs) and 8 rows of x the right one.  The order of inputs inside an instruction is free as long as both operands
-// have the same, so a lane takes its word's eight inputs as they lie in memory.  The eight warps of a block are WR rows of RT
-// row tiles x 8 / WR parts of the inputs, which they take in turn; their sums meet in shared memory in the order of the
-// warps, so that results do not change from call to call.
+// have the same, so a lane takes its word's eight inputs as they lie in memory.  The eight warps of a block take the tiles of its
+// RT row tiles in turn; their sums meet in shared memory in the order of the warps, so that results do not change from call to
+// call.
 //
 // Memory.  The kernel lives from bytes in flight (6.5 TB/s at about 1 us of latency under load are 44 KB for each SM), and
 // registers do not hold them: every warp has a ring of AHEAD stages in shared memory that it fills with 16-byte asynchronous
-// copies of its own, so that no barrier but the warp's own is needed.  Copies of x go through the first-level cache,
-// where the WR warps that work on the same inputs find them.
+// copies of its own, so that no barrier but the warp's own is needed.  The warps of a block work on different inputs; copies of x go
+// through the first-level cache, where the blocks of an SM find what another one fetched.  With one row that is worth up to a sixth
+// (2048 x 2048: 2.3 us, past it 2.7; 4096 x 8192: 7.8, 8.4; 8192 x 8192: 11.7, 12.0), with eight it may cost a tenth (8192 x 8192: 13.1,
+// 13.2; 4096 x 4096, groups of 32: 6.5, 5.8).
 #pragma once
 #include "lowbit_format.cuh"
 #include "per_device.h"
@@ -33,38 +35,24 @@ namespace lowbit {
 constexpr int kRowWarps = 8;
 constexpr int kRowThreads = kRowWarps * 32;
 
-template <typename T> struct Pair16;
-template <> struct Pair16<__half> {
-  static constexpr uint32_t magic = 0x64006400u;  // 1024, last bit 1
-  static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
-  // Codes 2 q and 2 q + 1 (in the order of the inputs) of a word, minus the zero point.
-  static __device__ __forceinline__ uint32_t code(uint32_t w, int q, uint32_t bias, uint32_t mask, uint32_t magic_in_register) {
-    return sub(and_or(w >> (4 * q), mask, magic_in_register), bias);
-  }
-  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-};
-template <> struct Pair16<__nv_bfloat16> {
-  static constexpr uint32_t magic = 0x43004300u;  // 128, last bit 1
-  static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
-    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
-  static __device__ __forceinline__ uint32_t code(uint32_t w, int q, uint32_t bias, uint32_t mask, uint32_t magic_in_register) {
-    return sub(and_or(w >> (4 * q), mask, magic_in_register), bias);
-  }
-  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-};
+// Codes 2 q and 2 q + 1 (in the order of the inputs) of a word, minus the zero point.
+template <typename T>
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, int q, uint32_t bias, uint32_t mask, uint32_t magic) {
+  return sub2<T>(and_or(w >> (4 * q), mask, magic), bias);
+}
+template <typename T> __device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma_16x8x16<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma_16x8x16<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 
 struct RowsParams {
   const void* x;   // rows on 16 bytes
@@ -77,19 +65,9 @@ struct RowsParams {
   int m, n, k, blocks;
 };
 
-__device__ __forceinline__ void rows_copy_cg(uint32_t to, const void* from, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void rows_copy_ca(uint32_t to, const void* from, int bytes) {
+// The first `bytes` of 16, zeros behind; through the first-level cache.
+__device__ __forceinline__ void copy_async_part(uint32_t to, const void* from, int bytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ uint32_t rows_lds(uint32_t a, int bytes) {
-  uint32_t v;
-  uint16_t h;
-  if (bytes == 4) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
-  else if (bytes == 2) { asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(a)); v = h; }
-  else asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(a));
-  return v;
 }
 
 // Bytes of a stage: codes, scales and zeros of RT row tiles, then 128 inputs of eight rows of x.
@@ -97,25 +75,23 @@ __host__ __device__ constexpr int rows_tile_bytes(int per) { return kW4TileBytes
 __host__ __device__ constexpr int rows_stage_bytes(int per, int rt) { return rt * rows_tile_bytes(per) + 8 * 256; }
 __host__ __device__ constexpr int rows_smem(int per, int rt, int ahead) { return kRowWarps * ahead * rows_stage_bytes(per, rt); }
 
-template <typename T, int PER, int RT, int WR, int AHEAD, bool ZEROS>
+template <typename T, int PER, int RT, int AHEAD, bool ZEROS>
 __global__ void __launch_bounds__(kRowThreads) w4_rows_kernel(const RowsParams p) {
-  constexpr int WK = kRowWarps / WR;
   constexpr int kTile = rows_tile_bytes(PER), kStage = rows_stage_bytes(PER, RT);
   static_assert(kRowWarps * 8 * (RT * 16 + 1) * 4 <= rows_smem(PER, RT, AHEAD), "the sums reuse the rings");
   extern __shared__ __align__(128) uint8_t smem_rows[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int wk = warp % WK, wr = warp / WK;
-  const int tile0 = (static_cast<int>(blockIdx.x) * WR + wr) * RT;  // first row tile of the warp
+  const int tile0 = static_cast<int>(blockIdx.x) * RT;  // first row tile of the block
   const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem_rows)) + warp * (AHEAD * kStage);
 
-  // where this lane's copies come from; they move on by WK tiles of 128 inputs
+  // where this lane's copies come from; they move on by a tile of 128 inputs for each warp of the block
   const uint8_t *codes[RT], *table[RT];
   const bool copies_table = lane < 2 * PER || (ZEROS && lane < 3 * PER);  // 2 PER pieces of scales, PER of zeros
-  const int table_step = WK * kW4Rows * PER * (lane < 2 * PER ? 2 : 1);
+  const int table_step = kRowWarps * kW4Rows * PER * (lane < 2 * PER ? 2 : 1);
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     // row tiles behind the weights read the last one and are not stored
-    const long long tile = static_cast<long long>(min(tile0 + r, w4_row_tiles(p.n) - 1)) * p.blocks + wk;
+    const long long tile = static_cast<long long>(min(tile0 + r, w4_row_tiles(p.n) - 1)) * p.blocks + warp;
     codes[r] = p.codes + tile * kW4TileBytes + lane * 16;
     table[r] = lane < 2 * PER ? p.scales + tile * (kW4Rows * 2 * PER) + lane * 16
                               : p.zeros + tile * (kW4Rows * PER) + (lane - 2 * PER) * 16;
@@ -125,16 +101,16 @@ __global__ void __launch_bounds__(kRowThreads) w4_rows_kernel(const RowsParams p
   // there reaches columns of the result that are not stored.
   const int xc = lane & 15, xrow = lane >> 4;
   const T* x = static_cast<const T*>(p.x) + xrow * p.ldx;
-  int fetch_k = wk * kW4Block + xc * 8, fetch_b = wk, fill = 0;
+  int fetch_k = warp * kW4Block + xc * 8, fetch_b = warp, fill = 0;
   auto fetch = [&]() {
     if (fetch_b < p.blocks) {
       const uint32_t to = ring + fill * kStage;
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
-        rows_copy_cg(to + r * kTile + lane * 16, codes[r], 16);
-        rows_copy_cg(to + r * kTile + 512 + lane * 16, codes[r] + 512, 16);
-        if (copies_table) rows_copy_cg(to + r * kTile + kW4TileBytes + lane * 16, table[r], 16);
-        codes[r] += WK * kW4TileBytes;
+        copy_async_16(to + r * kTile + lane * 16, codes[r], true);
+        copy_async_16(to + r * kTile + 512 + lane * 16, codes[r] + 512, true);
+        if (copies_table) copy_async_16(to + r * kTile + kW4TileBytes + lane * 16, table[r], true);
+        codes[r] += kRowWarps * kW4TileBytes;
         table[r] += table_step;
       }
       const int left = min(max(p.k - fetch_k, 0), 8) * 2;
@@ -142,10 +118,10 @@ __global__ void __launch_bounds__(kRowThreads) w4_rows_kernel(const RowsParams p
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if (2 * i + xrow < p.m)
-          rows_copy_ca(to + RT * kTile + (2 * i + xrow) * 256 + ((xc ^ (xrow << 2)) << 4), from + 2 * i * p.ldx, left);
+          copy_async_part(to + RT * kTile + (2 * i + xrow) * 256 + ((xc ^ (xrow << 2)) << 4), from + 2 * i * p.ldx, left);
     }
-    fetch_b += WK;
-    fetch_k += WK * kW4Block;
+    fetch_b += kRowWarps;
+    fetch_k += kRowWarps * kW4Block;
     fill = fill + 1 == AHEAD ? 0 : fill + 1;
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -154,9 +130,9 @@ __global__ void __launch_bounds__(kRowThreads) w4_rows_kernel(const RowsParams p
 #pragma unroll
   for (int a = 0; a < AHEAD - 1; ++a) fetch();
   int stage = 0;
-  const uint32_t mask = in_register(0x000f000fu), magic = in_register(Pair16<T>::magic);
+  const uint32_t mask = in_register(0x000f000fu), magic = in_register(Half<T>::magic);
   const uint32_t xat = g * 256 + ((t ^ ((g & 1) << 2)) << 4);  // of word 0; word j is 64 j further, exclusive-or
-  for (int b = wk; b < p.blocks; b += WK) {
+  for (int b = warp; b < p.blocks; b += kRowWarps) {
     asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 2) : "memory");
     __syncwarp();  // every lane's copies of this stage are there, and all have read the stage that is filled next
     fetch();
@@ -177,10 +153,10 @@ __global__ void __launch_bounds__(kRowThreads) w4_rows_kernel(const RowsParams p
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int entry = (8 * h + g) * PER + gr;
-          const uint16_t s = static_cast<uint16_t>(rows_lds(tile + kW4TileBytes + 2 * entry, 2));
+          const uint16_t s = static_cast<uint16_t>(lds_u16(tile + kW4TileBytes + 2 * entry));
           scale[h] = to_f32(*reinterpret_cast<const T*>(&s));
-          bias[h] = Pair16<T>::magic +
-                    (ZEROS ? __byte_perm(rows_lds(tile + kW4TileBytes + kW4Rows * 2 * PER + entry, 1), 0, 0x4040) : 0x00080008u);
+          bias[h] = Half<T>::magic +
+                    (ZEROS ? __byte_perm(lds_u8(tile + kW4TileBytes + kW4Rows * 2 * PER + entry), 0, 0x4040) : 0x00080008u);
         }
         float acc[4] = {};
 #pragma unroll
@@ -189,9 +165,9 @@ __global__ void __launch_bounds__(kRowThreads) w4_rows_kernel(const RowsParams p
           const uint32_t xw[4] = {xv[j].x, xv[j].y, xv[j].z, xv[j].w};
 #pragma unroll
           for (int q = 0; q < 4; q += 2) {
-            const uint32_t a4[4] = {Pair16<T>::code(lo[j], q, bias[0], mask, magic), Pair16<T>::code(hi[j], q, bias[1], mask, magic),
-                                    Pair16<T>::code(lo[j], q + 1, bias[0], mask, magic), Pair16<T>::code(hi[j], q + 1, bias[1], mask, magic)};
-            Pair16<T>::mma(acc, a4, xw[q], xw[q + 1]);
+            const uint32_t a4[4] = {code_pair<T>(lo[j], q, bias[0], mask, magic), code_pair<T>(hi[j], q, bias[1], mask, magic),
+                                    code_pair<T>(lo[j], q + 1, bias[0], mask, magic), code_pair<T>(hi[j], q + 1, bias[1], mask, magic)};
+            mma_16x8x16<T>(acc, a4, xw[q], xw[q + 1]);
           }
         }
         total[r][0] = fmaf(scale[0], acc[0], total[r][0]);
@@ -209,34 +185,34 @@ __global__ void __launch_bounds__(kRowThreads) w4_rows_kernel(const RowsParams p
 #pragma unroll
     for (int i = 0; i < 4; ++i) part[warp][2 * t + (i & 1)][r * 16 + g + 8 * (i >> 1)] = total[r][i];
   __syncthreads();
-  constexpr int kCols = WR * RT * 16;
+  constexpr int kCols = RT * 16;
   for (int e = threadIdx.x; e < p.m * kCols; e += kRowThreads) {
     const int row = e / kCols, c = e % kCols, col = static_cast<int>(blockIdx.x) * kCols + c;
     float s = 0.f;
 #pragma unroll
-    for (int w = 0; w < WK; ++w) s += part[c / (RT * 16) * WK + w][row][c % (RT * 16)];
+    for (int w = 0; w < kRowWarps; ++w) s += part[w][row][c];
     if (col < p.n) static_cast<T*>(p.y)[row * p.ldy + col] = from_f32<T>(s);
   }
 }
 
-template <typename T, int PER, int RT, int WR, int AHEAD, bool ZEROS>
+template <typename T, int PER, int RT, int AHEAD, bool ZEROS>
 int launch_rows_kernel(const RowsParams& p, cudaStream_t stream) {
   constexpr int kSmem = rows_smem(PER, RT, AHEAD);
   if (kSmem > 48 * 1024) {
     static PerDeviceOnce attr;
     const int rc = attr.run_once([] {
-      return static_cast<int>(cudaFuncSetAttribute(w4_rows_kernel<T, PER, RT, WR, AHEAD, ZEROS>,
+      return static_cast<int>(cudaFuncSetAttribute(w4_rows_kernel<T, PER, RT, AHEAD, ZEROS>,
                                                    cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
     });
     if (rc) return rc;
   }
-  w4_rows_kernel<T, PER, RT, WR, AHEAD, ZEROS><<<ceil_div(w4_row_tiles(p.n), RT * WR), kRowThreads, kSmem, stream>>>(p);
+  w4_rows_kernel<T, PER, RT, AHEAD, ZEROS><<<ceil_div(w4_row_tiles(p.n), RT), kRowThreads, kSmem, stream>>>(p);
   return static_cast<int>(cudaGetLastError());
 }
-template <typename T, int PER, int RT, int WR, int AHEAD>
+template <typename T, int PER, int RT, int AHEAD>
 int launch_rows(const RowsParams& p, cudaStream_t stream) {
-  return p.zeros ? launch_rows_kernel<T, PER, RT, WR, AHEAD, true>(p, stream)
-                 : launch_rows_kernel<T, PER, RT, WR, AHEAD, false>(p, stream);
+  return p.zeros ? launch_rows_kernel<T, PER, RT, AHEAD, true>(p, stream)
+                 : launch_rows_kernel<T, PER, RT, AHEAD, false>(p, stream);
 }
 
 }  // namespace lowbit
