@@ -303,8 +303,9 @@ int sb200_peer_wait(int* const* local_flags, int count, int value, unsigned wait
 size_t sb200_w4_codes_bytes(int n, int k);
 size_t sb200_w4_table_entries(int n, int k, int group);
 /* Quantise w (n x k, 16-bit), group by group.  zeros == NULL: scale = amax / 7, code = 8 + rint(w / scale).  Else, with
- * lo = min(0, w) and hi = max(0, w): scale = (hi - lo) / 15, zero = rint(-lo / scale), code = zero + rint(w / scale).  The
- * scale is rounded to `dtype` before the codes are made; codes are held within 0..15.  A group with an infinity or a NaN
+ * lo = min(0, w) and hi = max(0, w): scale = (hi - lo) / 15 (in fp32), zero = rint(-lo / scale), code = zero + rint(w / scale).  The
+ * scale is rounded to `dtype` before the codes are made; codes are held within 0..15.  Weights next to the largest f16 number may
+ * stand for more than it (their value in `dtype` is then infinite).  A group with an infinity or a NaN
  * (or whose hi - lo overflows) gets a scale that is not finite: its weights stand for NaN. */
 int sb200_w4_quantize(int dtype, const void* w, long long ldw, int n, int k, int group, void* codes, void* scales, void* zeros,
                       sb200_stream_t stream);

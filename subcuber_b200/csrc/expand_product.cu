@@ -14,9 +14,17 @@ namespace {
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
 constexpr int kMaxSlices = 16;
-constexpr int kDenseColumns = 1280;  // from here on two passes: rows through 8192 x 4096 4-bit weights, on the
-// way and in two passes: 512: 37 and 44 us, 1024: 64 and 63, 1280: 89 and 77, 4096: 202 and 181; columns of a gradient of 4096
-// channels from 4096 tokens: 512: 31 and 37 us, 1024: 41 and 42, 1280: 69 and 60, 2048: 72 and 64
+// From here on two passes.  On the way and in two passes, in us; rows through 4-bit weights:
+//   2048 x 2048:   512: 15 and 17, 1024: 20 and 18, 1280: 21 and 19, 2048: 21 and 20
+//   4096 x 4096:   512: 26 and 30, 1024: 33 and 34, 1280: 60 and 48, 2048: 59 and 54
+//   8192 x 4096:   512: 34 and 42, 1024: 59 and 62, 1280: 86 and 78, 2048: 112 and 110
+//   16384 x 4096:  512: 65 and 85, 1024: 115 and 124, 1280: 142 and 147, 2048: 206 and 202
+//   8192 x 8192:   512: 59 and 86, 1024: 111 and 131, 1280: 162 and 157, 2048: 217 and 221
+// columns of a gradient, tokens x channels:
+//   2048 x 1024:   512: 16 and 20, 1024: 17 and 24, 1280: 20 and 24, 2048: 23 and 25
+//   4096 x 4096:   512: 31 and 39, 1024: 39 and 43, 1280: 69 and 60, 2048: 69 and 65
+//   16384 x 2048:  512: 42 and 56, 1024: 68 and 76, 1280: 90 and 94, 2048: 118 and 113
+constexpr int kDenseColumns = 1280;
 constexpr size_t kPartBytes = size_t(64) << 20;  // most that the parts of a divided reduction may take
 
 struct Cut {
@@ -196,9 +204,9 @@ int launch_decode(const DecodeParams& p, cudaStream_t stream) {
   cfg.numAttrs = 1;
   // CTAs that divide the inputs of 128 rows: as many as fit on the device at once, one for each SM, or two where they have eight
   // tiles or more to go through (the runtime counts one).  A cluster lies within one group of SMs, which leaves some of
-  // them over.  16 rows, clusters of 1, 2, 4 and 8 CTAs in us: 128 x 4096: 15.9, 10.4, 7.5, 6.2; 4096 x 4096: 17.4, 11.7, 8.8,
-  // 9.8; 8192 x 1024: 7.2, 6.2, 7.2, 12.3; 8192 x 8192: 30.4, 18.6, 16.9, 21.8; 9472 x 4096: 17.8, 12.5, 16.9, 20.2;
-  // 16384 x 512: 5.6, 7.1, 10.9, 10.8; 16384 x 4096: 18.0, 17.0, 20.4, 29.7.
+  // them over.  16 rows, clusters of 1, 2, 4 and 8 CTAs in us: 128 x 4096: 16.6, 11.2, 8.2, 6.8; 4096 x 4096: 17.5, 11.8, 9.3,
+  // 10.2; 8192 x 1024: 7.4, 6.7, 8.2, 13.8; 8192 x 8192: 31.8, 19.6, 18.4, 24.0; 9472 x 4096: 18.2, 12.8, 18.4, 22.8;
+  // 16384 x 512: 6.3, 8.1, 13.1, 13.1 (no more than four, the tiles); 16384 x 4096: 18.7, 17.8, 22.8, 33.3.
   static std::atomic<int> room[kMaxDevices][kDecodeMaxRight / 16][4];  // clusters at once, plus one
   const int groups = ceil_div(p.n, kDecodeRows);
   int dev = -1, log2 = 3, least = 0;

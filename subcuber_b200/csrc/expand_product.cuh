@@ -6,20 +6,21 @@
 // reduction each CTA's converter warps (two groups of four, in turn) expand the 128 x 64 values of its own left rows into the swizzled shared-memory
 // tile that the tensor cores read; TMA brings the codes and the CTA's half of the right operand, so that no
 // converter has a load of its own in flight when it hands a tile to the tensor cores.  The expansion costs no pass over
-// memory: the operand travels in 4 or 8 bits and is never written out in 16.
+// memory: the operand travels in 4 or 8 bits and is never written out in 16.  (One rounding to 16 bits for each weight is what the
+// tensor cores ask of an operand whose scale changes along the reduction.)
 //   W4    the tile is K-major (a word of the format is the 16 bytes of eight neighbouring inputs); weights are rounded to 16
 //         bits once, code - zero is exact before.
 //   ACT8  the tile is MN-major (tokens are rows in memory, channels run along a row); every value is exact in 16 bits.
 //
 // A left tile is expanded once for every tile of columns.  With many of those it is cheaper to expand the operand once into 16
-// bits in the workspace and to multiply that (DENSE: the left tiles come by TMA too, there are no converters): 4096 rows
-// through 8192 x 4096 4-bit weights take 181 us, expanded on the way 202 us; a gradient of 4096 x 2048 from 4096 tokens
-// 64 and 72 us.
+// bits in the workspace and to multiply that (DENSE: the left tiles come by TMA too, there are no converters): 1280 rows
+// through 8192 x 4096 4-bit weights take 78 us, expanded on the way 86 us; a gradient of 4096 x 1280 from 4096 tokens
+// 60 and 69 us (expand_product.cu has more sizes).
 //
-// Bound.  Dense, a large product: the tensor pipe is busy for 79 % of the cycles, and under a long load the power limit lowers
-// the clock (4096 rows through 8192 x 4096: 1.5 PFLOP/s; a gradient of 4096 x 8192 from 16384 tokens 1.5 in a short run,
-// 1.1 in a long one).  Expanded on the way: tensor pipe 60 %, the converters issue in 41 % of the cycles, and
-// operands, codes and expanded tiles share the bandwidth of shared memory.  Small products: about 9 us for the launch, the
+// Bound.  Dense, a large product: the tensor pipe is busy for 89 % of the cycles (2048 rows; a gradient of 2048 x 2304: 75 %), and
+// under a long load the power limit lowers the clock (4096 rows through 8192 x 4096: 1.2 PFLOP/s in a long run, 1.5 in a short
+// one; a gradient of 4096 x 8192 from 16384 tokens 1.1 and 1.5).  Expanded on the way: tensor pipe 51 % (4-bit) and 55 % (8-bit), the
+// converters issue in 36 and 42 % of the cycles, and operands, codes and expanded tiles share the bandwidth of shared memory.  Small products: about 9 us for the launch, the
 // setup, the first loads, the last sums and the end, and 0.37 us for every step of 64 that a narrow tile takes.
 //
 // Sums.  The tensor cores chop when they add to an accumulator (measured on B200, exact products of normal values:

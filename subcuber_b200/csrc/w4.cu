@@ -257,7 +257,8 @@ int rows_product_any(const void* x, long long ldx, const W4& w, void* y, long lo
 }
 
 // Up to here, the columns of one warp instruction, the codes are multiplied as they are (w4_rows.cuh); more rows go to
-// tcgen05.mma (w4_decode.cuh).  8192 x 8192: 1 row 11.6 us, the other kernel 16.1; 8 rows 12.7 and 16.5; 9 rows 16.6.
+// tcgen05.mma (w4_decode.cuh).  In one run, this kernel and the other one: 8192 x 8192: 1 row 12.1 and 17.3 us, 8 rows 13.3 and 18.1,
+// 9 rows 18.3 (the other); 2048 x 2048: 1 row 2.3 and 5.9, 8 rows 2.4 and 6.4, 9 rows 6.8; 16384 x 4096: 8 rows 14.1 and 17.8.
 constexpr int kFewRows = 8;
 
 int check(const W4& w) {

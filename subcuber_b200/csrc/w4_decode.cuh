@@ -5,11 +5,15 @@
 // weights go where tcgen05.mma takes them from without another pass through shared memory: a thread expands a row of
 // 128 inputs in its registers and writes it to its lane of tensor memory, which is the left operand (128 rows x 16 inputs
 // an instruction); x, the right operand, comes to shared memory by TMA.  What a batch costs is then almost independent of its
-// rows: 8192 x 8192, groups of 128: 9 rows 16.6 us, 16 rows 17.0, 32 rows 17.7, 64 rows 19.4 (the bytes: 5.3 us; 2.0 TB/s).
+// rows: 8192 x 8192, groups of 128: 9 rows 17.9 us, 16 rows 18.4, 32 rows 19.2, 64 rows 21.0 (the bytes: 5.3 us; 1.9 TB/s).  64 rows are
+// what its shared memory and 256 columns of tensor memory hold; 65 rows in the next kernel take 36.0 us (4096 x 4096: 11.4 and 17.4).
 //
-// Bound.  Neither memory nor the tensor cores (6 % busy) nor one pipe: the integer pipe is active for 37 % of the cycles, issue for
-// half, and the warps wait on one another (load, expand, store to tensor memory, hand over).  About 15 instructions for
-// eight weights are the expansion; the scales are multiplied in here, one rounding to 16 bits for each weight.
+// Bound.  Neither memory nor the tensor cores (16 rows: 6 % busy, 64: 22 %) nor one pipe: the integer pipe is active for 36 % of the
+// cycles, issue for half, and the warps wait on one another (load, expand, store to tensor memory, hand over).  About 15 instructions
+// for eight weights are the expansion.  The scales are multiplied in here, one rounding to 16 bits for each weight: an accumulator
+// gathers groups whose scales differ, and scaling the sums of each group instead, as up to 8 rows, would mean emptying it every 32 to
+// 128 inputs.  Against exact weights that costs a third more error in the result (bf16, root mean square: 0.0022 of the result; its own
+// rounding alone is 0.0017).
 //
 // Split.  A CTA holds 128 rows; where rows are few, the CTAs of a cluster divide the inputs and add their sums over
 // distributed shared memory, rank by rank, so that results do not change from call to call.  Two CTAs share an SM: one

@@ -1,9 +1,9 @@
 // y = x W^T for up to 8 rows of x, weights in format W4.
 //
 // Bound.  The bytes of the weights are the floor (8192 x 8192, groups of 128: 34.6 MB, 5.3 us at the measured copy rate); one row
-// takes 11.9 us (2.9 TB/s), eight take 13.1.  What holds it there is the issue of instructions: a tile of 1 KiB costs a warp
+// takes 11.8 us (2.9 TB/s), eight take 12.8.  What holds it there is the issue of instructions: a tile of 1 KiB costs a warp
 // about 240, most of them logical operations and subtractions that turn codes into numbers; of the active cycles 60 %
-// issue, the integer pipe is busy for 58 % and the tensor pipe for 21 %.  Fewer than four operations for two codes
+// issue, the integer pipe is busy for 57 % and the tensor pipe for 21 %.  Fewer than four operations for two codes
 // (shift, and-or, subtract, and a quarter of the matrix instruction) were not found.
 //
 // Mathematics.  Codes are small whole numbers and exact in 16 bits, so that the matrix instruction multiplies (code -
@@ -22,8 +22,8 @@
 // registers do not hold them: every warp has a ring of AHEAD stages in shared memory that it fills with 16-byte asynchronous
 // copies of its own, so that no barrier but the warp's own is needed.  The warps of a block work on different inputs; copies of x go
 // through the first-level cache, where the blocks of an SM find what another one fetched.  With one row that is worth up to a sixth
-// (2048 x 2048: 2.3 us, past it 2.7; 4096 x 8192: 7.8, 8.4; 8192 x 8192: 11.7, 12.0), with eight it may cost a tenth (8192 x 8192: 13.1,
-// 13.2; 4096 x 4096, groups of 32: 6.5, 5.8).
+// (in one run, 2048 x 2048: 2.3 us, past it 2.7; 4096 x 8192: 7.8, 8.4; 8192 x 8192: 11.7, 12.0), with eight it may cost a tenth
+// (8192 x 8192: 13.1, 13.2; 4096 x 4096, groups of 32: 6.5, 5.8).
 #pragma once
 #include "lowbit_format.cuh"
 #include "per_device.h"

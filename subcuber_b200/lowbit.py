@@ -14,7 +14,14 @@ Activations saved in 8 bits for the backward pass (training):
 The formats and the exact rounding rules are described in include/subcuber_b200.h.  All compute happens in the CUDA
 library, asynchronously on the current stream of the operands' device; every call can be captured into a graph.  A
 workspace that is passed in serves one call at a time: calls that may overlap (other streams, two captured graphs that
-are replayed at once) need one each.  The reference project has no counterpart.
+are replayed at once) need one each.
+
+Every wait inside a kernel is bounded.  A product whose wait gave up (2 s, or the bound in `opts`) leaves an incomplete result and
+a status: `check=True` waits for the call and raises, or, with a workspace of one's own, its `check()` does at any time
+before the next call that uses it.  Without either nothing is reported.
+
+As with `runner.gemm` there is no autograd here: a result of tensors that require gradients does not.  The reference project has
+no counterpart.
 """
 from __future__ import annotations
 
@@ -120,7 +127,8 @@ class _Workspace:
         return self.ptr, self.nbytes
 
     def check(self) -> None:
-        """Wait for the call that used the workspace last and raise if a device-side wait gave up."""
+        """Wait for the calls so far and raise if a device-side wait of the last product in this workspace gave up (`gemm_w4` of up to 8
+        rows has no waits and leaves the status of the product before it)."""
         _status(self.ptr, self.device)
 
 
@@ -232,7 +240,8 @@ def dequantize_w4(w: WeightsW4, out: Optional[torch.Tensor] = None) -> torch.Ten
 
 class WorkspaceW4(_Workspace):
     """Device workspace for `gemm_w4` with up to `m` rows; for one call at a time.  `aligned`: the rows of x will start on 16
-    bytes (the default expects packed rows); else there is room for a copy of x."""
+    bytes (the default expects packed rows); else there is room for a copy of x.  From 65 rows on up to 64 MB, from 1280 rows on the
+    weights in 16 bits besides."""
 
     def __init__(self, m: int, w: WeightsW4, aligned: Optional[bool] = None):
         _extent("rows", m)
@@ -243,7 +252,8 @@ class WorkspaceW4(_Workspace):
 
 def gemm_w4(x: torch.Tensor, w: WeightsW4, out: Optional[torch.Tensor] = None, workspace: Optional[WorkspaceW4] = None,
             check: bool = False, opts=None) -> torch.Tensor:
-    """x @ W^T (m x out_features) for x (m x in_features) of the weights' type; sums in fp32.  `out` must not overlap x.
+    """x @ W^T (m x out_features) for x (m x in_features) of the weights' type; sums in fp32.  Up to 8 rows the codes and scales are
+    exact, with more the weights are those of `dequantize_w4`, rounded to their type.  `out` must not overlap x.
     `check` synchronises and raises if a device-side wait gave up; `opts` (`runner.options`): the bound of those waits."""
     _matrix("x", x, (w.dtype,))
     m, k = x.shape
