@@ -3,8 +3,9 @@
 // Bound.  The bytes of the weights are the floor (8192 x 8192, groups of 128: 34.6 MB, 5.3 us at the measured copy rate); one row
 // takes 11.8 us (2.9 TB/s), eight take 12.8.  What holds it there is the issue of instructions: a tile of 1 KiB costs a warp
 // about 240, most of them logical operations and subtractions that turn codes into numbers; of the active cycles 60 %
-// issue, the integer pipe is busy for 57 % and the tensor pipe for 21 %.  Fewer than four operations for two codes
-// (shift, and-or, subtract, and a quarter of the matrix instruction) were not found.
+// issue, the integer pipe is busy for 57 % and the tensor pipe for 21 %.  Two codes cost four
+// operations (shift, and-or, subtract, and a quarter of the matrix instruction); in f16 two of the three shifts of a word could go, since
+// the upper code of a byte, masked in place, is worth 16 units that a fused multiply-add takes off exactly.
 //
 // Mathematics.  Codes are small whole numbers and exact in 16 bits, so that the matrix instruction multiplies (code -
 // zero) with x without any rounding; the sums of one group are scaled in fp32 afterwards:
